@@ -10,11 +10,11 @@ include/lgx.h); there is no CPU fallback.
 from . import _lib
 from ._lib import build, version
 from .graph import CSRGraph, build_norm_adj, from_csr_arrays, from_sparse_coo, make_plan
-from .ops import (fill_normal, foldout_metrics, gather_scores, propagate, propagate_layer, score_dense,
-                  score_topk, spmm, topk_rows)
+from .ops import (MXTable, fill_normal, foldout_metrics, gather_scores, mx_dequantize, mx_quantize, propagate,
+                  propagate_layer, sample_rows, score_dense, score_mx, score_topk, spmm, topk_rows)
 
 __all__ = [
     "build", "version", "CSRGraph", "build_norm_adj", "from_csr_arrays", "from_sparse_coo", "make_plan",
     "propagate", "propagate_layer", "spmm", "score_dense", "score_topk", "topk_rows", "foldout_metrics",
-    "gather_scores", "fill_normal",
+    "gather_scores", "fill_normal", "MXTable", "mx_quantize", "mx_dequantize", "score_mx", "sample_rows",
 ]

@@ -20,6 +20,8 @@ CSRC = os.path.join(_HERE, "csrc")
 LGX_OK = 0
 LGX_DTYPE_F32 = 0
 LGX_DTYPE_BF16 = 1
+LGX_DTYPE_MXFP4 = 2
+LGX_DTYPE_F64 = 3
 LGX_LAYER_PLAIN, LGX_LAYER_FIRST, LGX_LAYER_MID, LGX_LAYER_LAST, LGX_LAYER_ONLY, LGX_LAYER_PARTIAL, LGX_LAYER_STACK = range(7)
 LGX_REDUCE_MAX, LGX_REDUCE_SUM = 0, 1
 LGX_STRAT_EXACT = 1
@@ -111,6 +113,14 @@ SIGNATURES = {
     "lgx_test_metrics_workspace": (_c_int, [_c_i64, _c_int, _sz_p]),
     "lgx_test_metrics": (_c_int, [_vp, _c_i64, _c_int, _vp, _vp, _vp, _vp, _c_int, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
     "lgx_gather_scores": (_c_int, [_vp, _vp, _c_i64, _c_i64, _c_i64, _vp, _vp, _c_i64, _vp, _vp]),
+    "lgx_mx_quantize": (_c_int, [_vp, _c_i64, _c_i64, _c_i64, _c_int, _vp, _vp, _vp]),
+    "lgx_mx_dequantize": (_c_int, [_vp, _vp, _c_i64, _c_i64, _c_int, _vp, _vp]),
+    "lgx_score_mx_workspace": (_c_int, [_c_i64, _c_i64, _c_int, _sz_p]),
+    "lgx_score_mx": (_c_int, [_vp, _vp, _c_int, _c_i64, _c_i64, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_int, _c_int,
+                              _vp, _vp, ctypes.c_size_t, _vp]),
+    "lgx_sample_rows_workspace": (_c_int, [_c_i64, _c_i64, _c_i64, _sz_p]),
+    "lgx_sample_rows": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _vp, _c_int, _c_i64, ctypes.c_double, _vp, _c_i64,
+                                 _vp, ctypes.c_double, _vp, ctypes.c_double, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
     "lgx_synth_edges": (_c_int, [ctypes.c_uint64, _vp, _c_i64, _vp, _vp, _c_i64, _c_i64, _vp, _vp, _vp]),
     "lgx_fill_normal": (_c_int, [_vp, _c_i64, ctypes.c_float, ctypes.c_uint64, _c_int, _vp]),
     "lgx_fill_normal_at": (_c_int, [_vp, _c_i64, _c_i64, ctypes.c_float, ctypes.c_uint64, _c_int, _vp]),

@@ -1,0 +1,360 @@
+// Microscaled 4-bit floating point tables: quantisation, its inverse, and full-catalog scoring over them.
+//
+// A row of d elements is cut into blocks of 32.  A block with largest magnitude a is stored as one byte
+// b = max(E(a) - 2, 0), E the f32 exponent field, standing for the scale 2^(b - 127), and 32 e2m1 codes of
+// x * 2^(127 - b): 4.25 bits an element, 1/7.5 of f32.  lgx_score_mx multiplies such rows on the block-scaled
+// matrix instructions, which take the codes and scale bytes as they are stored.
+#include "lgx_common.h"
+
+#include <algorithm>
+
+namespace lgx {
+namespace {
+
+constexpr int kBlock = 32;       // elements under one scale
+constexpr int64_t kMaxD = 65536;
+
+using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
+using f32x4 = float __attribute__((ext_vector_type(4)));
+using f32x2 = float __attribute__((ext_vector_type(2)));
+using f32x16 = float __attribute__((ext_vector_type(16)));
+using i32x8 = int __attribute__((ext_vector_type(8)));
+
+// the codes of 8 scaled elements, element 0 in the low nibble of byte 0 (v_cvt_scalef32_pk_fp4_f32 rounds
+// to nearest even and saturates at 6; the scale is applied by the caller, so its own is 1)
+__device__ __forceinline__ uint32_t pack8(const float (&y)[8]) {
+    uint32_t r = 0;
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, y[0], y[1], 1.0f, 0);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, y[2], y[3], 1.0f, 1);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, y[4], y[5], 1.0f, 2);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, y[6], y[7], 1.0f, 3);
+    return r;
+}
+
+__device__ __forceinline__ void load8_f32(const float* p, float (&x)[8]) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = a[j], x[4 + j] = b[j];
+}
+__device__ __forceinline__ void load8_bf16(const uint16_t* p, float (&x)[8]) {
+    const u32x4 a = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        x[2 * j] = __uint_as_float(a[j] << 16);
+        x[2 * j + 1] = __uint_as_float(a[j] & 0xffff0000u);
+    }
+}
+
+// 4 lanes per block, 8 elements a lane.  VEC: rows are 16-byte aligned and d % 8 == 0.  rows_of (optional):
+// the source row of every output row, a row outside [0, n_src) gives NaN blocks.
+template <bool BF16, bool VEC>
+__global__ __launch_bounds__(256) void mx_quantize_kernel(const void* __restrict__ X, const int64_t* __restrict__ rows_of,
+                                                          int64_t n_src, int64_t units, int64_t nb, int64_t d, int64_t ld,
+                                                          uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+    const int64_t unit = blockIdx.x * (int64_t)64 + (threadIdx.x >> 2);
+    const int sub = threadIdx.x & 3;
+    if (unit >= units) return;
+    const int64_t row = units <= UINT32_MAX ? (int64_t)((uint32_t)unit / (uint32_t)nb) : unit / nb;
+    const int64_t c0 = (unit - row * nb) * kBlock + sub * 8;
+    int64_t src = row;
+    bool bad = false;
+    if (rows_of) {
+        src = rows_of[row];
+        bad = src < 0 || src >= n_src;
+    }
+    float x[8] = {};
+    if (!bad) {
+        if (VEC) {
+            if (c0 < d) {
+                if (BF16)
+                    load8_bf16(static_cast<const uint16_t*>(X) + src * ld + c0, x);
+                else
+                    load8_f32(static_cast<const float*>(X) + src * ld + c0, x);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c0 + j < d)
+                    x[j] = BF16 ? bf16_to_f32(static_cast<const uint16_t*>(X)[src * ld + c0 + j])
+                                : static_cast<const float*>(X)[src * ld + c0 + j];
+        }
+    }
+    uint32_t a = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a = max(a, __float_as_uint(x[j]) & 0x7fffffffu);
+    a = max(a, (uint32_t)__shfl_xor((int)a, 1));
+    a = max(a, (uint32_t)__shfl_xor((int)a, 2));
+    const uint32_t e = a >> 23;
+    bad |= e == 255u;  // an infinity or a NaN
+    const uint32_t b = bad ? 255u : e > 2u ? e - 2u : 0u;
+    const float inv = __uint_as_float((254u - b) << 23);  // 2^(127 - b), b <= 252
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = x[j] * inv;
+    reinterpret_cast<uint32_t*>(codes)[unit * 4 + sub] = bad ? 0u : pack8(y);
+    if (sub == 0) scales[unit] = (uint8_t)b;
+}
+
+__device__ __forceinline__ float scale_value(uint32_t b) {  // 2^(b - 127); b = 0 is the subnormal 2^-127
+    return b == 255u ? __builtin_nanf("") : __uint_as_float(b ? b << 23 : 0x00400000u);
+}
+
+// 4 lanes per block, 8 elements a lane (the layout of the quantiser)
+template <bool BF16, bool VEC>
+__global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint8_t* __restrict__ codes,
+                                                            const uint8_t* __restrict__ scales, int64_t units, int64_t nb,
+                                                            int64_t d, void* __restrict__ out) {
+    const int64_t unit = blockIdx.x * (int64_t)64 + (threadIdx.x >> 2);
+    const int sub = threadIdx.x & 3;
+    if (unit >= units) return;
+    const int64_t row = units <= UINT32_MAX ? (int64_t)((uint32_t)unit / (uint32_t)nb) : unit / nb;
+    const int64_t c0 = (unit - row * nb) * kBlock + sub * 8;
+    if (c0 >= d) return;
+    const uint32_t c = reinterpret_cast<const uint32_t*>(codes)[unit * 4 + sub];
+    const float s = scale_value(scales[unit]);
+    f32x2 p[4];
+    p[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 0);
+    p[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 1);
+    p[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 2);
+    p[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 3);
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = p[j / 2][j % 2] * s;
+    if (BF16) {
+        uint16_t* o = static_cast<uint16_t*>(out) + row * d + c0;
+        if (VEC) {
+            u32x4 w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = f32_to_bf16(v[2 * j]) | (uint32_t)f32_to_bf16(v[2 * j + 1]) << 16;
+            *reinterpret_cast<u32x4*>(o) = w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c0 + j < d) o[j] = f32_to_bf16(v[j]);
+        }
+    } else {
+        float* o = static_cast<float*>(out) + row * d + c0;
+        if (VEC) {
+            *reinterpret_cast<f32x4*>(o) = f32x4{v[0], v[1], v[2], v[3]};
+            *reinterpret_cast<f32x4*>(o + 4) = f32x4{v[4], v[5], v[6], v[7]};
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c0 + j < d) o[j] = v[j];
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------ product
+// v_mfma_scale_f32_32x32x64 on e2m1 operands: lane l gives row l % 32 of A (users) and column l % 32 of B
+// (items), 32 consecutive codes of that row (16 bytes: one block, so one scale byte a lane), the lane's half
+// l / 32 picking the first or second 32 of the 64 products; result element i of lane l is user
+// 8 (i / 4) + 4 (l / 32) + i % 4, item l % 32.  Any assignment of a row's blocks to (step, half) gives the
+// same sum as long as both operands use it.
+struct MxArgs {
+    const uint8_t* q;
+    const uint8_t* qs;
+    const int64_t* user_rows;
+    int64_t n_q;
+    const uint8_t* it;
+    const uint8_t* its;
+    int64_t B, n_items, nb;
+    void* out;
+};
+
+__device__ __forceinline__ i32x8 frag(u32x4 v) {
+    return i32x8{(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0};
+}
+
+template <int KK>
+__device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c, uint32_t sa, uint32_t sb) {
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(frag(a), frag(b), c, 4, 4, KK, (int)sa, KK, (int)sb);
+}
+
+__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
+
+// the blocks of one chunk (4 steps of 64 products): 16 bytes of codes a step and one scale byte a step
+struct Chunk {
+    u32x4 c[4];
+    uint32_t s;
+};
+
+// blocks [first, first + 4) of one row, the ones at or past nb as zeros
+__device__ __forceinline__ void load_chunk(Chunk& f, const uint8_t* codes, const uint8_t* scales, int64_t row, int64_t nb,
+                                           int64_t first, bool valid) {
+    const u32x4* src = reinterpret_cast<const u32x4*>(codes) + row * nb;
+    const uint8_t* ss = scales + row * nb;
+    f.s = valid ? 0u : 0x7f7f7f7fu;
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+        const bool in = valid && first + kk < nb;
+        f.c[kk] = in ? src[first + kk] : u32x4{0, 0, 0, 0};
+        if (valid) f.s |= (in ? (uint32_t)ss[first + kk] : 127u) << (8 * kk);
+    }
+}
+
+// One wave: 32 users x 128 items, the items' tile t of lane l being item base + 4 (l % 32) + t, so that a
+// lane's four results of one user are neighbours in the output row (one 16-byte store).
+template <bool BF16, bool SIG>
+__global__ __launch_bounds__(256) void score_mx_kernel(MxArgs a) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int col = lane & 31, half = lane >> 5;
+    const int64_t base = (blockIdx.x * (int64_t)4 + wave) * 128;
+    if (base >= a.n_items) return;
+    const int64_t u0 = blockIdx.y * (int64_t)32;
+    const int64_t b = u0 + col;
+    const bool have = b < a.B;
+    int64_t qrow = b;
+    if (have && a.user_rows) qrow = a.user_rows[b];
+    const bool badq = have && (qrow < 0 || qrow >= a.n_q);
+    f32x16 acc[4] = {};
+    for (int64_t k0 = 0; k0 < a.nb; k0 += 8) {
+        Chunk q, it[4];
+        load_chunk(q, a.q, a.qs, qrow, a.nb, k0 + 4 * half, have && !badq);
+        if (badq) q.s = 0xffffffffu;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+            load_chunk(it[t], a.it, a.its, min(base + 4 * col + t, a.n_items - 1), a.nb, k0 + 4 * half, true);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[t] = mma<0>(q.c[0], it[t].c[0], acc[t], q.s, it[t].s);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[t] = mma<1>(q.c[1], it[t].c[1], acc[t], q.s, it[t].s);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[t] = mma<2>(q.c[2], it[t].c[2], acc[t], q.s, it[t].s);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[t] = mma<3>(q.c[3], it[t].c[3], acc[t], q.s, it[t].s);
+    }
+    const int64_t i0 = base + 4 * col;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int64_t u = u0 + 8 * (i / 4) + 4 * half + i % 4;
+        if (u >= a.B) continue;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            if (i0 + t >= a.n_items) continue;
+            float v = acc[t][i];
+            if (SIG) v = sigmoid(v);
+            if (BF16)
+                static_cast<uint16_t*>(a.out)[u * a.n_items + i0 + t] = f32_to_bf16(v);
+            else
+                static_cast<float*>(a.out)[u * a.n_items + i0 + t] = v;
+        }
+    }
+}
+
+bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+int launch_quantize(const void* X, const int64_t* rows_of, int64_t n_src, int64_t rows, int64_t d, int64_t ld, int dtype,
+                    uint8_t* codes, uint8_t* scales, hipStream_t stream) {
+    const int64_t nb = ceil_div(d, (int64_t)kBlock), units = rows * nb;
+    const int64_t grid = ceil_div(units, (int64_t)64);
+    LGX_REQUIRE(grid < (1LL << 31), LGX_ERR_UNSUPPORTED, "lgx_mx_quantize: %lld rows is too many", (long long)rows);
+    const int size = dtype == LGX_DTYPE_BF16 ? 2 : 4;
+    const bool vec = d % 8 == 0 && (ld * size) % 16 == 0 && aligned(X, 16);
+#define LGX_MXQ(BF, V)                                                                                          \
+    mx_quantize_kernel<BF, V><<<(unsigned)grid, 256, 0, stream>>>(X, rows_of, n_src, units, nb, d, ld, codes, scales)
+    if (dtype == LGX_DTYPE_BF16) {
+        if (vec) LGX_MXQ(true, true); else LGX_MXQ(true, false);
+    } else {
+        if (vec) LGX_MXQ(false, true); else LGX_MXQ(false, false);
+    }
+#undef LGX_MXQ
+    LGX_LAUNCH_CHECK();
+    return LGX_OK;
+}
+
+}  // namespace
+}  // namespace lgx
+
+using namespace lgx;
+
+extern "C" int lgx_mx_quantize(const void* X, int64_t rows, int64_t d, int64_t ld, int dtype, uint8_t* codes,
+                               uint8_t* scales, lgx_stream_t stream) {
+    LGX_REQUIRE(rows >= 0 && (rows == 0 || (X && codes && scales)), LGX_ERR_INVALID_ARG, "lgx_mx_quantize: bad arguments");
+    LGX_REQUIRE(dtype == LGX_DTYPE_F32 || dtype == LGX_DTYPE_BF16, LGX_ERR_INVALID_ARG, "lgx_mx_quantize: dtype");
+    LGX_REQUIRE(d >= 1 && d <= kMaxD && ld >= d, LGX_ERR_UNSUPPORTED, "lgx_mx_quantize: d=%lld outside [1, %lld] or ld=%lld < d",
+                (long long)d, (long long)kMaxD, (long long)ld);
+    LGX_REQUIRE(aligned(codes, 16), LGX_ERR_INVALID_ARG, "lgx_mx_quantize: codes must be 16-byte aligned");
+    if (rows == 0) return LGX_OK;
+    return launch_quantize(X, nullptr, rows, rows, d, ld, dtype, codes, scales, as_hip(stream));
+}
+
+extern "C" int lgx_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t d, int dtype, void* out,
+                                 lgx_stream_t stream_) {
+    hipStream_t stream = as_hip(stream_);
+    LGX_REQUIRE(rows >= 0 && (rows == 0 || (codes && scales && out)), LGX_ERR_INVALID_ARG,
+                "lgx_mx_dequantize: bad arguments");
+    LGX_REQUIRE(dtype == LGX_DTYPE_F32 || dtype == LGX_DTYPE_BF16, LGX_ERR_INVALID_ARG, "lgx_mx_dequantize: dtype");
+    LGX_REQUIRE(d >= 1 && d <= kMaxD, LGX_ERR_UNSUPPORTED, "lgx_mx_dequantize: d=%lld outside [1, %lld]", (long long)d,
+                (long long)kMaxD);
+    LGX_REQUIRE(aligned(codes, 16), LGX_ERR_INVALID_ARG, "lgx_mx_dequantize: codes must be 16-byte aligned");
+    if (rows == 0) return LGX_OK;
+    const int64_t nb = ceil_div(d, (int64_t)kBlock), units = rows * nb, grid = ceil_div(units, (int64_t)64);
+    LGX_REQUIRE(grid < (1LL << 31), LGX_ERR_UNSUPPORTED, "lgx_mx_dequantize: %lld rows is too many", (long long)rows);
+    const bool vec = d % 8 == 0 && aligned(out, 16);
+#define LGX_MXD(BF, V) mx_dequantize_kernel<BF, V><<<(unsigned)grid, 256, 0, stream>>>(codes, scales, units, nb, d, out)
+    if (dtype == LGX_DTYPE_BF16) {
+        if (vec) LGX_MXD(true, true); else LGX_MXD(true, false);
+    } else {
+        if (vec) LGX_MXD(false, true); else LGX_MXD(false, false);
+    }
+#undef LGX_MXD
+    LGX_LAUNCH_CHECK();
+    return LGX_OK;
+}
+
+extern "C" int lgx_score_mx_workspace(int64_t B, int64_t d, int q_dtype, size_t* ws_bytes) {
+    LGX_REQUIRE(ws_bytes && B >= 0 && d >= 1 && d <= kMaxD, LGX_ERR_INVALID_ARG, "lgx_score_mx_workspace: bad arguments");
+    const size_t nb = (size_t)ceil_div(d, (int64_t)kBlock);
+    *ws_bytes = q_dtype == LGX_DTYPE_MXFP4 ? 0 : align_up((size_t)B * nb * 16) + align_up((size_t)B * nb);
+    return LGX_OK;
+}
+
+extern "C" int lgx_score_mx(const void* Q, const uint8_t* q_scales, int q_dtype, int64_t n_q, int64_t q_ld,
+                            const int64_t* user_rows, const uint8_t* item_codes, const uint8_t* item_scales, int64_t B,
+                            int64_t n_items, int64_t d, int apply_sigmoid, int out_dtype, void* scores, void* ws,
+                            size_t ws_bytes, lgx_stream_t stream_) {
+    hipStream_t stream = as_hip(stream_);
+    LGX_REQUIRE(B >= 0 && n_items >= 0 && n_q >= 0, LGX_ERR_INVALID_ARG, "lgx_score_mx: negative size");
+    LGX_REQUIRE(q_dtype == LGX_DTYPE_F32 || q_dtype == LGX_DTYPE_BF16 || q_dtype == LGX_DTYPE_MXFP4, LGX_ERR_INVALID_ARG,
+                "lgx_score_mx: query dtype");
+    LGX_REQUIRE(out_dtype == LGX_DTYPE_F32 || out_dtype == LGX_DTYPE_BF16, LGX_ERR_INVALID_ARG, "lgx_score_mx: out dtype");
+    LGX_REQUIRE(d >= 1 && d <= kMaxD, LGX_ERR_UNSUPPORTED, "lgx_score_mx: d=%lld outside [1, %lld]", (long long)d,
+                (long long)kMaxD);
+    LGX_REQUIRE(n_items < INT32_MAX && B < INT32_MAX, LGX_ERR_UNSUPPORTED, "lgx_score_mx: 2^31 rows or more");
+    if (B == 0 || n_items == 0) return LGX_OK;
+    LGX_REQUIRE(Q && item_codes && item_scales && scores, LGX_ERR_INVALID_ARG, "lgx_score_mx: null pointer");
+    LGX_REQUIRE(user_rows || B <= n_q, LGX_ERR_INVALID_ARG, "lgx_score_mx: %lld queries of %lld rows", (long long)B,
+                (long long)n_q);
+    LGX_REQUIRE(aligned(item_codes, 16), LGX_ERR_INVALID_ARG, "lgx_score_mx: codes must be 16-byte aligned");
+    const int64_t nb = ceil_div(d, (int64_t)kBlock);
+    MxArgs a{static_cast<const uint8_t*>(Q), q_scales, user_rows, n_q, item_codes, item_scales, B, n_items, nb, scores};
+    if (q_dtype == LGX_DTYPE_MXFP4) {
+        LGX_REQUIRE(q_scales && aligned(Q, 16), LGX_ERR_INVALID_ARG, "lgx_score_mx: query codes must be 16-byte aligned, with scales");
+    } else {
+        LGX_REQUIRE(q_ld >= d, LGX_ERR_INVALID_ARG, "lgx_score_mx: q_ld=%lld < d", (long long)q_ld);
+        size_t need = 0;
+        lgx_score_mx_workspace(B, d, q_dtype, &need);
+        LGX_REQUIRE(ws && ws_bytes >= need && aligned(ws, 16), LGX_ERR_WORKSPACE, "lgx_score_mx: workspace %zu < %zu", ws_bytes, need);
+        uint8_t* codes = static_cast<uint8_t*>(ws);
+        uint8_t* scales = codes + align_up((size_t)B * nb * 16);
+        const int rc = launch_quantize(Q, user_rows, n_q, B, d, q_ld, q_dtype, codes, scales, stream);
+        if (rc) return rc;
+        a.q = codes;
+        a.qs = scales;
+        a.user_rows = nullptr;
+        a.n_q = B;
+    }
+    const int64_t gx = ceil_div(n_items, (int64_t)512), gy = ceil_div(B, (int64_t)32);
+    LGX_REQUIRE(gy < 65536, LGX_ERR_UNSUPPORTED, "lgx_score_mx: %lld queries is too many", (long long)B);
+    const dim3 grid((unsigned)gx, (unsigned)gy);
+    if (out_dtype == LGX_DTYPE_BF16) {
+        if (apply_sigmoid) score_mx_kernel<true, true><<<grid, 256, 0, stream>>>(a);
+        else score_mx_kernel<true, false><<<grid, 256, 0, stream>>>(a);
+    } else {
+        if (apply_sigmoid) score_mx_kernel<false, true><<<grid, 256, 0, stream>>>(a);
+        else score_mx_kernel<false, false><<<grid, 256, 0, stream>>>(a);
+    }
+    LGX_LAUNCH_CHECK();
+    return LGX_OK;
+}

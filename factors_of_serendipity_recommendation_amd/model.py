@@ -154,8 +154,17 @@ class LightGCN(BasicModel):
         """propagate methods for lightGCN (model.py:145-177): (users, items) views of one table."""
         return torch.split(self._light_out(), [self.num_users, self.num_items])
 
-    def getUsersRating(self, users):
+    def quantizeItems(self) -> ops.MXTable:
+        """The propagated item rows of the current weights, packed to MXFP4: the table a server keeps
+        for getUsersRating between weight updates."""
+        return ops.mx_quantize(self.computer()[1].detach())
+
+    def getUsersRating(self, users, items: Optional[ops.MXTable] = None):
+        """Sigmoid scores [B, m_items] (model.py:179-184).  items: a quantizeItems() table to score
+        against in 4 bits (the users' rows are quantised by the call) instead of the f32 rows."""
         all_users, all_items = self.computer()
+        if items is not None:
+            return ops.score_mx(all_users.detach(), items, user_rows=users.long(), apply_sigmoid=True)
         return ops.score_dense(all_users.detach(), all_items.detach(), user_rows=users.long(), apply_sigmoid=True)
 
     def getEmbedding(self, users, pos_items, neg_items):

@@ -486,6 +486,205 @@ def fill_normal(shape, std: float, seed: int, dtype=torch.float32, device="cuda"
     return t
 
 
+# ------------------------------------------------------------------------------------ 4-bit tables
+MX_BLOCK = 32  # elements that share one scale
+
+
+class MXTable:
+    """Embedding rows in microscaled 4-bit floating point (MXFP4), as ``lgx_mx_quantize`` packs them:
+    ``codes`` uint8 [rows, 16 nb] (element 2j of a row in the low nibble of byte j: sign << 3 | e2m1) and
+    ``scales`` uint8 [rows, nb] (b stands for 2^(b - 127), 255 for NaN), nb = ceil(d / 32).  17 bytes per 32
+    elements.  ``table[a:b]`` is a view of rows; ``to(device)`` moves both parts."""
+
+    __slots__ = ("codes", "scales", "d")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, d: int):
+        nb = -(-int(d) // MX_BLOCK)
+        if d < 1 or codes.dim() != 2 or scales.dim() != 2 or codes.shape[1] != 16 * nb or scales.shape[1] != nb \
+                or codes.shape[0] != scales.shape[0]:
+            raise ValueError(f"MXTable: codes {tuple(codes.shape)} / scales {tuple(scales.shape)} are not "
+                             f"[rows, {16 * nb}] / [rows, {nb}] (d = {d})")
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise TypeError("MXTable: codes and scales must be uint8")
+        if codes.device != scales.device:
+            raise ValueError(f"MXTable: codes on {codes.device}, scales on {scales.device}")
+        if not codes.is_contiguous() or not scales.is_contiguous() or codes.data_ptr() % 16:
+            raise ValueError("MXTable: codes and scales must be contiguous, codes 16-byte aligned")
+        self.codes, self.scales, self.d = codes, scales, int(d)
+
+    @property
+    def shape(self) -> Tuple[int, int]:
+        return (self.codes.shape[0], self.d)
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def __len__(self) -> int:
+        return self.codes.shape[0]
+
+    def __getitem__(self, rows: slice) -> "MXTable":
+        if not isinstance(rows, slice) or rows.step not in (None, 1):
+            raise TypeError("MXTable takes a slice of consecutive rows")
+        return MXTable(self.codes[rows], self.scales[rows], self.d)
+
+    def to(self, device) -> "MXTable":
+        return MXTable(self.codes.to(device), self.scales.to(device), self.d)
+
+
+def _one_device(what: str, *tensors) -> torch.device:
+    """The device all the given tensors (None skipped) live on; the call runs there, whatever the
+    current device is."""
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
+    return dev
+
+
+def _row_stride(x: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """x [rows, cols] with unit column stride and a row stride of at least cols, and that stride
+    (copied only where the given strides are others)."""
+    if x.stride(1) != 1 and x.shape[1] > 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
+        x = x.contiguous()
+    return x, max(x.stride(0), x.shape[1]) if x.shape[0] > 1 else x.shape[1]
+
+
+def mx_quantize(x: torch.Tensor) -> MXTable:
+    """Rows [rows, d] (f32 or bf16, any row stride) packed to MXFP4 (``lgx_mx_quantize``): per 32 elements
+    the scale 2^(floor(log2 max|x|) - 2), elements rounded to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6
+    scales (ties to the even code, 6 and above to 6).  A block with an infinity or a NaN decodes to NaN.
+    Not differentiable."""
+    require_gpu(x)
+    dt = _dtype_code(x)
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"mx_quantize: [rows, d] expected, got {tuple(x.shape)}")
+    x, ld = _row_stride(x)
+    rows, d = x.shape
+    nb = -(-d // MX_BLOCK)
+    with torch.cuda.device(x.device):
+        codes = torch.empty((rows, 16 * nb), dtype=torch.uint8, device=x.device)
+        scales = torch.empty((rows, nb), dtype=torch.uint8, device=x.device)
+        _lib.check(_lib.lib().lgx_mx_quantize(x.data_ptr(), rows, d, ld, dt, codes.data_ptr(), scales.data_ptr(),
+                                              _stream_ptr(x.device)), "lgx_mx_quantize")
+    return MXTable(codes, scales, d)
+
+
+def mx_dequantize(table: MXTable, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values of an MXTable as f32 or bf16 [rows, d] (``lgx_mx_dequantize``; exact in both)."""
+    require_gpu(table.codes)
+    out = torch.empty(table.shape, dtype=dtype, device=table.device)
+    dt = _dtype_code(out)
+    with torch.cuda.device(table.device):
+        _lib.check(_lib.lib().lgx_mx_dequantize(table.codes.data_ptr(), table.scales.data_ptr(), len(table), table.d, dt,
+                                                out.data_ptr(), _stream_ptr(table.device)), "lgx_mx_dequantize")
+    return out
+
+
+def score_mx(Q, items: MXTable, user_rows: Optional[torch.Tensor] = None, apply_sigmoid: bool = False,
+             dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """[B, I] scores against an MXFP4 item table (``lgx_score_mx``): ``score_dense`` for tables a quarter of
+    bf16's size.  Q [n, d] is an MXTable, or an f32 / bf16 tensor (any row stride) that the call
+    quantises; user_rows picks its rows as in score_dense (a row outside the table scores NaN).  out: an
+    optional contiguous [B, I] destination of type ``dtype`` (f32 or bf16).  Not differentiable."""
+    if not isinstance(items, MXTable):
+        raise TypeError("score_mx: items must be an MXTable (mx_quantize)")
+    packed = isinstance(Q, MXTable)
+    q = Q.codes if packed else Q
+    require_gpu(q, items.codes, user_rows, out)
+    dev = _one_device("score_mx", q, items.codes, user_rows, out)
+    q_dt = _lib.LGX_DTYPE_MXFP4 if packed else _dtype_code(q)
+    if q.dim() != 2 or Q.shape[1] != items.d:
+        raise ValueError(f"Q {tuple(Q.shape)} and items {items.shape} must be [*, d] with one d")
+    if dtype not in _DT:
+        raise TypeError(f"score_mx: unsupported score dtype {dtype}; use float32 or bfloat16")
+    q, q_ld = (q, 0) if packed else _row_stride(q)
+    n_q, n_items, d = q.shape[0], len(items), items.d
+    if user_rows is not None and user_rows.dim() != 1:
+        raise ValueError(f"score_mx: user_rows must be one-dimensional, got {tuple(user_rows.shape)}")
+    B = user_rows.numel() if user_rows is not None else n_q
+    with torch.cuda.device(dev):
+        rows = user_rows.to(torch.int64).contiguous() if user_rows is not None else None
+        if out is None:
+            out = torch.empty((B, n_items), dtype=dtype, device=dev)
+        elif out.dtype != dtype or tuple(out.shape) != (B, n_items) or not out.is_contiguous():
+            raise ValueError(f"score_mx: out must be a contiguous {dtype} [{B}, {n_items}] on {dev}")
+        L = _lib.lib()
+        ws = ctypes.c_size_t(0)
+        _lib.check(L.lgx_score_mx_workspace(B, d, q_dt, ctypes.byref(ws)), "lgx_score_mx_workspace")
+        work = torch.empty(ws.value, dtype=torch.uint8, device=dev) if ws.value else None
+        _lib.check(L.lgx_score_mx(q.data_ptr(), Q.scales.data_ptr() if packed else None, q_dt, n_q, q_ld, _ptr(rows),
+                                  items.codes.data_ptr(), items.scales.data_ptr(), B, n_items, d, int(apply_sigmoid),
+                                  _dtype_code(out), out.data_ptr(), _ptr(work), ws.value, _stream_ptr(dev)),
+                   "lgx_score_mx")
+    return out
+
+
+# ------------------------------------------------------------------------------------ draws
+def _row_setting(name: str, v, rows: int, dev: torch.device, dtype: torch.dtype, lo: float, hi: float):
+    """(value for all rows, per-row tensor or None) of one sample_rows setting."""
+    if torch.is_tensor(v):
+        if v.dim() != 1 or v.numel() != rows or v.device != dev:
+            raise ValueError(f"sample_rows: {name} must be a number or one per row ([{rows}] on {dev}), got "
+                             f"{tuple(v.shape)} on {v.device}")
+        if dtype == torch.int32 and v.dtype != torch.int32:
+            if v.dtype.is_floating_point or v.dtype == torch.bool:
+                raise TypeError(f"sample_rows: {name} must hold integers, got {v.dtype}")
+            v = v.clamp(0, 2 ** 31 - 1)
+        return 0, v.to(dtype).contiguous()
+    if not lo <= v <= hi:
+        raise ValueError(f"sample_rows: {name} = {v} outside [{lo}, {hi}]")
+    return v, None
+
+
+def sample_rows(S: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0,
+                min_p=0.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Draws from the softmax of score rows, from given random numbers (``lgx_sample_rows``).
+
+    S [rows, cols] f32 or bf16 (any row stride); u [rows] or [rows, n] f32 / f64 in [0, 1): n independent
+    draws per row, e.g. ``torch.rand``.  Per row the weights are exp((s - max s) / temperature), -inf and
+    NaN scores excluded; kept are the first top_k columns of the ranking (score descending, ties to the
+    lower column; 0 = all), of these the shortest prefix with top_p of their weight, of these the ones
+    with weight >= min_p.  A draw is the first kept column, in column order, whose cumulative weight
+    exceeds u times the whole.  temperature 0 is the best column.  Each setting is a number or a tensor
+    [rows] (then T <= 0 and NaN mean the best column, top_k <= 0 all).
+
+    Returns (columns int32, their probabilities f32), both shaped as u; -1 and 0 for a row with nothing to
+    draw from.  Not differentiable."""
+    require_gpu(S, u)
+    dev = _one_device("sample_rows", S, u)
+    dt = _dtype_code(S)
+    if S.dim() != 2:
+        raise ValueError(f"sample_rows: [rows, cols] expected, got {tuple(S.shape)}")
+    rows, cols = S.shape
+    if u.dtype not in (torch.float32, torch.float64):
+        raise TypeError(f"sample_rows: u must be float32 or float64, got {u.dtype}")
+    if u.dim() not in (1, 2) or u.shape[0] != rows:
+        raise ValueError(f"sample_rows: u must be [{rows}] or [{rows}, n], got {tuple(u.shape)}")
+    n = u.shape[1] if u.dim() == 2 else 1
+    with torch.cuda.device(dev):
+        t, t_rows = _row_setting("temperature", temperature, rows, dev, torch.float32, 0.0, float("inf"))
+        k, k_rows = _row_setting("top_k", top_k, rows, dev, torch.int32, 0, 2 ** 63 - 1)
+        p, p_rows = _row_setting("top_p", top_p, rows, dev, torch.float32, 0.0, 1.0)
+        m, m_rows = _row_setting("min_p", min_p, rows, dev, torch.float32, 0.0, 1.0)
+        idx = torch.empty(u.shape, dtype=torch.int32, device=dev)
+        prob = torch.empty(u.shape, dtype=torch.float32, device=dev)
+        if cols == 0:
+            return idx.fill_(-1), prob.zero_()
+        S, ld = _row_stride(S)
+        u = u.contiguous()
+        L = _lib.lib()
+        ws = ctypes.c_size_t(0)
+        _lib.check(L.lgx_sample_rows_workspace(rows, cols, n, ctypes.byref(ws)), "lgx_sample_rows_workspace")
+        work = torch.empty(ws.value, dtype=torch.uint8, device=dev) if ws.value else None
+        _lib.check(L.lgx_sample_rows(S.data_ptr(), dt, rows, cols, ld, u.data_ptr(),
+                                     _lib.LGX_DTYPE_F64 if u.dtype == torch.float64 else _lib.LGX_DTYPE_F32, n, float(t),
+                                     _ptr(t_rows), int(k), _ptr(k_rows), float(p), _ptr(p_rows), float(m), _ptr(m_rows),
+                                     idx.data_ptr(), prob.data_ptr(), _ptr(work), ws.value, _stream_ptr(dev)),
+                   "lgx_sample_rows")
+    return idx, prob
+
+
 # ------------------------------------------------------------------------------------ BPR loss
 def _bpr_args(light, ego_user, ego_item, users, pos, neg):
     require_gpu(light, ego_user, ego_item, users, pos, neg)

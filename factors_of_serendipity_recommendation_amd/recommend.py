@@ -67,6 +67,44 @@ def topk_candidates(emb_user: torch.Tensor, emb_item: torch.Tensor, candidates: 
     return ragged_topk(scores, indptr, items, K)
 
 
+def sample_recommendations(emb_user: torch.Tensor, emb_item, users: torch.Tensor, u: torch.Tensor,
+                           mask: Optional[Tuple[torch.Tensor, torch.Tensor]] = None, temperature=1.0, top_k=0,
+                           top_p=1.0, min_p=0.0,
+                           chunk_bytes: int = ops.DENSE_CHUNK_BYTES) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Recommendations drawn from the users' score distribution instead of its top-K: the full catalog's
+    scores of ``users`` (int64 rows of emb_user), their masked items excluded, then ops.sample_rows with the
+    given random numbers u [len(users)] or [len(users), n].
+
+    emb_item: the item rows (emb_user's dtype, scored by score_dense) or an MXTable of them (score_mx).
+    mask = (indptr int64 [len(users) + 1], indices int32), e.g. the train positives.  The settings are
+    sample_rows' own, each a number or one per user.  Users go in chunks of at most chunk_bytes of scores.
+    Returns (items int32, probabilities f32) shaped as u, on the device; -1 and 0 for a user whose
+    every item is masked."""
+    ops.require_gpu(emb_user, users, u)
+    packed = isinstance(emb_item, ops.MXTable)
+    n_users, n_items = users.numel(), emb_item.shape[0]
+    if users.dim() != 1 or u.shape[:1] != users.shape:
+        raise ValueError(f"users {tuple(users.shape)} and u {tuple(u.shape)} must list the same users")
+    if mask is not None and mask[0].numel() != n_users + 1:
+        raise ValueError(f"mask indptr must have {n_users + 1} entries, got {mask[0].numel()}")
+    if n_users and (int(users.min()) < 0 or int(users.max()) >= emb_user.shape[0]):
+        raise IndexError(f"user id out of range for {emb_user.shape[0]} users")
+    items = torch.empty(u.shape, dtype=torch.int32, device=u.device)
+    prob = torch.empty(u.shape, dtype=torch.float32, device=u.device)
+    settings = {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p}
+    step = ops.dense_chunk_users(n_items, chunk_bytes)
+    for c0 in range(0, n_users, step):
+        c1 = min(n_users, c0 + step)
+        score = ops.score_mx if packed else ops.score_dense
+        S = score(emb_user, emb_item, user_rows=users[c0:c1])
+        if mask is not None:
+            S.view(-1).index_fill_(0, ops.dense_mask_offsets(mask, n_items, c0, c1), float("-inf"))
+        items[c0:c1], prob[c0:c1] = ops.sample_rows(
+            S, u[c0:c1], **{n: v[c0:c1] if torch.is_tensor(v) else v for n, v in settings.items()})
+        del S
+    return items, prob
+
+
 def accuracy_cf(mat_candidate: Dict[int, List[int]], dataset_name: str, seed: int, K: int = 20,
                 data_root: str = "data", device="cuda") -> None:
     """recommend.accuracy_cf: same inputs (data/<ds>/emb_{item,user}.npy, candidate dict), same

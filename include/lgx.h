@@ -55,6 +55,8 @@ typedef struct ihipStream_t* lgx_stream_t; /* == hipStream_t */
 
 #define LGX_DTYPE_F32 0  /* fp32 storage, fp32 arithmetic */
 #define LGX_DTYPE_BF16 1 /* bf16 storage, fp32 accumulate */
+#define LGX_DTYPE_MXFP4 2 /* packed rows: e2m1 codes + one power-of-two scale per 32 elements (lgx_mx_quantize) */
+#define LGX_DTYPE_F64 3  /* the given random numbers of lgx_sample_rows only */
 
 /* layer epilogue modes of lgx_propagate_layer (model.py:163-175: embs.append + stack + mean) */
 #define LGX_LAYER_PLAIN 0 /* Y = A X                                                     */
@@ -430,6 +432,63 @@ int lgx_adam_step_dev(float* param, const float* grad, float* exp_avg, float* ex
 int lgx_list_dot_reduce(const void* table, int64_t d, int dtype, int64_t n_users, const int64_t* a_indptr,
                         const int32_t* a_items, const int64_t* b_indptr, const int32_t* b_items, int reduce,
                         float* out, lgx_stream_t stream);
+
+/* ---------------------------------------------------------------- 4-bit tables */
+/*
+ * Microscaled 4-bit floating point (MXFP4) rows: blocks of 32 consecutive elements of a row (the last
+ * one padded with zeros) share one power-of-two scale.  nb = ceil(d / 32):
+ *   codes  [rows, 16 nb] uint8, 16-byte aligned: element 2j of a row in the low nibble of byte j; a nibble
+ *          is sign << 3 | e2m1 (magnitudes 0, 0.5, 1, 1.5, 2, 3, 4, 6)
+ *   scales [rows, nb] uint8: b stands for 2^(b - 127), 255 for NaN (the whole block decodes to NaN)
+ * lgx_mx_quantize: X [rows, d] f32 or bf16, row stride ld >= d elements.  b = max(E - 2, 0) with E the
+ * exponent field of the block's largest magnitude, so that magnitude lands in [4, 8); elements round to
+ * the nearest magnitude, ties to the even code, and saturate at 6.  A block holding an infinity or a NaN
+ * gets b = 255.  1 <= d <= 65536.
+ * lgx_mx_dequantize: -> out [rows, d] f32 or bf16 contiguous; every value is exact in both types.
+ */
+int lgx_mx_quantize(const void* X, int64_t rows, int64_t d, int64_t ld, int dtype, uint8_t* codes, uint8_t* scales,
+                    lgx_stream_t stream);
+int lgx_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t d, int dtype, void* out,
+                      lgx_stream_t stream);
+/*
+ * scores[b, i] = <Q row of b, item i> over an MXFP4 item table (optionally sigmoid), [B, n_items] in
+ * out_dtype (f32 or bf16), on the block-scaled matrix instructions (f32 accumulation).
+ *   Q [n_q, d]: q_dtype MXFP4 (Q = codes, q_scales = scales, q_ld ignored), or f32 / bf16 with row stride
+ *   q_ld (q_scales NULL), which the call first quantises as lgx_mx_quantize does.
+ *   user_rows [B] int64 (NULL: row b, B <= n_q): the rows of Q; a row outside [0, n_q) is never read and
+ *   scores NaN.  n_items < 2^31, 1 <= d <= 65536.  Workspace: lgx_score_mx_workspace (0 for MXFP4 queries).
+ */
+int lgx_score_mx_workspace(int64_t B, int64_t d, int q_dtype, size_t* ws_bytes);
+int lgx_score_mx(const void* Q, const uint8_t* q_scales, int q_dtype, int64_t n_q, int64_t q_ld,
+                 const int64_t* user_rows, const uint8_t* item_codes, const uint8_t* item_scales, int64_t B,
+                 int64_t n_items, int64_t d, int apply_sigmoid, int out_dtype, void* scores, void* ws, size_t ws_bytes,
+                 lgx_stream_t stream);
+
+/* ---------------------------------------------------------------- draws from score rows */
+/*
+ * n_draws independent draws per row of S [rows, cols] (f32 or bf16, row stride ld >= cols) from the
+ * row's softmax, restricted to its best columns.  With m the row's largest score:
+ *   weight w_i = exp((s_i - m) / T); scores of -inf and NaN are excluded; +inf shares the row equally.
+ *   ranking: higher score first, ties -> lower column.  Kept are, in this order:
+ *   top_k  the first top_k columns (top_k <= 0: all);
+ *   top_p  of these the shortest prefix whose weight reaches top_p of theirs, one at least (top_p >= 1: all);
+ *   min_p  of these the ones with w_i >= min_p.
+ *   A draw with the given number u is the first kept column i, in column order, with
+ *   sum_{j <= i, kept} w_j > u * sum_{kept} w_j.  T not above 0 (or NaN): the best column.  A
+ *   NaN top_p or min_p restricts nothing; a min_p above 1 counts as 1.
+ * out_idx [rows, n_draws] int32, out_prob [rows, n_draws] f32 = w_i / sum_{kept} w_j (NULL: not wanted).  A
+ * row with nothing to draw from gives -1 and 0.
+ *   u [rows, n_draws] f32 or f64 (u_dtype) in [0, 1); values outside are taken as the nearest end.
+ *   Each setting is one value for all rows or, where the *_rows pointer is given, one per row.
+ * Weights and their sums are held in 64 bits, so that the column does not depend on how the sums
+ * are split; results are the same for every call.  1 <= cols < 2^31.
+ */
+int lgx_sample_rows_workspace(int64_t rows, int64_t cols, int64_t n_draws, size_t* ws_bytes);
+int lgx_sample_rows(const void* S, int dtype, int64_t rows, int64_t cols, int64_t ld, const void* u, int u_dtype,
+                    int64_t n_draws, double temperature, const float* temperature_rows, int64_t top_k,
+                    const int32_t* top_k_rows, double top_p, const float* top_p_rows, double min_p,
+                    const float* min_p_rows, int32_t* out_idx, float* out_prob, void* ws, size_t ws_bytes,
+                    lgx_stream_t stream);
 
 /* ---------------------------------------------------------------- synthetic graphs (bench) */
 /*

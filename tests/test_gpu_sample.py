@@ -1,0 +1,301 @@
+"""GPU: draws from score rows (lgx_sample_rows) against the definition in 64 bits on the host.
+
+The drawn columns must be equal: the kernel's weights and sums carry 64 bits, as the reference's do, so
+they differ only where a random number lies within ~1e-14 of a border.  Probabilities are one rounding to
+f32 off: 2^-24 relative, plus 1e-12 for the weights."""
+import numpy as np
+import pytest
+import torch
+
+import factors_of_serendipity_recommendation_amd as lgx
+from factors_of_serendipity_recommendation_amd import ops, recommend
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def ref_row(s, u, T=1.0, k=0, p=1.0, minp=0.0):
+    """(columns, probabilities) of the draws u from one row, the kept set as a list of columns."""
+    live = np.flatnonzero(s > -np.inf)  # NaN compares false
+    if not live.size:
+        return np.full(len(u), -1), np.zeros(len(u))
+    s = s[live].astype(np.float64)
+    top = s.max()
+    if not T > 0:
+        live, s, w = live[s == top][:1], s[s == top][:1], np.ones(1)
+    else:
+        with np.errstate(invalid="ignore", over="ignore", under="ignore"):
+            w = np.where(s == top, 1.0, 0.0 if top == np.inf else np.exp((s - top) / T))
+    rank = np.lexsort((live, -s))
+    if k > 0:
+        rank = rank[:k]
+    if p < 1:
+        before = np.concatenate(([0.0], np.cumsum(w[rank])))
+        rank = rank[:max(1, int(np.searchsorted(before[:-1], p * before[-1], side="left")))]
+    rank = np.sort(rank)
+    live, w = live[rank], w[rank]
+    if minp > 0:
+        keep = w >= min(minp, 1.0)
+        live, w = live[keep], w[keep]
+    c = np.cumsum(w)
+    j = np.minimum(np.searchsorted(c, u * c[-1], side="right"), np.flatnonzero(w > 0)[-1])
+    return live[j], w[j] / c[-1]
+
+
+def check(S, u, **kw):
+    idx, prob = lgx.sample_rows(S, u, **kw)
+    assert idx.shape == u.shape and prob.shape == u.shape and idx.dtype == torch.int32
+    Sh, uh = S.double().cpu().numpy(), u.double().cpu().numpy().reshape(S.shape[0], -1)
+    names = {"temperature": "T", "top_k": "k", "top_p": "p", "min_p": "minp"}
+    for r in range(S.shape[0]):
+        row = {names[n]: (v[r].item() if torch.is_tensor(v) else v) for n, v in kw.items()}
+        wi, wp = ref_row(Sh[r], uh[r], **row)
+        gi, gp = idx.view(S.shape[0], -1)[r].cpu().numpy(), prob.view(S.shape[0], -1)[r].double().cpu().numpy()
+        assert np.array_equal(gi, wi), (r, row, gi, wi)
+        assert (np.abs(gp - wp) <= (2.0 ** -24 + 1e-12) * wp + 1e-45).all(), (r, gp, wp)
+    return idx, prob
+
+
+def scores(rows, cols, seed, dtype=torch.float32, sigma=1.5, masked=0.05):
+    g = torch.Generator().manual_seed(seed)
+    s = torch.randn(rows, cols, generator=g) * sigma
+    s[torch.rand(rows, cols, generator=g) < masked] = float("-inf")
+    return s.to(dtype).to(DEV), torch.rand(rows, 5, generator=g).to(DEV)
+
+
+SETTINGS = [{}, {"temperature": 0.3}, {"top_k": 1}, {"top_k": 7}, {"top_k": 300}, {"top_p": 0.9}, {"top_p": 0.1},
+            {"min_p": 0.05}, {"top_k": 50, "top_p": 0.8, "temperature": 0.7},
+            {"top_k": 1000, "top_p": 0.95, "min_p": 0.02, "temperature": 1.3}, {"temperature": 0.0},
+            {"top_p": 0.0}, {"min_p": 1.0}, {"top_p": 1e-3, "top_k": 3}, {"temperature": 50.0, "top_p": 0.5}]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 2), (2, 63), (5, 64), (4, 65), (3, 1000), (2, 4097), (9, 2120),
+                                       (2, 40981), (3, 12288)])
+def test_draws_match_the_definition(rows, cols, dtype):
+    for j, kw in enumerate(SETTINGS):
+        S, u = scores(rows, cols, 100 * j + cols, dtype)
+        check(S, u, **kw)
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 100003), (2, 250000), (1, 1000000)])
+def test_long_rows(rows, cols):
+    for j, kw in enumerate([{}, {"top_p": 0.9}, {"top_k": 100, "temperature": 0.5}, {"top_k": 5000, "top_p": 0.9},
+                            {"min_p": 0.1}]):
+        S, u = scores(rows, cols, j, sigma=2.0)
+        check(S, u, **kw)
+    S, u = scores(rows, cols, 9, torch.bfloat16)
+    check(S, u, top_p=0.7)
+
+
+def test_many_draws_and_given_numbers_at_the_ends():
+    S, _ = scores(3, 5000, 1)
+    u = torch.rand(3, 777, generator=torch.Generator().manual_seed(2), dtype=torch.float64)
+    u[:, 0], u[:, 1], u[:, 2] = 0.0, 1.0 - 2.0 ** -53, 2.0 ** -60
+    check(S, u.to(DEV), top_p=0.9)
+    check(S, u.float().clamp(max=1 - 2.0 ** -24).to(DEV))
+    check(S, u.to(DEV)[:, 0].contiguous(), top_k=40)
+    a = lgx.sample_rows(S, torch.full((3, 2), 5.0, device=DEV))[0]  # outside [0, 1): the nearest end
+    b = lgx.sample_rows(S, torch.tensor([[-1.0, 0.0]] * 3, device=DEV))[0]
+    assert (a >= 0).all() and torch.equal(b[:, 0], b[:, 1])
+
+
+def test_equal_scores_are_cut_and_drawn_in_column_order():
+    S = torch.zeros(4, 1000, device=DEV)
+    S[:, 500] = float("-inf")
+    u = torch.tensor([[0.0, 0.25, 0.5, 0.999]] * 4, device=DEV)
+    idx, prob = check(S, u, top_k=torch.tensor([4, 8, 0, 999], dtype=torch.int32, device=DEV))
+    assert idx[0].tolist() == [0, 1, 2, 3] and prob[0].tolist() == [0.25] * 4  # a border belongs to the next column
+    idx, _ = check(S, u, top_p=0.5)      # 999 equal columns: the first 500 hold 500/999 >= 0.5
+    assert idx[0, 3].item() == 499
+    S[:, 300:400] = 1.0
+    check(S, u, top_k=101)
+    check(S, u, top_k=100)
+    check(S, u, top_p=0.3)
+    check(S.bfloat16(), u, top_k=150, top_p=0.9)
+    # one value on both sides of zero, and both zeros
+    S = torch.cat((torch.full((1, 700), -0.0, device=DEV), torch.zeros(1, 700, device=DEV)), 1)
+    check(S, u[:1], top_k=900)
+
+
+def test_masked_infinite_and_undefined_scores():
+    inf, nan, low = float("inf"), float("nan"), torch.finfo(torch.float32).min
+    S = torch.full((10, 300), -inf, device=DEV)
+    S[1, 250] = -3.0                                   # one column left
+    S[2] = nan                                         # nothing defined
+    S[3, 10:20], S[3, 15] = 1.0, nan
+    S[4] = low                                         # a mask of the type's lowest value everywhere
+    S[5], S[5, 7] = low, 0.0
+    S[6], S[6, 8], S[6, 100] = 1.0, inf, inf           # infinities share the row
+    S[7], S[7, ::2] = torch.finfo(torch.float32).max, low
+    S[8] = torch.linspace(-1e-40, 1e-40, 300, device=DEV)
+    S[9], S[9, 299] = -1000.0, 500.0                   # weights that underflow
+    u = torch.rand(10, 9, generator=torch.Generator().manual_seed(0)).to(DEV)
+    u[:, 0] = 0.0
+    for kw in ({}, {"top_k": 3}, {"top_p": 0.5}, {"min_p": 0.5}, {"temperature": 0.0}, {"temperature": 1e-30},
+               {"temperature": 1e30}, {"temperature": float("inf")}):
+        idx, prob = check(S, u, **kw)
+        assert (idx[[0, 2]] == -1).all() and (prob[[0, 2]] == 0).all() and (idx[1] == 250).all()
+        assert set(idx[6].tolist()) <= {8, 100}
+    check(S.bfloat16(), u, top_p=0.5)
+
+
+def test_settings_per_row():
+    S, u = scores(64, 3000, 4)
+    g = torch.Generator().manual_seed(1)
+
+    def pick(values, dtype):
+        return torch.tensor(values, dtype=dtype)[torch.randint(0, len(values), (64,), generator=g)].to(DEV)
+
+    kw = {"temperature": pick([0.0, -1.0, 0.5, 2.0, float("nan")], torch.float32),
+          "top_k": pick([-5, 0, 1, 30, 3000, 2 ** 31 - 1], torch.int32),
+          "top_p": pick([0.0, 0.5, 0.99, 1.0], torch.float32), "min_p": pick([0.0, 0.01, 1.0, 2.0, -1.0], torch.float32)}
+    check(S, u, **kw)
+    a = lgx.sample_rows(S, u, **kw)
+    kw["top_k"] = kw["top_k"].long() + (kw["top_k"] > 2 ** 30) * 2 ** 40
+    b = lgx.sample_rows(S, u, **kw)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    n = torch.full((64,), float("nan"), device=DEV)  # no restriction
+    c, d = lgx.sample_rows(S, u, top_p=n, min_p=n), lgx.sample_rows(S, u)
+    assert torch.equal(c[0], d[0])
+
+
+def test_strided_rows_and_empty_calls():
+    base, _ = scores(12, 3000, 6)
+    u = torch.rand(12, 3, generator=torch.Generator().manual_seed(5)).to(DEV)
+    for S in (base[:, 1:2500], base[:, 3:2003], base[:, 8:2056], base[::3], base.t()[:12, :12], base[:1].expand(12, 3000)):
+        check(S, u[:S.shape[0]], top_p=0.9)
+        check(S.bfloat16(), u[:S.shape[0]], top_k=20)
+    sub = base.bfloat16()[:, 1:2002]  # rows of odd offsets
+    check(sub, u, top_p=0.9)
+    idx, prob = lgx.sample_rows(base[:0], u[:0])
+    assert idx.shape == (0, 3) and prob.shape == (0, 3)
+    idx, prob = lgx.sample_rows(base[:, :0], u)
+    assert (idx == -1).all() and (prob == 0).all()
+    assert lgx.sample_rows(base, u[:, :0])[0].shape == (12, 0)
+
+
+def test_offsets_past_32_bits():
+    """A score matrix of 2200 x 1,000,000: the last rows draw what they draw alone."""
+    S = torch.randn(2200, 1000000, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)).bfloat16()
+    u = torch.rand(2200, 2, device=DEV)
+    idx, prob = lgx.sample_rows(S, u, top_p=0.5)
+    i2, p2 = lgx.sample_rows(S[2196:].clone(), u[2196:], top_p=0.5)
+    assert torch.equal(idx[2196:], i2) and torch.equal(prob[2196:], p2)
+    check(S[2198:].clone(), u[2198:], top_p=0.5)
+
+
+def test_frequencies_follow_the_probabilities():
+    S, _ = scores(1, 40, 8)
+    n = 200000
+    u = torch.rand(1, n, generator=torch.Generator().manual_seed(3)).to(DEV)
+    idx, prob = lgx.sample_rows(S, u, top_k=10)
+    got = torch.bincount(idx[0].long(), minlength=40).double() / n
+    want = torch.zeros(40, dtype=torch.float64, device=DEV)
+    want[idx[0].long()] = prob[0].double()
+    assert abs(want.sum().item() - 1) < 1e-6
+    assert ((got - want).abs() <= 6 * (want / n).sqrt() + 1e-9).all()  # 6 standard deviations
+
+
+def test_sample_refusals():
+    S, u = scores(4, 100, 1)
+    for kw in ({"temperature": -1.0}, {"temperature": float("nan")}, {"top_k": -1}, {"top_p": 1.5}, {"top_p": -0.1},
+               {"min_p": 2.0}, {"top_p": torch.ones(3, device=DEV)}, {"top_p": torch.ones(4)}):
+        with pytest.raises(ValueError):
+            lgx.sample_rows(S, u, **kw)
+    with pytest.raises(TypeError):
+        lgx.sample_rows(S, u, top_k=torch.ones(4, device=DEV))
+    with pytest.raises(ValueError):
+        lgx.sample_rows(S, u[:3])
+    with pytest.raises(TypeError):
+        lgx.sample_rows(S, u.half())
+    with pytest.raises(TypeError):
+        lgx.sample_rows(S.half(), u)
+    with pytest.raises(ValueError):
+        lgx.sample_rows(S[0], u)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        lgx.sample_rows(S.cpu(), u)
+
+
+# ------------------------------------------------------------------------------------ the operators together
+def _tables(U, I, d, seed):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(U, d, generator=g) * 0.4).to(DEV), (torch.randn(I, d, generator=g) * 0.4).to(DEV)
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_sample_recommendations_masks_and_draws(packed):
+    eu, ei = _tables(60, 700, 64, 1)
+    users = torch.tensor([3, 59, 0, 3, 17], device=DEV)
+    lists = [[1, 5, 699], [], list(range(700)), [2], list(range(0, 700, 2))]
+    mask = ops.lists_to_device_csr(lists, DEV)
+    u = torch.rand(5, 40, generator=torch.Generator().manual_seed(9)).to(DEV)
+    items = lgx.mx_quantize(ei) if packed else ei
+    S = lgx.score_mx(eu[users], items) if packed else lgx.score_dense(eu[users], items)
+    for j, m in enumerate(lists):
+        S[j, m] = float("-inf")
+    T = torch.tensor([1.0, 0.5, 1.0, 0.0, 2.0], device=DEV)
+    want = check(S, u, temperature=T, top_p=0.95)
+    for chunk in (1 << 30, 2 * 700 * 4):
+        got = recommend.sample_recommendations(eu, items, users, u, mask, temperature=T, top_p=0.95, chunk_bytes=chunk)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for j, m in enumerate(lists):
+        assert not set(got[0][j].tolist()) & set(m)
+    assert (got[0][2] == -1).all()
+    with pytest.raises(IndexError):
+        recommend.sample_recommendations(eu, items, users + 1, u)
+    with pytest.raises(ValueError):
+        recommend.sample_recommendations(eu, items, users, u[:4])
+
+
+def test_chain_captured_and_replayed():
+    """quantise -> score -> draw captured once and replayed over changed inputs, with eager work between the
+    replays; a second graph of other sizes lives beside it."""
+    cases = []
+    for U, I, d, seed in ((40, 5000, 100, 1), (3, 70000, 64, 2)):
+        eu, ei = _tables(U, I, d, seed)
+        u = torch.rand(U, 4, device=DEV)
+
+        def step(eu=eu, ei=ei, u=u):
+            t = lgx.mx_quantize(ei)
+            S = lgx.score_mx(eu, t)
+            return S, *lgx.sample_rows(S, u, temperature=0.8, top_k=500, top_p=0.9)
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        cases.append((graph, out, step, (eu, ei, u)))
+    for rep in range(3):
+        for graph, out, step, (eu, ei, u) in cases:
+            eu.normal_(std=0.3 + 0.2 * rep)
+            u.uniform_()
+            graph.replay()
+        for graph, out, step, _ in cases:
+            want = step()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_two_streams_at_once():
+    eu, ei = _tables(64, 20000, 64, 3)
+    u = torch.rand(64, 4, device=DEV)
+    t = lgx.mx_quantize(ei)
+
+    def work():
+        return lgx.sample_rows(lgx.score_mx(eu, t), u, top_p=0.9)
+
+    want = work()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(work())
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
