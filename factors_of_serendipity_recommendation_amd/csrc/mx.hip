@@ -173,73 +173,218 @@ __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c, uint32_t sa, u
 
 __device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
 
-// the blocks of one chunk (4 steps of 64 products): 16 bytes of codes a step and one scale byte a step
-struct Chunk {
-    u32x4 c[4];
+using u32u = uint32_t __attribute__((aligned(1)));
+using u16u = uint16_t __attribute__((aligned(1)));
+
+// HB steps of 64 products of one row: 16 bytes of codes and one scale byte a step
+template <int HB>
+struct Frag {
+    u32x4 c[HB];
     uint32_t s;
 };
 
-// blocks [first, first + 4) of one row, the ones at or past nb as zeros
-__device__ __forceinline__ void load_chunk(Chunk& f, const uint8_t* codes, const uint8_t* scales, int64_t row, int64_t nb,
-                                           int64_t first, bool valid) {
-    const u32x4* src = reinterpret_cast<const u32x4*>(codes) + row * nb;
-    const uint8_t* ss = scales + row * nb;
-    f.s = valid ? 0u : 0x7f7f7f7fu;
+// blocks [first, first + HB) of one row; the ones at or past nb, and all of them without `valid`, are zeros.
+// The row is `row` rows behind codes / scales (for items a wave-uniform address, so that a lane holds 32-bit
+// offsets only: 128 rows of at most 2048 blocks).
+template <int HB, typename Row>
+__device__ __forceinline__ void load_frag(Frag<HB>& f, const uint8_t* codes, const uint8_t* scales, Row row, int nb, int first,
+                                          bool valid) {
+    const Row blk = row * (Row)nb + (Row)first;
+    const u32x4* src = reinterpret_cast<const u32x4*>(codes + blk * 16);
+    const uint8_t* ss = scales + blk;
+    f.s = 0x7f7f7f7fu;
+    if (valid && first + HB <= nb) {
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-        const bool in = valid && first + kk < nb;
-        f.c[kk] = in ? src[first + kk] : u32x4{0, 0, 0, 0};
-        if (valid) f.s |= (in ? (uint32_t)ss[first + kk] : 127u) << (8 * kk);
+        for (int kk = 0; kk < HB; ++kk) f.c[kk] = src[kk];
+        if (HB == 4) {
+            f.s = *reinterpret_cast<const u32u*>(ss);
+        } else if (HB == 2) {
+            f.s = *reinterpret_cast<const u16u*>(ss);
+        } else {
+            f.s = 0;
+#pragma unroll
+            for (int kk = 0; kk < HB; ++kk) f.s |= (uint32_t)ss[kk] << (8 * kk);
+        }
+    } else {
+#pragma unroll
+        for (int kk = 0; kk < HB; ++kk) {
+            f.c[kk] = u32x4{0, 0, 0, 0};
+            if (valid && first + kk < nb) {
+                f.c[kk] = src[kk];
+                f.s ^= (0x7fu ^ ss[kk]) << (8 * kk);
+            }
+        }
     }
 }
 
-// One wave: 32 users x 128 items, the items' tile t of lane l being item base + 4 (l % 32) + t, so that a
-// lane's four results of one user are neighbours in the output row (one 16-byte store).
+template <int HB>
+__device__ __forceinline__ void copy_frag(Frag<HB>& to, const Frag<HB>& from) {
+#pragma unroll
+    for (int kk = 0; kk < HB; ++kk) to.c[kk] = from.c[kk];
+    to.s = from.s;
+}
+
+// the row of Q behind query b: -1 without one, -2 for an id outside the table
+__device__ __forceinline__ int64_t query_row(const MxArgs& a, int64_t b) {
+    if (b >= a.B) return -1;
+    if (!a.user_rows) return b;
+    const int64_t r = a.user_rows[b];
+    return r >= 0 && r < a.n_q ? r : -2;
+}
+template <int HB>
+__device__ __forceinline__ void load_query(Frag<HB>& f, const MxArgs& a, int64_t row, int first) {
+    load_frag<HB, int64_t>(f, a.q, a.qs, row, (int)a.nb, first, row >= 0);
+    if (row == -2) f.s = 0xffffffffu;  // NaN scales
+}
+
+// items past the end repeat the last one
+__device__ __forceinline__ uint32_t item_row(const MxArgs& a, int64_t base, int j) {
+    return (uint32_t)min((int64_t)j, a.n_items - 1 - base);
+}
+
+template <int HB>
+__device__ __forceinline__ void mma_steps(f32x16 (&acc)[4], const Frag<HB>& q, const Frag<HB> (&it)[4]) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) acc[t] = mma<0>(q.c[0], it[t].c[0], acc[t], q.s, it[t].s);
+    if (HB > 1)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[t] = mma<1>(q.c[HB > 1 ? 1 : 0], it[t].c[HB > 1 ? 1 : 0], acc[t], q.s, it[t].s);
+    if (HB > 2)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[t] = mma<2>(q.c[HB > 2 ? 2 : 0], it[t].c[HB > 2 ? 2 : 0], acc[t], q.s, it[t].s);
+    if (HB > 3)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[t] = mma<3>(q.c[HB > 3 ? 3 : 0], it[t].c[HB > 3 ? 3 : 0], acc[t], q.s, it[t].s);
+}
+
+// rows of the score matrix start at any multiple of an element
+using f32x4u = float __attribute__((ext_vector_type(4), aligned(4)));
+using u32x2u = uint32_t __attribute__((ext_vector_type(2), aligned(2)));
+
+// 32 users x 128 items of results.  The items' tile t of lane l is item base + 4 (l % 32) + t, so that a lane's
+// four results of one user are neighbours in the output row: one 16-byte store (512 bytes of a row per
+// half-wave).
 template <bool BF16, bool SIG>
-__global__ __launch_bounds__(256) void score_mx_kernel(MxArgs a) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int col = lane & 31, half = lane >> 5;
-    const int64_t base = (blockIdx.x * (int64_t)4 + wave) * 128;
-    if (base >= a.n_items) return;
-    const int64_t u0 = blockIdx.y * (int64_t)32;
-    const int64_t b = u0 + col;
-    const bool have = b < a.B;
-    int64_t qrow = b;
-    if (have && a.user_rows) qrow = a.user_rows[b];
-    const bool badq = have && (qrow < 0 || qrow >= a.n_q);
-    f32x16 acc[4] = {};
-    for (int64_t k0 = 0; k0 < a.nb; k0 += 8) {
-        Chunk q, it[4];
-        load_chunk(q, a.q, a.qs, qrow, a.nb, k0 + 4 * half, have && !badq);
-        if (badq) q.s = 0xffffffffu;
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-            load_chunk(it[t], a.it, a.its, min(base + 4 * col + t, a.n_items - 1), a.nb, k0 + 4 * half, true);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) acc[t] = mma<0>(q.c[0], it[t].c[0], acc[t], q.s, it[t].s);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) acc[t] = mma<1>(q.c[1], it[t].c[1], acc[t], q.s, it[t].s);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) acc[t] = mma<2>(q.c[2], it[t].c[2], acc[t], q.s, it[t].s);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) acc[t] = mma<3>(q.c[3], it[t].c[3], acc[t], q.s, it[t].s);
-    }
-    const int64_t i0 = base + 4 * col;
+__device__ __forceinline__ void store_tile(const MxArgs& a, const f32x16 (&acc)[4], int64_t u0, int64_t base, int lane) {
+    const int64_t left = a.n_items - base - 4 * (lane & 31);
+    if (left <= 0) return;
+    // a wave-uniform row plus a 32-bit lane offset (n_items < 2^27)
+    const uint32_t off = (uint32_t)(4 * (lane >> 5)) * (uint32_t)a.n_items + 4u * (lane & 31);
+    const int64_t u_lane = u0 + 4 * (lane >> 5);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        const int64_t u = u0 + 8 * (i / 4) + 4 * half + i % 4;
-        if (u >= a.B) continue;
+        const int64_t r = 8 * (i / 4) + i % 4;
+        if (u_lane + r >= a.B) continue;
+        float v[4];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            if (i0 + t >= a.n_items) continue;
-            float v = acc[t][i];
-            if (SIG) v = sigmoid(v);
-            if (BF16)
-                static_cast<uint16_t*>(a.out)[u * a.n_items + i0 + t] = f32_to_bf16(v);
-            else
-                static_cast<float*>(a.out)[u * a.n_items + i0 + t] = v;
+        for (int t = 0; t < 4; ++t) v[t] = SIG ? sigmoid(acc[t][i]) : acc[t][i];
+        if (BF16) {
+            uint16_t* o = static_cast<uint16_t*>(a.out) + (u0 + r) * a.n_items + base + off;
+            if (left >= 4) {
+                *reinterpret_cast<u32x2u*>(o) = u32x2u{f32_to_bf16(v[0]) | (uint32_t)f32_to_bf16(v[1]) << 16,
+                                                       f32_to_bf16(v[2]) | (uint32_t)f32_to_bf16(v[3]) << 16};
+            } else {
+                o[0] = f32_to_bf16(v[0]);
+                if (left > 1) o[1] = f32_to_bf16(v[1]);
+                if (left > 2) o[2] = f32_to_bf16(v[2]);
+            }
+        } else {
+            float* o = static_cast<float*>(a.out) + (u0 + r) * a.n_items + base + off;
+            if (left >= 4) {
+                *reinterpret_cast<f32x4u*>(o) = f32x4u{v[0], v[1], v[2], v[3]};
+            } else {
+                o[0] = v[0];
+                if (left > 1) o[1] = v[1];
+                if (left > 2) o[2] = v[2];
+            }
         }
     }
+}
+
+constexpr int kUserTiles = 8;  // tiles of 32 users a workgroup of score_mx_short walks
+
+// Rows of at most 8 blocks (d <= 256), HB = ceil(nb / 2): a wave keeps 128 items in registers and walks the
+// users' tiles; the next tile's rows are loaded before this one's scores are stored, so that no load waits
+// behind a store.  Bound by the writes of the score matrix.
+template <int HB, bool BF16, bool SIG>
+__global__ __launch_bounds__(256, 2) void score_mx_short(MxArgs a) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 31;
+    const int first = HB * (lane >> 5);
+    const int64_t base = (blockIdx.x * (int64_t)4 + wave) * 128;
+    if (base >= a.n_items) return;
+    const int64_t u_end = min(a.B, (blockIdx.y + (int64_t)1) * (kUserTiles * 32));
+    int64_t u0 = blockIdx.y * (int64_t)(kUserTiles * 32);
+    Frag<HB> it[4], q;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+        load_frag<HB, uint32_t>(it[t], a.it + base * a.nb * 16, a.its + base * a.nb, item_row(a, base, 4 * col + t), (int)a.nb,
+                                first, true);
+    load_query<HB>(q, a, query_row(a, u0 + col), first);
+    for (; u0 < u_end; u0 += 32) {
+        Frag<HB> next;
+        if (u0 + 32 < u_end) load_query<HB>(next, a, query_row(a, u0 + 32 + col), first);
+        f32x16 acc[4] = {};
+        mma_steps<HB>(acc, q, it);
+        store_tile<BF16, SIG>(a, acc, u0, base, lane);
+        copy_frag<HB>(q, next);
+    }
+}
+
+// Longer rows: a wave holds 64 users x 128 items of results and walks the blocks, 8 at a
+// time.  WU waves of
+// the workgroup take the next 64 users each, the others the next 128 items.
+template <int WU, bool BF16, bool SIG>
+__global__ __launch_bounds__(256, 2) void score_mx_long(MxArgs a) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 31;
+    const int64_t base = (blockIdx.x * (int64_t)(4 / WU) + wave / WU) * 128;
+    const int64_t u0 = (blockIdx.y * (int64_t)WU + wave % WU) * 64;
+    if (base >= a.n_items || u0 >= a.B) return;
+    const int64_t r0 = query_row(a, u0 + col), r1 = query_row(a, u0 + 32 + col);
+    f32x16 acc0[4] = {}, acc1[4] = {};
+    const uint8_t* codes = a.it + base * a.nb * 16;
+    const uint8_t* scales = a.its + base * a.nb;
+    uint32_t rows[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) rows[t] = item_row(a, base, 4 * col + t);
+    for (int k0 = 0; k0 < (int)a.nb; k0 += 8) {
+        const int first = k0 + 4 * (lane >> 5);
+        Frag<4> it[4], q0, q1;
+        load_query<4>(q0, a, r0, first);
+        load_query<4>(q1, a, r1, first);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) load_frag<4, uint32_t>(it[t], codes, scales, rows[t], (int)a.nb, first, true);
+        mma_steps<4>(acc0, q0, it);
+        mma_steps<4>(acc1, q1, it);
+    }
+    store_tile<BF16, SIG>(a, acc0, u0, base, lane);
+    if (u0 + 32 < a.B) store_tile<BF16, SIG>(a, acc1, u0 + 32, base, lane);
+}
+
+template <bool BF16, bool SIG>
+int launch_score(const MxArgs& a, hipStream_t stream) {
+    if (a.nb <= 8) {
+        const int64_t gy = ceil_div(a.B, (int64_t)(kUserTiles * 32));
+        LGX_REQUIRE(gy < 65536, LGX_ERR_UNSUPPORTED, "lgx_score_mx: %lld queries is too many", (long long)a.B);
+        const dim3 grid((unsigned)ceil_div(a.n_items, (int64_t)512), (unsigned)gy);
+        switch ((a.nb + 1) / 2) {
+            case 1: score_mx_short<1, BF16, SIG><<<grid, 256, 0, stream>>>(a); break;
+            case 2: score_mx_short<2, BF16, SIG><<<grid, 256, 0, stream>>>(a); break;
+            case 3: score_mx_short<3, BF16, SIG><<<grid, 256, 0, stream>>>(a); break;
+            default: score_mx_short<4, BF16, SIG><<<grid, 256, 0, stream>>>(a); break;
+        }
+    } else {
+        const int wu = a.B > 128 ? 4 : a.B > 64 ? 2 : 1;  // waves side by side over the users
+        const int64_t gy = ceil_div(a.B, (int64_t)(64 * wu));
+        LGX_REQUIRE(gy < 65536, LGX_ERR_UNSUPPORTED, "lgx_score_mx: %lld queries is too many", (long long)a.B);
+        const dim3 grid((unsigned)ceil_div(a.n_items, (int64_t)(512 / wu)), (unsigned)gy);
+        if (wu == 4) score_mx_long<4, BF16, SIG><<<grid, 256, 0, stream>>>(a);
+        else if (wu == 2) score_mx_long<2, BF16, SIG><<<grid, 256, 0, stream>>>(a);
+        else score_mx_long<1, BF16, SIG><<<grid, 256, 0, stream>>>(a);
+    }
+    LGX_LAUNCH_CHECK();
+    return LGX_OK;
 }
 
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
@@ -321,7 +466,8 @@ extern "C" int lgx_score_mx(const void* Q, const uint8_t* q_scales, int q_dtype,
     LGX_REQUIRE(out_dtype == LGX_DTYPE_F32 || out_dtype == LGX_DTYPE_BF16, LGX_ERR_INVALID_ARG, "lgx_score_mx: out dtype");
     LGX_REQUIRE(d >= 1 && d <= kMaxD, LGX_ERR_UNSUPPORTED, "lgx_score_mx: d=%lld outside [1, %lld]", (long long)d,
                 (long long)kMaxD);
-    LGX_REQUIRE(n_items < INT32_MAX && B < INT32_MAX, LGX_ERR_UNSUPPORTED, "lgx_score_mx: 2^31 rows or more");
+    LGX_REQUIRE(n_items < (1LL << 27), LGX_ERR_UNSUPPORTED, "lgx_score_mx: %lld items is too many (< 2^27)",
+                (long long)n_items);
     if (B == 0 || n_items == 0) return LGX_OK;
     LGX_REQUIRE(Q && item_codes && item_scales && scores, LGX_ERR_INVALID_ARG, "lgx_score_mx: null pointer");
     LGX_REQUIRE(user_rows || B <= n_q, LGX_ERR_INVALID_ARG, "lgx_score_mx: %lld queries of %lld rows", (long long)B,
@@ -345,16 +491,6 @@ extern "C" int lgx_score_mx(const void* Q, const uint8_t* q_scales, int q_dtype,
         a.user_rows = nullptr;
         a.n_q = B;
     }
-    const int64_t gx = ceil_div(n_items, (int64_t)512), gy = ceil_div(B, (int64_t)32);
-    LGX_REQUIRE(gy < 65536, LGX_ERR_UNSUPPORTED, "lgx_score_mx: %lld queries is too many", (long long)B);
-    const dim3 grid((unsigned)gx, (unsigned)gy);
-    if (out_dtype == LGX_DTYPE_BF16) {
-        if (apply_sigmoid) score_mx_kernel<true, true><<<grid, 256, 0, stream>>>(a);
-        else score_mx_kernel<true, false><<<grid, 256, 0, stream>>>(a);
-    } else {
-        if (apply_sigmoid) score_mx_kernel<false, true><<<grid, 256, 0, stream>>>(a);
-        else score_mx_kernel<false, false><<<grid, 256, 0, stream>>>(a);
-    }
-    LGX_LAUNCH_CHECK();
-    return LGX_OK;
+    if (out_dtype == LGX_DTYPE_BF16) return apply_sigmoid ? launch_score<true, true>(a, stream) : launch_score<true, false>(a, stream);
+    return apply_sigmoid ? launch_score<false, true>(a, stream) : launch_score<false, false>(a, stream);
 }
