@@ -322,7 +322,10 @@ __global__ __launch_bounds__(256, 2) void score_mx_short(MxArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31;
     const int first = HB * (lane >> 5);
-    const int64_t base = (blockIdx.x * (int64_t)4 + wave) * 128;
+    // workgroups go to the 8 XCDs in turn; rows whose stores share lines put neighbours on one XCD, so that one
+    // L2 sees both parts of a line (2048 x 40,981: 94 -> 75 us; whole-line rows 793 -> 804)
+    const uint32_t bx = NT ? blockIdx.x : blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8;
+    const int64_t base = (bx * (int64_t)4 + wave) * 128;
     if (base >= a.n_items) return;
     const int64_t u_end = min(a.B, (blockIdx.y + (int64_t)1) * (kUserTiles * 32));
     int64_t u0 = blockIdx.y * (int64_t)(kUserTiles * 32);
@@ -378,7 +381,8 @@ int launch_score(const MxArgs& a, hipStream_t stream) {
     if (a.nb <= 8) {
         const int64_t gy = ceil_div(a.B, (int64_t)(kUserTiles * 32));
         LGX_REQUIRE(gy < 65536, LGX_ERR_UNSUPPORTED, "lgx_score_mx: %lld queries is too many", (long long)a.B);
-        const dim3 grid((unsigned)ceil_div(a.n_items, (int64_t)512), (unsigned)gy);
+        const int64_t gx = ceil_div(a.n_items, (int64_t)512);
+        const dim3 grid((unsigned)(NT ? gx : 8 * ceil_div(gx, (int64_t)8)), (unsigned)gy);
         switch ((a.nb + 1) / 2) {
             case 1: score_mx_short<1, BF16, SIG, NT><<<grid, 256, 0, stream>>>(a); break;
             case 2: score_mx_short<2, BF16, SIG, NT><<<grid, 256, 0, stream>>>(a); break;
