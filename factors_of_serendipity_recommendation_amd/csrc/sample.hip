@@ -73,22 +73,21 @@ struct Vec {
     }
 };
 
-// f(score, column) over columns [lo, hi) by `width` lanes, this one being `me`; a lane takes its columns in
-// ascending order
+// f(four scores, column of the first) over columns [lo, hi) by `width` lanes, this one being `me`; a lane takes
+// its columns in ascending order, U groups at a time; columns past the end come as -inf
 template <bool BF16, int U, typename F>
-__device__ __forceinline__ void for_columns(const void* s, int64_t lo, int64_t hi, int me, int width, F f) {
+__device__ __forceinline__ void for_groups(const void* s, int64_t lo, int64_t hi, int me, int width, F f) {
     constexpr int N = Vec<BF16>::N;
     int64_t i = lo + (int64_t)me * N;
     const int64_t step = (int64_t)width * N;
-    for (; i + (U - 1) * step + N <= hi; i += U * step) {
-        Vec<BF16> v[U];
+    if (U > 1)
+        for (; i + (U - 1) * step + N <= hi; i += U * step) {
+            Vec<BF16> v[U];
 #pragma unroll
-        for (int k = 0; k < U; ++k) v[k].load(s, i + k * step);
+            for (int k = 0; k < U; ++k) v[k].load(s, i + k * step);
 #pragma unroll
-        for (int k = 0; k < U; ++k)
-#pragma unroll
-            for (int j = 0; j < N; ++j) f(v[k].v[j], i + k * step + j);
-    }
+            for (int k = 0; k < U; ++k) f(v[k].v, (int)(i + k * step));
+        }
 #pragma unroll 1
     for (; i < hi; i += step) {
         Vec<BF16> v;
@@ -96,8 +95,7 @@ __device__ __forceinline__ void for_columns(const void* s, int64_t lo, int64_t h
             v.load(s, i);
         else
             v.load_tail(s, i, hi);
-#pragma unroll
-        for (int j = 0; j < N; ++j) f(v.v[j], i + j);
+        f(v.v, (int)i);
     }
 }
 
@@ -105,47 +103,61 @@ __device__ __forceinline__ void for_columns(const void* s, int64_t lo, int64_t h
 __device__ __forceinline__ uint32_t score_key(float s) {
     return s > -INFINITY ? ord_f32(s + 0.0f) : 0u;
 }
-__device__ __forceinline__ uint64_t column_key(float s, int64_t i) {
+__device__ __forceinline__ uint64_t column_key(float s, int i) {
     return (uint64_t)score_key(s) << 32 | (0xffffffffu - (uint32_t)i);
 }
 
-// 2^(y + e) for y <= 0: y = n + f, |f| <= 1/2, and the Taylor polynomial of e^(f ln 2) of degree 11, whose
-// coefficients are ln(2)^k / k! (remainder below 0.347^12 / 12! < 7e-15)
-__device__ __forceinline__ double exp2_f64(double y, int e) {
-    y = fmax(y, -1100.0);
-    const double big = y + 6755399441055744.0;  // 1.5 * 2^52: the low word is rint(y)
-    const double f = y - (big - 6755399441055744.0);
-    constexpr double L = 0.69314718055994530942;
-    constexpr double c2 = L * L / 2, c3 = c2 * L / 3, c4 = c3 * L / 4, c5 = c4 * L / 5, c6 = c5 * L / 6, c7 = c6 * L / 7,
-                     c8 = c7 * L / 8, c9 = c8 * L / 9, c10 = c9 * L / 10, c11 = c10 * L / 11;
-    double r = fma(c11, f, c10);
-    r = fma(r, f, c9);
-    r = fma(r, f, c8);
-    r = fma(r, f, c7);
-    r = fma(r, f, c6);
-    r = fma(r, f, c5);
-    r = fma(r, f, c4);
-    r = fma(r, f, c3);
-    r = fma(r, f, c2);
-    r = fma(r, f, L);
-    r = fma(r, f, 1.0);
-    return ldexp(r, (int)(uint32_t)__double_as_longlong(big) + e);
+// where the ranking is cut: columns scoring above s, and those scoring s up to column i
+struct Cut {
+    float s;
+    int i;
+    __device__ __forceinline__ bool keeps(float v, int col) const { return (v > s) | ((v == s) & (col <= i)); }
+};
+constexpr float kNone = -INFINITY;  // Cut{kNone, -1}: every column with a score
+
+// one f64 multiply-add with its addend in scalar registers (the compiler copies a constant addend into vector
+// registers before every step: 10 more instructions a weight)
+__device__ __forceinline__ double fma_const(double a, double b, double c) {
+    double r;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
+    return r;
 }
 
-// Weights against the row's best score m: exp((s - m) / T), 1 for s == m (an infinite m too), 0 for excluded ones
+// Weights exp((s - m) / T) against the row's best score m, a finite one; 0 for -inf and NaN, which the maximum turns into
+// a distance of 2^-1100.  2^y = 2^n 2^f with n = rint(y) and for 2^f, |f| <= 1/2, the polynomial that equals it at 0 and
+// at nine Chebyshev nodes (within 4e-14 relative, exact at f = 0: equal scores weigh the same power of two)
 struct Weigh {
-    double m, c;  // c = log2(e) / T
-    float top;
-    int unit;     // log2 of the fixed-point unit
-    __device__ __forceinline__ double operator()(float s) const {
-        const double w = exp2_f64(((double)s - m) * c, 0);
-        return s == top ? 1.0 : s > -INFINITY ? w : 0.0;
+    double m, c;   // c = log2(e) / T
+    double floor;  // the distance whose weight underflows
+    int unit;      // log2 of the fixed-point unit
+    __device__ __forceinline__ Weigh(float top, double T, int cols) {
+        m = (double)top;
+        c = 1.4426950408889634074 / fmin(T, 1e300);
+        floor = -1100.0 / c;
+        unit = 62;  // the sum of all weights is at most cols
+        while (unit > 0 && (1ll << (62 - unit)) < (int64_t)cols) --unit;
+        unit = min(unit, 51);
     }
+    __device__ __forceinline__ double scaled(float s, int e) const {
+        const double d = fmax((double)s - m, floor);
+        const double big = fma(d, c, 6755399441055744.0);  // 1.5 * 2^52: the low word is n
+        const double f = fma(d, c, 6755399441055744.0 - big);
+        double r = fma_const(f, 1.0203121063391729e-07, 1.3255224878668817e-06);
+        r = fma_const(r, f, 1.525268684626772e-05);
+        r = fma_const(r, f, 0.00015403455852453838);
+        r = fma_const(r, f, 0.0013333558179043112);
+        r = fma_const(r, f, 0.009618129159402558);
+        r = fma_const(r, f, 0.055504108664760424);
+        r = fma_const(r, f, 0.2402265069581299);
+        r = fma_const(r, f, 0.6931471805599453);
+        r = fma(r, f, 1.0);
+        return ldexp(r, (int)(uint32_t)__double_as_longlong(big) + e);
+    }
+    __device__ __forceinline__ double operator()(float s) const { return scaled(s, 0); }
     // w in units of 2^-unit, rounded; w 2^unit <= 2^51, so that adding 2^52 leaves it in the low bits
     __device__ __forceinline__ uint64_t fixed(float s) const {
-        const double w = exp2_f64(((double)s - m) * c, unit) + 4503599627370496.0;
-        const uint64_t v = (uint64_t)__double_as_longlong(w) & 0xfffffffffffffull;
-        return s == top ? 1ull << unit : s > -INFINITY ? v : 0ull;
+        const double w = scaled(s, unit) + 4503599627370496.0;
+        return (uint64_t)__double_as_longlong(w) & 0xfffffffffffffull;
     }
 };
 
@@ -153,32 +165,45 @@ struct Weigh {
 __device__ __forceinline__ double shfl_f64(double v, int src) { return __longlong_as_double((int64_t)shfl_u64(__double_as_longlong(v), src)); }
 __device__ __forceinline__ double shfl_xor_f64(double v, int m) { return __longlong_as_double((int64_t)shfl_xor_u64(__double_as_longlong(v), m)); }
 
-__device__ __forceinline__ double wave_sum_f64(double v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += shfl_xor_f64(v, o);
+// v from the lane that a DPP row operation names, 0 where it names none
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp_u64(uint64_t v) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf, false);
+    return (uint64_t)hi << 32 | lo;
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_f64(double v) {
+    return __longlong_as_double((int64_t)dpp_u64<CTRL, ROWS>((uint64_t)__double_as_longlong(v)));
+}
+// inclusive sums over the lanes: shifts within a row of 16, then the last lane of row 0 into row 1 and of row 2 into row
+// 3, then lane 31 into the upper half
+__device__ __forceinline__ double wave_scan_f64(double v) {
+    v += dpp_f64<0x111, 0xf>(v);
+    v += dpp_f64<0x112, 0xf>(v);
+    v += dpp_f64<0x114, 0xf>(v);
+    v += dpp_f64<0x118, 0xf>(v);
+    v += dpp_f64<0x142, 0xa>(v);
+    v += dpp_f64<0x143, 0xc>(v);
     return v;
 }
-__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += shfl_xor_u64(v, o);
+__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {
+    v += dpp_u64<0x111, 0xf>(v);
+    v += dpp_u64<0x112, 0xf>(v);
+    v += dpp_u64<0x114, 0xf>(v);
+    v += dpp_u64<0x118, 0xf>(v);
+    v += dpp_u64<0x142, 0xa>(v);
+    v += dpp_u64<0x143, 0xc>(v);
     return v;
 }
-// inclusive prefix sums over the lanes
-__device__ __forceinline__ double wave_scan_f64(double v, int lane) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double t = shfl_f64(v, lane >= o ? lane - o : lane);
-        if (lane >= o) v += t;
-    }
-    return v;
-}
-__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v, int lane) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint64_t t = shfl_u64(v, lane >= o ? lane - o : lane);
-        if (lane >= o) v += t;
-    }
-    return v;
+__device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
+    v = max(v, dpp_u64<0x111, 0xf>(v));
+    v = max(v, dpp_u64<0x112, 0xf>(v));
+    v = max(v, dpp_u64<0x114, 0xf>(v));
+    v = max(v, dpp_u64<0x118, 0xf>(v));
+    v = max(v, dpp_u64<0x142, 0xa>(v));
+    v = max(v, dpp_u64<0x143, 0xc>(v));
+    return v;  // lane 63 holds it
 }
 
 struct Shared {
@@ -193,21 +218,22 @@ struct Shared {
 
 // sum / maximum over the workgroup, the same value in every thread
 __device__ uint64_t block_sum_u64(uint64_t v, Shared& sh) {
-    v = wave_sum_u64(v);
+    v = wave_scan_u64(v);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh.part[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 63) sh.part[threadIdx.x >> 6] = v;
     __syncthreads();
     uint64_t s = 0;
+#pragma unroll
     for (int i = 0; i < kWaves; ++i) s += sh.part[i];
     return s;
 }
 __device__ uint64_t block_max_u64(uint64_t v, Shared& sh) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = max(v, shfl_xor_u64(v, o));
+    v = wave_max_u64(v);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh.part[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 63) sh.part[threadIdx.x >> 6] = v;
     __syncthreads();
     uint64_t s = 0;
+#pragma unroll
     for (int i = 0; i < kWaves; ++i) s = max(s, sh.part[i]);
     return s;
 }
@@ -220,33 +246,38 @@ __device__ __forceinline__ void clear_hist(Shared& sh) {
 }
 
 // The bin in which the running sum of hist, from bin 0 on, reaches `target`: sum before it < target <= sum with
-// it; the last bin that holds anything if the whole falls short.  -> sh.bin, sh.below = the sum before it
+// it; the last bin that holds anything if the whole falls short, bin 0 of an empty histogram.
+// -> sh.bin, sh.below = the sum before it
 __device__ void find_bin(double target, Shared& sh) {
+    constexpr int per = kBins / kThreads;
+    const int tid = threadIdx.x;
+    if (tid == 0) {
+        sh.bin = 0;
+        sh.below = 0;
+    }
     __syncthreads();
-    if (threadIdx.x < 64) {
-        const int lane = threadIdx.x;
-        constexpr int per = kBins / 64;
-        uint64_t own = 0;
-        for (int j = 0; j < per; ++j) own += sh.hist[lane * per + j];
-        const uint64_t incl = wave_scan_u64(own, lane);
-        const uint64_t hit = __ballot(own > 0 && (double)incl >= target);
-        const uint64_t any = __ballot(own > 0);
-        const int pick = hit ? __builtin_ctzll(hit) : any ? 63 - __builtin_clzll(any) : 0;
-        if (lane == pick) {
-            uint64_t run = incl - own;
-            int last = lane * per;
-            uint64_t at = run;
-            for (int j = 0; j < per; ++j) {
-                const uint64_t h = sh.hist[lane * per + j];
-                if (!h) continue;
-                last = lane * per + j;
-                at = run;
-                if ((double)(run + h) >= target) break;
-                run += h;
-            }
-            sh.bin = (uint32_t)last;
-            sh.below = at;
+    uint64_t h[per], own = 0;
+#pragma unroll
+    for (int j = 0; j < per; ++j) own += h[j] = sh.hist[tid * per + j];
+    const uint64_t incl = wave_scan_u64(own);
+    if ((tid & 63) == 63) sh.part[tid >> 6] = incl;
+    __syncthreads();
+    uint64_t run = incl - own, all = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        if (w < (tid >> 6)) run += sh.part[w];
+        all += sh.part[w];
+    }
+    target = fmin(target, (double)all);
+#pragma unroll
+    for (int j = 0; j < per; ++j) {
+        const uint64_t next = run + h[j];
+        // the first bin that reaches it (a target of 0 or less: the first that holds anything)
+        if (h[j] && (double)next >= target && (run == 0 || (double)run < target)) {
+            sh.bin = (uint32_t)(tid * per + j);
+            sh.below = run;
         }
+        run = next;
     }
     __syncthreads();
 }
@@ -281,7 +312,7 @@ __device__ void scan_list(int n, Shared& sh) {
         const int lane = threadIdx.x, lo = lane * per, hi = min(n, lo + per);
         double own = 0.0;
         for (int j = lo; j < hi; ++j) own += sh.w[j];
-        double run = wave_scan_f64(own, lane) - own;
+        double run = wave_scan_f64(own) - own;
         for (int j = lo; j < hi; ++j) sh.w[j] = run += sh.w[j];
     }
     __syncthreads();
@@ -307,47 +338,47 @@ __device__ __forceinline__ double draw_number(const SampleArgs& a, int64_t row, 
     return fmin(fmax(u, 0.0), 1.0);
 }
 
-// what one reading of a row (or a part of it) gives
+// one reading of the columns [lo, hi): the best one as a key (0 without one), and the lowest score above -1e30 (lower
+// ones are masks, and share the last bin)
 struct Top {
-    uint64_t best;  // largest column key
-    uint64_t live;  // columns that are not excluded
-    float low;      // smallest live score above -1e30 (lower ones are masks, and share the last bin)
+    uint64_t best;
+    float low;
 };
 template <bool BF16>
 __device__ __forceinline__ Top scan_top(const void* s, int64_t lo, int64_t hi, int me, int width) {
     float best = -INFINITY, low = INFINITY;
-    int64_t at = -1;
-    uint32_t live = 0;
-    for_columns<BF16, 2>(s, lo, hi, me, width, [&](float v, int64_t i) {
-        if (v > best) {
-            best = v;
-            at = i;
+    int at = -1;
+    for_groups<BF16, 4>(s, lo, hi, me, width, [&](const float (&v)[4], int i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) low = fminf(low, v[j] > -1e30f ? v[j] : INFINITY);
+        if (fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) > best) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (v[j] > best) {
+                    best = v[j];
+                    at = i + j;
+                }
         }
-        live += v > -INFINITY;
-        if (v > -1e30f) low = fminf(low, v);
     });
-    return Top{at < 0 ? 0ull : column_key(best, at), live, low};
+    return Top{at < 0 ? 0ull : column_key(best, at), low};
 }
 
-// equal steps of the distance to the best score; 0 is the best bin
+// equal steps of the distance to the best score.  A score belongs to bin b < kBins - 1 iff b <= at(s) < b + 1,
+// what is farther (and NaN) to the last one
 struct Binning {
     float top, inv;
-    __device__ __forceinline__ int operator()(float s) const {
-        // NaN and -inf never get here; top - s is inf at most
-        return s == top ? 0 : (int)fminf((top - s) * inv, (float)(kBins - 1));
-    }
+    __device__ __forceinline__ float at(float s) const { return (top - s) * inv; }
+    __device__ __forceinline__ int operator()(float s) const { return (int)fminf(at(s), (float)(kBins - 1)); }
 };
-__device__ __forceinline__ Binning make_binning(float top, float low, double reach) {
-    const double range = fmin((double)top - (double)low, reach);
-    // at least one f32 step per bin; an infinite or undefined range leaves all in bin 0 or the last one
-    const double inv = (double)(kBins - 1) / range;
-    return Binning{top, inv < 1e37 && inv > 0.0 ? (float)inv : inv > 0.0 ? 1e37f : 0.0f};
+__device__ __forceinline__ Binning make_binning(float top, double range) {
+    const double inv = (double)(kBins - 1) / range;  // a range of 0: all the best score's equals in bin 0
+    return Binning{top, (float)fmin(inv, 1e30)};
 }
 
 // The cut of top_k (MASS false: `target` columns) or top_p (`target` of the fixed weights), among the columns of
 // key >= cut, by descent over the score bits; ties are counted off in column order
 template <bool BF16, bool MASS>
-__device__ uint64_t descend(const void* s, int cols, uint64_t cut, double target, const Weigh& weigh, Shared& sh) {
+__device__ Cut descend(const void* s, int cols, const Cut& cut, double target, const Weigh& weigh, Shared& sh) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     uint64_t above = 0;   // counted in better bins than this digit's
     uint32_t prefix = 0;  // the score bits found so far
@@ -357,26 +388,29 @@ __device__ uint64_t descend(const void* s, int cols, uint64_t cut, double target
         const int open = digit == 0 ? 32 : digit == 1 ? 21 : 10;  // bits not yet found
         const uint32_t mask = (1u << (open - shift)) - 1u;
         clear_hist(sh);
-        for_columns<BF16, 1>(s, 0, cols, tid, kThreads, [&](float v, int64_t i) {
-            const uint64_t key = column_key(v, i);
-            const uint32_t k = (uint32_t)(key >> 32);
-            if (k && key >= cut && (open == 32 || (k >> open) == (prefix >> open)))
-                atomicAdd((unsigned long long*)&sh.hist[mask - ((k >> shift) & mask)],
-                          (unsigned long long)(MASS ? weigh.fixed(v) : 1ull));
+        for_groups<BF16, 1>(s, 0, cols, tid, kThreads, [&](const float (&v)[4], int i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t k = score_key(v[j]);
+                if (cut.keeps(v[j], i + j) && (open == 32 || (k >> open) == (prefix >> open)))
+                    atomicAdd((unsigned long long*)&sh.hist[mask - ((k >> shift) & mask)],
+                              (unsigned long long)(MASS ? weigh.fixed(v[j]) : 1ull));
+            }
         });
         find_bin(target - (double)above, sh);
         prefix |= (mask - sh.bin) << shift;
         above += sh.below;
     }
     __syncthreads();
-    const uint64_t each = MASS ? max(weigh.fixed(unord_f32(prefix)), (uint64_t)1) : 1ull;
+    const float value = unord_f32(prefix);
+    const uint64_t each = MASS ? max(weigh.fixed(value), (uint64_t)1) : 1ull;
     const double want_f = ceil((target - (double)above) / (double)each);
     int64_t want = want_f < 1.0 ? 1 : (int64_t)fmin(want_f, (double)cols);
-    int64_t found = -1;  // the column of the last one taken
+    int found = -1;  // the column of the last one taken
     for (int64_t i0 = 0; i0 < cols; i0 += kThreads) {
         const int64_t i = i0 + tid;
-        const uint64_t key = i < cols ? column_key(load_score<BF16>(s, i), i) : 0ull;
-        const bool eq = (uint32_t)(key >> 32) == prefix && key >= cut;
+        const float v = i < cols ? load_score<BF16>(s, i) : kNone;
+        const bool eq = v == value && cut.keeps(v, (int)i);
         const uint64_t m = __ballot(eq);
         __syncthreads();
         if (lane == 0) sh.part[wave] = (uint64_t)__popcll(m);
@@ -387,12 +421,11 @@ __device__ uint64_t descend(const void* s, int cols, uint64_t cut, double target
             all += (int64_t)sh.part[w];
         }
         before += __popcll(m & ((1ull << lane) - 1));
-        if (eq && before < want) found = i;
+        if (eq && before < want) found = (int)i;
         want -= all;
         if (want <= 0) break;
     }
-    const uint64_t last = block_max_u64((uint64_t)(found + 1), sh);
-    return max(cut, (uint64_t)prefix << 32 | (0xffffffffu - (uint32_t)(last - 1)));
+    return Cut{value, (int)block_max_u64((uint64_t)(found + 1), sh) - 1};
 }
 
 // sh.key[0, n) holds the row's best n columns, unsorted, n <= kList, at least min(top_k, live) of them: the
@@ -448,6 +481,31 @@ __device__ void finish_list(const SampleArgs& a, int64_t row, const Row& r, int 
     }
 }
 
+// A row with infinite scores: those columns share it equally, and their ranking is the column order
+template <bool BF16>
+__device__ void draw_infinite(const SampleArgs& a, int64_t row, const Row& r, const void* s, Shared& sh) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    uint64_t n = 0;
+    for (int64_t i = tid; i < a.cols; i += kThreads) n += load_score<BF16>(s, i) == INFINITY;
+    int64_t keep = (int64_t)block_sum_u64(n, sh);
+    if (r.top_k > 0) keep = min(keep, r.top_k);
+    if (r.top_p < 1.0) keep = max((int64_t)1, (int64_t)ceil(r.top_p * (double)keep));
+    for (int64_t j = wave; j < a.n_draws; j += kWaves) {
+        int64_t rank = min((int64_t)(draw_number(a, row, j) * (double)keep), keep - 1), at = -1;
+        for (int64_t i0 = 0; i0 < a.cols && at < 0; i0 += 64) {
+            const uint64_t m = __ballot(i0 + lane < a.cols && load_score<BF16>(s, min(i0 + lane, a.cols - 1)) == INFINITY);
+            const bool mine = (m >> lane & 1) && __popcll(m & ((1ull << lane) - 1)) == rank;
+            const uint64_t hit = __ballot(mine);
+            if (hit) at = i0 + __builtin_ctzll(hit);
+            rank -= __popcll(m);
+        }
+        if (lane == 0) {
+            a.out_idx[row * a.n_draws + j] = (int32_t)at;
+            if (a.out_prob) a.out_prob[row * a.n_draws + j] = (float)(1.0 / (double)keep);
+        }
+    }
+}
+
 template <bool BF16>
 __global__ __launch_bounds__(kThreads, 4) void sample_rows_kernel(SampleArgs a) {
     __shared__ Shared sh;
@@ -461,58 +519,75 @@ __global__ __launch_bounds__(kThreads, 4) void sample_rows_kernel(SampleArgs a) 
 
     const Top mine = scan_top<BF16>(s, 0, cols, tid, kThreads);
     const uint64_t best = block_max_u64(mine.best, sh);
-    const uint64_t live = block_sum_u64(mine.live, sh);
-    if (live == 0 || !(r.T > 0.0) || r.top_k == 1) {
+    if (best == 0 || !(r.T > 0.0) || r.top_k == 1) {
         for (int64_t j = tid; j < a.n_draws; j += kThreads) {
-            a.out_idx[row * a.n_draws + j] = live ? key_index(best) : -1;
-            if (a.out_prob) a.out_prob[row * a.n_draws + j] = live ? 1.0f : 0.0f;
+            a.out_idx[row * a.n_draws + j] = best ? key_index(best) : -1;
+            if (a.out_prob) a.out_prob[row * a.n_draws + j] = best ? 1.0f : 0.0f;
         }
         return;
     }
-    const float low = unord_f32(~(uint32_t)block_max_u64((uint64_t)(~ord_f32(mine.low)), sh));
     const float top = key_score(best);
-    int unit = 62;  // the sum of all weights is at most cols
-    while (unit > 0 && (1ll << (62 - unit)) < (int64_t)cols) --unit;
-    const Weigh weigh{(double)top, 1.4426950408889634074 / r.T, top, min(unit, 51)};
+    if (top == INFINITY) {
+        draw_infinite<BF16>(a, row, r, s, sh);
+        return;
+    }
+    const Weigh weigh(top, r.T, cols);
 
-    uint64_t cut = 1ull << 32;  // every column with a score
-    if (r.top_k > 0 && (uint64_t)r.top_k < live) {
-        const Binning bin = make_binning(top, low, INFINITY);
+    Cut cut{kNone, -1};
+    if (r.top_k > 0 && r.top_k < cols) {
+        const float low = unord_f32(~(uint32_t)block_max_u64((uint64_t)(~ord_f32(mine.low)), sh));
+        const Binning bin = make_binning(top, fmax((double)top - (double)low, 0.0));
         clear_hist(sh);
-        for_columns<BF16, 2>(s, 0, cols, tid, kThreads, [&](float v, int64_t) {
-            if (v > -INFINITY) atomicAdd((unsigned*)&sh.hist[bin(v)], 1u);
+        for_groups<BF16, 2>(s, 0, cols, tid, kThreads, [&](const float (&v)[4], int) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (v[j] > kNone) atomicAdd((unsigned*)&sh.hist[bin(v[j])], 1u);
         });
         find_bin((double)r.top_k, sh);
         const int b = (int)sh.bin;
         const uint64_t before = sh.below, in_bin = sh.hist[b];
         const bool list = before + in_bin <= kList;
         if (list || in_bin <= kList) {
-            for_columns<BF16, 2>(s, 0, cols, tid, kThreads, [&](float v, int64_t i) {
-                if (v > -INFINITY) {
-                    const int at = bin(v);
-                    if (list ? at <= b : at == b) sh.key[atomicAdd(&sh.n, 1u)] = column_key(v, i);
+            const float from = list ? -INFINITY : (float)b, to = b == kBins - 1 ? NAN : (float)(b + 1);
+            for_groups<BF16, 2>(s, 0, cols, tid, kThreads, [&](const float (&v)[4], int i) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float x = bin.at(v[j]);
+                    if ((x >= from) & !(x >= to) & (v[j] > kNone)) sh.key[atomicAdd(&sh.n, 1u)] = column_key(v[j], i + j);
                 }
             });
             __syncthreads();
             if (list) {
-                finish_list(a, row, r, (int)(before + in_bin), weigh, sh);
+                finish_list(a, row, r, (int)sh.n, weigh, sh);
                 return;
             }
             sort_keys((int)in_bin, sh);
-            cut = sh.key[(uint64_t)r.top_k - before - 1];
+            const uint64_t key = sh.key[min((uint64_t)r.top_k - before, in_bin) - 1];
+            cut = Cut{key_score(key), key_index(key)};
         } else {
             cut = descend<BF16, false>(s, cols, cut, (double)r.top_k, weigh, sh);
         }
     }
     if (r.top_p < 1.0) {
         // a column of weight below (1 - p) Z / cols is never kept (all such together weigh less than the
-        // (1 - p) Z that are dropped), and Z >= 1
-        const double reach = r.T * (log((double)cols / (1.0 - r.top_p)) + 1e-3);
-        const Binning bin = make_binning(top, low, reach);
+        // (1 - p) Z that are dropped), and Z >= 1; they share the last bin, summed in registers
+        const Binning bin = make_binning(top, fmin(r.T, 1e30) * (log((double)cols / (1.0 - r.top_p)) + 1e-3));
+        const bool all = cut.s == kNone;
         clear_hist(sh);
-        for_columns<BF16, 1>(s, 0, cols, tid, kThreads, [&](float v, int64_t i) {
-            if (column_key(v, i) >= cut) atomicAdd((unsigned long long*)&sh.hist[bin(v)], (unsigned long long)weigh.fixed(v));
+        uint64_t rest = 0;
+        for_groups<BF16, 1>(s, 0, cols, tid, kThreads, [&](const float (&v)[4], int i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (!all && !cut.keeps(v[j], i + j)) continue;
+                const uint64_t w = weigh.fixed(v[j]);
+                const int b = bin(v[j]);
+                if (b < kBins - 1)
+                    atomicAdd((unsigned long long*)&sh.hist[b], (unsigned long long)w);
+                else
+                    rest += w;
+            }
         });
+        if (rest) atomicAdd((unsigned long long*)&sh.hist[kBins - 1], (unsigned long long)rest);
         __syncthreads();
         uint64_t sum = 0;
         for (int j = tid; j < kBins; j += kThreads) sum += sh.hist[j];
@@ -520,16 +595,38 @@ __global__ __launch_bounds__(kThreads, 4) void sample_rows_kernel(SampleArgs a) 
         find_bin(target, sh);
         const int b = (int)sh.bin;
         const uint64_t before = sh.below;
-        for_columns<BF16, 2>(s, 0, cols, tid, kThreads, [&](float v, int64_t i) {
-            const uint64_t key = column_key(v, i);
-            if (key >= cut && bin(v) == b) {
-                const uint32_t at = atomicAdd(&sh.n, 1u);
-                if (at < kList) sh.key[at] = key;
+        const float from = (float)b, to = b == kBins - 1 ? NAN : (float)(b + 1);
+        for_groups<BF16, 4>(s, 0, cols, tid, kThreads, [&](const float (&v)[4], int i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float x = bin.at(v[j]);
+                if ((x >= from) & !(x >= to) & cut.keeps(v[j], i + j)) {
+                    const uint32_t at = atomicAdd(&sh.n, 1u);
+                    if (at < kList) sh.key[at] = column_key(v[j], i + j);
+                }
             }
         });
         __syncthreads();
         const int n = (int)min(sh.n, (uint32_t)kList + 1);
-        if (n <= kList) {
+        if (n > 0 && n <= kThreads) {
+            // each thread adds up what ranks before its column: the last one below the target is the cut
+            if (tid < n) sh.hist[tid] = weigh.fixed(key_score(sh.key[tid]));
+            __syncthreads();
+            uint64_t mine = ~0ull;
+            if (tid < n) {
+                mine = sh.key[tid];
+                uint64_t sum = before;
+                bool first = true;
+                for (int j = 0; j < n; ++j) {
+                    const bool better = sh.key[j] > mine;
+                    sum += better ? sh.hist[j] : 0;
+                    first &= !better;
+                }
+                if (!((double)sum < target) && !(first && before == 0)) mine = ~0ull;
+            }
+            const uint64_t key = ~block_max_u64(~mine, sh);
+            cut = Cut{key_score(key), key_index(key)};
+        } else if (n > 0 && n <= kList) {
             sort_keys(n, sh);
             // the last column whose sum before it is below the target
             for (int j = tid; j < n; j += kThreads) sh.hist[j] = weigh.fixed(key_score(sh.key[j]));
@@ -539,7 +636,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_rows_kernel(SampleArgs a) 
                 const int lo = lane * per, hi = min(n, lo + per);
                 uint64_t own = 0;
                 for (int j = lo; j < hi; ++j) own += sh.hist[j];
-                uint64_t run = before + wave_scan_u64(own, lane) - own;
+                uint64_t run = before + wave_scan_u64(own) - own;
                 int last = 0;
                 for (int j = lo; j < hi; ++j) {
                     if ((double)run < target) last = j;
@@ -550,27 +647,30 @@ __global__ __launch_bounds__(kThreads, 4) void sample_rows_kernel(SampleArgs a) 
                 if (lane == 0) sh.bin = (uint32_t)last;
             }
             __syncthreads();
-            cut = max(cut, sh.key[sh.bin]);
+            const uint64_t key = sh.key[sh.bin];
+            cut = Cut{key_score(key), key_index(key)};
         } else {
             cut = descend<BF16, true>(s, cols, cut, target, weigh, sh);
         }
     }
 
     // weights of the kept columns, summed per segment
-    constexpr int kStep = 64 * N;
-    const int64_t seg_len = ((int64_t)cols + kSegs * kStep - 1) / (kSegs * kStep) * kStep;
+    constexpr int kStep = 64 * N;  // at least four steps of a wave, so that their one reduction is shared
+    const int64_t seg_len = max(((int64_t)cols + kSegs * kStep - 1) / (kSegs * kStep), (int64_t)(cols > 16 * kStep * kWaves ? 4 : 1)) * kStep;
     const int n_segs = (int)(((int64_t)cols + seg_len - 1) / seg_len);
-    auto kept = [&](float v, int64_t i) -> double {
-        const double w = column_key(v, i) >= cut ? weigh(v) : 0.0;
-        return w >= r.min_p ? w : 0.0;
+    auto kept = [&](float v, int i) -> double {
+        const double w = weigh(v);
+        return (cut.keeps(v, i) & (w >= r.min_p)) ? w : 0.0;
     };
     __syncthreads();
     for (int g = wave; g < n_segs; g += kWaves) {
         double w = 0.0;
-        for_columns<BF16, 1>(s, g * seg_len, min((int64_t)cols, (g + 1) * seg_len), lane, 64,
-                             [&](float v, int64_t i) { w += kept(v, i); });
-        w = wave_sum_f64(w);
-        if (lane == 0) sh.seg[g + 1] = w;
+        for_groups<BF16, 1>(s, g * seg_len, min((int64_t)cols, (g + 1) * seg_len), lane, 64, [&](const float (&v)[4], int i) {
+            if (fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) >= cut.s)
+                w += (kept(v[0], i) + kept(v[1], i + 1)) + (kept(v[2], i + 2) + kept(v[3], i + 3));
+        });
+        w = wave_scan_f64(w);
+        if (lane == 63) sh.seg[g + 1] = w;
     }
     __syncthreads();
     if (tid < 64) {
@@ -578,7 +678,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_rows_kernel(SampleArgs a) 
         const int lo = lane * per, hi = min(n_segs, lo + per);
         double own = 0.0;
         for (int j = lo; j < hi; ++j) own += sh.seg[j + 1];
-        double run = wave_scan_f64(own, lane) - own;
+        double run = wave_scan_f64(own) - own;
         for (int j = lo; j < hi; ++j) sh.seg[j + 1] = run += sh.seg[j + 1];
         if (lane == 0) sh.seg[0] = 0.0;
     }
@@ -606,8 +706,8 @@ __global__ __launch_bounds__(kThreads, 4) void sample_rows_kernel(SampleArgs a) 
                 v.load_tail(s, i, end);
             double w[N], own = 0.0;
 #pragma unroll
-            for (int k = 0; k < N; ++k) own += w[k] = kept(v.v[k], i + k);
-            double c = run + wave_scan_f64(own, lane) - own;
+            for (int k = 0; k < N; ++k) own += w[k] = kept(v.v[k], (int)i + k);
+            double c = run + wave_scan_f64(own) - own;
             // this lane's first column past the target, or without one its last of any weight
             int at = -1, tail = -1;
             double wa = 0.0, wt = 0.0;
