@@ -2,11 +2,13 @@
 //
 // The kept columns are a prefix of the row's ranking (score descending, ties to the lower column), so they are
 // described by one 64-bit key (wave_topk.h's make_key): column i is kept iff its key is at least the cut.
-// A cut is found through a histogram of 2048 equal steps of the distance to the row's best score, of counts for
-// top_k and of weights for top_p: the bin in which the running sum reaches its target is gathered and sorted.
-// A top_k of at most ~kList columns gathers all of them, and what follows works on that list alone.  A bin that
-// holds more than kList columns (many equal scores, scores of very different sizes) is opened by a descent
-// over the 32 score bits instead.
+// top_k: with the row cut into kThreads x 4 classes of columns, the top_k-th largest of the classes' best scores is
+// at most the top_k-th largest score, so that what reaches it holds the top_k columns and hardly more: one
+// reading finds that bound, a second gathers a list in LDS, and everything else happens on that list.
+// top_p: a histogram of the distances to the best score, in 4096 equal steps, counts columns; a count times the weight
+// in the middle of its step is close enough to name the step in which the running weight reaches its target.  The next
+// reading sums the exact weights of everything better, and gathers that step's columns, among which the cut is
+// found.  What does not fit (a top_k of thousands, a step full of equal scores) takes a descent over the 32 score bits.
 //
 // Which column a given number draws depends on every weight before it, and with a million columns the borders
 // between columns lie 1e-6 of the total apart, so 24 bits are not enough: weights are computed in f64 and
@@ -21,8 +23,8 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
-constexpr int kBins = 2048;
-constexpr int kList = 2048;  // columns that are sorted in LDS
+constexpr int kBins = 4096;  // of 32 bits, or half as many of 64
+constexpr int kList = 2048;  // columns that are gathered in LDS
 constexpr int kSegs = 1024;  // column segments with sums of their own: a draw scans one of them
 
 struct SampleArgs {
@@ -159,6 +161,10 @@ struct Weigh {
         const double w = scaled(s, unit) + 4503599627370496.0;
         return (uint64_t)__double_as_longlong(w) & 0xfffffffffffffull;
     }
+    // the same, but at least 1 for a weight that f64 does not round to 0: a column that is kept can be drawn
+    __device__ __forceinline__ uint64_t fixed_kept(float s) const {
+        return max(fixed(s), (uint64_t)(scaled(s, 0) > 0.0 ? 1 : 0));
+    }
 };
 
 // ------------------------------------------------------------------------------------ wave and workgroup steps
@@ -207,13 +213,19 @@ __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
 }
 
 struct Shared {
-    uint64_t hist[kBins];
-    uint64_t key[kList];    // gathered columns
-    double w[kList];        // their weights, then the running sums of the kept ones
-    double seg[kSegs + 1];
+    union {
+        uint64_t wide[kBins / 2];
+        uint32_t count[kBins];
+    };
+    uint64_t key[kList];  // gathered columns
+    union {
+        double w[kList];  // their weights, then the running sums of the kept ones
+        double seg[kSegs + 1];
+    };
     uint64_t part[kWaves];
+    double dpart[kWaves];
     uint64_t below;
-    uint32_t bin, n;
+    uint32_t bin, bin2, n;
 };
 
 // sum / maximum over the workgroup, the same value in every thread
@@ -238,27 +250,38 @@ __device__ uint64_t block_max_u64(uint64_t v, Shared& sh) {
     return s;
 }
 
+__device__ double block_sum_f64(double v, Shared& sh) {
+    v = wave_scan_f64(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) sh.dpart[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double s = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) s += sh.dpart[i];
+    return s;
+}
+
 __device__ __forceinline__ void clear_hist(Shared& sh) {
     __syncthreads();
-    for (int j = threadIdx.x; j < kBins; j += kThreads) sh.hist[j] = 0;
+    for (int j = threadIdx.x; j < kBins / 2; j += kThreads) sh.wide[j] = 0;
     if (threadIdx.x == 0) sh.n = 0;
     __syncthreads();
 }
 
-// The bin in which the running sum of hist, from bin 0 on, reaches `target`: sum before it < target <= sum with
+// The bin in which the running sum of the histogram, from bin 0 on, reaches `target`: sum before it < target <= sum with
 // it; the last bin that holds anything if the whole falls short, bin 0 of an empty histogram.
 // -> sh.bin, sh.below = the sum before it
-__device__ void find_bin(double target, Shared& sh) {
-    constexpr int per = kBins / kThreads;
+template <typename C>
+__device__ void find_bin(const C* hist, double target, Shared& sh) {
+    constexpr int per = kBins * 4 / (int)sizeof(C) / kThreads;
     const int tid = threadIdx.x;
     if (tid == 0) {
         sh.bin = 0;
         sh.below = 0;
     }
     __syncthreads();
-    uint64_t h[per], own = 0;
-#pragma unroll
-    for (int j = 0; j < per; ++j) own += h[j] = sh.hist[tid * per + j];
+    uint64_t own = 0;
+    for (int j = 0; j < per; ++j) own += hist[tid * per + j];
     const uint64_t incl = wave_scan_u64(own);
     if ((tid & 63) == 63) sh.part[tid >> 6] = incl;
     __syncthreads();
@@ -269,16 +292,17 @@ __device__ void find_bin(double target, Shared& sh) {
         all += sh.part[w];
     }
     target = fmin(target, (double)all);
-#pragma unroll
-    for (int j = 0; j < per; ++j) {
-        const uint64_t next = run + h[j];
-        // the first bin that reaches it (a target of 0 or less: the first that holds anything)
-        if (h[j] && (double)next >= target && (run == 0 || (double)run < target)) {
-            sh.bin = (uint32_t)(tid * per + j);
-            sh.below = run;
+    // one thread holds it (with a target of 0 or less: the first bin that holds anything)
+    if (own && (double)(run + own) >= target && (run == 0 || (double)run < target))
+        for (int j = 0; j < per; ++j) {
+            const uint64_t h = hist[tid * per + j], next = run + h;
+            if (h && (double)next >= target) {
+                sh.bin = (uint32_t)(tid * per + j);
+                sh.below = run;
+                break;
+            }
+            run = next;
         }
-        run = next;
-    }
     __syncthreads();
 }
 
@@ -338,20 +362,16 @@ __device__ __forceinline__ double draw_number(const SampleArgs& a, int64_t row, 
     return fmin(fmax(u, 0.0), 1.0);
 }
 
-// one reading of the columns [lo, hi): the best one as a key (0 without one), and the lowest score above -1e30 (lower
-// ones are masks, and share the last bin)
-struct Top {
-    uint64_t best;
-    float low;
-};
+// v_med3 ignores NaN (so does the maximum, but the compiler first makes signalling NaN quiet: two instructions)
+__device__ __forceinline__ float max_of(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
+
+// the best of the columns [lo, hi) as a key, 0 without one
 template <bool BF16>
-__device__ __forceinline__ Top scan_top(const void* s, int64_t lo, int64_t hi, int me, int width) {
-    float best = -INFINITY, low = INFINITY;
+__device__ __forceinline__ uint64_t scan_best(const void* s, int64_t lo, int64_t hi, int me, int width) {
+    float best = kNone;
     int at = -1;
     for_groups<BF16, 4>(s, lo, hi, me, width, [&](const float (&v)[4], int i) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) low = fminf(low, v[j] > -1e30f ? v[j] : INFINITY);
-        if (fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) > best) {
+        if (max_of(max_of(v[0], v[1]), max_of(v[2], v[3])) > best) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 if (v[j] > best) {
@@ -360,7 +380,7 @@ __device__ __forceinline__ Top scan_top(const void* s, int64_t lo, int64_t hi, i
                 }
         }
     });
-    return Top{at < 0 ? 0ull : column_key(best, at), low};
+    return at < 0 ? 0ull : column_key(best, at);
 }
 
 // equal steps of the distance to the best score.  A score belongs to bin b < kBins - 1 iff b <= at(s) < b + 1,
@@ -393,11 +413,11 @@ __device__ Cut descend(const void* s, int cols, const Cut& cut, double target, c
             for (int j = 0; j < 4; ++j) {
                 const uint32_t k = score_key(v[j]);
                 if (cut.keeps(v[j], i + j) && (open == 32 || (k >> open) == (prefix >> open)))
-                    atomicAdd((unsigned long long*)&sh.hist[mask - ((k >> shift) & mask)],
+                    atomicAdd((unsigned long long*)&sh.wide[mask - ((k >> shift) & mask)],
                               (unsigned long long)(MASS ? weigh.fixed(v[j]) : 1ull));
             }
         });
-        find_bin(target - (double)above, sh);
+        find_bin(sh.wide, target - (double)above, sh);
         prefix |= (mask - sh.bin) << shift;
         above += sh.below;
     }
@@ -429,8 +449,54 @@ __device__ Cut descend(const void* s, int cols, const Cut& cut, double target, c
 }
 
 // sh.key[0, n) holds the row's best n columns, unsorted, n <= kList, at least min(top_k, live) of them: the
-// restrictions and the draws on that list
+// restrictions and the draws on that list, a column per thread.  A column's rank, the weight that ranks before it, and
+// the kept weight up to it in column order are sums over the list.
+__device__ void finish_short(const SampleArgs& a, int64_t row, const Row& r, int n, const Weigh& weigh, Shared& sh) {
+    const int tid = threadIdx.x;
+    const uint64_t mine = tid < n ? sh.key[tid] : 0;
+    const uint64_t w = tid < n ? weigh.fixed_kept(key_score(mine)) : 0;
+    if (tid < n) sh.wide[tid] = w;
+    __syncthreads();
+    int rank = 0;
+    uint64_t better = 0;
+    for (int j = 0; j < n; ++j) {
+        const bool b = sh.key[j] > mine;
+        rank += b;
+        better += b ? sh.wide[j] : 0;
+    }
+    bool keep = tid < n && rank < r.top_k;
+    if (r.top_p < 1.0) {
+        const double target = r.top_p * (double)block_sum_u64(keep ? w : 0, sh);
+        keep &= rank == 0 || (double)better < target;
+    }
+    keep &= (w > 0) & (weigh(key_score(mine)) >= r.min_p);
+    __syncthreads();
+    if (tid < n) sh.wide[tid] = keep ? w : 0;
+    __syncthreads();
+    uint64_t upto = 0, total = 0;
+    for (int j = 0; j < n; ++j) {
+        const uint64_t x = sh.wide[j];
+        total += x;
+        upto += (uint32_t)sh.key[j] >= (uint32_t)mine ? x : 0;  // the low half falls with the column
+    }
+    if (!keep) return;
+    const float prob = (float)(ldexp(weigh(key_score(mine)), weigh.unit) / (double)total);
+    for (int64_t j = 0; j < a.n_draws; ++j) {
+        const double target = draw_number(a, row, j) * (double)total;
+        // a number at the end of the range: the last column
+        if (((double)upto > target || upto == total) && (upto == w || (double)(upto - w) <= target)) {
+            a.out_idx[row * a.n_draws + j] = key_index(mine);
+            if (a.out_prob) a.out_prob[row * a.n_draws + j] = prob;
+        }
+    }
+}
+
+// the same for longer lists: sorted by rank, cut, and sorted by column
 __device__ void finish_list(const SampleArgs& a, int64_t row, const Row& r, int n, const Weigh& weigh, Shared& sh) {
+    if (n <= kThreads) {
+        finish_short(a, row, r, n, weigh, sh);
+        return;
+    }
     sort_keys(n, sh);
     n = (int)min((int64_t)n, r.top_k);
     for (int j = threadIdx.x; j < n; j += kThreads) sh.w[j] = weigh(key_score(sh.key[j]));
@@ -455,10 +521,10 @@ __device__ void finish_list(const SampleArgs& a, int64_t row, const Row& r, int 
         const uint64_t key = sh.key[j];
         const double w = weigh(key_score(key));
         // ~column descending = column ascending; the score rides along in the low half
-        sh.hist[j] = w >= r.min_p ? (uint64_t)(uint32_t)key << 32 | (uint32_t)(key >> 32) : 0ull;
+        sh.wide[j] = w >= r.min_p ? (uint64_t)(uint32_t)key << 32 | (uint32_t)(key >> 32) : 0ull;
     }
     __syncthreads();
-    for (int j = threadIdx.x; j < keep; j += kThreads) sh.key[j] = sh.hist[j];
+    for (int j = threadIdx.x; j < keep; j += kThreads) sh.key[j] = sh.wide[j];
     sort_keys(keep, sh);
     for (int j = threadIdx.x; j < keep; j += kThreads) {
         const uint64_t key = sh.key[j];
@@ -507,7 +573,7 @@ __device__ void draw_infinite(const SampleArgs& a, int64_t row, const Row& r, co
 }
 
 template <bool BF16>
-__global__ __launch_bounds__(kThreads, 4) void sample_rows_kernel(SampleArgs a) {
+__global__ __launch_bounds__(kThreads, 6) void sample_rows_kernel(SampleArgs a) {
     __shared__ Shared sh;
     constexpr int N = Vec<BF16>::N;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -517,38 +583,97 @@ __global__ __launch_bounds__(kThreads, 4) void sample_rows_kernel(SampleArgs a) 
     const int cols = (int)a.cols;
     const Row r = row_settings(a, row);
 
-    const Top mine = scan_top<BF16>(s, 0, cols, tid, kThreads);
-    const uint64_t best = block_max_u64(mine.best, sh);
-    if (best == 0 || !(r.T > 0.0) || r.top_k == 1) {
+    if (!(r.T > 0.0) || r.top_k == 1 || r.top_p <= 0.0) {
+        const uint64_t best = block_max_u64(scan_best<BF16>(s, 0, cols, tid, kThreads), sh);
         for (int64_t j = tid; j < a.n_draws; j += kThreads) {
             a.out_idx[row * a.n_draws + j] = best ? key_index(best) : -1;
             if (a.out_prob) a.out_prob[row * a.n_draws + j] = best ? 1.0f : 0.0f;
         }
         return;
     }
-    const float top = key_score(best);
+    float best[4] = {kNone, kNone, kNone, kNone}, low = INFINITY;
+    for_groups<BF16, 4>(s, 0, cols, tid, kThreads, [&](const float (&v)[4], int) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) best[j] = max_of(best[j], v[j]);
+        low = v[0] > -1e30f ? fminf(low, v[0]) : low;  // of a quarter of the columns: it only sets the bins' width
+    });
+    const float top = unord_f32((uint32_t)block_max_u64(ord_f32(max_of(max_of(best[0], best[1]), max_of(best[2], best[3]))), sh));
+    if (top == kNone) {
+        for (int64_t j = tid; j < a.n_draws; j += kThreads) {
+            a.out_idx[row * a.n_draws + j] = -1;
+            if (a.out_prob) a.out_prob[row * a.n_draws + j] = 0.0f;
+        }
+        return;
+    }
     if (top == INFINITY) {
         draw_infinite<BF16>(a, row, r, s, sh);
         return;
     }
+    low = unord_f32(~(uint32_t)block_max_u64((uint64_t)(~ord_f32(low)), sh));
+    const double range = fmax((double)top - (double)low, 0.0);
     const Weigh weigh(top, r.T, cols);
 
     Cut cut{kNone, -1};
     if (r.top_k > 0 && r.top_k < cols) {
-        const float low = unord_f32(~(uint32_t)block_max_u64((uint64_t)(~ord_f32(mine.low)), sh));
-        const Binning bin = make_binning(top, fmax((double)top - (double)low, 0.0));
+        // a list of the columns that reach the classes' bound
+        float to = NAN;  // all columns
+        Binning bin{top, 0.0f};
+        bool list = cols <= kList;
+        if (!list && r.top_k <= kList) {
+            float least = INFINITY;
+            uint64_t classes = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (best[j] > kNone) {
+                    ++classes;
+                    least = fminf(least, best[j]);
+                }
+            list = block_sum_u64(classes, sh) >= (uint64_t)r.top_k;
+            least = unord_f32(~(uint32_t)block_max_u64((uint64_t)(~ord_f32(least)), sh));
+            if (list) {
+                bin = make_binning(top, (double)top - (double)least);
+                clear_hist(sh);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (best[j] > kNone) atomicAdd(&sh.count[bin(best[j])], 1u);
+                __syncthreads();
+                find_bin(sh.count, (double)r.top_k, sh);
+                if (sh.bin < kBins - 1) to = (float)(sh.bin + 1);
+            }
+        }
+        if (list) {
+            __syncthreads();
+            if (tid == 0) sh.n = 0;
+            __syncthreads();
+            for_groups<BF16, 4>(s, 0, cols, tid, kThreads, [&](const float (&v)[4], int i) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (!(bin.at(v[j]) >= to) & (v[j] > kNone)) {
+                        const uint32_t at = atomicAdd(&sh.n, 1u);
+                        if (at < kList) sh.key[at] = column_key(v[j], i + j);
+                    }
+            });
+            __syncthreads();
+            if (sh.n <= kList) {
+                finish_list(a, row, r, (int)sh.n, weigh, sh);
+                return;
+            }
+        }
+        // the step of the top_k-th column
+        bin = make_binning(top, range);
         clear_hist(sh);
         for_groups<BF16, 2>(s, 0, cols, tid, kThreads, [&](const float (&v)[4], int) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (v[j] > kNone) atomicAdd((unsigned*)&sh.hist[bin(v[j])], 1u);
+                if (v[j] > kNone) atomicAdd(&sh.count[bin(v[j])], 1u);
         });
-        find_bin((double)r.top_k, sh);
+        __syncthreads();
+        find_bin(sh.count, (double)r.top_k, sh);
         const int b = (int)sh.bin;
-        const uint64_t before = sh.below, in_bin = sh.hist[b];
-        const bool list = before + in_bin <= kList;
-        if (list || in_bin <= kList) {
-            const float from = list ? -INFINITY : (float)b, to = b == kBins - 1 ? NAN : (float)(b + 1);
+        const uint64_t before = sh.below, in_bin = sh.count[b];
+        if (in_bin > 0 && in_bin <= kList) {
+            const float from = (float)b;
+            to = b == kBins - 1 ? NAN : (float)(b + 1);
             for_groups<BF16, 2>(s, 0, cols, tid, kThreads, [&](const float (&v)[4], int i) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -556,11 +681,6 @@ __global__ __launch_bounds__(kThreads, 4) void sample_rows_kernel(SampleArgs a) 
                     if ((x >= from) & !(x >= to) & (v[j] > kNone)) sh.key[atomicAdd(&sh.n, 1u)] = column_key(v[j], i + j);
                 }
             });
-            __syncthreads();
-            if (list) {
-                finish_list(a, row, r, (int)sh.n, weigh, sh);
-                return;
-            }
             sort_keys((int)in_bin, sh);
             const uint64_t key = sh.key[min((uint64_t)r.top_k - before, in_bin) - 1];
             cut = Cut{key_score(key), key_index(key)};
@@ -568,102 +688,149 @@ __global__ __launch_bounds__(kThreads, 4) void sample_rows_kernel(SampleArgs a) 
             cut = descend<BF16, false>(s, cols, cut, (double)r.top_k, weigh, sh);
         }
     }
+
+    constexpr int kStep = 64 * N;  // at least four steps of a wave in a segment, so that its one reduction is shared
+    const int64_t seg_len = max(((int64_t)cols + kSegs * kStep - 1) / (kSegs * kStep), (int64_t)(cols > 16 * kStep * kWaves ? 4 : 1)) * kStep;
+    const int n_segs = (int)(((int64_t)cols + seg_len - 1) / seg_len);
+    bool summed = false;
     if (r.top_p < 1.0) {
-        // a column of weight below (1 - p) Z / cols is never kept (all such together weigh less than the
-        // (1 - p) Z that are dropped), and Z >= 1; they share the last bin, summed in registers
-        const Binning bin = make_binning(top, fmin(r.T, 1e30) * (log((double)cols / (1.0 - r.top_p)) + 1e-3));
+        // A column of weight below (1 - p) Z / cols is never kept (all such together weigh less than the (1 - p) Z that are
+        // dropped), and Z >= 1.  What lies e^-12 below that shares the last bin, and adds at most e^-12 (1 - p) to the sums
+        // here.
+        const Binning bin = make_binning(top, fmin(range, fmin(r.T, 1e30) * (log((double)cols / (1.0 - r.top_p)) + 12.0)));
         const bool all = cut.s == kNone;
         clear_hist(sh);
-        uint64_t rest = 0;
-        for_groups<BF16, 1>(s, 0, cols, tid, kThreads, [&](const float (&v)[4], int i) {
+        for_groups<BF16, 2>(s, 0, cols, tid, kThreads, [&](const float (&v)[4], int i) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                if (!all && !cut.keeps(v[j], i + j)) continue;
-                const uint64_t w = weigh.fixed(v[j]);
                 const int b = bin(v[j]);
-                if (b < kBins - 1)
-                    atomicAdd((unsigned long long*)&sh.hist[b], (unsigned long long)w);
-                else
-                    rest += w;
+                if ((all | cut.keeps(v[j], i + j)) & (b < kBins - 1)) atomicAdd(&sh.count[b], 1u);
             }
         });
-        if (rest) atomicAdd((unsigned long long*)&sh.hist[kBins - 1], (unsigned long long)rest);
         __syncthreads();
-        uint64_t sum = 0;
-        for (int j = tid; j < kBins; j += kThreads) sum += sh.hist[j];
-        const double target = r.top_p * (double)block_sum_u64(sum, sh);
-        find_bin(target, sh);
-        const int b = (int)sh.bin;
-        const uint64_t before = sh.below;
-        const float from = (float)b, to = b == kBins - 1 ? NAN : (float)(b + 1);
-        for_groups<BF16, 4>(s, 0, cols, tid, kThreads, [&](const float (&v)[4], int i) {
+        // the steps in which the running weight is within 1e-4 of its target: the middle's weight stands for a step's, an
+        // error of its width squared (of T) / 24, 2e-6 at most for a range of 28 T
+        constexpr int per = kBins / kThreads;
+        const double wide = bin.inv > 0.0f ? 1.0 / (double)bin.inv : 0.0;
+        double own = 0.0;
+        for (int j = 0; j < per; ++j) {
+            const uint32_t c = sh.count[tid * per + j];
+            if (c) own += (double)c * weigh((float)((double)top - wide * (tid * per + j + 0.5)));
+        }
+        const double incl = wave_scan_f64(own);
+        if (lane == 63) sh.dpart[wave] = incl;
+        if (tid == 0) {
+            sh.bin = kBins - 1;
+            sh.bin2 = kBins - 1;
+        }
+        __syncthreads();
+        double run = incl - own, sum = 0.0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float x = bin.at(v[j]);
-                if ((x >= from) & !(x >= to) & cut.keeps(v[j], i + j)) {
-                    const uint32_t at = atomicAdd(&sh.n, 1u);
-                    if (at < kList) sh.key[at] = column_key(v[j], i + j);
-                }
-            }
-        });
+        for (int w = 0; w < kWaves; ++w) {
+            if (w < wave) run += sh.dpart[w];
+            sum += sh.dpart[w];
+        }
+        const double t1 = (r.top_p - 1e-4) * sum, t2 = fmin(r.top_p + 1e-4, 1.0 - 1e-13) * sum;
+        uint32_t f1 = kBins - 1, f2 = kBins - 1;
+        for (int j = 0; j < per; ++j) {
+            const int b = tid * per + j;
+            const uint32_t c = sh.count[b];
+            if (!c) continue;
+            const double next = run + (double)c * weigh((float)((double)top - wide * (b + 0.5)));
+            if (next >= t1) f1 = min(f1, (uint32_t)b);
+            if (next >= t2) f2 = min(f2, (uint32_t)b);
+            run = next;
+        }
+        if (f1 < kBins - 1) atomicMin(&sh.bin, f1);
+        if (f2 < kBins - 1) atomicMin(&sh.bin2, f2);
         __syncthreads();
-        const int n = (int)min(sh.n, (uint32_t)kList + 1);
-        if (n > 0 && n <= kThreads) {
+        const int b1 = (int)sh.bin, b2 = (int)sh.bin2;
+        uint64_t inside = 0;
+        for (int j = 0; j < per; ++j) {
+            const int b = tid * per + j;
+            if (b >= b1 && b <= b2) inside += sh.count[b];
+        }
+        inside = block_sum_u64(inside, sh);
+        if (b2 < kBins - 1 && inside > 0 && inside <= kList) {
+            // exact weights: all, and per segment of the better steps; the columns of [b1, b2] are gathered
+            const float from = (float)b1, to = (float)(b2 + 1);
+            double z = 0.0, better = 0.0;
+            for (int g = wave; g < n_segs; g += kWaves) {
+                double w = 0.0;
+                for_groups<BF16, 1>(s, g * seg_len, min((int64_t)cols, (g + 1) * seg_len), lane, 64, [&](const float (&v)[4], int i) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        double x = weigh(v[j]);
+                        const float d = bin.at(v[j]);
+                        const bool ok = all | cut.keeps(v[j], i + j);
+                        z += ok ? x : 0.0;
+                        x = d < from ? x : 0.0;
+                        better += x;
+                        w += x >= r.min_p ? x : 0.0;
+                        if (!(d < from) & (d < to) & ok) {
+                            const uint32_t at = atomicAdd(&sh.n, 1u);
+                            if (at < kList) sh.key[at] = column_key(v[j], i + j);
+                        }
+                    }
+                });
+                w = wave_scan_f64(w);
+                if (lane == 63) sh.seg[g + 1] = w;
+            }
+            z = block_sum_f64(z, sh);
+            better = block_sum_f64(better, sh);
+            const double target = r.top_p * z;
+            const int n = (int)min(sh.n, (uint32_t)kList);
             // each thread adds up what ranks before its column: the last one below the target is the cut
-            if (tid < n) sh.hist[tid] = weigh.fixed(key_score(sh.key[tid]));
+            for (int j = tid; j < n; j += kThreads) sh.wide[j] = weigh.fixed(key_score(sh.key[j]));
             __syncthreads();
-            uint64_t mine = ~0ull;
-            if (tid < n) {
-                mine = sh.key[tid];
-                uint64_t sum = before;
-                bool first = true;
+            uint64_t last = 0, whole = 0;  // of the keys below the target the smallest, complemented
+            for (int c = tid; c < n; c += kThreads) {
+                const uint64_t mine = sh.key[c];
+                uint64_t sum_before = 0;
+                whole = 0;
                 for (int j = 0; j < n; ++j) {
-                    const bool better = sh.key[j] > mine;
-                    sum += better ? sh.hist[j] : 0;
-                    first &= !better;
+                    const uint64_t x = sh.wide[j];
+                    whole += x;
+                    sum_before += sh.key[j] > mine ? x : 0;
                 }
-                if (!((double)sum < target) && !(first && before == 0)) mine = ~0ull;
+                if (better + ldexp((double)sum_before, -weigh.unit) < target) last = max(last, ~mine);
             }
-            const uint64_t key = ~block_max_u64(~mine, sh);
-            cut = Cut{key_score(key), key_index(key)};
-        } else if (n > 0 && n <= kList) {
-            sort_keys(n, sh);
-            // the last column whose sum before it is below the target
-            for (int j = tid; j < n; j += kThreads) sh.hist[j] = weigh.fixed(key_score(sh.key[j]));
-            __syncthreads();
-            if (tid < 64) {
-                constexpr int per = kList / 64;
-                const int lo = lane * per, hi = min(n, lo + per);
-                uint64_t own = 0;
-                for (int j = lo; j < hi; ++j) own += sh.hist[j];
-                uint64_t run = before + wave_scan_u64(own) - own;
-                int last = 0;
-                for (int j = lo; j < hi; ++j) {
-                    if ((double)run < target) last = j;
-                    run += sh.hist[j];
+            const uint64_t key = ~block_max_u64(last, sh);
+            whole = block_max_u64(whole, sh);
+            // the step was the right one
+            if (better < target && better + ldexp((double)whole, -weigh.unit) >= target) {
+                cut = Cut{key_score(key), key_index(key)};
+                __syncthreads();
+                for (int j = tid; j < n_segs; j += kThreads) sh.wide[j] = 0;
+                __syncthreads();
+                for (int j = tid; j < n; j += kThreads) {
+                    const uint64_t k = sh.key[j];
+                    const float v = key_score(k);
+                    if (k >= key && weigh(v) >= r.min_p)
+                        atomicAdd((unsigned long long*)&sh.wide[key_index(k) / seg_len], (unsigned long long)weigh.fixed_kept(v));
                 }
+                __syncthreads();
+                for (int j = tid; j < n_segs; j += kThreads) sh.seg[j + 1] += ldexp((double)sh.wide[j], -weigh.unit);
+                summed = true;
+            }
+        }
+        if (!summed) {
+            uint64_t sum_fixed = 0;
+            for_groups<BF16, 1>(s, 0, cols, tid, kThreads, [&](const float (&v)[4], int i) {
 #pragma unroll
-                for (int o = 32; o > 0; o >>= 1) last = max(last, __shfl_xor(last, o, 64));
-                if (lane == 0) sh.bin = (uint32_t)last;
-            }
-            __syncthreads();
-            const uint64_t key = sh.key[sh.bin];
-            cut = Cut{key_score(key), key_index(key)};
-        } else {
-            cut = descend<BF16, true>(s, cols, cut, target, weigh, sh);
+                for (int j = 0; j < 4; ++j) sum_fixed += cut.keeps(v[j], i + j) ? weigh.fixed(v[j]) : 0;
+            });
+            cut = descend<BF16, true>(s, cols, cut, r.top_p * (double)block_sum_u64(sum_fixed, sh), weigh, sh);
         }
     }
 
     // weights of the kept columns, summed per segment
-    constexpr int kStep = 64 * N;  // at least four steps of a wave, so that their one reduction is shared
-    const int64_t seg_len = max(((int64_t)cols + kSegs * kStep - 1) / (kSegs * kStep), (int64_t)(cols > 16 * kStep * kWaves ? 4 : 1)) * kStep;
-    const int n_segs = (int)(((int64_t)cols + seg_len - 1) / seg_len);
     auto kept = [&](float v, int i) -> double {
         const double w = weigh(v);
         return (cut.keeps(v, i) & (w >= r.min_p)) ? w : 0.0;
     };
     __syncthreads();
-    for (int g = wave; g < n_segs; g += kWaves) {
+    for (int g = summed ? n_segs : wave; g < n_segs; g += kWaves) {
         double w = 0.0;
         for_groups<BF16, 1>(s, g * seg_len, min((int64_t)cols, (g + 1) * seg_len), lane, 64, [&](const float (&v)[4], int i) {
             if (fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) >= cut.s)
