@@ -572,277 +572,253 @@ __device__ void draw_infinite(const SampleArgs& a, int64_t row, const Row& r, co
     }
 }
 
+// The columns' segments: `len` columns each, a multiple of a wave's step and at least four of those in a long row (so
+// that their one reduction is shared), and at most kSegs of them
+struct Segments {
+    int64_t len;
+    int n;
+    __host__ __device__ explicit Segments(int64_t cols) {
+        constexpr int64_t step = 64 * 4;
+        const int64_t least = (cols + kSegs * step - 1) / (kSegs * step);
+        len = (cols > 16 * step * kWaves && least < 4 ? 4 : least) * step;
+        n = (int)((cols + len - 1) / len);
+    }
+};
+
+// what the first reading finds: the best scores of the thread's four classes of columns, and a low score that sets the
+// width of the steps (of a quarter of the columns, masks of the type's lowest value left out)
+struct Maxima {
+    float best[4], low;
+};
 template <bool BF16>
-__global__ __launch_bounds__(kThreads, 6) void sample_rows_kernel(SampleArgs a) {
-    __shared__ Shared sh;
-    constexpr int N = Vec<BF16>::N;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t row = blockIdx.x;
-    const void* s = BF16 ? (const void*)(static_cast<const uint16_t*>(a.S) + row * a.ld)
-                         : (const void*)(static_cast<const float*>(a.S) + row * a.ld);
-    const int cols = (int)a.cols;
-    const Row r = row_settings(a, row);
-
-    if (!(r.T > 0.0) || r.top_k == 1 || r.top_p <= 0.0) {
-        const uint64_t best = block_max_u64(scan_best<BF16>(s, 0, cols, tid, kThreads), sh);
-        for (int64_t j = tid; j < a.n_draws; j += kThreads) {
-            a.out_idx[row * a.n_draws + j] = best ? key_index(best) : -1;
-            if (a.out_prob) a.out_prob[row * a.n_draws + j] = best ? 1.0f : 0.0f;
-        }
-        return;
-    }
-    float best[4] = {kNone, kNone, kNone, kNone}, low = INFINITY;
-    for_groups<BF16, 4>(s, 0, cols, tid, kThreads, [&](const float (&v)[4], int) {
+__device__ __forceinline__ Maxima scan_maxima(const void* s, int64_t lo, int64_t hi) {
+    Maxima m{{kNone, kNone, kNone, kNone}, INFINITY};
+    for_groups<BF16, 4>(s, lo, hi, threadIdx.x, kThreads, [&](const float (&v)[4], int) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) best[j] = max_of(best[j], v[j]);
-        low = v[0] > -1e30f ? fminf(low, v[0]) : low;  // of a quarter of the columns: it only sets the bins' width
+        for (int j = 0; j < 4; ++j) m.best[j] = max_of(m.best[j], v[j]);
+        m.low = v[0] > -1e30f ? fminf(m.low, v[0]) : m.low;
     });
-    const float top = unord_f32((uint32_t)block_max_u64(ord_f32(max_of(max_of(best[0], best[1]), max_of(best[2], best[3]))), sh));
-    if (top == kNone) {
-        for (int64_t j = tid; j < a.n_draws; j += kThreads) {
-            a.out_idx[row * a.n_draws + j] = -1;
-            if (a.out_prob) a.out_prob[row * a.n_draws + j] = 0.0f;
+    return m;
+}
+__device__ __forceinline__ uint64_t order_of(float f) { return ord_f32(f); }
+__device__ __forceinline__ uint64_t reverse_order_of(float f) { return (uint32_t)~ord_f32(f); }
+__device__ __forceinline__ float of_reverse_order(uint64_t o) { return unord_f32(~(uint32_t)o); }
+
+// a score that at least k of the workgroup's classes reach, so at least k columns do; kNone without k classes
+__device__ float class_bound(const Maxima& m, int64_t k, Shared& sh) {
+    float least = INFINITY, most = kNone;
+    uint64_t classes = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (m.best[j] > kNone) {
+            ++classes;
+            least = fminf(least, m.best[j]);
+            most = max_of(most, m.best[j]);
         }
-        return;
-    }
-    if (top == INFINITY) {
-        draw_infinite<BF16>(a, row, r, s, sh);
-        return;
-    }
-    low = unord_f32(~(uint32_t)block_max_u64((uint64_t)(~ord_f32(low)), sh));
+    if (block_sum_u64(classes, sh) < (uint64_t)k) return kNone;
+    least = of_reverse_order(block_max_u64(reverse_order_of(least), sh));
+    most = unord_f32((uint32_t)block_max_u64(order_of(most), sh));
+    const Binning bin = make_binning(most, (double)most - (double)least);
+    clear_hist(sh);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (m.best[j] > kNone) atomicAdd(&sh.count[bin(m.best[j])], 1u);
+    __syncthreads();
+    find_bin(sh.count, (double)k, sh);
+    // the least class at or before that bin
+    float bound = INFINITY;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (m.best[j] > kNone && bin(m.best[j]) <= (int)sh.bin) bound = fminf(bound, m.best[j]);
+    return of_reverse_order(block_max_u64(reverse_order_of(bound), sh));
+}
+
+// the columns of [lo, hi) that `take` names go to keys[0, kList), counted in n beyond that
+template <bool BF16, typename Take>
+__device__ __forceinline__ void gather(const void* s, int64_t lo, int64_t hi, uint64_t* keys, uint32_t* n, Take take) {
+    for_groups<BF16, 4>(s, lo, hi, threadIdx.x, kThreads, [&](const float (&v)[4], int i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (take(v[j], i + j)) {
+                const uint32_t at = atomicAdd(n, 1u);
+                if (at < kList) keys[at] = column_key(v[j], i + j);
+            }
+    });
+}
+
+// steps of the distance to the best score for top_p.  A column of weight below (1 - p) Z / cols is never kept (all such
+// together weigh less than the (1 - p) Z that are dropped), and Z >= 1.  What lies e^-12 below that shares the last step,
+// and adds at most e^-12 (1 - p) to the sums.
+__device__ __forceinline__ Binning mass_binning(float top, float low, const Row& r, int64_t cols) {
     const double range = fmax((double)top - (double)low, 0.0);
-    const Weigh weigh(top, r.T, cols);
+    return make_binning(top, fmin(range, fmin(r.T, 1e30) * (log((double)cols / (1.0 - r.top_p)) + 12.0)));
+}
 
-    Cut cut{kNone, -1};
-    if (r.top_k > 0 && r.top_k < cols) {
-        // a list of the columns that reach the classes' bound
-        float to = NAN;  // all columns
-        Binning bin{top, 0.0f};
-        bool list = cols <= kList;
-        if (!list && r.top_k <= kList) {
-            float least = INFINITY;
-            uint64_t classes = 0;
+// counts of the columns [lo, hi) that the cut keeps, without the last step, into sh.count
+template <bool BF16>
+__device__ __forceinline__ void count_steps(const void* s, int64_t lo, int64_t hi, const Binning& bin, const Cut& cut, Shared& sh) {
+    const bool all = cut.s == kNone;
+    for_groups<BF16, 2>(s, lo, hi, threadIdx.x, kThreads, [&](const float (&v)[4], int i) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (best[j] > kNone) {
-                    ++classes;
-                    least = fminf(least, best[j]);
-                }
-            list = block_sum_u64(classes, sh) >= (uint64_t)r.top_k;
-            least = unord_f32(~(uint32_t)block_max_u64((uint64_t)(~ord_f32(least)), sh));
-            if (list) {
-                bin = make_binning(top, (double)top - (double)least);
-                clear_hist(sh);
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (best[j] > kNone) atomicAdd(&sh.count[bin(best[j])], 1u);
-                __syncthreads();
-                find_bin(sh.count, (double)r.top_k, sh);
-                if (sh.bin < kBins - 1) to = (float)(sh.bin + 1);
-            }
+        for (int j = 0; j < 4; ++j) {
+            const int b = bin(v[j]);
+            if ((all | cut.keeps(v[j], i + j)) & (b < kBins - 1)) atomicAdd(&sh.count[b], 1u);
         }
-        if (list) {
-            __syncthreads();
-            if (tid == 0) sh.n = 0;
-            __syncthreads();
-            for_groups<BF16, 4>(s, 0, cols, tid, kThreads, [&](const float (&v)[4], int i) {
+    });
+}
+
+// The steps [first, last] in which the running weight of sh.count is within 1e-4 of top_p of the whole, and the columns in
+// them.  The weight in a step's middle stands for all of it, an error of the step's width (in T) squared / 24, 2e-6 at
+// most for a range of 28 T.
+struct Window {
+    int first, last;
+    uint64_t columns;
+    float from, to;
+    __device__ __forceinline__ bool usable() const { return last < kBins - 1 && columns > 0 && columns <= kList; }
+};
+__device__ Window mass_window(const Binning& bin, float top, double top_p, const Weigh& weigh, Shared& sh) {
+    constexpr int per = kBins / kThreads;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const double wide = 1.0 / (double)bin.inv;
+    auto step_weight = [&](int b) { return (double)sh.count[b] * weigh((float)((double)top - wide * (b + 0.5))); };
+    double own = 0.0;
+    for (int j = 0; j < per; ++j)
+        if (sh.count[tid * per + j]) own += step_weight(tid * per + j);
+    const double incl = wave_scan_f64(own);
+    __syncthreads();
+    if (lane == 63) sh.dpart[wave] = incl;
+    if (tid == 0) sh.bin = sh.bin2 = kBins - 1;
+    __syncthreads();
+    double run = incl - own, sum = 0.0;
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (!(bin.at(v[j]) >= to) & (v[j] > kNone)) {
-                        const uint32_t at = atomicAdd(&sh.n, 1u);
-                        if (at < kList) sh.key[at] = column_key(v[j], i + j);
-                    }
-            });
-            __syncthreads();
-            if (sh.n <= kList) {
-                finish_list(a, row, r, (int)sh.n, weigh, sh);
-                return;
-            }
-        }
-        // the step of the top_k-th column
-        bin = make_binning(top, range);
-        clear_hist(sh);
-        for_groups<BF16, 2>(s, 0, cols, tid, kThreads, [&](const float (&v)[4], int) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (v[j] > kNone) atomicAdd(&sh.count[bin(v[j])], 1u);
-        });
-        __syncthreads();
-        find_bin(sh.count, (double)r.top_k, sh);
-        const int b = (int)sh.bin;
-        const uint64_t before = sh.below, in_bin = sh.count[b];
-        if (in_bin > 0 && in_bin <= kList) {
-            const float from = (float)b;
-            to = b == kBins - 1 ? NAN : (float)(b + 1);
-            for_groups<BF16, 2>(s, 0, cols, tid, kThreads, [&](const float (&v)[4], int i) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float x = bin.at(v[j]);
-                    if ((x >= from) & !(x >= to) & (v[j] > kNone)) sh.key[atomicAdd(&sh.n, 1u)] = column_key(v[j], i + j);
-                }
-            });
-            sort_keys((int)in_bin, sh);
-            const uint64_t key = sh.key[min((uint64_t)r.top_k - before, in_bin) - 1];
-            cut = Cut{key_score(key), key_index(key)};
-        } else {
-            cut = descend<BF16, false>(s, cols, cut, (double)r.top_k, weigh, sh);
-        }
+    for (int w = 0; w < kWaves; ++w) {
+        if (w < wave) run += sh.dpart[w];
+        sum += sh.dpart[w];
     }
+    const double t1 = (top_p - 1e-4) * sum, t2 = fmin(top_p + 1e-4, 1.0 - 1e-13) * sum;
+    uint32_t f1 = kBins - 1, f2 = kBins - 1;
+    for (int j = 0; j < per; ++j) {
+        const int b = tid * per + j;
+        if (!sh.count[b]) continue;
+        run += step_weight(b);
+        if (run >= t1) f1 = min(f1, (uint32_t)b);
+        if (run >= t2) f2 = min(f2, (uint32_t)b);
+    }
+    if (f1 < kBins - 1) atomicMin(&sh.bin, f1);
+    if (f2 < kBins - 1) atomicMin(&sh.bin2, f2);
+    __syncthreads();
+    Window w{(int)sh.bin, (int)sh.bin2, 0, (float)sh.bin, (float)(sh.bin2 + 1)};
+    uint64_t inside = 0;
+    for (int j = 0; j < per; ++j) {
+        const int b = tid * per + j;
+        if (b >= w.first && b <= w.last) inside += sh.count[b];
+    }
+    w.columns = block_sum_u64(inside, sh);
+    return w;
+}
 
-    constexpr int kStep = 64 * N;  // at least four steps of a wave in a segment, so that its one reduction is shared
-    const int64_t seg_len = max(((int64_t)cols + kSegs * kStep - 1) / (kSegs * kStep), (int64_t)(cols > 16 * kStep * kWaves ? 4 : 1)) * kStep;
-    const int n_segs = (int)(((int64_t)cols + seg_len - 1) / seg_len);
-    bool summed = false;
-    if (r.top_p < 1.0) {
-        // A column of weight below (1 - p) Z / cols is never kept (all such together weigh less than the (1 - p) Z that are
-        // dropped), and Z >= 1.  What lies e^-12 below that shares the last bin, and adds at most e^-12 (1 - p) to the sums
-        // here.
-        const Binning bin = make_binning(top, fmin(range, fmin(r.T, 1e30) * (log((double)cols / (1.0 - r.top_p)) + 12.0)));
-        const bool all = cut.s == kNone;
-        clear_hist(sh);
-        for_groups<BF16, 2>(s, 0, cols, tid, kThreads, [&](const float (&v)[4], int i) {
+// One reading of the segments [g0, g1) with exact weights: z = all that the cut keeps, better = what lies before the
+// window, seg[g + 1] = of that what min_p keeps.  The window's columns are gathered.  z and better of this lane.
+template <bool BF16>
+__device__ __forceinline__ void sum_window(const void* s, int64_t cols, const Segments& segs, int g0, int g1, const Binning& bin,
+                                           const Window& win, const Cut& cut, const Weigh& weigh, double min_p, double* seg,
+                                           uint64_t* keys, uint32_t* n, double& z, double& better) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const bool all = cut.s == kNone;
+    z = better = 0.0;
+    for (int g = g0 + wave; g < g1; g += kWaves) {
+        double w = 0.0;
+        for_groups<BF16, 1>(s, g * segs.len, min(cols, (g + 1) * segs.len), lane, 64, [&](const float (&v)[4], int i) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int b = bin(v[j]);
-                if ((all | cut.keeps(v[j], i + j)) & (b < kBins - 1)) atomicAdd(&sh.count[b], 1u);
-            }
-        });
-        __syncthreads();
-        // the steps in which the running weight is within 1e-4 of its target: the middle's weight stands for a step's, an
-        // error of its width squared (of T) / 24, 2e-6 at most for a range of 28 T
-        constexpr int per = kBins / kThreads;
-        const double wide = bin.inv > 0.0f ? 1.0 / (double)bin.inv : 0.0;
-        double own = 0.0;
-        for (int j = 0; j < per; ++j) {
-            const uint32_t c = sh.count[tid * per + j];
-            if (c) own += (double)c * weigh((float)((double)top - wide * (tid * per + j + 0.5)));
-        }
-        const double incl = wave_scan_f64(own);
-        if (lane == 63) sh.dpart[wave] = incl;
-        if (tid == 0) {
-            sh.bin = kBins - 1;
-            sh.bin2 = kBins - 1;
-        }
-        __syncthreads();
-        double run = incl - own, sum = 0.0;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            if (w < wave) run += sh.dpart[w];
-            sum += sh.dpart[w];
-        }
-        const double t1 = (r.top_p - 1e-4) * sum, t2 = fmin(r.top_p + 1e-4, 1.0 - 1e-13) * sum;
-        uint32_t f1 = kBins - 1, f2 = kBins - 1;
-        for (int j = 0; j < per; ++j) {
-            const int b = tid * per + j;
-            const uint32_t c = sh.count[b];
-            if (!c) continue;
-            const double next = run + (double)c * weigh((float)((double)top - wide * (b + 0.5)));
-            if (next >= t1) f1 = min(f1, (uint32_t)b);
-            if (next >= t2) f2 = min(f2, (uint32_t)b);
-            run = next;
-        }
-        if (f1 < kBins - 1) atomicMin(&sh.bin, f1);
-        if (f2 < kBins - 1) atomicMin(&sh.bin2, f2);
-        __syncthreads();
-        const int b1 = (int)sh.bin, b2 = (int)sh.bin2;
-        uint64_t inside = 0;
-        for (int j = 0; j < per; ++j) {
-            const int b = tid * per + j;
-            if (b >= b1 && b <= b2) inside += sh.count[b];
-        }
-        inside = block_sum_u64(inside, sh);
-        if (b2 < kBins - 1 && inside > 0 && inside <= kList) {
-            // exact weights: all, and per segment of the better steps; the columns of [b1, b2] are gathered
-            const float from = (float)b1, to = (float)(b2 + 1);
-            double z = 0.0, better = 0.0;
-            for (int g = wave; g < n_segs; g += kWaves) {
-                double w = 0.0;
-                for_groups<BF16, 1>(s, g * seg_len, min((int64_t)cols, (g + 1) * seg_len), lane, 64, [&](const float (&v)[4], int i) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        double x = weigh(v[j]);
-                        const float d = bin.at(v[j]);
-                        const bool ok = all | cut.keeps(v[j], i + j);
-                        z += ok ? x : 0.0;
-                        x = d < from ? x : 0.0;
-                        better += x;
-                        w += x >= r.min_p ? x : 0.0;
-                        if (!(d < from) & (d < to) & ok) {
-                            const uint32_t at = atomicAdd(&sh.n, 1u);
-                            if (at < kList) sh.key[at] = column_key(v[j], i + j);
-                        }
-                    }
-                });
-                w = wave_scan_f64(w);
-                if (lane == 63) sh.seg[g + 1] = w;
-            }
-            z = block_sum_f64(z, sh);
-            better = block_sum_f64(better, sh);
-            const double target = r.top_p * z;
-            const int n = (int)min(sh.n, (uint32_t)kList);
-            // each thread adds up what ranks before its column: the last one below the target is the cut
-            for (int j = tid; j < n; j += kThreads) sh.wide[j] = weigh.fixed(key_score(sh.key[j]));
-            __syncthreads();
-            uint64_t last = 0, whole = 0;  // of the keys below the target the smallest, complemented
-            for (int c = tid; c < n; c += kThreads) {
-                const uint64_t mine = sh.key[c];
-                uint64_t sum_before = 0;
-                whole = 0;
-                for (int j = 0; j < n; ++j) {
-                    const uint64_t x = sh.wide[j];
-                    whole += x;
-                    sum_before += sh.key[j] > mine ? x : 0;
+                double x = weigh(v[j]);
+                const float d = bin.at(v[j]);
+                const bool ok = all | cut.keeps(v[j], i + j);
+                z += ok ? x : 0.0;
+                x = d < win.from ? x : 0.0;
+                better += x;
+                w += x >= min_p ? x : 0.0;
+                if (!(d < win.from) & (d < win.to) & ok) {
+                    const uint32_t at = atomicAdd(n, 1u);
+                    if (at < kList) keys[at] = column_key(v[j], i + j);
                 }
-                if (better + ldexp((double)sum_before, -weigh.unit) < target) last = max(last, ~mine);
             }
-            const uint64_t key = ~block_max_u64(last, sh);
-            whole = block_max_u64(whole, sh);
-            // the step was the right one
-            if (better < target && better + ldexp((double)whole, -weigh.unit) >= target) {
-                cut = Cut{key_score(key), key_index(key)};
-                __syncthreads();
-                for (int j = tid; j < n_segs; j += kThreads) sh.wide[j] = 0;
-                __syncthreads();
-                for (int j = tid; j < n; j += kThreads) {
-                    const uint64_t k = sh.key[j];
-                    const float v = key_score(k);
-                    if (k >= key && weigh(v) >= r.min_p)
-                        atomicAdd((unsigned long long*)&sh.wide[key_index(k) / seg_len], (unsigned long long)weigh.fixed_kept(v));
-                }
-                __syncthreads();
-                for (int j = tid; j < n_segs; j += kThreads) sh.seg[j + 1] += ldexp((double)sh.wide[j], -weigh.unit);
-                summed = true;
-            }
-        }
-        if (!summed) {
-            uint64_t sum_fixed = 0;
-            for_groups<BF16, 1>(s, 0, cols, tid, kThreads, [&](const float (&v)[4], int i) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) sum_fixed += cut.keeps(v[j], i + j) ? weigh.fixed(v[j]) : 0;
-            });
-            cut = descend<BF16, true>(s, cols, cut, r.top_p * (double)block_sum_u64(sum_fixed, sh), weigh, sh);
-        }
-    }
-
-    // weights of the kept columns, summed per segment
-    auto kept = [&](float v, int i) -> double {
-        const double w = weigh(v);
-        return (cut.keeps(v, i) & (w >= r.min_p)) ? w : 0.0;
-    };
-    __syncthreads();
-    for (int g = summed ? n_segs : wave; g < n_segs; g += kWaves) {
-        double w = 0.0;
-        for_groups<BF16, 1>(s, g * seg_len, min((int64_t)cols, (g + 1) * seg_len), lane, 64, [&](const float (&v)[4], int i) {
-            if (fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) >= cut.s)
-                w += (kept(v[0], i) + kept(v[1], i + 1)) + (kept(v[2], i + 2) + kept(v[3], i + 3));
         });
         w = wave_scan_f64(w);
-        if (lane == 63) sh.seg[g + 1] = w;
+        if (lane == 63) seg[g + 1] = w;
     }
+}
+
+// The cut of top_p among the window's columns sh.key[0, n), and their kept weights added to the segments.  False if the
+// exact sums show that the cut lies elsewhere.
+__device__ bool resolve_window(int n, double z, double better, const Row& r, const Segments& segs, const Weigh& weigh, Cut& cut, Shared& sh) {
+    const int tid = threadIdx.x;
+    const double target = r.top_p * z;
+    for (int j = tid; j < n; j += kThreads) sh.wide[j] = weigh.fixed(key_score(sh.key[j]));
+    __syncthreads();
+    // each thread adds up what ranks before its columns: the last one below the target is the cut
+    uint64_t last = 0, whole = 0;  // of the keys below the target the smallest, complemented
+    for (int c = tid; c < n; c += kThreads) {
+        const uint64_t mine = sh.key[c];
+        uint64_t sum = 0;
+        whole = 0;
+        for (int j = 0; j < n; ++j) {
+            const uint64_t x = sh.wide[j];
+            whole += x;
+            sum += sh.key[j] > mine ? x : 0;
+        }
+        if (better + ldexp((double)sum, -weigh.unit) < target) last = max(last, ~mine);
+    }
+    const uint64_t key = ~block_max_u64(last, sh);
+    whole = block_max_u64(whole, sh);
+    if (!(better < target && better + ldexp((double)whole, -weigh.unit) >= target)) return false;
+    cut = Cut{key_score(key), key_index(key)};
+    __syncthreads();
+    for (int j = tid; j < segs.n; j += kThreads) sh.wide[j] = 0;
+    __syncthreads();
+    for (int j = tid; j < n; j += kThreads) {
+        const uint64_t k = sh.key[j];
+        const float v = key_score(k);
+        if (k >= key && weigh(v) >= r.min_p)
+            atomicAdd((unsigned long long*)&sh.wide[key_index(k) / segs.len], (unsigned long long)weigh.fixed_kept(v));
+    }
+    __syncthreads();
+    for (int j = tid; j < segs.n; j += kThreads) sh.seg[j + 1] += ldexp((double)sh.wide[j], -weigh.unit);
+    return true;
+}
+
+__device__ __forceinline__ double kept_weight(float v, int i, const Cut& cut, const Weigh& weigh, double min_p) {
+    const double w = weigh(v);
+    return (cut.keeps(v, i) & (w >= min_p)) ? w : 0.0;
+}
+
+// weights of the kept columns of segments [g0, g1) -> seg[g + 1]
+template <bool BF16>
+__device__ __forceinline__ void sum_segments(const void* s, int64_t cols, const Segments& segs, int g0, int g1, const Cut& cut,
+                                             const Weigh& weigh, double min_p, double* seg) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int g = g0 + wave; g < g1; g += kWaves) {
+        double w = 0.0;
+        for_groups<BF16, 1>(s, g * segs.len, min(cols, (g + 1) * segs.len), lane, 64, [&](const float (&v)[4], int i) {
+            if (max_of(max_of(v[0], v[1]), max_of(v[2], v[3])) >= cut.s)
+                w += (kept_weight(v[0], i, cut, weigh, min_p) + kept_weight(v[1], i + 1, cut, weigh, min_p)) +
+                     (kept_weight(v[2], i + 2, cut, weigh, min_p) + kept_weight(v[3], i + 3, cut, weigh, min_p));
+        });
+        w = wave_scan_f64(w);
+        if (lane == 63) seg[g + 1] = w;
+    }
+}
+
+// the draws part, part + parts, ... (in groups of kWaves) from the segment sums sh.seg[1, n]
+template <bool BF16>
+__device__ void draw_columns(const SampleArgs& a, int64_t row, const Row& r, const void* s, const Segments& segs, const Cut& cut,
+                             const Weigh& weigh, int part, int parts, Shared& sh) {
+    constexpr int N = Vec<BF16>::N, kStep = 64 * N;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     __syncthreads();
     if (tid < 64) {
         constexpr int per = kSegs / 64;
-        const int lo = lane * per, hi = min(n_segs, lo + per);
+        const int lo = lane * per, hi = min(segs.n, lo + per);
         double own = 0.0;
         for (int j = lo; j < hi; ++j) own += sh.seg[j + 1];
         double run = wave_scan_f64(own) - own;
@@ -850,21 +826,21 @@ __global__ __launch_bounds__(kThreads, 6) void sample_rows_kernel(SampleArgs a) 
         if (lane == 0) sh.seg[0] = 0.0;
     }
     __syncthreads();
-    const double total = sh.seg[n_segs];
-    int last_seg = n_segs - 1;  // the last segment with any weight
+    const double total = sh.seg[segs.n];
+    int last_seg = segs.n - 1;  // the last segment with any weight
     while (last_seg > 0 && !(sh.seg[last_seg + 1] > sh.seg[last_seg])) --last_seg;
-    for (int64_t j = wave; j < a.n_draws; j += kWaves) {
+    for (int64_t j = wave + (int64_t)part * kWaves; j < a.n_draws; j += (int64_t)parts * kWaves) {
         const double target = draw_number(a, row, j) * total;
         int lo = 0, hi = last_seg;  // the first segment whose end passes the target
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
             if (sh.seg[mid + 1] > target) hi = mid; else lo = mid + 1;
         }
-        const int64_t end = min((int64_t)cols, (lo + 1) * seg_len);
+        const int64_t end = min(a.cols, (lo + 1) * segs.len);
         double run = sh.seg[lo];
         int64_t pick = -1;
         double wp = 0.0;
-        for (int64_t i0 = lo * seg_len; i0 < end; i0 += kStep) {
+        for (int64_t i0 = lo * segs.len; i0 < end; i0 += kStep) {
             Vec<BF16> v;
             const int64_t i = i0 + lane * N;
             if (i + N <= end)
@@ -873,7 +849,7 @@ __global__ __launch_bounds__(kThreads, 6) void sample_rows_kernel(SampleArgs a) 
                 v.load_tail(s, i, end);
             double w[N], own = 0.0;
 #pragma unroll
-            for (int k = 0; k < N; ++k) own += w[k] = kept(v.v[k], (int)i + k);
+            for (int k = 0; k < N; ++k) own += w[k] = kept_weight(v.v[k], (int)i + k, cut, weigh, r.min_p);
             double c = run + wave_scan_f64(own) - own;
             // this lane's first column past the target, or without one its last of any weight
             int at = -1, tail = -1;
@@ -906,6 +882,358 @@ __global__ __launch_bounds__(kThreads, 6) void sample_rows_kernel(SampleArgs a) 
     }
 }
 
+__device__ __forceinline__ void all_draws(const SampleArgs& a, int64_t row, int32_t idx, float prob) {
+    for (int64_t j = threadIdx.x; j < a.n_draws; j += kThreads) {
+        a.out_idx[row * a.n_draws + j] = idx;
+        if (a.out_prob) a.out_prob[row * a.n_draws + j] = prob;
+    }
+}
+__device__ __forceinline__ bool best_only(const Row& r) { return !(r.T > 0.0) || r.top_k == 1 || r.top_p <= 0.0; }
+
+template <bool BF16>
+__device__ __forceinline__ const void* row_scores(const SampleArgs& a, int64_t row) {
+    return BF16 ? (const void*)(static_cast<const uint16_t*>(a.S) + row * a.ld)
+                : (const void*)(static_cast<const float*>(a.S) + row * a.ld);
+}
+
+// A whole row by one workgroup
+template <bool BF16>
+__device__ void sample_row(const SampleArgs& a, int64_t row, const Row& r, Shared& sh) {
+    const int tid = threadIdx.x;
+    const void* s = row_scores<BF16>(a, row);
+    const int cols = (int)a.cols;
+    if (best_only(r)) {
+        const uint64_t best = block_max_u64(scan_best<BF16>(s, 0, cols, tid, kThreads), sh);
+        all_draws(a, row, best ? key_index(best) : -1, best ? 1.0f : 0.0f);
+        return;
+    }
+    const Maxima m = scan_maxima<BF16>(s, 0, cols);
+    const float top = unord_f32((uint32_t)block_max_u64(order_of(max_of(max_of(m.best[0], m.best[1]), max_of(m.best[2], m.best[3]))), sh));
+    if (top == kNone) {
+        all_draws(a, row, -1, 0.0f);
+        return;
+    }
+    if (top == INFINITY) {
+        draw_infinite<BF16>(a, row, r, s, sh);
+        return;
+    }
+    const float low = of_reverse_order(block_max_u64(reverse_order_of(m.low), sh));
+    const Weigh weigh(top, r.T, cols);
+
+    Cut cut{kNone, -1};
+    if (r.top_k > 0 && r.top_k < cols) {
+        // a list of the columns that reach the classes' bound, or of all
+        float bound = kNone;
+        if (cols > kList && r.top_k <= kList) bound = class_bound(m, r.top_k, sh);
+        if (cols <= kList || bound > kNone) {
+            __syncthreads();
+            if (tid == 0) sh.n = 0;
+            __syncthreads();
+            gather<BF16>(s, 0, cols, sh.key, &sh.n, [&](float v, int) { return (v >= bound) & (v > kNone); });
+            __syncthreads();
+            if (sh.n <= kList) {
+                finish_list(a, row, r, (int)sh.n, weigh, sh);
+                return;
+            }
+        }
+        // the step of the top_k-th column
+        const Binning bin = make_binning(top, fmax((double)top - (double)low, 0.0));
+        clear_hist(sh);
+        for_groups<BF16, 2>(s, 0, cols, tid, kThreads, [&](const float (&v)[4], int) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (v[j] > kNone) atomicAdd(&sh.count[bin(v[j])], 1u);
+        });
+        __syncthreads();
+        find_bin(sh.count, (double)r.top_k, sh);
+        const int b = (int)sh.bin;
+        const uint64_t before = sh.below, in_bin = sh.count[b];
+        if (in_bin > 0 && in_bin <= kList) {
+            gather<BF16>(s, 0, cols, sh.key, &sh.n, [&](float v, int) { return (v > kNone) && bin(v) == b; });
+            sort_keys((int)in_bin, sh);
+            const uint64_t key = sh.key[min((uint64_t)r.top_k - before, in_bin) - 1];
+            cut = Cut{key_score(key), key_index(key)};
+        } else {
+            cut = descend<BF16, false>(s, cols, cut, (double)r.top_k, weigh, sh);
+        }
+    }
+    const Segments segs(cols);
+    bool summed = false;
+    if (r.top_p < 1.0) {
+        const Binning bin = mass_binning(top, low, r, cols);
+        clear_hist(sh);
+        count_steps<BF16>(s, 0, cols, bin, cut, sh);
+        __syncthreads();
+        const Window win = mass_window(bin, top, r.top_p, weigh, sh);
+        if (win.usable()) {
+            double z, better;
+            sum_window<BF16>(s, cols, segs, 0, segs.n, bin, win, cut, weigh, r.min_p, sh.seg, sh.key, &sh.n, z, better);
+            z = block_sum_f64(z, sh);
+            better = block_sum_f64(better, sh);
+            summed = resolve_window((int)min(sh.n, (uint32_t)kList), z, better, r, segs, weigh, cut, sh);
+        }
+        if (!summed) {
+            uint64_t sum = 0;
+            for_groups<BF16, 1>(s, 0, cols, tid, kThreads, [&](const float (&v)[4], int i) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum += cut.keeps(v[j], i + j) ? weigh.fixed(v[j]) : 0;
+            });
+            cut = descend<BF16, true>(s, cols, cut, r.top_p * (double)block_sum_u64(sum, sh), weigh, sh);
+        }
+    }
+    if (!summed) {
+        __syncthreads();
+        sum_segments<BF16>(s, cols, segs, 0, segs.n, cut, weigh, r.min_p, sh.seg);
+    }
+    draw_columns<BF16>(a, row, r, s, segs, cut, weigh, 0, 1, sh);
+}
+
+template <bool BF16>
+__global__ __launch_bounds__(kThreads, 6) void sample_rows_kernel(SampleArgs a) {
+    __shared__ Shared sh;
+    sample_row<BF16>(a, blockIdx.x, row_settings(a, blockIdx.x), sh);
+}
+
+// ------------------------------------------------------------------------------------ few long rows
+// The same steps with a row cut into `parts` runs of segments, a workgroup each, and a launch per reading; what the
+// workgroups of a row tell each other goes through the workspace, in integers whose order does not matter or in slots
+// of their own.  A row that needs one of the rare ways is left to its first workgroup in the last launch.
+struct RowState {          // all zero at the start
+    uint64_t best;         // best column key (rows that draw the best column only)
+    uint32_t top, low;     // order bits of the best score, reversed ones of the low score
+    uint32_t bound;        // reversed order bits of the least of the parts' class bounds
+    uint32_t n;            // columns gathered
+    uint32_t count[kBins];
+};
+struct SplitArgs {
+    RowState* state;
+    uint64_t* keys;  // [rows, kList]
+    double* seg;     // [rows, kSegs + 1]
+    double* sums;    // [rows, parts, 2]: z, better
+    int parts;
+};
+
+__global__ __launch_bounds__(256) void sample_clear(uint32_t* p, int64_t n) {
+    for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n; i += gridDim.x * (int64_t)256) p[i] = 0;
+}
+
+// the segments of this workgroup
+struct Part {
+    int g0, g1;
+    int64_t lo, hi;
+    __device__ __forceinline__ Part(const Segments& segs, int64_t cols, int part, int parts) {
+        const int per = (segs.n + parts - 1) / parts;
+        g0 = min(segs.n, part * per);
+        g1 = min(segs.n, g0 + per);
+        lo = min(cols, g0 * segs.len);
+        hi = min(cols, g1 * segs.len);
+    }
+};
+__device__ __forceinline__ bool listed(const SampleArgs& a, const Row& r) { return r.top_k > 0 && r.top_k < a.cols; }
+// rows that the middle launches have nothing to do for
+__device__ __forceinline__ bool settled(const Row& r, float top) { return best_only(r) || top == kNone || top == INFINITY; }
+
+template <bool BF16>
+__global__ __launch_bounds__(kThreads, 6) void sample_split_top(SampleArgs a, SplitArgs p) {
+    __shared__ Shared sh;
+    const int64_t row = blockIdx.y;
+    const Row r = row_settings(a, row);
+    const Part part(Segments(a.cols), a.cols, blockIdx.x, p.parts);
+    if (part.lo >= part.hi) return;
+    RowState* st = p.state + row;
+    const void* s = row_scores<BF16>(a, row);
+    if (best_only(r)) {
+        const uint64_t best = block_max_u64(scan_best<BF16>(s, part.lo, part.hi, threadIdx.x, kThreads), sh);
+        if (threadIdx.x == 0) atomicMax((unsigned long long*)&st->best, (unsigned long long)best);
+        return;
+    }
+    const Maxima m = scan_maxima<BF16>(s, part.lo, part.hi);
+    const uint32_t top = (uint32_t)block_max_u64(order_of(max_of(max_of(m.best[0], m.best[1]), max_of(m.best[2], m.best[3]))), sh);
+    const uint32_t low = (uint32_t)block_max_u64(reverse_order_of(m.low), sh);
+    uint32_t bound = 0;
+    // with ceil(top_k / parts) columns of every part at or above the least of the parts' bounds, top_k are
+    if (listed(a, r))
+        bound = (uint32_t)reverse_order_of(r.top_k <= kList ? class_bound(m, (r.top_k + p.parts - 1) / p.parts, sh) : kNone);
+    if (threadIdx.x == 0) {
+        atomicMax(&st->top, top);
+        atomicMax(&st->low, low);
+        if (bound) atomicMax(&st->bound, bound);
+    }
+}
+
+template <bool BF16>
+__global__ __launch_bounds__(kThreads, 6) void sample_split_find(SampleArgs a, SplitArgs p) {
+    __shared__ Shared sh;
+    const int64_t row = blockIdx.y;
+    const Row r = row_settings(a, row);
+    const Part part(Segments(a.cols), a.cols, blockIdx.x, p.parts);
+    RowState* st = p.state + row;
+    const float top = unord_f32(st->top);
+    if (part.lo >= part.hi || settled(r, top)) return;
+    const void* s = row_scores<BF16>(a, row);
+    if (listed(a, r)) {
+        const float bound = of_reverse_order(st->bound);
+        if (bound > kNone) gather<BF16>(s, part.lo, part.hi, p.keys + row * kList, &st->n, [&](float v, int) { return v >= bound; });
+    } else if (r.top_p < 1.0) {
+        clear_hist(sh);
+        count_steps<BF16>(s, part.lo, part.hi, mass_binning(top, of_reverse_order(st->low), r, a.cols), Cut{kNone, -1}, sh);
+        __syncthreads();
+        for (int j = threadIdx.x; j < kBins; j += kThreads)
+            if (sh.count[j]) atomicAdd(&st->count[j], sh.count[j]);
+    }
+}
+
+template <bool BF16>
+__global__ __launch_bounds__(kThreads, 6) void sample_split_sum(SampleArgs a, SplitArgs p) {
+    __shared__ Shared sh;
+    const int64_t row = blockIdx.y;
+    const Row r = row_settings(a, row);
+    const Segments segs(a.cols);
+    const Part part(segs, a.cols, blockIdx.x, p.parts);
+    RowState* st = p.state + row;
+    const float top = unord_f32(st->top);
+    if (part.lo >= part.hi || settled(r, top) || listed(a, r)) return;
+    const void* s = row_scores<BF16>(a, row);
+    const Weigh weigh(top, r.T, (int)a.cols);
+    double* seg = p.seg + row * (kSegs + 1);
+    if (!(r.top_p < 1.0)) {
+        sum_segments<BF16>(s, a.cols, segs, part.g0, part.g1, Cut{kNone, -1}, weigh, r.min_p, seg);
+        return;
+    }
+    for (int j = threadIdx.x; j < kBins; j += kThreads) sh.count[j] = st->count[j];
+    __syncthreads();
+    const Binning bin = mass_binning(top, of_reverse_order(st->low), r, a.cols);
+    const Window win = mass_window(bin, top, r.top_p, weigh, sh);
+    if (!win.usable()) return;
+    double z, better;
+    sum_window<BF16>(s, a.cols, segs, part.g0, part.g1, bin, win, Cut{kNone, -1}, weigh, r.min_p, seg, p.keys + row * kList, &st->n, z, better);
+    z = block_sum_f64(z, sh);
+    better = block_sum_f64(better, sh);
+    if (threadIdx.x == 0) {
+        double* o = p.sums + (row * p.parts + blockIdx.x) * 2;
+        o[0] = z;
+        o[1] = better;
+    }
+}
+
+template <bool BF16>
+__global__ __launch_bounds__(kThreads, 4) void sample_split_draw(SampleArgs a, SplitArgs p) {
+    __shared__ Shared sh;
+    const int64_t row = blockIdx.y;
+    const int tid = threadIdx.x;
+    const bool first = blockIdx.x == 0;
+    const Row r = row_settings(a, row);
+    const Segments segs(a.cols);
+    const RowState* st = p.state + row;
+    const void* s = row_scores<BF16>(a, row);
+    const float top = unord_f32(st->top);
+    if (best_only(r)) {
+        if (first) all_draws(a, row, st->best ? key_index(st->best) : -1, st->best ? 1.0f : 0.0f);
+        return;
+    }
+    if (top == kNone || st->top == 0) {
+        if (first) all_draws(a, row, -1, 0.0f);
+        return;
+    }
+    if (top == INFINITY) {
+        if (first) draw_infinite<BF16>(a, row, r, s, sh);
+        return;
+    }
+    const Weigh weigh(top, r.T, (int)a.cols);
+    const int n = (int)min(st->n, (uint32_t)kList + 1);
+    bool alone = n > kList;
+    if (listed(a, r)) {
+        if (!first) return;
+        alone |= !(of_reverse_order(st->bound) > kNone);
+        if (!alone) {
+            for (int j = tid; j < n; j += kThreads) sh.key[j] = p.keys[row * kList + j];
+            __syncthreads();
+            finish_list(a, row, r, n, weigh, sh);
+            return;
+        }
+    }
+    Cut cut{kNone, -1};
+    if (!alone) {
+        const double* seg = p.seg + row * (kSegs + 1);
+        if (r.top_p < 1.0) {
+            for (int j = tid; j < kBins; j += kThreads) sh.count[j] = st->count[j];
+            __syncthreads();
+            const Binning bin = mass_binning(top, of_reverse_order(st->low), r, a.cols);
+            alone = !mass_window(bin, top, r.top_p, weigh, sh).usable();
+            if (!alone) {
+                __syncthreads();
+                for (int j = tid; j < segs.n; j += kThreads) sh.seg[j + 1] = seg[j + 1];
+                for (int j = tid; j < n; j += kThreads) sh.key[j] = p.keys[row * kList + j];
+                double z = 0.0, better = 0.0;
+                for (int j = 0; j < p.parts; ++j) {
+                    if (Part(segs, a.cols, j, p.parts).g0 >= segs.n) break;
+                    z += p.sums[(row * p.parts + j) * 2];
+                    better += p.sums[(row * p.parts + j) * 2 + 1];
+                }
+                __syncthreads();
+                alone = !resolve_window(n, z, better, r, segs, weigh, cut, sh);
+            }
+        } else {
+            for (int j = tid; j < segs.n; j += kThreads) sh.seg[j + 1] = seg[j + 1];
+        }
+    }
+    if (alone) {
+        __syncthreads();
+        if (first) sample_row<BF16>(a, row, r, sh);
+        return;
+    }
+    draw_columns<BF16>(a, row, r, s, segs, cut, weigh, blockIdx.x, gridDim.x, sh);
+}
+
+// How many workgroups share a row: enough to fill the chip with three each, of at least four segments
+int split_parts(int64_t rows, int64_t cols) {
+    if (rows <= 0 || cols <= 32768) return 1;
+    const Segments segs(cols);
+    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(ceil_div((int64_t)768, rows), segs.n / 4));
+    return (int)ceil_div((int64_t)segs.n, ceil_div((int64_t)segs.n, parts));  // none without a segment
+}
+
+// the workspace: states, keys, segment sums, sums
+struct SplitLayout {
+    size_t keys, seg, sums, bytes;
+    SplitLayout(int64_t rows, int parts) {
+        keys = align_up((size_t)rows * sizeof(RowState));
+        seg = keys + align_up((size_t)rows * kList * 8);
+        sums = seg + align_up((size_t)rows * (kSegs + 1) * 8);
+        bytes = parts > 1 ? sums + align_up((size_t)rows * parts * 16) : 0;
+    }
+};
+
+template <bool BF16>
+int launch_sample(const SampleArgs& a, void* ws, int parts, hipStream_t stream) {
+    if (parts == 1) {
+        sample_rows_kernel<BF16><<<(unsigned)a.rows, kThreads, 0, stream>>>(a);
+        LGX_LAUNCH_CHECK();
+        return LGX_OK;
+    }
+    const SplitLayout l(a.rows, parts);
+    char* w = static_cast<char*>(ws);
+    const SplitArgs p{reinterpret_cast<RowState*>(w), reinterpret_cast<uint64_t*>(w + l.keys), reinterpret_cast<double*>(w + l.seg),
+                      reinterpret_cast<double*>(w + l.sums), parts};
+    const int64_t words = a.rows * (int64_t)(sizeof(RowState) / 4);
+    sample_clear<<<(unsigned)std::min<int64_t>(1024, ceil_div(words, (int64_t)256)), 256, 0, stream>>>(reinterpret_cast<uint32_t*>(w), words);
+    LGX_LAUNCH_CHECK();
+    const dim3 grid((unsigned)parts, (unsigned)a.rows);
+    sample_split_top<BF16><<<grid, kThreads, 0, stream>>>(a, p);
+    LGX_LAUNCH_CHECK();
+    // without any top_k or top_p there is nothing to find
+    if (a.k_rows || a.p_rows || a.top_k > 0 || a.top_p < 1.0) {
+        sample_split_find<BF16><<<grid, kThreads, 0, stream>>>(a, p);
+        LGX_LAUNCH_CHECK();
+    }
+    sample_split_sum<BF16><<<grid, kThreads, 0, stream>>>(a, p);
+    LGX_LAUNCH_CHECK();
+    const int64_t draws = std::min<int64_t>(ceil_div(a.n_draws, (int64_t)kWaves), parts);
+    sample_split_draw<BF16><<<dim3((unsigned)draws, (unsigned)a.rows), kThreads, 0, stream>>>(a, p);
+    LGX_LAUNCH_CHECK();
+    return LGX_OK;
+}
+
 }  // namespace
 }  // namespace lgx
 
@@ -914,7 +1242,7 @@ using namespace lgx;
 extern "C" int lgx_sample_rows_workspace(int64_t rows, int64_t cols, int64_t n_draws, size_t* ws_bytes) {
     LGX_REQUIRE(ws_bytes && rows >= 0 && cols >= 1 && n_draws >= 0, LGX_ERR_INVALID_ARG,
                 "lgx_sample_rows_workspace: bad arguments");
-    *ws_bytes = 0;
+    *ws_bytes = SplitLayout(rows, split_parts(rows, cols)).bytes;
     return LGX_OK;
 }
 
@@ -932,14 +1260,11 @@ extern "C" int lgx_sample_rows(const void* S, int dtype, int64_t rows, int64_t c
     if (rows == 0 || n_draws == 0) return LGX_OK;
     LGX_REQUIRE(rows < (1LL << 31), LGX_ERR_UNSUPPORTED, "lgx_sample_rows: %lld rows is too many", (long long)rows);
     LGX_REQUIRE(S && u && out_idx, LGX_ERR_INVALID_ARG, "lgx_sample_rows: null pointer");
-    (void)ws;
-    (void)ws_bytes;
+    const int parts = split_parts(rows, cols);
+    const size_t need = SplitLayout(rows, parts).bytes;
+    LGX_REQUIRE(need == 0 || (ws && ws_bytes >= need && reinterpret_cast<uintptr_t>(ws) % 16 == 0), LGX_ERR_WORKSPACE,
+                "lgx_sample_rows: workspace %zu < %zu", ws_bytes, need);
     const SampleArgs a{S, rows, cols, ld, u, u_dtype == LGX_DTYPE_F64, n_draws, temperature, top_p, min_p, top_k,
                        temperature_rows, top_p_rows, min_p_rows, top_k_rows, out_idx, out_prob};
-    if (dtype == LGX_DTYPE_BF16)
-        sample_rows_kernel<true><<<(unsigned)rows, kThreads, 0, stream>>>(a);
-    else
-        sample_rows_kernel<false><<<(unsigned)rows, kThreads, 0, stream>>>(a);
-    LGX_LAUNCH_CHECK();
-    return LGX_OK;
+    return dtype == LGX_DTYPE_BF16 ? launch_sample<true>(a, ws, parts, stream) : launch_sample<false>(a, ws, parts, stream);
 }
