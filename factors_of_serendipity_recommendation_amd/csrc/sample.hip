@@ -2,9 +2,9 @@
 //
 // The kept columns are a prefix of the row's ranking (score descending, ties to the lower column), so they are
 // described by one 64-bit key (wave_topk.h's make_key): column i is kept iff its key is at least the cut.
-// top_k: with the row cut into kThreads x 4 classes of columns, the top_k-th largest of the classes' best scores is
-// at most the top_k-th largest score, so that what reaches it holds the top_k columns and hardly more: one
-// reading finds that bound, a second gathers a list in LDS, and everything else happens on that list.
+// top_k: the first columns are cut into kThreads x 4 classes; the top_k-th largest of the classes' best scores is at
+// most the row's top_k-th largest score, so that what reaches it holds the top_k columns.  One reading of the row gathers
+// those as a list in LDS, and everything else happens on that list.
 // top_p: a histogram of the distances to the best score, in 4096 equal steps, counts columns; a count times the weight
 // in the middle of its step is close enough to name the step in which the running weight reaches its target.  The next
 // reading sums the exact weights of everything better, and gathers that step's columns, among which the cut is
@@ -24,7 +24,10 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
 constexpr int kBins = 4096;  // of 32 bits, or half as many of 64
+constexpr int kTopBins = 512;  // the first of them, whose columns' places within the step are summed too
 constexpr int kList = 2048;  // columns that are gathered in LDS
+constexpr int kAim = 384;  // columns a list is made of, where one chunk in several is looked at first
+constexpr int kShort = 256;  // columns that are compared with each other, a step per pair, instead of sorted
 constexpr int kSegs = 1024;  // column segments with sums of their own: a draw scans one of them
 
 struct SampleArgs {
@@ -217,7 +220,8 @@ struct Shared {
         uint64_t wide[kBins / 2];
         uint32_t count[kBins];
     };
-    uint64_t key[kList];  // gathered columns
+    uint64_t place[kTopBins];  // in 2^-16 of a step
+    uint64_t key[kList];       // gathered columns
     union {
         double w[kList];  // their weights, then the running sums of the kept ones
         double seg[kSegs + 1];
@@ -225,11 +229,11 @@ struct Shared {
     uint64_t part[kWaves];
     double dpart[kWaves];
     uint64_t below;
-    uint32_t bin, bin2, n;
+    uint32_t bin, bin2, bin3, n;
 };
 
 // sum / maximum over the workgroup, the same value in every thread
-__device__ uint64_t block_sum_u64(uint64_t v, Shared& sh) {
+__device__ __forceinline__ uint64_t block_sum_u64(uint64_t v, Shared& sh) {
     v = wave_scan_u64(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 63) sh.part[threadIdx.x >> 6] = v;
@@ -239,7 +243,7 @@ __device__ uint64_t block_sum_u64(uint64_t v, Shared& sh) {
     for (int i = 0; i < kWaves; ++i) s += sh.part[i];
     return s;
 }
-__device__ uint64_t block_max_u64(uint64_t v, Shared& sh) {
+__device__ __forceinline__ uint64_t block_max_u64(uint64_t v, Shared& sh) {
     v = wave_max_u64(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 63) sh.part[threadIdx.x >> 6] = v;
@@ -250,7 +254,7 @@ __device__ uint64_t block_max_u64(uint64_t v, Shared& sh) {
     return s;
 }
 
-__device__ double block_sum_f64(double v, Shared& sh) {
+__device__ __forceinline__ double block_sum_f64(double v, Shared& sh) {
     v = wave_scan_f64(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 63) sh.dpart[threadIdx.x >> 6] = v;
@@ -272,7 +276,7 @@ __device__ __forceinline__ void clear_hist(Shared& sh) {
 // it; the last bin that holds anything if the whole falls short, bin 0 of an empty histogram.
 // -> sh.bin, sh.below = the sum before it
 template <typename C>
-__device__ void find_bin(const C* hist, double target, Shared& sh) {
+__device__ __forceinline__ void find_bin(const C* hist, double target, Shared& sh) {
     constexpr int per = kBins * 4 / (int)sizeof(C) / kThreads;
     const int tid = threadIdx.x;
     if (tid == 0) {
@@ -307,7 +311,7 @@ __device__ void find_bin(const C* hist, double target, Shared& sh) {
 }
 
 // bitonic sort of sh.key[0, n), descending, n <= kList; keys past n become 0
-__device__ void sort_keys(int n, Shared& sh) {
+__device__ __forceinline__ void sort_keys(int n, Shared& sh) {
     int size = 64;
     while (size < n) size <<= 1;
     __syncthreads();
@@ -329,7 +333,7 @@ __device__ void sort_keys(int n, Shared& sh) {
 }
 
 // sh.w[0, n) -> its inclusive running sums, in order
-__device__ void scan_list(int n, Shared& sh) {
+__device__ __forceinline__ void scan_list(int n, Shared& sh) {
     constexpr int per = kList / 64;
     __syncthreads();
     if (threadIdx.x < 64) {
@@ -398,7 +402,7 @@ __device__ __forceinline__ Binning make_binning(float top, double range) {
 // The cut of top_k (MASS false: `target` columns) or top_p (`target` of the fixed weights), among the columns of
 // key >= cut, by descent over the score bits; ties are counted off in column order
 template <bool BF16, bool MASS>
-__device__ Cut descend(const void* s, int cols, const Cut& cut, double target, const Weigh& weigh, Shared& sh) {
+__device__ __forceinline__ Cut descend(const void* s, int cols, const Cut& cut, double target, const Weigh& weigh, Shared& sh) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     uint64_t above = 0;   // counted in better bins than this digit's
     uint32_t prefix = 0;  // the score bits found so far
@@ -451,15 +455,16 @@ __device__ Cut descend(const void* s, int cols, const Cut& cut, double target, c
 // sh.key[0, n) holds the row's best n columns, unsorted, n <= kList, at least min(top_k, live) of them: the
 // restrictions and the draws on that list, a column per thread.  A column's rank, the weight that ranks before it, and
 // the kept weight up to it in column order are sums over the list.
-__device__ void finish_short(const SampleArgs& a, int64_t row, const Row& r, int n, const Weigh& weigh, Shared& sh) {
+__device__ __forceinline__ void finish_short(const SampleArgs& a, int64_t row, const Row& r, int n, const Weigh& weigh, Shared& sh) {
     const int tid = threadIdx.x;
+    const int n_wave = __builtin_amdgcn_readfirstlane(tid) < n ? n : 0;  // waves without a column skip the loops
     const uint64_t mine = tid < n ? sh.key[tid] : 0;
     const uint64_t w = tid < n ? weigh.fixed_kept(key_score(mine)) : 0;
     if (tid < n) sh.wide[tid] = w;
     __syncthreads();
     int rank = 0;
     uint64_t better = 0;
-    for (int j = 0; j < n; ++j) {
+    for (int j = 0; j < n_wave; ++j) {
         const bool b = sh.key[j] > mine;
         rank += b;
         better += b ? sh.wide[j] : 0;
@@ -474,7 +479,7 @@ __device__ void finish_short(const SampleArgs& a, int64_t row, const Row& r, int
     if (tid < n) sh.wide[tid] = keep ? w : 0;
     __syncthreads();
     uint64_t upto = 0, total = 0;
-    for (int j = 0; j < n; ++j) {
+    for (int j = 0; j < n_wave; ++j) {
         const uint64_t x = sh.wide[j];
         total += x;
         upto += (uint32_t)sh.key[j] >= (uint32_t)mine ? x : 0;  // the low half falls with the column
@@ -491,9 +496,36 @@ __device__ void finish_short(const SampleArgs& a, int64_t row, const Row& r, int
     }
 }
 
+// A longer list is cut to little more than its best top_k: a histogram of its scores names the step of the top_k-th
+__device__ __forceinline__ int shrink_list(int n, int64_t top_k, Shared& sh) {
+    const int tid = threadIdx.x;
+    constexpr int per = kList / kThreads;
+    uint64_t mine[per], most = 0, least = 0;  // least: complemented
+#pragma unroll
+    for (int j = 0; j < per; ++j) {
+        mine[j] = tid + j * kThreads < n ? sh.key[tid + j * kThreads] : 0;
+        most = max(most, mine[j]);
+        if (mine[j]) least = max(least, ~mine[j]);
+    }
+    const float top = key_score(block_max_u64(most, sh)), low = key_score(~block_max_u64(least, sh));
+    const Binning bin = make_binning(top, (double)top - (double)low);
+    clear_hist(sh);
+#pragma unroll
+    for (int j = 0; j < per; ++j)
+        if (mine[j]) atomicAdd(&sh.count[bin(key_score(mine[j]))], 1u);
+    __syncthreads();
+    find_bin(sh.count, (double)top_k, sh);
+#pragma unroll
+    for (int j = 0; j < per; ++j)
+        if (mine[j] && bin(key_score(mine[j])) <= (int)sh.bin) sh.key[atomicAdd(&sh.n, 1u)] = mine[j];
+    __syncthreads();
+    return (int)sh.n;
+}
+
 // the same for longer lists: sorted by rank, cut, and sorted by column
-__device__ void finish_list(const SampleArgs& a, int64_t row, const Row& r, int n, const Weigh& weigh, Shared& sh) {
-    if (n <= kThreads) {
+__device__ __forceinline__ void finish_list(const SampleArgs& a, int64_t row, const Row& r, int n, const Weigh& weigh, Shared& sh) {
+    if (n > kShort && r.top_k < n) n = shrink_list(n, r.top_k, sh);
+    if (n <= kShort) {
         finish_short(a, row, r, n, weigh, sh);
         return;
     }
@@ -549,7 +581,7 @@ __device__ void finish_list(const SampleArgs& a, int64_t row, const Row& r, int 
 
 // A row with infinite scores: those columns share it equally, and their ranking is the column order
 template <bool BF16>
-__device__ void draw_infinite(const SampleArgs& a, int64_t row, const Row& r, const void* s, Shared& sh) {
+__device__ __forceinline__ void draw_infinite(const SampleArgs& a, int64_t row, const Row& r, const void* s, Shared& sh) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     uint64_t n = 0;
     for (int64_t i = tid; i < a.cols; i += kThreads) n += load_score<BF16>(s, i) == INFINITY;
@@ -590,22 +622,29 @@ struct Segments {
 struct Maxima {
     float best[4], low;
 };
+constexpr int64_t kChunk = kThreads * 4;  // columns of one step of the workgroup
+// of every `stride`-th chunk of [lo, hi)
 template <bool BF16>
-__device__ __forceinline__ Maxima scan_maxima(const void* s, int64_t lo, int64_t hi) {
+__device__ __forceinline__ Maxima scan_maxima(const void* s, int64_t lo, int64_t hi, int64_t stride) {
     Maxima m{{kNone, kNone, kNone, kNone}, INFINITY};
-    for_groups<BF16, 4>(s, lo, hi, threadIdx.x, kThreads, [&](const float (&v)[4], int) {
+    for_groups<BF16, 4>(s, lo, hi, threadIdx.x, kThreads * stride, [&](const float (&v)[4], int) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) m.best[j] = max_of(m.best[j], v[j]);
         m.low = v[0] > -1e30f ? fminf(m.low, v[0]) : m.low;
     });
     return m;
 }
+// For a list of about kAim columns of those that reach the top_k-th of the chunks looked at, at least two of them (sorted
+// and periodic rows look like others this way)
+__device__ __forceinline__ int64_t list_stride(int64_t lo, int64_t hi, int64_t top_k) {
+    return max((int64_t)1, min((int64_t)kAim / top_k, (hi - lo) / (2 * kChunk)));
+}
 __device__ __forceinline__ uint64_t order_of(float f) { return ord_f32(f); }
 __device__ __forceinline__ uint64_t reverse_order_of(float f) { return (uint32_t)~ord_f32(f); }
 __device__ __forceinline__ float of_reverse_order(uint64_t o) { return unord_f32(~(uint32_t)o); }
 
 // a score that at least k of the workgroup's classes reach, so at least k columns do; kNone without k classes
-__device__ float class_bound(const Maxima& m, int64_t k, Shared& sh) {
+__device__ __forceinline__ float class_bound(const Maxima& m, int64_t k, Shared& sh) {
     float least = INFINITY, most = kNone;
     uint64_t classes = 0;
 #pragma unroll
@@ -633,61 +672,86 @@ __device__ float class_bound(const Maxima& m, int64_t k, Shared& sh) {
     return of_reverse_order(block_max_u64(reverse_order_of(bound), sh));
 }
 
-// the columns of [lo, hi) that `take` names go to keys[0, kList), counted in n beyond that
-template <bool BF16, typename Take>
-__device__ __forceinline__ void gather(const void* s, int64_t lo, int64_t hi, uint64_t* keys, uint32_t* n, Take take) {
+// a list keys[0, kList), counted in n beyond that
+template <typename Keys, typename Count>
+__device__ __forceinline__ void push(Keys keys, Count n, uint64_t key) {
+    const uint32_t at = atomicAdd(n, 1u);
+    if (at < kList) keys[at] = key;
+}
+// put(key) for the columns of [lo, hi) that `take` names
+template <bool BF16, typename Take, typename Put>
+__device__ __forceinline__ void gather(const void* s, int64_t lo, int64_t hi, Take take, Put put) {
     for_groups<BF16, 4>(s, lo, hi, threadIdx.x, kThreads, [&](const float (&v)[4], int i) {
+        if (take(v[0]) | take(v[1]) | take(v[2]) | take(v[3])) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (take(v[j], i + j)) {
-                const uint32_t at = atomicAdd(n, 1u);
-                if (at < kList) keys[at] = column_key(v[j], i + j);
-            }
-    });
-}
-
-// steps of the distance to the best score for top_p.  A column of weight below (1 - p) Z / cols is never kept (all such
-// together weigh less than the (1 - p) Z that are dropped), and Z >= 1.  What lies e^-12 below that shares the last step,
-// and adds at most e^-12 (1 - p) to the sums.
-__device__ __forceinline__ Binning mass_binning(float top, float low, const Row& r, int64_t cols) {
-    const double range = fmax((double)top - (double)low, 0.0);
-    return make_binning(top, fmin(range, fmin(r.T, 1e30) * (log((double)cols / (1.0 - r.top_p)) + 12.0)));
-}
-
-// counts of the columns [lo, hi) that the cut keeps, without the last step, into sh.count
-template <bool BF16>
-__device__ __forceinline__ void count_steps(const void* s, int64_t lo, int64_t hi, const Binning& bin, const Cut& cut, Shared& sh) {
-    const bool all = cut.s == kNone;
-    for_groups<BF16, 2>(s, lo, hi, threadIdx.x, kThreads, [&](const float (&v)[4], int i) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int b = bin(v[j]);
-            if ((all | cut.keeps(v[j], i + j)) & (b < kBins - 1)) atomicAdd(&sh.count[b], 1u);
+            for (int j = 0; j < 4; ++j)
+                if (take(v[j])) put(column_key(v[j], i + j));
         }
     });
 }
 
-// The steps [first, last] in which the running weight of sh.count is within 1e-4 of top_p of the whole, and the columns in
-// them.  The weight in a step's middle stands for all of it, an error of the step's width (in T) squared / 24, 2e-6 at
-// most for a range of 28 T.
+// Steps of the distance to the best score for top_p.  A column of weight below (1 - p) Z / cols is never kept (all such
+// together weigh less than the (1 - p) Z that are dropped), and Z >= 1.  What lies e^-12 below that shares the last step,
+// and adds at most e^-12 (1 - p) to the sums; so does what lies a tenth of the range below the low score, which is that
+// of a quarter of the columns.
+__device__ __forceinline__ Binning mass_binning(float top, float low, const Row& r, int64_t cols) {
+    const double range = fmax((double)top - (double)low, 0.0);
+    return make_binning(top, fmin(1.1 * range, fmin(r.T, 1e30) * (log((double)cols / (1.0 - r.top_p)) + 12.0)));
+}
+
+// counts of the columns [lo, hi) that the cut keeps, without the last step, into sh.count, and the first steps' places
+template <bool BF16>
+__device__ __forceinline__ void count_steps(const void* s, int64_t lo, int64_t hi, const Binning& bin, const Cut& cut, Shared& sh) {
+    const bool all = cut.s == kNone;
+    clear_hist(sh);
+    for (int j = threadIdx.x; j < kTopBins; j += kThreads) sh.place[j] = 0;
+    __syncthreads();
+    for_groups<BF16, 2>(s, lo, hi, threadIdx.x, kThreads, [&](const float (&v)[4], int i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float x = fminf(bin.at(v[j]), (float)(kBins - 1));
+            const int b = (int)x;
+            if ((all | cut.keeps(v[j], i + j)) & (b < kBins - 1)) {
+                atomicAdd(&sh.count[b], 1u);
+                if (b < kTopBins) atomicAdd((unsigned long long*)&sh.place[b], (unsigned long long)((x - (float)b) * 65536.0f));
+            }
+        }
+    });
+}
+
+// The steps [first, last] that may hold the column in which the running weight reaches top_p of the whole, and the columns
+// in them; the likeliest step alone where those are too many.  The weight w at the mean place of a step's columns stands
+// for each of them.  Past the first steps, where single columns weigh little, the middle is their place: they lie anywhere
+// in the step's width of d, an error of w d / (T sqrt 12) each.  Four times its root of squares, and 5e-6 of the whole
+// (the slope of their number within a step), are allowed for.
 struct Window {
     int first, last;
     uint64_t columns;
     float from, to;
     __device__ __forceinline__ bool usable() const { return last < kBins - 1 && columns > 0 && columns <= kList; }
 };
-__device__ Window mass_window(const Binning& bin, float top, double top_p, const Weigh& weigh, Shared& sh) {
+__device__ __forceinline__ Window mass_window(const Binning& bin, double T, double top_p, const Weigh& weigh, Shared& sh) {
     constexpr int per = kBins / kThreads;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const double wide = 1.0 / (double)bin.inv;
-    auto step_weight = [&](int b) { return (double)sh.count[b] * weigh((float)((double)top - wide * (b + 0.5))); };
-    double own = 0.0;
-    for (int j = 0; j < per; ++j)
-        if (sh.count[tid * per + j]) own += step_weight(tid * per + j);
+    auto step_weight = [&](int b) {
+        const double place = b < kTopBins ? (double)sh.place[b] / (65536.0 * (double)sh.count[b]) : 0.5;
+        return weigh((float)((double)bin.top - wide * (b + place)));
+    };
+    double own = 0.0, square = 0.0;
+    for (int j = 0; j < per; ++j) {
+        const double c = (double)sh.count[tid * per + j];
+        if (c > 0.0) {
+            const double w = step_weight(tid * per + j);
+            own += c * w;
+            if (tid * per + j >= kTopBins) square += c * w * w;
+        }
+    }
+    const double error = 4.0 * wide / (T * sqrt(12.0)) * sqrt(block_sum_f64(square, sh));
     const double incl = wave_scan_f64(own);
     __syncthreads();
     if (lane == 63) sh.dpart[wave] = incl;
-    if (tid == 0) sh.bin = sh.bin2 = kBins - 1;
+    if (tid == 0) sh.bin = sh.bin2 = sh.bin3 = kBins - 1;
     __syncthreads();
     double run = incl - own, sum = 0.0;
 #pragma unroll
@@ -695,17 +759,20 @@ __device__ Window mass_window(const Binning& bin, float top, double top_p, const
         if (w < wave) run += sh.dpart[w];
         sum += sh.dpart[w];
     }
-    const double t1 = (top_p - 1e-4) * sum, t2 = fmin(top_p + 1e-4, 1.0 - 1e-13) * sum;
-    uint32_t f1 = kBins - 1, f2 = kBins - 1;
+    const double all = (1.0 - 1e-13) * sum, t3 = fmin(top_p * sum, all);
+    const double t1 = t3 - 5e-6 * sum - error, t2 = fmin(t3 + 5e-6 * sum + error, all);
+    uint32_t f1 = kBins - 1, f2 = kBins - 1, f3 = kBins - 1;
     for (int j = 0; j < per; ++j) {
         const int b = tid * per + j;
         if (!sh.count[b]) continue;
-        run += step_weight(b);
+        run += (double)sh.count[b] * step_weight(b);
         if (run >= t1) f1 = min(f1, (uint32_t)b);
         if (run >= t2) f2 = min(f2, (uint32_t)b);
+        if (run >= t3) f3 = min(f3, (uint32_t)b);
     }
     if (f1 < kBins - 1) atomicMin(&sh.bin, f1);
     if (f2 < kBins - 1) atomicMin(&sh.bin2, f2);
+    if (f3 < kBins - 1) atomicMin(&sh.bin3, f3);
     __syncthreads();
     Window w{(int)sh.bin, (int)sh.bin2, 0, (float)sh.bin, (float)(sh.bin2 + 1)};
     uint64_t inside = 0;
@@ -714,76 +781,110 @@ __device__ Window mass_window(const Binning& bin, float top, double top_p, const
         if (b >= w.first && b <= w.last) inside += sh.count[b];
     }
     w.columns = block_sum_u64(inside, sh);
+    if (w.columns > kList) w = Window{(int)sh.bin3, (int)sh.bin3, sh.count[sh.bin3], (float)sh.bin3, (float)(sh.bin3 + 1)};
     return w;
 }
 
 // One reading of the segments [g0, g1) with exact weights: z = all that the cut keeps, better = what lies before the
-// window, seg[g + 1] = of that what min_p keeps.  The window's columns are gathered.  z and better of this lane.
-template <bool BF16>
+// window, sum(g, .) = of that what min_p keeps.  The window's columns are put.  z and better of this lane.
+template <bool BF16, bool ALL, typename Put, typename Sum>
 __device__ __forceinline__ void sum_window(const void* s, int64_t cols, const Segments& segs, int g0, int g1, const Binning& bin,
-                                           const Window& win, const Cut& cut, const Weigh& weigh, double min_p, double* seg,
-                                           uint64_t* keys, uint32_t* n, double& z, double& better) {
+                                           const Window& win, const Cut& cut, const Weigh& weigh, double min_p, Put put,
+                                           Sum sum, double& z, double& better) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const bool all = cut.s == kNone;
     z = better = 0.0;
     for (int g = g0 + wave; g < g1; g += kWaves) {
         double w = 0.0;
         for_groups<BF16, 1>(s, g * segs.len, min(cols, (g + 1) * segs.len), lane, 64, [&](const float (&v)[4], int i) {
+            bool in[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 double x = weigh(v[j]);
                 const float d = bin.at(v[j]);
-                const bool ok = all | cut.keeps(v[j], i + j);
+                const bool ok = ALL || cut.keeps(v[j], i + j);
                 z += ok ? x : 0.0;
                 x = d < win.from ? x : 0.0;
-                better += x;
-                w += x >= min_p ? x : 0.0;
-                if (!(d < win.from) & (d < win.to) & ok) {
-                    const uint32_t at = atomicAdd(n, 1u);
-                    if (at < kList) keys[at] = column_key(v[j], i + j);
+                if (min_p > 0.0) {
+                    better += x;
+                    w += x >= min_p ? x : 0.0;
+                } else {
+                    w += x;
                 }
+                in[j] = !(d < win.from) & (d < win.to) & ok;
+            }
+            if (in[0] | in[1] | in[2] | in[3]) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (in[j]) put(column_key(v[j], i + j));
             }
         });
+        if (!(min_p > 0.0)) better += w;
         w = wave_scan_f64(w);
-        if (lane == 63) seg[g + 1] = w;
+        if (lane == 63) sum(g, w);
     }
 }
 
 // The cut of top_p among the window's columns sh.key[0, n), and their kept weights added to the segments.  False if the
 // exact sums show that the cut lies elsewhere.
-__device__ bool resolve_window(int n, double z, double better, const Row& r, const Segments& segs, const Weigh& weigh, Cut& cut, Shared& sh) {
+__device__ __forceinline__ bool resolve_window(int n, double z, double better, const Binning& bin, const Window& win, const Row& r, const Segments& segs, const Weigh& weigh, Cut& cut, Shared& sh) {
     const int tid = threadIdx.x;
-    const double target = r.top_p * z;
-    for (int j = tid; j < n; j += kThreads) sh.wide[j] = weigh.fixed(key_score(sh.key[j]));
+    const double target = r.top_p * z, scale = ldexp(1.0, -weigh.unit);
+    // 2048 smaller steps within the window, of weights, and the columns of the one that reaches the target
+    constexpr int kFine = kBins / 2, per = kList / kThreads;
+    const float fine = (float)kFine / (win.to - win.from);
+    uint64_t mine[per], whole = 0;
+    int at[per];
+    clear_hist(sh);
+#pragma unroll
+    for (int j = 0; j < per; ++j) {
+        mine[j] = tid + j * kThreads < n ? sh.key[tid + j * kThreads] : 0;
+        at[j] = -1;
+        if (mine[j]) {
+            const float v = key_score(mine[j]);
+            const uint64_t w = weigh.fixed(v);
+            whole += w;
+            at[j] = min(kFine - 1, (int)((bin.at(v) - win.from) * fine));
+            atomicAdd((unsigned long long*)&sh.wide[at[j]], (unsigned long long)w);
+        }
+    }
+    whole = block_sum_u64(whole, sh);
+    if (!(better < target && better + (double)whole * scale >= target)) return false;
+    find_bin(sh.wide, (target - better) / scale, sh);
+    const int b = (int)sh.bin;
+    const double before = better + (double)sh.below * scale;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < per; ++j)
+        if (at[j] == b) {
+            const uint32_t k = atomicAdd(&sh.n, 1u);
+            sh.key[k] = mine[j];
+            sh.wide[k] = weigh.fixed(key_score(mine[j]));
+        }
     __syncthreads();
     // each thread adds up what ranks before its columns: the last one below the target is the cut
-    uint64_t last = 0, whole = 0;  // of the keys below the target the smallest, complemented
-    for (int c = tid; c < n; c += kThreads) {
-        const uint64_t mine = sh.key[c];
+    const int m = (int)sh.n;
+    uint64_t last = 0;  // of the keys below the target the smallest, complemented
+    for (int c = tid; c < m; c += kThreads) {
         uint64_t sum = 0;
-        whole = 0;
-        for (int j = 0; j < n; ++j) {
-            const uint64_t x = sh.wide[j];
-            whole += x;
-            sum += sh.key[j] > mine ? x : 0;
-        }
-        if (better + ldexp((double)sum, -weigh.unit) < target) last = max(last, ~mine);
+        for (int j = 0; j < m; ++j) sum += sh.key[j] > sh.key[c] ? sh.wide[j] : 0;
+        if (before + (double)sum * scale < target) last = max(last, ~sh.key[c]);
     }
-    const uint64_t key = ~block_max_u64(last, sh);
-    whole = block_max_u64(whole, sh);
-    if (!(better < target && better + ldexp((double)whole, -weigh.unit) >= target)) return false;
+    last = block_max_u64(last, sh);
+    if (!last) return false;
+    const uint64_t key = ~last;
     cut = Cut{key_score(key), key_index(key)};
     __syncthreads();
     for (int j = tid; j < segs.n; j += kThreads) sh.wide[j] = 0;
     __syncthreads();
-    for (int j = tid; j < n; j += kThreads) {
-        const uint64_t k = sh.key[j];
+#pragma unroll
+    for (int j = 0; j < per; ++j) {
+        const uint64_t k = mine[j];
         const float v = key_score(k);
-        if (k >= key && weigh(v) >= r.min_p)
+        if (k && k >= key && weigh(v) >= r.min_p)
             atomicAdd((unsigned long long*)&sh.wide[key_index(k) / segs.len], (unsigned long long)weigh.fixed_kept(v));
     }
     __syncthreads();
-    for (int j = tid; j < segs.n; j += kThreads) sh.seg[j + 1] += ldexp((double)sh.wide[j], -weigh.unit);
+    for (int j = tid; j < segs.n; j += kThreads) sh.seg[j + 1] += (double)sh.wide[j] * scale;
     return true;
 }
 
@@ -792,10 +893,10 @@ __device__ __forceinline__ double kept_weight(float v, int i, const Cut& cut, co
     return (cut.keeps(v, i) & (w >= min_p)) ? w : 0.0;
 }
 
-// weights of the kept columns of segments [g0, g1) -> seg[g + 1]
-template <bool BF16>
+// weights of the kept columns of segments [g0, g1) -> sum(g, .)
+template <bool BF16, typename Sum>
 __device__ __forceinline__ void sum_segments(const void* s, int64_t cols, const Segments& segs, int g0, int g1, const Cut& cut,
-                                             const Weigh& weigh, double min_p, double* seg) {
+                                             const Weigh& weigh, double min_p, Sum sum) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int g = g0 + wave; g < g1; g += kWaves) {
         double w = 0.0;
@@ -805,13 +906,13 @@ __device__ __forceinline__ void sum_segments(const void* s, int64_t cols, const 
                      (kept_weight(v[2], i + 2, cut, weigh, min_p) + kept_weight(v[3], i + 3, cut, weigh, min_p));
         });
         w = wave_scan_f64(w);
-        if (lane == 63) seg[g + 1] = w;
+        if (lane == 63) sum(g, w);
     }
 }
 
 // the draws part, part + parts, ... (in groups of kWaves) from the segment sums sh.seg[1, n]
 template <bool BF16>
-__device__ void draw_columns(const SampleArgs& a, int64_t row, const Row& r, const void* s, const Segments& segs, const Cut& cut,
+__device__ __forceinline__ void draw_columns(const SampleArgs& a, int64_t row, const Row& r, const void* s, const Segments& segs, const Cut& cut,
                              const Weigh& weigh, int part, int parts, Shared& sh) {
     constexpr int N = Vec<BF16>::N, kStep = 64 * N;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -896,9 +997,29 @@ __device__ __forceinline__ const void* row_scores(const SampleArgs& a, int64_t r
                 : (const void*)(static_cast<const float*>(a.S) + row * a.ld);
 }
 
+__device__ __forceinline__ bool listed(const SampleArgs& a, const Row& r) { return r.top_k > 0 && r.top_k < a.cols; }
+
+__device__ __forceinline__ float best_of(const Maxima& m, Shared& sh) {
+    return unord_f32((uint32_t)block_max_u64(order_of(max_of(max_of(m.best[0], m.best[1]), max_of(m.best[2], m.best[3]))), sh));
+}
+
+// the draws of a row whose top_k columns are among sh.key[0, n)
+template <bool BF16>
+__device__ __forceinline__ void draw_list(const SampleArgs& a, int64_t row, const Row& r, const void* s, int n, Shared& sh) {
+    uint64_t best = 0;
+    for (int j = threadIdx.x; j < n; j += kThreads) best = max(best, sh.key[j]);
+    best = block_max_u64(best, sh);
+    if (!best)
+        all_draws(a, row, -1, 0.0f);
+    else if (key_score(best) == INFINITY)
+        draw_infinite<BF16>(a, row, r, s, sh);
+    else
+        finish_list(a, row, r, n, Weigh(key_score(best), r.T, (int)a.cols), sh);
+}
+
 // A whole row by one workgroup
 template <bool BF16>
-__device__ void sample_row(const SampleArgs& a, int64_t row, const Row& r, Shared& sh) {
+__device__ __forceinline__ void sample_row(const SampleArgs& a, int64_t row, const Row& r, Shared& sh) {
     const int tid = threadIdx.x;
     const void* s = row_scores<BF16>(a, row);
     const int cols = (int)a.cols;
@@ -907,8 +1028,29 @@ __device__ void sample_row(const SampleArgs& a, int64_t row, const Row& r, Share
         all_draws(a, row, best ? key_index(best) : -1, best ? 1.0f : 0.0f);
         return;
     }
-    const Maxima m = scan_maxima<BF16>(s, 0, cols);
-    const float top = unord_f32((uint32_t)block_max_u64(order_of(max_of(max_of(m.best[0], m.best[1]), max_of(m.best[2], m.best[3]))), sh));
+    const bool by_k = listed(a, r), by_p = r.top_p < 1.0;
+    const auto to_list = [&](uint64_t key) { push(sh.key, &sh.n, key); };
+    // the list of the columns that reach the bound of the first ones
+    if (by_k && r.top_k <= kList / 2) {
+        float bound = kNone;
+        if (cols > kList) {
+            const Maxima m = scan_maxima<BF16>(s, 0, cols, list_stride(0, cols, r.top_k));
+            bound = class_bound(m, r.top_k, sh);
+        }
+        if (cols <= kList || bound > kNone) {
+            __syncthreads();
+            if (tid == 0) sh.n = 0;
+            __syncthreads();
+            gather<BF16>(s, 0, cols, [&](float v) { return (v >= bound) & (v > kNone); }, to_list);
+            __syncthreads();
+            if (sh.n <= kList) {
+                draw_list<BF16>(a, row, r, s, (int)sh.n, sh);
+                return;
+            }
+        }
+    }
+    const Maxima m = scan_maxima<BF16>(s, 0, cols, 1);
+    const float top = best_of(m, sh), low = of_reverse_order(block_max_u64(reverse_order_of(m.low), sh));
     if (top == kNone) {
         all_draws(a, row, -1, 0.0f);
         return;
@@ -917,25 +1059,9 @@ __device__ void sample_row(const SampleArgs& a, int64_t row, const Row& r, Share
         draw_infinite<BF16>(a, row, r, s, sh);
         return;
     }
-    const float low = of_reverse_order(block_max_u64(reverse_order_of(m.low), sh));
     const Weigh weigh(top, r.T, cols);
-
     Cut cut{kNone, -1};
-    if (r.top_k > 0 && r.top_k < cols) {
-        // a list of the columns that reach the classes' bound, or of all
-        float bound = kNone;
-        if (cols > kList && r.top_k <= kList) bound = class_bound(m, r.top_k, sh);
-        if (cols <= kList || bound > kNone) {
-            __syncthreads();
-            if (tid == 0) sh.n = 0;
-            __syncthreads();
-            gather<BF16>(s, 0, cols, sh.key, &sh.n, [&](float v, int) { return (v >= bound) & (v > kNone); });
-            __syncthreads();
-            if (sh.n <= kList) {
-                finish_list(a, row, r, (int)sh.n, weigh, sh);
-                return;
-            }
-        }
+    if (by_k) {
         // the step of the top_k-th column
         const Binning bin = make_binning(top, fmax((double)top - (double)low, 0.0));
         clear_hist(sh);
@@ -949,7 +1075,7 @@ __device__ void sample_row(const SampleArgs& a, int64_t row, const Row& r, Share
         const int b = (int)sh.bin;
         const uint64_t before = sh.below, in_bin = sh.count[b];
         if (in_bin > 0 && in_bin <= kList) {
-            gather<BF16>(s, 0, cols, sh.key, &sh.n, [&](float v, int) { return (v > kNone) && bin(v) == b; });
+            gather<BF16>(s, 0, cols, [&](float v) { return (v > kNone) & (bin(v) == b); }, to_list);
             sort_keys((int)in_bin, sh);
             const uint64_t key = sh.key[min((uint64_t)r.top_k - before, in_bin) - 1];
             cut = Cut{key_score(key), key_index(key)};
@@ -958,19 +1084,22 @@ __device__ void sample_row(const SampleArgs& a, int64_t row, const Row& r, Share
         }
     }
     const Segments segs(cols);
+    const auto to_seg = [&](int g, double w) { sh.seg[g + 1] = w; };
     bool summed = false;
-    if (r.top_p < 1.0) {
+    if (by_p) {
         const Binning bin = mass_binning(top, low, r, cols);
-        clear_hist(sh);
         count_steps<BF16>(s, 0, cols, bin, cut, sh);
         __syncthreads();
-        const Window win = mass_window(bin, top, r.top_p, weigh, sh);
+        const Window win = mass_window(bin, r.T, r.top_p, weigh, sh);
         if (win.usable()) {
             double z, better;
-            sum_window<BF16>(s, cols, segs, 0, segs.n, bin, win, cut, weigh, r.min_p, sh.seg, sh.key, &sh.n, z, better);
+            if (by_k)
+                sum_window<BF16, false>(s, cols, segs, 0, segs.n, bin, win, cut, weigh, r.min_p, to_list, to_seg, z, better);
+            else
+                sum_window<BF16, true>(s, cols, segs, 0, segs.n, bin, win, cut, weigh, r.min_p, to_list, to_seg, z, better);
             z = block_sum_f64(z, sh);
             better = block_sum_f64(better, sh);
-            summed = resolve_window((int)min(sh.n, (uint32_t)kList), z, better, r, segs, weigh, cut, sh);
+            summed = resolve_window((int)min(sh.n, (uint32_t)kList), z, better, bin, win, r, segs, weigh, cut, sh);
         }
         if (!summed) {
             uint64_t sum = 0;
@@ -983,7 +1112,7 @@ __device__ void sample_row(const SampleArgs& a, int64_t row, const Row& r, Share
     }
     if (!summed) {
         __syncthreads();
-        sum_segments<BF16>(s, cols, segs, 0, segs.n, cut, weigh, r.min_p, sh.seg);
+        sum_segments<BF16>(s, cols, segs, 0, segs.n, cut, weigh, r.min_p, to_seg);
     }
     draw_columns<BF16>(a, row, r, s, segs, cut, weigh, 0, 1, sh);
 }
@@ -1001,15 +1130,16 @@ __global__ __launch_bounds__(kThreads, 6) void sample_rows_kernel(SampleArgs a) 
 struct RowState {          // all zero at the start
     uint64_t best;         // best column key (rows that draw the best column only)
     uint32_t top, low;     // order bits of the best score, reversed ones of the low score
-    uint32_t bound;        // reversed order bits of the least of the parts' class bounds
+    uint32_t bound;        // order bits of a score that top_k columns reach (top_k)
     uint32_t n;            // columns gathered
     uint32_t count[kBins];
+    uint64_t place[kTopBins];
 };
 struct SplitArgs {
     RowState* state;
     uint64_t* keys;  // [rows, kList]
     double* seg;     // [rows, kSegs + 1]
-    double* sums;    // [rows, parts, 2]: z, better
+    double* sums;    // [rows, parts, 2]: z, better (top_p); order bits of the part's class bound (top_k)
     int parts;
 };
 
@@ -1029,9 +1159,15 @@ struct Part {
         hi = min(cols, g1 * segs.len);
     }
 };
-__device__ __forceinline__ bool listed(const SampleArgs& a, const Row& r) { return r.top_k > 0 && r.top_k < a.cols; }
-// rows that the middle launches have nothing to do for
-__device__ __forceinline__ bool settled(const Row& r, float top) { return best_only(r) || top == kNone || top == INFINITY; }
+__device__ __forceinline__ void load_steps(const RowState* st, Shared& sh) {
+    for (int j = threadIdx.x; j < kBins; j += kThreads) sh.count[j] = st->count[j];
+    for (int j = threadIdx.x; j < kTopBins; j += kThreads) sh.place[j] = st->place[j];
+}
+__device__ __forceinline__ bool finite(float top) { return top > kNone && top < INFINITY; }
+
+// Every part gives the score of its j-th best class; the ceil(top_k / j)-th best of those is one that top_k columns reach.
+// j is a little more than their average share.
+__device__ __forceinline__ int64_t part_rank(int64_t top_k, int parts) { return 5 * top_k / (4 * parts) + 1; }
 
 template <bool BF16>
 __global__ __launch_bounds__(kThreads, 6) void sample_split_top(SampleArgs a, SplitArgs p) {
@@ -1047,18 +1183,31 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_top(SampleArgs a, Sp
         if (threadIdx.x == 0) atomicMax((unsigned long long*)&st->best, (unsigned long long)best);
         return;
     }
-    const Maxima m = scan_maxima<BF16>(s, part.lo, part.hi);
-    const uint32_t top = (uint32_t)block_max_u64(order_of(max_of(max_of(m.best[0], m.best[1]), max_of(m.best[2], m.best[3]))), sh);
+    const bool by_k = listed(a, r);
+    if (by_k && r.top_k > kList / 2) return;
+    const Maxima m = scan_maxima<BF16>(s, part.lo, part.hi, by_k ? list_stride(part.lo, part.hi, r.top_k) : 1);
+    if (by_k) {
+        const float bound = class_bound(m, part_rank(r.top_k, p.parts), sh);
+        if (threadIdx.x == 0) reinterpret_cast<uint64_t*>(p.sums)[(row * p.parts + blockIdx.x) * 2] = order_of(bound);
+        return;
+    }
+    const uint32_t top = (uint32_t)order_of(best_of(m, sh));
     const uint32_t low = (uint32_t)block_max_u64(reverse_order_of(m.low), sh);
-    uint32_t bound = 0;
-    // with ceil(top_k / parts) columns of every part at or above the least of the parts' bounds, top_k are
-    if (listed(a, r))
-        bound = (uint32_t)reverse_order_of(r.top_k <= kList ? class_bound(m, (r.top_k + p.parts - 1) / p.parts, sh) : kNone);
     if (threadIdx.x == 0) {
         atomicMax(&st->top, top);
         atomicMax(&st->low, low);
-        if (bound) atomicMax(&st->bound, bound);
     }
+}
+
+// the workgroup's list behind the row's
+__device__ __forceinline__ void append_list(uint64_t* keys, uint32_t* count, Shared& sh) {
+    __syncthreads();
+    const uint32_t n = sh.n;
+    if (threadIdx.x == 0) sh.bin = atomicAdd(count, n);
+    __syncthreads();
+    const uint32_t at = sh.bin;
+    for (uint32_t j = threadIdx.x; j < min(n, (uint32_t)kList); j += kThreads)
+        if (at + j < kList) keys[at + j] = sh.key[j];
 }
 
 template <bool BF16>
@@ -1068,18 +1217,30 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_find(SampleArgs a, S
     const Row r = row_settings(a, row);
     const Part part(Segments(a.cols), a.cols, blockIdx.x, p.parts);
     RowState* st = p.state + row;
-    const float top = unord_f32(st->top);
-    if (part.lo >= part.hi || settled(r, top)) return;
+    if (part.lo >= part.hi || best_only(r)) return;
     const void* s = row_scores<BF16>(a, row);
     if (listed(a, r)) {
-        const float bound = of_reverse_order(st->bound);
-        if (bound > kNone) gather<BF16>(s, part.lo, part.hi, p.keys + row * kList, &st->n, [&](float v, int) { return v >= bound; });
-    } else if (r.top_p < 1.0) {
-        clear_hist(sh);
-        count_steps<BF16>(s, part.lo, part.hi, mass_binning(top, of_reverse_order(st->low), r, a.cols), Cut{kNone, -1}, sh);
+        if (r.top_k > kList / 2) return;
+        for (int j = threadIdx.x; j < p.parts; j += kThreads)
+            sh.key[j] = reinterpret_cast<const uint64_t*>(p.sums)[(row * p.parts + j) * 2];
+        sort_keys(p.parts, sh);
+        const int64_t j = part_rank(r.top_k, p.parts);
+        const uint32_t order = (uint32_t)sh.key[(r.top_k + j - 1) / j - 1];
+        const float bound = unord_f32(order);
+        if (threadIdx.x == 0 && blockIdx.x == 0) st->bound = order;
+        if (!(bound > kNone)) return;
+        __syncthreads();
+        if (threadIdx.x == 0) sh.n = 0;
+        __syncthreads();
+        gather<BF16>(s, part.lo, part.hi, [&](float v) { return v >= bound; }, [&](uint64_t key) { push(sh.key, &sh.n, key); });
+        append_list(p.keys + row * kList, &st->n, sh);
+    } else if (r.top_p < 1.0 && finite(unord_f32(st->top))) {
+        count_steps<BF16>(s, part.lo, part.hi, mass_binning(unord_f32(st->top), of_reverse_order(st->low), r, a.cols), Cut{kNone, -1}, sh);
         __syncthreads();
         for (int j = threadIdx.x; j < kBins; j += kThreads)
             if (sh.count[j]) atomicAdd(&st->count[j], sh.count[j]);
+        for (int j = threadIdx.x; j < kTopBins; j += kThreads)
+            if (sh.place[j]) atomicAdd((unsigned long long*)&st->place[j], (unsigned long long)sh.place[j]);
     }
 }
 
@@ -1091,22 +1252,26 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_sum(SampleArgs a, Sp
     const Segments segs(a.cols);
     const Part part(segs, a.cols, blockIdx.x, p.parts);
     RowState* st = p.state + row;
-    const float top = unord_f32(st->top);
-    if (part.lo >= part.hi || settled(r, top) || listed(a, r)) return;
+    if (part.lo >= part.hi || best_only(r) || listed(a, r)) return;
     const void* s = row_scores<BF16>(a, row);
-    const Weigh weigh(top, r.T, (int)a.cols);
     double* seg = p.seg + row * (kSegs + 1);
+    const float top = unord_f32(st->top);
+    if (!finite(top)) return;
+    const Weigh weigh(top, r.T, (int)a.cols);
     if (!(r.top_p < 1.0)) {
-        sum_segments<BF16>(s, a.cols, segs, part.g0, part.g1, Cut{kNone, -1}, weigh, r.min_p, seg);
+        sum_segments<BF16>(s, a.cols, segs, part.g0, part.g1, Cut{kNone, -1}, weigh, r.min_p, [&](int g, double w) { seg[g + 1] = w; });
         return;
     }
-    for (int j = threadIdx.x; j < kBins; j += kThreads) sh.count[j] = st->count[j];
-    __syncthreads();
     const Binning bin = mass_binning(top, of_reverse_order(st->low), r, a.cols);
-    const Window win = mass_window(bin, top, r.top_p, weigh, sh);
+    load_steps(st, sh);
+    if (threadIdx.x == 0) sh.n = 0;
+    __syncthreads();
+    const Window win = mass_window(bin, r.T, r.top_p, weigh, sh);
     if (!win.usable()) return;
     double z, better;
-    sum_window<BF16>(s, a.cols, segs, part.g0, part.g1, bin, win, Cut{kNone, -1}, weigh, r.min_p, seg, p.keys + row * kList, &st->n, z, better);
+    sum_window<BF16, true>(s, a.cols, segs, part.g0, part.g1, bin, win, Cut{kNone, -1}, weigh, r.min_p,
+                           [&](uint64_t key) { push(sh.key, &sh.n, key); }, [&](int g, double w) { seg[g + 1] = w; }, z, better);
+    append_list(p.keys + row * kList, &st->n, sh);
     z = block_sum_f64(z, sh);
     better = block_sum_f64(better, sh);
     if (threadIdx.x == 0) {
@@ -1126,56 +1291,47 @@ __global__ __launch_bounds__(kThreads, 4) void sample_split_draw(SampleArgs a, S
     const Segments segs(a.cols);
     const RowState* st = p.state + row;
     const void* s = row_scores<BF16>(a, row);
-    const float top = unord_f32(st->top);
     if (best_only(r)) {
         if (first) all_draws(a, row, st->best ? key_index(st->best) : -1, st->best ? 1.0f : 0.0f);
         return;
     }
-    if (top == kNone || st->top == 0) {
-        if (first) all_draws(a, row, -1, 0.0f);
-        return;
-    }
-    if (top == INFINITY) {
-        if (first) draw_infinite<BF16>(a, row, r, s, sh);
-        return;
-    }
-    const Weigh weigh(top, r.T, (int)a.cols);
     const int n = (int)min(st->n, (uint32_t)kList + 1);
     bool alone = n > kList;
-    if (listed(a, r)) {
+    const bool by_k = listed(a, r);
+    if (by_k && !alone && unord_f32(st->bound) > kNone) {  // 0, a NaN, where none was found
         if (!first) return;
-        alone |= !(of_reverse_order(st->bound) > kNone);
-        if (!alone) {
-            for (int j = tid; j < n; j += kThreads) sh.key[j] = p.keys[row * kList + j];
-            __syncthreads();
-            finish_list(a, row, r, n, weigh, sh);
-            return;
-        }
+        for (int j = tid; j < n; j += kThreads) sh.key[j] = p.keys[row * kList + j];
+        __syncthreads();
+        draw_list<BF16>(a, row, r, s, n, sh);
+        return;
     }
+    alone |= by_k;
     Cut cut{kNone, -1};
-    if (!alone) {
-        const double* seg = p.seg + row * (kSegs + 1);
-        if (r.top_p < 1.0) {
-            for (int j = tid; j < kBins; j += kThreads) sh.count[j] = st->count[j];
+    const double* seg = p.seg + row * (kSegs + 1);
+    const bool by_p = r.top_p < 1.0;
+    const float top = unord_f32(st->top);
+    const Weigh weigh(top, r.T, (int)a.cols);
+    alone |= !finite(top);
+    if (!alone && by_p) {
+        const Binning bin = mass_binning(top, of_reverse_order(st->low), r, a.cols);
+        load_steps(st, sh);
+        __syncthreads();
+        const Window win = mass_window(bin, r.T, r.top_p, weigh, sh);
+        alone = !win.usable();
+        if (!alone) {
             __syncthreads();
-            const Binning bin = mass_binning(top, of_reverse_order(st->low), r, a.cols);
-            alone = !mass_window(bin, top, r.top_p, weigh, sh).usable();
-            if (!alone) {
-                __syncthreads();
-                for (int j = tid; j < segs.n; j += kThreads) sh.seg[j + 1] = seg[j + 1];
-                for (int j = tid; j < n; j += kThreads) sh.key[j] = p.keys[row * kList + j];
-                double z = 0.0, better = 0.0;
-                for (int j = 0; j < p.parts; ++j) {
-                    if (Part(segs, a.cols, j, p.parts).g0 >= segs.n) break;
-                    z += p.sums[(row * p.parts + j) * 2];
-                    better += p.sums[(row * p.parts + j) * 2 + 1];
-                }
-                __syncthreads();
-                alone = !resolve_window(n, z, better, r, segs, weigh, cut, sh);
-            }
-        } else {
             for (int j = tid; j < segs.n; j += kThreads) sh.seg[j + 1] = seg[j + 1];
+            for (int j = tid; j < n; j += kThreads) sh.key[j] = p.keys[row * kList + j];
+            double z = 0.0, better = 0.0;
+            for (int j = 0; j < p.parts; ++j) {
+                z += p.sums[(row * p.parts + j) * 2];
+                better += p.sums[(row * p.parts + j) * 2 + 1];
+            }
+            __syncthreads();
+            alone = !resolve_window(n, z, better, bin, win, r, segs, weigh, cut, sh);
         }
+    } else if (!alone) {
+        for (int j = tid; j < segs.n; j += kThreads) sh.seg[j + 1] = seg[j + 1];
     }
     if (alone) {
         __syncthreads();
@@ -1185,11 +1341,13 @@ __global__ __launch_bounds__(kThreads, 4) void sample_split_draw(SampleArgs a, S
     draw_columns<BF16>(a, row, r, s, segs, cut, weigh, blockIdx.x, gridDim.x, sh);
 }
 
-// How many workgroups share a row: enough to fill the chip with three each, of at least four segments
+// How many workgroups share a row: none where a workgroup per row fills the chip (three fit a CU), else enough to fill it
+// four times over (rows with other settings cost other amounts), of at least four segments
+constexpr int64_t kFill = 768, kSplitGroups = 4 * kFill;
 int split_parts(int64_t rows, int64_t cols) {
-    if (rows <= 0 || cols <= 32768) return 1;
+    if (rows <= 0 || rows >= kFill || cols <= 32768) return 1;
     const Segments segs(cols);
-    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(ceil_div((int64_t)768, rows), segs.n / 4));
+    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(kSplitGroups / rows, segs.n / 4));
     return (int)ceil_div((int64_t)segs.n, ceil_div((int64_t)segs.n, parts));  // none without a segment
 }
 
