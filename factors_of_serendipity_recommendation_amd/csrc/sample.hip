@@ -50,57 +50,87 @@ __device__ __forceinline__ float load_score(const void* s, int64_t i) {
     return BF16 ? bf16_to_f32(static_cast<const uint16_t*>(s)[i]) : static_cast<const float*>(s)[i];
 }
 
-// four scores from any element offset
+// four scores from any element offset, as they lie in memory: what is on its way is not looked at
 template <bool BF16>
 struct Vec {
     static constexpr int N = 4;
-    float v[N];
+    using F = float __attribute__((ext_vector_type(4), aligned(4)));
+    using U = uint32_t __attribute__((ext_vector_type(2), aligned(2)));
+    F f;
+    U u;
     __device__ __forceinline__ void load(const void* s, int64_t i) {
-        if (BF16) {
-            using U = uint32_t __attribute__((ext_vector_type(2), aligned(2)));
-            const U q = *reinterpret_cast<const U*>(static_cast<const uint16_t*>(s) + i);
-#pragma unroll
-            for (int j = 0; j < N; j += 2) {
-                v[j] = __uint_as_float(q[j / 2] << 16);
-                v[j + 1] = __uint_as_float(q[j / 2] & 0xffff0000u);
-            }
-        } else {
-            using F = float __attribute__((ext_vector_type(4), aligned(4)));
-            const F q = *reinterpret_cast<const F*>(static_cast<const float*>(s) + i);
-#pragma unroll
-            for (int j = 0; j < N; ++j) v[j] = q[j % 4];
-        }
+        if (BF16)
+            u = *reinterpret_cast<const U*>(static_cast<const uint16_t*>(s) + i);
+        else
+            f = *reinterpret_cast<const F*>(static_cast<const float*>(s) + i);
     }
-    // columns at or past `end` as -inf, which no step takes
-    __device__ __forceinline__ void load_tail(const void* s, int64_t i, int64_t end) {
+    __device__ __forceinline__ void none() {  // four excluded scores
+        f = F{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        u = U{0xff80ff80u, 0xff80ff80u};
+    }
+    __device__ __forceinline__ void values(float (&v)[4]) const {
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = i + j < end ? load_score<BF16>(s, i + j) : -INFINITY;
+        for (int j = 0; j < N; ++j) v[j] = BF16 ? __uint_as_float(j % 2 ? u[j / 2] & 0xffff0000u : u[j / 2] << 16) : f[j];
     }
 };
+// columns at or past `end` as -inf, which no step takes
+template <bool BF16>
+__device__ __forceinline__ void load_tail(float (&v)[4], const void* s, int64_t i, int64_t end) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = i + j < end ? load_score<BF16>(s, i + j) : -INFINITY;
+}
 
 // f(four scores, column of the first) over columns [lo, hi) by `width` lanes, this one being `me`; a lane takes
-// its columns in ascending order, U groups at a time; columns past the end come as -inf
+// its columns in ascending order.  U = 1, 2: so many groups at a time with the next ones on their way (f takes long); U = 4:
+// four groups on their way at once.  What is past the end comes as -inf
 template <bool BF16, int U, typename F>
 __device__ __forceinline__ void for_groups(const void* s, int64_t lo, int64_t hi, int me, int width, F f) {
     constexpr int N = Vec<BF16>::N;
+    const int64_t step = (int64_t)width * N, whole = lo + (hi - lo) / N * N;  // the end of the whole groups
     int64_t i = lo + (int64_t)me * N;
-    const int64_t step = (int64_t)width * N;
-    if (U > 1)
-        for (; i + (U - 1) * step + N <= hi; i += U * step) {
-            Vec<BF16> v[U];
-#pragma unroll
-            for (int k = 0; k < U; ++k) v[k].load(s, i + k * step);
-#pragma unroll
-            for (int k = 0; k < U; ++k) f(v[k].v, (int)(i + k * step));
-        }
+    Vec<BF16> v[U];
+    auto take = [&](const Vec<BF16>& g, int64_t at) {
+        float x[4];
+        g.values(x);
+        f(x, (int)at);
+    };
+    if (U >= 4) {
 #pragma unroll 1
-    for (; i < hi; i += step) {
-        Vec<BF16> v;
-        if (i + N <= hi)
-            v.load(s, i);
-        else
-            v.load_tail(s, i, hi);
-        f(v.v, (int)i);
+        for (; i < whole; i += U * step) {
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                v[k].none();
+                if (i + k * step < whole) v[k].load(s, i + k * step);
+            }
+#pragma unroll
+            for (int k = 0; k < U; ++k) take(v[k], i + k * step);
+        }
+    } else {
+        const int64_t last = whole - N - (U - 1) * step;  // the last place of U whole groups
+        bool more = i <= last;
+        if (more)
+            for (int k = 0; k < U; ++k) v[k].load(s, i + k * step);
+#pragma unroll 1
+        while (more) {
+            Vec<BF16> next[U];
+            const int64_t at = i;
+            i += U * step;
+            more = i <= last;
+            if (more)
+                for (int k = 0; k < U; ++k) next[k].load(s, i + k * step);
+            for (int k = 0; k < U; ++k) take(v[k], at + k * step);
+            for (int k = 0; k < U; ++k) v[k] = next[k];
+        }
+        if (U > 1 && i < whole) {  // one group less
+            v[0].load(s, i);
+            take(v[0], i);
+        }
+    }
+    if (whole < hi && (whole - lo) / N % width == me) {  // the lane whose turn it is takes the last columns
+        float x[4];
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[j] = whole + j < hi ? load_score<BF16>(s, whole + j) : -INFINITY;
+        f(x, (int)whole);
     }
 }
 
@@ -254,6 +284,18 @@ __device__ __forceinline__ uint64_t block_max_u64(uint64_t v, Shared& sh) {
     return s;
 }
 
+// the maximum of a and of b
+__device__ __forceinline__ void block_max2(uint32_t& a, uint32_t& b, Shared& sh) {
+    const uint64_t x = wave_max_u64(a), y = wave_max_u64(b);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) sh.part[threadIdx.x >> 6] = x << 32 | y;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+        a = max(a, (uint32_t)(sh.part[i] >> 32));
+        b = max(b, (uint32_t)sh.part[i]);
+    }
+}
 __device__ __forceinline__ double block_sum_f64(double v, Shared& sh) {
     v = wave_scan_f64(v);
     __syncthreads();
@@ -307,6 +349,34 @@ __device__ __forceinline__ void find_bin(const C* hist, double target, Shared& s
             }
             run = next;
         }
+    __syncthreads();
+}
+
+// The same over kThreads bins of 64 bits in sh.wide, a thread each; needs a sum above 0.  A target past the sum counts as
+// the sum.
+__device__ __forceinline__ void clear_fine(Shared& sh) {
+    __syncthreads();
+    sh.wide[threadIdx.x] = 0;
+    if (threadIdx.x == 0) sh.n = 0;
+    __syncthreads();
+}
+__device__ __forceinline__ void find_fine(double target, Shared& sh) {
+    const int tid = threadIdx.x;
+    __syncthreads();
+    const uint64_t own = sh.wide[tid], incl = wave_scan_u64(own);
+    if ((tid & 63) == 63) sh.part[tid >> 6] = incl;
+    __syncthreads();
+    uint64_t run = incl - own, all = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        if (w < (tid >> 6)) run += sh.part[w];
+        all += sh.part[w];
+    }
+    target = fmin(target, (double)all);
+    if (own && (double)(run + own) >= target && (run == 0 || (double)run < target)) {
+        sh.bin = (uint32_t)tid;
+        sh.below = run;
+    }
     __syncthreads();
 }
 
@@ -391,11 +461,13 @@ __device__ __forceinline__ uint64_t scan_best(const void* s, int64_t lo, int64_t
 // what is farther (and NaN) to the last one
 struct Binning {
     float top, inv;
+    // of kThreads bins
+    __device__ __forceinline__ int fine(float s) const { return (int)fminf(at(s), (float)(kThreads - 1)); }
     __device__ __forceinline__ float at(float s) const { return (top - s) * inv; }
     __device__ __forceinline__ int operator()(float s) const { return (int)fminf(at(s), (float)(kBins - 1)); }
 };
-__device__ __forceinline__ Binning make_binning(float top, double range) {
-    const double inv = (double)(kBins - 1) / range;  // a range of 0: all the best score's equals in bin 0
+__device__ __forceinline__ Binning make_binning(float top, double range, int bins = kBins) {
+    const double inv = (double)(bins - 1) / range;  // a range of 0: all the best score's equals in bin 0
     return Binning{top, (float)fmin(inv, 1e30)};
 }
 
@@ -464,10 +536,17 @@ __device__ __forceinline__ void finish_short(const SampleArgs& a, int64_t row, c
     __syncthreads();
     int rank = 0;
     uint64_t better = 0;
-    for (int j = 0; j < n_wave; ++j) {
-        const bool b = sh.key[j] > mine;
-        rank += b;
-        better += b ? sh.wide[j] : 0;
+    if (r.top_p < 1.0) {
+#pragma unroll 4
+        for (int j = 0; j < n_wave; ++j) {
+            const uint64_t x = sh.wide[j];
+            const bool b = sh.key[j] > mine;
+            rank += b;
+            better += b ? x : 0;
+        }
+    } else {
+#pragma unroll 8
+        for (int j = 0; j < n_wave; ++j) rank += sh.key[j] > mine;
     }
     bool keep = tid < n && rank < r.top_k;
     if (r.top_p < 1.0) {
@@ -478,21 +557,43 @@ __device__ __forceinline__ void finish_short(const SampleArgs& a, int64_t row, c
     __syncthreads();
     if (tid < n) sh.wide[tid] = keep ? w : 0;
     __syncthreads();
-    uint64_t upto = 0, total = 0;
+    uint64_t upto = 0;
+#pragma unroll 4
     for (int j = 0; j < n_wave; ++j) {
         const uint64_t x = sh.wide[j];
-        total += x;
         upto += (uint32_t)sh.key[j] >= (uint32_t)mine ? x : 0;  // the low half falls with the column
     }
-    if (!keep) return;
-    const float prob = (float)(ldexp(weigh(key_score(mine)), weigh.unit) / (double)total);
-    for (int64_t j = 0; j < a.n_draws; ++j) {
-        const double target = draw_number(a, row, j) * (double)total;
-        // a number at the end of the range: the last column
-        if (((double)upto > target || upto == total) && (upto == w || (double)(upto - w) <= target)) {
-            a.out_idx[row * a.n_draws + j] = key_index(mine);
-            if (a.out_prob) a.out_prob[row * a.n_draws + j] = prob;
+    const uint64_t total = block_max_u64(keep ? upto : 0, sh);  // (the barriers also end the loop above)
+    const auto put = [&](int64_t j, uint64_t key) {
+        a.out_idx[row * a.n_draws + j] = key_index(key);
+        if (a.out_prob) a.out_prob[row * a.n_draws + j] = (float)(ldexp(weigh(key_score(key)), weigh.unit) / (double)total);
+    };
+    // a draw is the column with upto - w <= target < upto; a number at the end of the range counts as the last column's
+    if (a.n_draws <= n) {
+        for (int j = tid; j < (int)a.n_draws; j += kThreads) sh.wide[j] = min((uint64_t)(draw_number(a, row, j) * (double)total), total - 1);
+        __syncthreads();
+        if (keep)
+#pragma unroll 4
+            for (int j = 0; j < (int)a.n_draws; ++j) {
+                const uint64_t target = sh.wide[j];
+                if ((target < upto) & (target >= upto - w)) put(j, mine);
+            }
+        return;
+    }
+    if (tid < n) sh.wide[tid] = keep ? upto : 0;
+    __syncthreads();
+    for (int64_t j = tid; j < a.n_draws; j += kThreads) {
+        const uint64_t target = min((uint64_t)(draw_number(a, row, j) * (double)total), total - 1);
+        uint64_t least = ~0ull;
+        int at = 0;
+#pragma unroll 4
+        for (int c = 0; c < n; ++c) {
+            const uint64_t x = sh.wide[c];
+            const bool nearer = (x > target) & (x < least);
+            least = nearer ? x : least;
+            at = nearer ? c : at;
         }
+        put(j, sh.key[at]);
     }
 }
 
@@ -500,24 +601,26 @@ __device__ __forceinline__ void finish_short(const SampleArgs& a, int64_t row, c
 __device__ __forceinline__ int shrink_list(int n, int64_t top_k, Shared& sh) {
     const int tid = threadIdx.x;
     constexpr int per = kList / kThreads;
-    uint64_t mine[per], most = 0, least = 0;  // least: complemented
+    uint64_t mine[per];
+    uint32_t most = 0, least = 0;  // order bits, reversed ones
 #pragma unroll
     for (int j = 0; j < per; ++j) {
         mine[j] = tid + j * kThreads < n ? sh.key[tid + j * kThreads] : 0;
-        most = max(most, mine[j]);
-        if (mine[j]) least = max(least, ~mine[j]);
+        const uint32_t order = (uint32_t)(mine[j] >> 32);
+        most = max(most, order);
+        if (order) least = max(least, ~order);
     }
-    const float top = key_score(block_max_u64(most, sh)), low = key_score(~block_max_u64(least, sh));
-    const Binning bin = make_binning(top, (double)top - (double)low);
-    clear_hist(sh);
+    block_max2(most, least, sh);
+    const float top = unord_f32(most);
+    const Binning bin = make_binning(top, (double)top - (double)unord_f32(~least), kThreads);
+    clear_fine(sh);
 #pragma unroll
     for (int j = 0; j < per; ++j)
-        if (mine[j]) atomicAdd(&sh.count[bin(key_score(mine[j]))], 1u);
-    __syncthreads();
-    find_bin(sh.count, (double)top_k, sh);
+        if (mine[j]) atomicAdd((unsigned long long*)&sh.wide[bin.fine(key_score(mine[j]))], 1ull);
+    find_fine((double)top_k, sh);
 #pragma unroll
     for (int j = 0; j < per; ++j)
-        if (mine[j] && bin(key_score(mine[j])) <= (int)sh.bin) sh.key[atomicAdd(&sh.n, 1u)] = mine[j];
+        if (mine[j] && bin.fine(key_score(mine[j])) <= (int)sh.bin) sh.key[atomicAdd(&sh.n, 1u)] = mine[j];
     __syncthreads();
     return (int)sh.n;
 }
@@ -645,31 +748,30 @@ __device__ __forceinline__ float of_reverse_order(uint64_t o) { return unord_f32
 
 // a score that at least k of the workgroup's classes reach, so at least k columns do; kNone without k classes
 __device__ __forceinline__ float class_bound(const Maxima& m, int64_t k, Shared& sh) {
-    float least = INFINITY, most = kNone;
+    uint32_t least = 0, most = 0;  // reversed order bits, order bits
     uint64_t classes = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
         if (m.best[j] > kNone) {
             ++classes;
-            least = fminf(least, m.best[j]);
-            most = max_of(most, m.best[j]);
+            least = max(least, (uint32_t)reverse_order_of(m.best[j]));
+            most = max(most, (uint32_t)order_of(m.best[j]));
         }
     if (block_sum_u64(classes, sh) < (uint64_t)k) return kNone;
-    least = of_reverse_order(block_max_u64(reverse_order_of(least), sh));
-    most = unord_f32((uint32_t)block_max_u64(order_of(most), sh));
-    const Binning bin = make_binning(most, (double)most - (double)least);
-    clear_hist(sh);
+    block_max2(least, most, sh);
+    const float top = unord_f32(most);
+    const Binning bin = make_binning(top, (double)top - (double)of_reverse_order(least), kThreads);
+    clear_fine(sh);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-        if (m.best[j] > kNone) atomicAdd(&sh.count[bin(m.best[j])], 1u);
-    __syncthreads();
-    find_bin(sh.count, (double)k, sh);
+        if (m.best[j] > kNone) atomicAdd((unsigned long long*)&sh.wide[bin.fine(m.best[j])], 1ull);
+    find_fine((double)k, sh);
     // the least class at or before that bin
-    float bound = INFINITY;
+    uint64_t bound = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-        if (m.best[j] > kNone && bin(m.best[j]) <= (int)sh.bin) bound = fminf(bound, m.best[j]);
-    return of_reverse_order(block_max_u64(reverse_order_of(bound), sh));
+        if (m.best[j] > kNone && bin.fine(m.best[j]) <= (int)sh.bin) bound = max(bound, reverse_order_of(m.best[j]));
+    return of_reverse_order(block_max_u64(bound, sh));
 }
 
 // a list keys[0, kList), counted in n beyond that
@@ -724,6 +826,11 @@ __device__ __forceinline__ void count_steps(const void* s, int64_t lo, int64_t h
 // for each of them.  Past the first steps, where single columns weigh little, the middle is their place: they lie anywhere
 // in the step's width of d, an error of w d / (T sqrt 12) each.  Four times its root of squares, and 5e-6 of the whole
 // (the slope of their number within a step), are allowed for.
+__device__ __forceinline__ double exp2_step(double distance, const Weigh& weigh) {
+    Weigh one = weigh;
+    one.m = 0.0;
+    return one((float)-distance);
+}
 struct Window {
     int first, last;
     uint64_t columns;
@@ -734,19 +841,29 @@ __device__ __forceinline__ Window mass_window(const Binning& bin, double T, doub
     constexpr int per = kBins / kThreads;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const double wide = 1.0 / (double)bin.inv;
-    auto step_weight = [&](int b) {
-        const double place = b < kTopBins ? (double)sh.place[b] / (65536.0 * (double)sh.count[b]) : 0.5;
-        return weigh((float)((double)bin.top - wide * (b + place)));
-    };
-    double own = 0.0, square = 0.0;
-    for (int j = 0; j < per; ++j) {
-        const double c = (double)sh.count[tid * per + j];
-        if (c > 0.0) {
-            const double w = step_weight(tid * per + j);
-            own += c * w;
-            if (tid * per + j >= kTopBins) square += c * w * w;
+    const int b0 = tid * per;
+    double w[per], own = 0.0, square = 0.0;
+    uint32_t count[per];
+#pragma unroll
+    for (int j = 0; j < per; ++j) count[j] = sh.count[b0 + j];
+    if (b0 < kTopBins) {
+#pragma unroll
+        for (int j = 0; j < per; ++j) {
+            const float place = (float)sh.place[b0 + j] / (65536.0f * (float)max(count[j], 1u));
+            w[j] = (double)count[j] * weigh((float)((double)bin.top - wide * (b0 + j + (double)place)));
+        }
+    } else {
+        double x = weigh((float)((double)bin.top - wide * (b0 + 0.5)));
+        const double ratio = exp2_step(wide, weigh);
+#pragma unroll
+        for (int j = 0; j < per; ++j) {
+            w[j] = (double)count[j] * x;
+            square = fma(w[j], x, square);
+            x *= ratio;
         }
     }
+#pragma unroll
+    for (int j = 0; j < per; ++j) own += w[j];
     const double error = 4.0 * wide / (T * sqrt(12.0)) * sqrt(block_sum_f64(square, sh));
     const double incl = wave_scan_f64(own);
     __syncthreads();
@@ -755,34 +872,28 @@ __device__ __forceinline__ Window mass_window(const Binning& bin, double T, doub
     __syncthreads();
     double run = incl - own, sum = 0.0;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-        if (w < wave) run += sh.dpart[w];
-        sum += sh.dpart[w];
+    for (int v = 0; v < kWaves; ++v) {
+        if (v < wave) run += sh.dpart[v];
+        sum += sh.dpart[v];
     }
     const double all = (1.0 - 1e-13) * sum, t3 = fmin(top_p * sum, all);
-    const double t1 = t3 - 5e-6 * sum - error, t2 = fmin(t3 + 5e-6 * sum + error, all);
-    uint32_t f1 = kBins - 1, f2 = kBins - 1, f3 = kBins - 1;
+    const double t1 = fmax(t3 - 5e-6 * sum - error, 1e-300), t2 = fmin(t3 + 5e-6 * sum + error, all);
+#pragma unroll
     for (int j = 0; j < per; ++j) {
-        const int b = tid * per + j;
-        if (!sh.count[b]) continue;
-        run += (double)sh.count[b] * step_weight(b);
-        if (run >= t1) f1 = min(f1, (uint32_t)b);
-        if (run >= t2) f2 = min(f2, (uint32_t)b);
-        if (run >= t3) f3 = min(f3, (uint32_t)b);
+        const double next = run + w[j];
+        if (next >= t1 && run < t1) sh.bin = b0 + j;
+        if (next >= t2 && run < t2) sh.bin2 = b0 + j;
+        if (next >= t3 && run < t3) sh.bin3 = b0 + j;
+        run = next;
     }
-    if (f1 < kBins - 1) atomicMin(&sh.bin, f1);
-    if (f2 < kBins - 1) atomicMin(&sh.bin2, f2);
-    if (f3 < kBins - 1) atomicMin(&sh.bin3, f3);
     __syncthreads();
-    Window w{(int)sh.bin, (int)sh.bin2, 0, (float)sh.bin, (float)(sh.bin2 + 1)};
+    Window win{(int)sh.bin, (int)sh.bin2, 0, (float)sh.bin, (float)(sh.bin2 + 1)};
     uint64_t inside = 0;
-    for (int j = 0; j < per; ++j) {
-        const int b = tid * per + j;
-        if (b >= w.first && b <= w.last) inside += sh.count[b];
-    }
-    w.columns = block_sum_u64(inside, sh);
-    if (w.columns > kList) w = Window{(int)sh.bin3, (int)sh.bin3, sh.count[sh.bin3], (float)sh.bin3, (float)(sh.bin3 + 1)};
-    return w;
+#pragma unroll
+    for (int j = 0; j < per; ++j) inside += b0 + j >= win.first && b0 + j <= win.last ? count[j] : 0;
+    win.columns = block_sum_u64(inside, sh);
+    if (win.columns > kList) win = Window{(int)sh.bin3, (int)sh.bin3, sh.count[sh.bin3], (float)sh.bin3, (float)(sh.bin3 + 1)};
+    return win;
 }
 
 // One reading of the segments [g0, g1) with exact weights: z = all that the cut keeps, better = what lies before the
@@ -829,27 +940,28 @@ __device__ __forceinline__ void sum_window(const void* s, int64_t cols, const Se
 __device__ __forceinline__ bool resolve_window(int n, double z, double better, const Binning& bin, const Window& win, const Row& r, const Segments& segs, const Weigh& weigh, Cut& cut, Shared& sh) {
     const int tid = threadIdx.x;
     const double target = r.top_p * z, scale = ldexp(1.0, -weigh.unit);
-    // 2048 smaller steps within the window, of weights, and the columns of the one that reaches the target
-    constexpr int kFine = kBins / 2, per = kList / kThreads;
-    const float fine = (float)kFine / (win.to - win.from);
-    uint64_t mine[per], whole = 0;
+    // kThreads smaller steps within the window, of weights, and the columns of the one that reaches the target
+    constexpr int per = kList / kThreads;
+    const float fine = (float)kThreads / (win.to - win.from);
+    uint64_t mine[per], whole = 0, w[per];
     int at[per];
-    clear_hist(sh);
+    clear_fine(sh);
 #pragma unroll
     for (int j = 0; j < per; ++j) {
         mine[j] = tid + j * kThreads < n ? sh.key[tid + j * kThreads] : 0;
         at[j] = -1;
+        w[j] = 0;
         if (mine[j]) {
             const float v = key_score(mine[j]);
-            const uint64_t w = weigh.fixed(v);
-            whole += w;
-            at[j] = min(kFine - 1, (int)((bin.at(v) - win.from) * fine));
-            atomicAdd((unsigned long long*)&sh.wide[at[j]], (unsigned long long)w);
+            w[j] = weigh.fixed(v);
+            whole += w[j];
+            at[j] = min(kThreads - 1, (int)((bin.at(v) - win.from) * fine));
+            atomicAdd((unsigned long long*)&sh.wide[at[j]], (unsigned long long)w[j]);
         }
     }
     whole = block_sum_u64(whole, sh);
-    if (!(better < target && better + (double)whole * scale >= target)) return false;
-    find_bin(sh.wide, (target - better) / scale, sh);
+    if (!whole || !(better < target && better + (double)whole * scale >= target)) return false;
+    find_fine((target - better) / scale, sh);
     const int b = (int)sh.bin;
     const double before = better + (double)sh.below * scale;
     __syncthreads();
@@ -858,7 +970,7 @@ __device__ __forceinline__ bool resolve_window(int n, double z, double better, c
         if (at[j] == b) {
             const uint32_t k = atomicAdd(&sh.n, 1u);
             sh.key[k] = mine[j];
-            sh.wide[k] = weigh.fixed(key_score(mine[j]));
+            sh.wide[k] = w[j];
         }
     __syncthreads();
     // each thread adds up what ranks before its columns: the last one below the target is the cut
@@ -881,7 +993,7 @@ __device__ __forceinline__ bool resolve_window(int n, double z, double better, c
         const uint64_t k = mine[j];
         const float v = key_score(k);
         if (k && k >= key && weigh(v) >= r.min_p)
-            atomicAdd((unsigned long long*)&sh.wide[key_index(k) / segs.len], (unsigned long long)weigh.fixed_kept(v));
+            atomicAdd((unsigned long long*)&sh.wide[(uint32_t)key_index(k) / (uint32_t)segs.len], (unsigned long long)weigh.fixed_kept(v));
     }
     __syncthreads();
     for (int j = tid; j < segs.n; j += kThreads) sh.seg[j + 1] += (double)sh.wide[j] * scale;
@@ -918,8 +1030,7 @@ __device__ __forceinline__ void draw_columns(const SampleArgs& a, int64_t row, c
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     __syncthreads();
     if (tid < 64) {
-        constexpr int per = kSegs / 64;
-        const int lo = lane * per, hi = min(segs.n, lo + per);
+        const int per = (segs.n + 63) / 64, lo = lane * per, hi = min(segs.n, lo + per);
         double own = 0.0;
         for (int j = lo; j < hi; ++j) own += sh.seg[j + 1];
         double run = wave_scan_f64(own) - own;
@@ -939,43 +1050,57 @@ __device__ __forceinline__ void draw_columns(const SampleArgs& a, int64_t row, c
         }
         const int64_t end = min(a.cols, (lo + 1) * segs.len);
         double run = sh.seg[lo];
-        int64_t pick = -1;
+        int64_t pick = -1, fallback = -1;  // without a column past the target: the segment's last of any weight
         double wp = 0.0;
-        for (int64_t i0 = lo * segs.len; i0 < end; i0 += kStep) {
-            Vec<BF16> v;
-            const int64_t i = i0 + lane * N;
-            if (i + N <= end)
-                v.load(s, i);
-            else
-                v.load_tail(s, i, end);
-            double w[N], own = 0.0;
+        // four steps of the wave on their way at once
+        constexpr int kAhead = 4;
+        for (int64_t i0 = lo * segs.len; i0 < end && pick < 0; i0 += kAhead * kStep) {
+            float v[kAhead][4];
 #pragma unroll
-            for (int k = 0; k < N; ++k) own += w[k] = kept_weight(v.v[k], (int)i + k, cut, weigh, r.min_p);
-            double c = run + wave_scan_f64(own) - own;
-            // this lane's first column past the target, or without one its last of any weight
-            int at = -1, tail = -1;
-            double wa = 0.0, wt = 0.0;
-#pragma unroll
-            for (int k = 0; k < N; ++k) {
-                c += w[k];
-                if (w[k] > 0.0) {
-                    tail = k;
-                    wt = w[k];
-                    if (at < 0 && c > target) {
-                        at = k;
-                        wa = w[k];
-                    }
+            for (int t = 0; t < kAhead; ++t) {
+                const int64_t i = i0 + t * kStep + lane * N;
+                if (i + N <= end) {
+                    Vec<BF16> x;
+                    x.load(s, i);
+                    x.values(v[t]);
+                } else {
+                    load_tail<BF16>(v[t], s, i, end);
                 }
             }
-            const uint64_t pass = __ballot(at >= 0), any = __ballot(tail >= 0);
-            if (any) {
-                const int l = pass ? __builtin_ctzll(pass) : 63 - __builtin_clzll(any);
-                pick = i0 + l * N + __shfl(pass ? at : tail, l, 64);
-                wp = shfl_f64(pass ? wa : wt, l);
-                if (pass) break;
+#pragma unroll
+            for (int t = 0; t < kAhead; ++t) {
+                if (pick >= 0) break;
+                const int64_t i = i0 + t * kStep + lane * N;
+                double w[N], own = 0.0;
+#pragma unroll
+                for (int k = 0; k < N; ++k) own += w[k] = kept_weight(v[t][k], (int)i + k, cut, weigh, r.min_p);
+                double c = run + wave_scan_f64(own) - own;
+                // this lane's first column past the target, or without one its last of any weight
+                int at = -1, tail = -1;
+                double wa = 0.0, wt = 0.0;
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    c += w[k];
+                    if (w[k] > 0.0) {
+                        tail = k;
+                        wt = w[k];
+                        if (at < 0 && c > target) {
+                            at = k;
+                            wa = w[k];
+                        }
+                    }
+                }
+                const uint64_t pass = __ballot(at >= 0), any = __ballot(tail >= 0);
+                if (any) {
+                    const int l = pass ? __builtin_ctzll(pass) : 63 - __builtin_clzll(any);
+                    const int64_t col = i0 + t * kStep + l * N + __shfl(pass ? at : tail, l, 64);
+                    wp = shfl_f64(pass ? wa : wt, l);
+                    if (pass) pick = col; else fallback = col;
+                }
+                run = shfl_f64(c, 63);
             }
-            run = shfl_f64(c, 63);
         }
+        if (pick < 0) pick = fallback;
         if (lane == 0) {
             a.out_idx[row * a.n_draws + j] = (int32_t)pick;
             if (a.out_prob) a.out_prob[row * a.n_draws + j] = (float)(wp / total);
@@ -1017,8 +1142,9 @@ __device__ __forceinline__ void draw_list(const SampleArgs& a, int64_t row, cons
         finish_list(a, row, r, n, Weigh(key_score(best), r.T, (int)a.cols), sh);
 }
 
-// A whole row by one workgroup
-template <bool BF16>
+// A whole row by one workgroup.  K, P: there may be a top_k, a top_p (a kernel without the one's steps keeps its weights in
+// registers)
+template <bool BF16, bool K, bool P>
 __device__ __forceinline__ void sample_row(const SampleArgs& a, int64_t row, const Row& r, Shared& sh) {
     const int tid = threadIdx.x;
     const void* s = row_scores<BF16>(a, row);
@@ -1028,7 +1154,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int64_t row, con
         all_draws(a, row, best ? key_index(best) : -1, best ? 1.0f : 0.0f);
         return;
     }
-    const bool by_k = listed(a, r), by_p = r.top_p < 1.0;
+    const bool by_k = K && listed(a, r), by_p = P && r.top_p < 1.0;
     const auto to_list = [&](uint64_t key) { push(sh.key, &sh.n, key); };
     // the list of the columns that reach the bound of the first ones
     if (by_k && r.top_k <= kList / 2) {
@@ -1093,7 +1219,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int64_t row, con
         const Window win = mass_window(bin, r.T, r.top_p, weigh, sh);
         if (win.usable()) {
             double z, better;
-            if (by_k)
+            if (K && by_k)
                 sum_window<BF16, false>(s, cols, segs, 0, segs.n, bin, win, cut, weigh, r.min_p, to_list, to_seg, z, better);
             else
                 sum_window<BF16, true>(s, cols, segs, 0, segs.n, bin, win, cut, weigh, r.min_p, to_list, to_seg, z, better);
@@ -1117,10 +1243,10 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int64_t row, con
     draw_columns<BF16>(a, row, r, s, segs, cut, weigh, 0, 1, sh);
 }
 
-template <bool BF16>
+template <bool BF16, bool K, bool P>
 __global__ __launch_bounds__(kThreads, 6) void sample_rows_kernel(SampleArgs a) {
     __shared__ Shared sh;
-    sample_row<BF16>(a, blockIdx.x, row_settings(a, blockIdx.x), sh);
+    sample_row<BF16, K, P>(a, blockIdx.x, row_settings(a, blockIdx.x), sh);
 }
 
 // ------------------------------------------------------------------------------------ few long rows
@@ -1335,7 +1461,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_split_draw(SampleArgs a, S
     }
     if (alone) {
         __syncthreads();
-        if (first) sample_row<BF16>(a, row, r, sh);
+        if (first) sample_row<BF16, true, true>(a, row, r, sh);
         return;
     }
     draw_columns<BF16>(a, row, r, s, segs, cut, weigh, blockIdx.x, gridDim.x, sh);
@@ -1365,7 +1491,13 @@ struct SplitLayout {
 template <bool BF16>
 int launch_sample(const SampleArgs& a, void* ws, int parts, hipStream_t stream) {
     if (parts == 1) {
-        sample_rows_kernel<BF16><<<(unsigned)a.rows, kThreads, 0, stream>>>(a);
+        const unsigned grid = (unsigned)a.rows;
+        if (a.k_rows || (a.top_k > 0 && a.top_k < a.cols))
+            sample_rows_kernel<BF16, true, true><<<grid, kThreads, 0, stream>>>(a);
+        else if (a.p_rows || a.top_p < 1.0)
+            sample_rows_kernel<BF16, false, true><<<grid, kThreads, 0, stream>>>(a);
+        else
+            sample_rows_kernel<BF16, false, false><<<grid, kThreads, 0, stream>>>(a);
         LGX_LAUNCH_CHECK();
         return LGX_OK;
     }
