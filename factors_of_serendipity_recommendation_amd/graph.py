@@ -321,7 +321,13 @@ class CSRGraph:
                               self.indptr.cpu().numpy()), shape=(self.n_rows, self.n_cols))
 
 
+# the current stream's handle without a Stream object around it (2 us of a small call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream_ptr(device: torch.device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 

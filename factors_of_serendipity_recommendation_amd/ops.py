@@ -6,6 +6,7 @@ is no CPU path.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 from typing import Optional, Sequence, Tuple
@@ -512,6 +513,13 @@ class MXTable:
             raise ValueError("MXTable: codes and scales must be contiguous, codes 16-byte aligned")
         self.codes, self.scales, self.d = codes, scales, int(d)
 
+    @classmethod
+    def _packed(cls, codes: torch.Tensor, scales: torch.Tensor, d: int) -> "MXTable":
+        """mx_quantize's own output, which needs no checks (they cost more than a small table's kernel)."""
+        t = object.__new__(cls)
+        t.codes, t.scales, t.d = codes, scales, d
+        return t
+
     @property
     def shape(self) -> Tuple[int, int]:
         return (self.codes.shape[0], self.d)
@@ -532,6 +540,15 @@ class MXTable:
         return MXTable(self.codes.to(device), self.scales.to(device), self.d)
 
 
+_HERE = contextlib.nullcontext()
+
+
+def _on(dev: torch.device):
+    """The context of a call on `dev`: nothing where that is the current device already (entering and
+    leaving torch.cuda.device costs as much as a small launch)."""
+    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
 def _one_device(what: str, *tensors) -> torch.device:
     """The device all the given tensors (None skipped) live on; the call runs there, whatever the
     current device is."""
@@ -545,9 +562,11 @@ def _one_device(what: str, *tensors) -> torch.device:
 def _row_stride(x: torch.Tensor) -> Tuple[torch.Tensor, int]:
     """x [rows, cols] with unit column stride and a row stride of at least cols, and that stride
     (copied only where the given strides are others)."""
-    if x.stride(1) != 1 and x.shape[1] > 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
-        x = x.contiguous()
-    return x, max(x.stride(0), x.shape[1]) if x.shape[0] > 1 else x.shape[1]
+    rows, cols = x.shape
+    ld, unit = x.stride()
+    if (unit != 1 and cols > 1) or (rows > 1 and ld < cols):
+        x, ld = x.contiguous(), cols
+    return x, ld if rows > 1 else cols
 
 
 def mx_quantize(x: torch.Tensor) -> MXTable:
@@ -562,22 +581,23 @@ def mx_quantize(x: torch.Tensor) -> MXTable:
     x, ld = _row_stride(x)
     rows, d = x.shape
     nb = -(-d // MX_BLOCK)
-    with torch.cuda.device(x.device):
-        codes = torch.empty((rows, 16 * nb), dtype=torch.uint8, device=x.device)
-        scales = torch.empty((rows, nb), dtype=torch.uint8, device=x.device)
+    with _on(x.device):
+        codes = x.new_empty((rows, 16 * nb), dtype=torch.uint8)
+        scales = x.new_empty((rows, nb), dtype=torch.uint8)
         _lib.check(_lib.lib().lgx_mx_quantize(x.data_ptr(), rows, d, ld, dt, codes.data_ptr(), scales.data_ptr(),
                                               _stream_ptr(x.device)), "lgx_mx_quantize")
-    return MXTable(codes, scales, d)
+    return MXTable._packed(codes, scales, d)
 
 
 def mx_dequantize(table: MXTable, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The values of an MXTable as f32 or bf16 [rows, d] (``lgx_mx_dequantize``; exact in both)."""
     require_gpu(table.codes)
-    out = torch.empty(table.shape, dtype=dtype, device=table.device)
+    codes, rows, dev = table.codes, table.codes.shape[0], table.codes.device
+    out = codes.new_empty((rows, table.d), dtype=dtype)
     dt = _dtype_code(out)
-    with torch.cuda.device(table.device):
-        _lib.check(_lib.lib().lgx_mx_dequantize(table.codes.data_ptr(), table.scales.data_ptr(), len(table), table.d, dt,
-                                                out.data_ptr(), _stream_ptr(table.device)), "lgx_mx_dequantize")
+    with _on(dev):
+        _lib.check(_lib.lib().lgx_mx_dequantize(codes.data_ptr(), table.scales.data_ptr(), rows, table.d, dt,
+                                                out.data_ptr(), _stream_ptr(dev)), "lgx_mx_dequantize")
     return out
 
 
@@ -603,16 +623,16 @@ def score_mx(Q, items: MXTable, user_rows: Optional[torch.Tensor] = None, apply_
     if user_rows is not None and user_rows.dim() != 1:
         raise ValueError(f"score_mx: user_rows must be one-dimensional, got {tuple(user_rows.shape)}")
     B = user_rows.numel() if user_rows is not None else n_q
-    with torch.cuda.device(dev):
+    with _on(dev):
         rows = user_rows.to(torch.int64).contiguous() if user_rows is not None else None
         if out is None:
-            out = torch.empty((B, n_items), dtype=dtype, device=dev)
+            out = q.new_empty((B, n_items), dtype=dtype)
         elif out.dtype != dtype or tuple(out.shape) != (B, n_items) or not out.is_contiguous():
             raise ValueError(f"score_mx: out must be a contiguous {dtype} [{B}, {n_items}] on {dev}")
         L = _lib.lib()
         ws = ctypes.c_size_t(0)
         _lib.check(L.lgx_score_mx_workspace(B, d, q_dt, ctypes.byref(ws)), "lgx_score_mx_workspace")
-        work = torch.empty(ws.value, dtype=torch.uint8, device=dev) if ws.value else None
+        work = q.new_empty(ws.value, dtype=torch.uint8) if ws.value else None
         _lib.check(L.lgx_score_mx(q.data_ptr(), Q.scales.data_ptr() if packed else None, q_dt, n_q, q_ld, _ptr(rows),
                                   items.codes.data_ptr(), items.scales.data_ptr(), B, n_items, d, int(apply_sigmoid),
                                   _dtype_code(out), out.data_ptr(), _ptr(work), ws.value, _stream_ptr(dev)),
@@ -662,13 +682,13 @@ def sample_rows(S: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     if u.dim() not in (1, 2) or u.shape[0] != rows:
         raise ValueError(f"sample_rows: u must be [{rows}] or [{rows}, n], got {tuple(u.shape)}")
     n = u.shape[1] if u.dim() == 2 else 1
-    with torch.cuda.device(dev):
+    with _on(dev):
         t, t_rows = _row_setting("temperature", temperature, rows, dev, torch.float32, 0.0, float("inf"))
         k, k_rows = _row_setting("top_k", top_k, rows, dev, torch.int32, 0, 2 ** 63 - 1)
         p, p_rows = _row_setting("top_p", top_p, rows, dev, torch.float32, 0.0, 1.0)
         m, m_rows = _row_setting("min_p", min_p, rows, dev, torch.float32, 0.0, 1.0)
-        idx = torch.empty(u.shape, dtype=torch.int32, device=dev)
-        prob = torch.empty(u.shape, dtype=torch.float32, device=dev)
+        idx = u.new_empty(u.shape, dtype=torch.int32)
+        prob = u.new_empty(u.shape, dtype=torch.float32)
         if cols == 0:
             return idx.fill_(-1), prob.zero_()
         S, ld = _row_stride(S)
@@ -676,7 +696,7 @@ def sample_rows(S: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
         L = _lib.lib()
         ws = ctypes.c_size_t(0)
         _lib.check(L.lgx_sample_rows_workspace(rows, cols, n, ctypes.byref(ws)), "lgx_sample_rows_workspace")
-        work = torch.empty(ws.value, dtype=torch.uint8, device=dev) if ws.value else None
+        work = u.new_empty(ws.value, dtype=torch.uint8) if ws.value else None
         _lib.check(L.lgx_sample_rows(S.data_ptr(), dt, rows, cols, ld, u.data_ptr(),
                                      _lib.LGX_DTYPE_F64 if u.dtype == torch.float64 else _lib.LGX_DTYPE_F32, n, float(t),
                                      _ptr(t_rows), int(k), _ptr(k_rows), float(p), _ptr(p_rows), float(m), _ptr(m_rows),
