@@ -7,6 +7,7 @@
 #include "lgx_common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace lgx {
 namespace {
@@ -345,35 +346,113 @@ __global__ __launch_bounds__(256, 2) void score_mx_short(MxArgs a) {
     }
 }
 
-// Longer rows: a wave holds 64 users x 128 items of results and walks the blocks, 8 at a
-// time.  WU waves of
-// the workgroup take the next 64 users each, the others the next 128 items.
-template <int WU, bool BF16, bool SIG, bool NT>
-__global__ __launch_bounds__(256, 2) void score_mx_long(MxArgs a) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col = lane & 31;
-    const int64_t base = (blockIdx.x * (int64_t)(4 / WU) + wave / WU) * 128;
-    const int64_t u0 = (blockIdx.y * (int64_t)WU + wave % WU) * 64;
-    if (base >= a.n_items || u0 >= a.B) return;
-    const int64_t r0 = query_row(a, u0 + col), r1 = query_row(a, u0 + 32 + col);
-    f32x16 acc0[4] = {}, acc1[4] = {};
-    const uint8_t* codes = a.it + base * a.nb * 16;
-    const uint8_t* scales = a.its + base * a.nb;
-    uint32_t rows[4];
+// Longer rows.  A workgroup holds UW x NU x 32 users against 4 / UW x 128 items, a wave NU x 32 x 128 of them, and walks the
+// blocks 8 at a time through LDS: read from there a row's 16 bytes a lane cost a line each (333 x 91,599 x 1000: 93 us, its
+// address unit busy throughout), while 8 lanes fetch the 128 bytes of a row together.  The next 8 blocks are on their way
+// in registers during the products.  Block b of a row lies at slot b ^ (r % 8) of the row's 128 bytes, of an item's at b ^ (r / 4 %
+// 8), so that 8 lanes that read one block of 8 rows (items: every fourth) touch all banks.
+template <int UW, int NU, bool BF16, bool SIG, bool NT>
+__global__ __launch_bounds__(256, 2) void score_mx_long(MxArgs a, int user_tiles) {
+    constexpr int kUsers = UW * NU * 32, kItems = 4 / UW * 128, kRows = kUsers + kItems;
+    constexpr int kUnits = kRows / 32, kScales = (kRows + 255) / 256;
+    __shared__ u32x4 codes[kRows * 8];
+    __shared__ uint32_t scales[kRows * 2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // the user tiles of one item tile run side by side on one XCD (workgroups go to the 8 XCDs in turn)
+    const int64_t turn = blockIdx.x / 8;
+    const int64_t base = (turn / user_tiles * 8 + blockIdx.x % 8) * kItems, u0 = turn % user_tiles * kUsers;
+    if (base >= a.n_items) return;
+    const int nb = (int)a.nb, blk = tid & 7, row0 = tid >> 3;
+    const uint8_t* it = a.it + base * nb * 16;
+    const uint8_t* its = a.its + base * nb;
+    const int last_item = (int)min((int64_t)kItems, a.n_items - base) - 1;  // rows past it repeat it
+    int64_t q_row[UW * NU];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) rows[t] = item_row(a, base, 4 * col + t);
-    for (int k0 = 0; k0 < (int)a.nb; k0 += 8) {
-        const int first = k0 + 4 * (lane >> 5);
-        Frag<4> it[4], q0, q1;
-        load_query<4>(q0, a, r0, first);
-        load_query<4>(q1, a, r1, first);
+    for (int j = 0; j < UW * NU; ++j) q_row[j] = query_row(a, u0 + row0 + 32 * j);
+    int64_t s_row[kScales];  // users: as query_row; items: the row
 #pragma unroll
-        for (int t = 0; t < 4; ++t) load_frag<4, uint32_t>(it[t], codes, scales, rows[t], (int)a.nb, first, true);
-        mma_steps<4>(acc0, q0, it);
-        mma_steps<4>(acc1, q1, it);
+    for (int j = 0; j < kScales; ++j) {
+        const int r = tid + 256 * j;
+        s_row[j] = r < kUsers ? query_row(a, u0 + r) : min(r - kUsers, last_item);
     }
-    store_tile<BF16, SIG, NT>(a, acc0, u0, base, lane);
-    if (u0 + 32 < a.B) store_tile<BF16, SIG, NT>(a, acc1, u0 + 32, base, lane);
+    u32x4 c[kUnits];
+    uint32_t sc[kScales][2];
+    auto fetch = [&](int k0) {
+        const bool in = k0 + blk < nb;
+#pragma unroll
+        for (int j = 0; j < kUnits; ++j) {
+            c[j] = u32x4{0, 0, 0, 0};
+            if (j < UW * NU) {
+                if (in && q_row[j < UW * NU ? j : 0] >= 0)
+                    c[j] = *reinterpret_cast<const u32x4*>(a.q + (q_row[j < UW * NU ? j : 0] * nb + k0 + blk) * 16);
+            } else if (in) {
+                const uint32_t r = (uint32_t)min(row0 + 32 * (j - UW * NU), last_item);
+                c[j] = *reinterpret_cast<const u32x4*>(it + (r * (uint32_t)nb + (uint32_t)(k0 + blk)) * 16u);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kScales; ++j) {
+            const int r = tid + 256 * j;
+            const bool user = r < kUsers;
+            sc[j][0] = sc[j][1] = user && s_row[j] == -2 ? 0xffffffffu : 0x7f7f7f7fu;
+            if (r >= kRows || s_row[j] < 0) continue;
+            const uint8_t* p = user ? a.qs + s_row[j] * nb + k0 : its + s_row[j] * nb + k0;
+            if (k0 + 8 <= nb) {
+                sc[j][0] = *reinterpret_cast<const u32u*>(p);
+                sc[j][1] = *reinterpret_cast<const u32u*>(p + 4);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (k0 + k < nb) sc[j][k / 4] ^= (0x7fu ^ p[k]) << (8 * (k % 4));
+            }
+        }
+    };
+    auto stage = [&]() {
+#pragma unroll
+        for (int j = 0; j < kUnits; ++j) codes[(row0 + 32 * j) * 8 + (blk ^ ((j < UW * NU ? row0 : row0 >> 2) & 7))] = c[j];
+#pragma unroll
+        for (int j = 0; j < kScales; ++j)
+            if (tid + 256 * j < kRows) {
+                scales[(tid + 256 * j) * 2] = sc[j][0];
+                scales[(tid + 256 * j) * 2 + 1] = sc[j][1];
+            }
+    };
+    const int col = lane & 31, half = lane >> 5;
+    const int users = wave % UW * NU * 32, items = wave / UW * 128;  // this wave's within the workgroup's
+    f32x16 acc[NU][4] = {};
+    fetch(0);
+    for (int k0 = 0; k0 < nb; k0 += 8) {
+        __syncthreads();
+        stage();
+        __syncthreads();
+        if (k0 + 8 < nb) fetch(k0 + 8);
+        uint32_t sq[NU], si[4];
+#pragma unroll
+        for (int u = 0; u < NU; ++u) sq[u] = scales[(users + 32 * u + col) * 2 + half];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) si[t] = scales[(kUsers + items + 4 * col + t) * 2 + half];
+        auto step = [&](auto kk) {
+            constexpr int KK = decltype(kk)::value;
+            u32x4 q[NU];
+#pragma unroll
+            for (int u = 0; u < NU; ++u) q[u] = codes[(users + 32 * u + col) * 8 + ((4 * half + KK) ^ (col & 7))];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int r = kUsers + items + 4 * col + t;
+                const u32x4 x = codes[r * 8 + ((4 * half + KK) ^ (col & 7))];
+#pragma unroll
+                for (int u = 0; u < NU; ++u) acc[u][t] = mma<KK>(q[u], x, acc[u][t], sq[u], si[t]);
+            }
+        };
+        step(std::integral_constant<int, 0>{});
+        step(std::integral_constant<int, 1>{});
+        step(std::integral_constant<int, 2>{});
+        step(std::integral_constant<int, 3>{});
+    }
+    if (base + items >= a.n_items) return;
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+        if (u0 + users + 32 * u < a.B) store_tile<BF16, SIG, NT>(a, acc[u], u0 + users + 32 * u, base + items, lane);
 }
 
 template <bool BF16, bool SIG, bool NT>
@@ -390,13 +469,14 @@ int launch_score(const MxArgs& a, hipStream_t stream) {
             default: score_mx_short<4, BF16, SIG, NT><<<grid, 256, 0, stream>>>(a); break;
         }
     } else {
-        const int wu = a.B > 128 ? 4 : a.B > 64 ? 2 : 1;  // waves side by side over the users
-        const int64_t gy = ceil_div(a.B, (int64_t)(64 * wu));
-        LGX_REQUIRE(gy < 65536, LGX_ERR_UNSUPPORTED, "lgx_score_mx: %lld queries is too many", (long long)a.B);
-        const dim3 grid((unsigned)ceil_div(a.n_items, (int64_t)(512 / wu)), (unsigned)gy);
-        if (wu == 4) score_mx_long<4, BF16, SIG, NT><<<grid, 256, 0, stream>>>(a);
-        else if (wu == 2) score_mx_long<2, BF16, SIG, NT><<<grid, 256, 0, stream>>>(a);
-        else score_mx_long<1, BF16, SIG, NT><<<grid, 256, 0, stream>>>(a);
+        // two waves side by side over the users where there are enough of them
+        const int uw = a.B > 32 ? 2 : 1, nu = a.B > 64 ? 2 : 1;
+        const int64_t user_tiles = ceil_div(a.B, (int64_t)(uw * nu * 32));
+        const int64_t grid = 8 * ceil_div(ceil_div(a.n_items, (int64_t)(512 / uw)), (int64_t)8) * user_tiles;
+        LGX_REQUIRE(grid < (1LL << 31), LGX_ERR_UNSUPPORTED, "lgx_score_mx: %lld queries is too many", (long long)a.B);
+        if (nu == 2) score_mx_long<2, 2, BF16, SIG, NT><<<(unsigned)grid, 256, 0, stream>>>(a, (int)user_tiles);
+        else if (uw == 2) score_mx_long<2, 1, BF16, SIG, NT><<<(unsigned)grid, 256, 0, stream>>>(a, (int)user_tiles);
+        else score_mx_long<1, 1, BF16, SIG, NT><<<(unsigned)grid, 256, 0, stream>>>(a, (int)user_tiles);
     }
     LGX_LAUNCH_CHECK();
     return LGX_OK;
