@@ -46,6 +46,18 @@ __device__ __forceinline__ void load8_bf16(const uint16_t* p, float (&x)[8]) {
     }
 }
 
+// two values to bf16, round to nearest even (one instruction)
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+    using B2 = __bf16 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), B2));
+}
+
+// the scale byte of a block whose largest magnitude has the bits a
+__device__ __forceinline__ uint32_t scale_byte(uint32_t a) {
+    const uint32_t e = a >> 23;
+    return e == 255u ? 255u : e > 2u ? e - 2u : 0u;
+}
+
 // 4 lanes per block, 8 elements a lane.  VEC: rows are 16-byte aligned and d % 8 == 0.  rows_of (optional):
 // the source row of every output row, a row outside [0, n_src) gives NaN blocks.
 template <bool BF16, bool VEC>
@@ -85,9 +97,8 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const void* __restrict
     for (int j = 0; j < 8; ++j) a = max(a, __float_as_uint(x[j]) & 0x7fffffffu);
     a = max(a, (uint32_t)__shfl_xor((int)a, 1));
     a = max(a, (uint32_t)__shfl_xor((int)a, 2));
-    const uint32_t e = a >> 23;
-    bad |= e == 255u;  // an infinity or a NaN
-    const uint32_t b = bad ? 255u : e > 2u ? e - 2u : 0u;
+    const uint32_t b = bad ? 255u : scale_byte(a);
+    bad |= b == 255u;
     const float inv = __uint_as_float((254u - b) << 23);  // 2^(127 - b), b <= 252
     float y[8];
 #pragma unroll
@@ -126,7 +137,7 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint8_t* __res
         if (VEC) {
             u32x4 w;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = f32_to_bf16(v[2 * j]) | (uint32_t)f32_to_bf16(v[2 * j + 1]) << 16;
+            for (int j = 0; j < 4; ++j) w[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
             *reinterpret_cast<u32x4*>(o) = w;
         } else {
 #pragma unroll
@@ -161,6 +172,8 @@ struct MxArgs {
     const uint8_t* its;
     int64_t B, n_items, nb;
     void* out;
+    int64_t d, q_ld;  // of f32 / bf16 queries
+    bool q_vec;       // their rows start at multiples of 16 bytes and d % 8 == 0
 };
 
 __device__ __forceinline__ i32x8 frag(u32x4 v) {
@@ -233,8 +246,51 @@ __device__ __forceinline__ int64_t query_row(const MxArgs& a, int64_t b) {
     const int64_t r = a.user_rows[b];
     return r >= 0 && r < a.n_q ? r : -2;
 }
-template <int HB>
+// QD: the queries' type.  f32 and bf16 ones are quantised here, 32 elements of a row by one lane
+template <int QD, int HB>
 __device__ __forceinline__ void load_query(Frag<HB>& f, const MxArgs& a, int64_t row, int first) {
+    if (QD != LGX_DTYPE_MXFP4) {
+        f.s = 0x7f7f7f7fu;
+#pragma unroll
+        for (int kk = 0; kk < HB; ++kk) {
+            f.c[kk] = u32x4{0, 0, 0, 0};
+            const int c0 = (first + kk) * kBlock;
+            if (row < 0 || c0 >= a.d) continue;
+            float x[4][8] = {};
+            uint32_t most = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int64_t at = row * a.q_ld + c0 + 8 * i;
+                if (a.q_vec) {
+                    if (c0 + 8 * i < a.d) {
+                        if (QD == LGX_DTYPE_BF16)
+                            load8_bf16(reinterpret_cast<const uint16_t*>(a.q) + at, x[i]);
+                        else
+                            load8_f32(reinterpret_cast<const float*>(a.q) + at, x[i]);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (c0 + 8 * i + j < a.d)
+                            x[i][j] = QD == LGX_DTYPE_BF16 ? bf16_to_f32(reinterpret_cast<const uint16_t*>(a.q)[at + j])
+                                                           : reinterpret_cast<const float*>(a.q)[at + j];
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(x[i][j]) & 0x7fffffffu);
+            }
+            const uint32_t b = scale_byte(most);
+            const float inv = __uint_as_float((254u - b) << 23);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[i][j] *= inv;
+                f.c[kk][i] = b == 255u ? 0u : pack8(x[i]);
+            }
+            f.s ^= (0x7fu ^ b) << (8 * kk);
+        }
+        if (row == -2) f.s = 0xffffffffu;
+        return;
+    }
     load_frag<HB, int64_t>(f, a.q, a.qs, row, (int)a.nb, first, row >= 0);
     if (row == -2) f.s = 0xffffffffu;  // NaN scales
 }
@@ -292,9 +348,7 @@ __device__ __forceinline__ void store_tile(const MxArgs& a, const f32x16 (&acc)[
         if (BF16) {
             uint16_t* o = static_cast<uint16_t*>(a.out) + (u0 + r) * a.n_items + base + off;
             if (left >= 4) {
-                put<NT>(u32x2u{f32_to_bf16(v[0]) | (uint32_t)f32_to_bf16(v[1]) << 16,
-                               f32_to_bf16(v[2]) | (uint32_t)f32_to_bf16(v[3]) << 16},
-                        reinterpret_cast<u32x2u*>(o));
+                put<NT>(u32x2u{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])}, reinterpret_cast<u32x2u*>(o));
             } else {
                 o[0] = f32_to_bf16(v[0]);
                 if (left > 1) o[1] = f32_to_bf16(v[1]);
@@ -335,14 +389,47 @@ __global__ __launch_bounds__(256, 2) void score_mx_short(MxArgs a) {
     for (int t = 0; t < 4; ++t)
         load_frag<HB, uint32_t>(it[t], a.it + base * a.nb * 16, a.its + base * a.nb, item_row(a, base, 4 * col + t), (int)a.nb,
                                 first, true);
-    load_query<HB>(q, a, query_row(a, u0 + col), first);
+    load_query<LGX_DTYPE_MXFP4, HB>(q, a, query_row(a, u0 + col), first);
     for (; u0 < u_end; u0 += 32) {
         Frag<HB> next;
-        if (u0 + 32 < u_end) load_query<HB>(next, a, query_row(a, u0 + 32 + col), first);
+        if (u0 + 32 < u_end) load_query<LGX_DTYPE_MXFP4, HB>(next, a, query_row(a, u0 + 32 + col), first);
         f32x16 acc[4] = {};
         mma_steps<HB>(acc, q, it);
         store_tile<BF16, SIG, NT>(a, acc, u0, base, lane);
         copy_frag<HB>(q, next);
+    }
+}
+
+// The same for one tile of users: a wave keeps that, quantised by itself, and walks the items, the next 128 on their way.
+// Bound by the reading of the table.
+template <int QD, int HB, bool BF16, bool SIG, bool NT>
+__global__ __launch_bounds__(256, 2) void score_mx_few(MxArgs a) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 31;
+    const int first = HB * (lane >> 5);
+    const int64_t stride = gridDim.x * (int64_t)512;
+    int64_t base = (blockIdx.x * (int64_t)4 + wave) * 128;
+    if (base >= a.n_items) return;
+    auto load_items = [&](Frag<HB> (&it)[4], int64_t at) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+            load_frag<HB, uint32_t>(it[t], a.it + at * a.nb * 16, a.its + at * a.nb, item_row(a, at, 4 * col + t), (int)a.nb, first, true);
+    };
+    Frag<HB> it[4], q;
+    load_items(it, base);
+    load_query<QD, HB>(q, a, query_row(a, col), first);
+#pragma unroll 1
+    for (;;) {
+        const int64_t next_base = base + stride;
+        Frag<HB> next[4];
+        if (next_base < a.n_items) load_items(next, next_base);
+        f32x16 acc[4] = {};
+        mma_steps<HB>(acc, q, it);
+        store_tile<BF16, SIG, NT>(a, acc, 0, base, lane);
+        if (next_base >= a.n_items) break;
+        base = next_base;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) copy_frag<HB>(it[t], next[t]);
     }
 }
 
@@ -455,19 +542,30 @@ __global__ __launch_bounds__(256, 2) void score_mx_long(MxArgs a, int user_tiles
         if (u0 + users + 32 * u < a.B) store_tile<BF16, SIG, NT>(a, acc[u], u0 + users + 32 * u, base + items, lane);
 }
 
+#define LGX_MX_STEPS(KERNEL, ...)                                        \
+    switch ((a.nb + 1) / 2) {                                            \
+        case 1: KERNEL(1, __VA_ARGS__); break;                           \
+        case 2: KERNEL(2, __VA_ARGS__); break;                           \
+        case 3: KERNEL(3, __VA_ARGS__); break;                           \
+        default: KERNEL(4, __VA_ARGS__); break;                          \
+    }
+#define LGX_MX_FEW(HB, QD) score_mx_few<QD, HB, BF16, SIG, NT><<<grid, 256, 0, stream>>>(a)
+#define LGX_MX_SHORT(HB, ...) score_mx_short<HB, BF16, SIG, NT><<<grid, 256, 0, stream>>>(a)
+
 template <bool BF16, bool SIG, bool NT>
-int launch_score(const MxArgs& a, hipStream_t stream) {
-    if (a.nb <= 8) {
+int launch_score(const MxArgs& a, int q_dtype, hipStream_t stream) {
+    if (a.nb <= 8 && a.B <= 32) {
+        // two workgroups a CU
+        const dim3 grid((unsigned)std::min<int64_t>(512, ceil_div(a.n_items, (int64_t)512)));
+        if (q_dtype == LGX_DTYPE_F32) { LGX_MX_STEPS(LGX_MX_FEW, LGX_DTYPE_F32) }
+        else if (q_dtype == LGX_DTYPE_BF16) { LGX_MX_STEPS(LGX_MX_FEW, LGX_DTYPE_BF16) }
+        else { LGX_MX_STEPS(LGX_MX_FEW, LGX_DTYPE_MXFP4) }
+    } else if (a.nb <= 8) {
         const int64_t gy = ceil_div(a.B, (int64_t)(kUserTiles * 32));
         LGX_REQUIRE(gy < 65536, LGX_ERR_UNSUPPORTED, "lgx_score_mx: %lld queries is too many", (long long)a.B);
         const int64_t gx = ceil_div(a.n_items, (int64_t)512);
         const dim3 grid((unsigned)(NT ? gx : 8 * ceil_div(gx, (int64_t)8)), (unsigned)gy);
-        switch ((a.nb + 1) / 2) {
-            case 1: score_mx_short<1, BF16, SIG, NT><<<grid, 256, 0, stream>>>(a); break;
-            case 2: score_mx_short<2, BF16, SIG, NT><<<grid, 256, 0, stream>>>(a); break;
-            case 3: score_mx_short<3, BF16, SIG, NT><<<grid, 256, 0, stream>>>(a); break;
-            default: score_mx_short<4, BF16, SIG, NT><<<grid, 256, 0, stream>>>(a); break;
-        }
+        LGX_MX_STEPS(LGX_MX_SHORT, 0)
     } else {
         // two waves side by side over the users where there are enough of them
         const int uw = a.B > 32 ? 2 : 1, nu = a.B > 64 ? 2 : 1;
@@ -481,6 +579,10 @@ int launch_score(const MxArgs& a, hipStream_t stream) {
     LGX_LAUNCH_CHECK();
     return LGX_OK;
 }
+
+// One tile of users over rows of at most 8 blocks: every wave of score_mx_few quantises it for itself (a launch less: 57 ->
+// 52 us for a call of 1 x 1 M x 256 by itself); with more of them, once for all by a launch of its own
+bool quantised_inside(int64_t B, int64_t d) { return B <= 32 && d <= 8 * kBlock; }
 
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
@@ -546,7 +648,7 @@ extern "C" int lgx_mx_dequantize(const uint8_t* codes, const uint8_t* scales, in
 extern "C" int lgx_score_mx_workspace(int64_t B, int64_t d, int q_dtype, size_t* ws_bytes) {
     LGX_REQUIRE(ws_bytes && B >= 0 && d >= 1 && d <= kMaxD, LGX_ERR_INVALID_ARG, "lgx_score_mx_workspace: bad arguments");
     const size_t nb = (size_t)ceil_div(d, (int64_t)kBlock);
-    *ws_bytes = q_dtype == LGX_DTYPE_MXFP4 ? 0 : align_up((size_t)B * nb * 16) + align_up((size_t)B * nb);
+    *ws_bytes = q_dtype == LGX_DTYPE_MXFP4 || quantised_inside(B, d) ? 0 : align_up((size_t)B * nb * 16) + align_up((size_t)B * nb);
     return LGX_OK;
 }
 
@@ -569,27 +671,31 @@ extern "C" int lgx_score_mx(const void* Q, const uint8_t* q_scales, int q_dtype,
                 (long long)n_q);
     LGX_REQUIRE(aligned(item_codes, 16), LGX_ERR_INVALID_ARG, "lgx_score_mx: codes must be 16-byte aligned");
     const int64_t nb = ceil_div(d, (int64_t)kBlock);
-    MxArgs a{static_cast<const uint8_t*>(Q), q_scales, user_rows, n_q, item_codes, item_scales, B, n_items, nb, scores};
+    MxArgs a{static_cast<const uint8_t*>(Q), q_scales, user_rows, n_q, item_codes, item_scales, B, n_items, nb, scores, d, q_ld, false};
     if (q_dtype == LGX_DTYPE_MXFP4) {
         LGX_REQUIRE(q_scales && aligned(Q, 16), LGX_ERR_INVALID_ARG, "lgx_score_mx: query codes must be 16-byte aligned, with scales");
     } else {
         LGX_REQUIRE(q_ld >= d, LGX_ERR_INVALID_ARG, "lgx_score_mx: q_ld=%lld < d", (long long)q_ld);
         size_t need = 0;
         lgx_score_mx_workspace(B, d, q_dtype, &need);
-        LGX_REQUIRE(ws && ws_bytes >= need && aligned(ws, 16), LGX_ERR_WORKSPACE, "lgx_score_mx: workspace %zu < %zu", ws_bytes, need);
-        uint8_t* codes = static_cast<uint8_t*>(ws);
-        uint8_t* scales = codes + align_up((size_t)B * nb * 16);
-        const int rc = launch_quantize(Q, user_rows, n_q, B, d, q_ld, q_dtype, codes, scales, stream);
-        if (rc) return rc;
-        a.q = codes;
-        a.qs = scales;
-        a.user_rows = nullptr;
-        a.n_q = B;
+        a.q_vec = d % 8 == 0 && q_ld * (q_dtype == LGX_DTYPE_BF16 ? 2 : 4) % 16 == 0 && aligned(Q, 16);
+        LGX_REQUIRE(need == 0 || (ws && ws_bytes >= need && aligned(ws, 16)), LGX_ERR_WORKSPACE, "lgx_score_mx: workspace %zu < %zu", ws_bytes, need);
+        if (!quantised_inside(B, d)) {
+            uint8_t* codes = static_cast<uint8_t*>(ws);
+            uint8_t* scales = codes + align_up((size_t)B * nb * 16);
+            const int rc = launch_quantize(Q, user_rows, n_q, B, d, q_ld, q_dtype, codes, scales, stream);
+            if (rc) return rc;
+            a.q = codes;
+            a.qs = scales;
+            a.user_rows = nullptr;
+            a.n_q = B;
+            q_dtype = LGX_DTYPE_MXFP4;
+        }
     }
     // Rows that start on a 128-byte line write whole lines, which go past the L2 (1024 x 1 M f32: 0.79 against
     // 0.94 ms); the ends of other rows' stores share lines, which the L2 merges (2048 x 40,981: 119 us past it).
     const bool nt = aligned(scores, 128) && n_items * (out_dtype == LGX_DTYPE_BF16 ? 2 : 4) % 128 == 0;
-#define LGX_SMX(BF, SG) (nt ? launch_score<BF, SG, true>(a, stream) : launch_score<BF, SG, false>(a, stream))
+#define LGX_SMX(BF, SG) (nt ? launch_score<BF, SG, true>(a, q_dtype, stream) : launch_score<BF, SG, false>(a, q_dtype, stream))
     if (out_dtype == LGX_DTYPE_BF16) return apply_sigmoid ? LGX_SMX(true, true) : LGX_SMX(true, false);
     return apply_sigmoid ? LGX_SMX(false, true) : LGX_SMX(false, false);
 #undef LGX_SMX

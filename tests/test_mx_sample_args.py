@@ -65,10 +65,10 @@ def test_score_entry_point_refuses_bad_arguments():
     L = _lib.lib()
     ws = ctypes.c_size_t()
     assert L.lgx_score_mx_workspace(10, 100, 2, ctypes.byref(ws)) == 0 and ws.value == 0
-    assert L.lgx_score_mx_workspace(10, 100, 0, ctypes.byref(ws)) == 0 and ws.value >= 10 * 4 * 17
+    assert L.lgx_score_mx_workspace(40, 100, 0, ctypes.byref(ws)) == 0 and ws.value >= 40 * 4 * 17
     assert L.lgx_score_mx_workspace(10, 0, 0, ctypes.byref(ws)) == 1
 
-    def call(Q=P, qs=P, qd=2, n_q=4, ld=0, rows=None, codes=P, scales=P, B=4, n=100, d=64, od=0, out=P, work=None, wb=0):
+    def call(Q=P, qs=P, qd=2, n_q=40, ld=0, rows=None, codes=P, scales=P, B=40, n=100, d=64, od=0, out=P, work=None, wb=0):
         return L.lgx_score_mx(Q, qs, qd, n_q, ld, rows, codes, scales, B, n, d, 0, od, out, work, wb, None)
 
     assert call(B=0) == 0 and call(n=0) == 0
@@ -77,7 +77,7 @@ def test_score_entry_point_refuses_bad_arguments():
     assert call(d=0) == 3 and call(d=65537) == 3
     assert call(n=2 ** 31) == 3
     assert call(Q=None) == 1 and call(codes=None) == 1 and call(scales=None) == 1 and call(out=None) == 1
-    assert call(B=5) == 1 and b"5 queries of 4 rows" in _err()
+    assert call(B=41) == 1 and b"41 queries of 40 rows" in _err()
     assert call(codes=ODD) == 1 and call(Q=ODD) == 1 and call(qs=None) == 1
     assert call(qd=0, ld=63, work=P, wb=1 << 20) == 1
     assert call(qd=0, ld=64) == 4 and b"workspace" in _err()
