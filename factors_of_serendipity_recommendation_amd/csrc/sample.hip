@@ -68,6 +68,13 @@ struct Vec {
         f = F{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         u = U{0xff80ff80u, 0xff80ff80u};
     }
+    // the values are there from here on (a loop that enters with loads on their way would wait for its own first thing)
+    __device__ __forceinline__ void arrive() {
+        if (BF16)
+            asm volatile("" : "+v"(u));
+        else
+            asm volatile("" : "+v"(f));
+    }
     __device__ __forceinline__ void values(float (&v)[4]) const {
 #pragma unroll
         for (int j = 0; j < N; ++j) v[j] = BF16 ? __uint_as_float(j % 2 ? u[j / 2] & 0xffff0000u : u[j / 2] << 16) : f[j];
@@ -108,8 +115,10 @@ __device__ __forceinline__ void for_groups(const void* s, int64_t lo, int64_t hi
     } else {
         const int64_t last = whole - N - (U - 1) * step;  // the last place of U whole groups
         bool more = i <= last;
-        if (more)
+        if (more) {
             for (int k = 0; k < U; ++k) v[k].load(s, i + k * step);
+            for (int k = 0; k < U; ++k) v[k].arrive();
+        }
 #pragma unroll 1
         while (more) {
             Vec<BF16> next[U];
@@ -173,20 +182,41 @@ struct Weigh {
         while (unit > 0 && (1ll << (62 - unit)) < (int64_t)cols) --unit;
         unit = min(unit, 51);
     }
+    template <int N>
+    __device__ __forceinline__ void scaled(const float (&s)[N], int e, double (&w)[N]) const {
+        if (N > 2) {
+            const float s0[2] = {s[0], s[1 % N]}, s1[2] = {s[2 % N], s[3 % N]};
+            double w0[2], w1[2];
+            scaled<2>(s0, e, w0);
+            scaled<2>(s1, e, w1);
+            w[0] = w0[0]; w[1 % N] = w0[1]; w[2 % N] = w1[0]; w[3 % N] = w1[1];
+            return;
+        }
+        double f[N];
+        int n[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const double d = fmax((double)s[j] - m, floor);
+            const double big = fma(d, c, 6755399441055744.0);  // 1.5 * 2^52: the low word is n
+            f[j] = fma(d, c, 6755399441055744.0 - big);
+            n[j] = (int)(uint32_t)__double_as_longlong(big) + e;
+            w[j] = 1.0203121063391729e-07;
+        }
+        // step by step over all of them: one after the other they would wait for each step
+        constexpr double k[8] = {1.3255224878668817e-06, 1.525268684626772e-05, 0.00015403455852453838, 0.0013333558179043112,
+                                 0.009618129159402558, 0.055504108664760424, 0.2402265069581299, 0.6931471805599453};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j < N; ++j) w[j] = fma_const(w[j], f[j], k[i]);
+#pragma unroll
+        for (int j = 0; j < N; ++j) w[j] = ldexp(fma(w[j], f[j], 1.0), n[j]);
+    }
     __device__ __forceinline__ double scaled(float s, int e) const {
-        const double d = fmax((double)s - m, floor);
-        const double big = fma(d, c, 6755399441055744.0);  // 1.5 * 2^52: the low word is n
-        const double f = fma(d, c, 6755399441055744.0 - big);
-        double r = fma_const(f, 1.0203121063391729e-07, 1.3255224878668817e-06);
-        r = fma_const(r, f, 1.525268684626772e-05);
-        r = fma_const(r, f, 0.00015403455852453838);
-        r = fma_const(r, f, 0.0013333558179043112);
-        r = fma_const(r, f, 0.009618129159402558);
-        r = fma_const(r, f, 0.055504108664760424);
-        r = fma_const(r, f, 0.2402265069581299);
-        r = fma_const(r, f, 0.6931471805599453);
-        r = fma(r, f, 1.0);
-        return ldexp(r, (int)(uint32_t)__double_as_longlong(big) + e);
+        const float v[1] = {s};
+        double w[1];
+        scaled<1>(v, e, w);
+        return w[0];
     }
     __device__ __forceinline__ double operator()(float s) const { return scaled(s, 0); }
     // w in units of 2^-unit, rounded; w 2^unit <= 2^51, so that adding 2^52 leaves it in the low bits
@@ -793,25 +823,37 @@ __device__ __forceinline__ void gather(const void* s, int64_t lo, int64_t hi, Ta
 }
 
 // Steps of the distance to the best score for top_p.  A column of weight below (1 - p) Z / cols is never kept (all such
-// together weigh less than the (1 - p) Z that are dropped), and Z >= 1.  What lies e^-12 below that shares the last step,
-// and adds at most e^-12 (1 - p) to the sums; so does what lies a tenth of the range below the low score, which is that
-// of a quarter of the columns.
-__device__ __forceinline__ Binning mass_binning(float top, float low, const Row& r, int64_t cols) {
-    const double range = fmax((double)top - (double)low, 0.0);
-    return make_binning(top, fmin(1.1 * range, fmin(r.T, 1e30) * (log((double)cols / (1.0 - r.top_p)) + 12.0)));
-}
+// together weigh less than the (1 - p) Z that are dropped), and Z >= 1: that far below the best score is the reach.  What
+// lies 12 T below that shares the last step, and adds at most e^-12 (1 - p) to the sums; so does what lies a tenth of the
+// range below the low score, which is that of some of the columns.
+struct Steps {
+    double range, reach, margin;
+    // top, low: of the columns looked at.  margin: room above them for the others
+    __device__ __forceinline__ Steps(float top, float low, const Row& r, int64_t cols) {
+        range = fmax((double)top - (double)low, 0.0);
+        reach = fmin(r.T, 1e30) * (log((double)cols / (1.0 - r.top_p)) + 12.0);
+        margin = fmin(0.25 * range, 0.25 * reach);
+    }
+    __device__ __forceinline__ Binning bins(float top, double room) const {
+        const float first = (float)((double)top + room);
+        return make_binning(first, (double)first - (double)top + fmin(1.1 * range, reach));
+    }
+};
 
-// counts of the columns [lo, hi) that the cut keeps, without the last step, into sh.count, and the first steps' places
+// counts of the columns [lo, hi) that the cut keeps, without the last step, into sh.count, and the first steps' places.
+// top: this thread's best score (one above the first step counts there, and shows by that)
 template <bool BF16>
-__device__ __forceinline__ void count_steps(const void* s, int64_t lo, int64_t hi, const Binning& bin, const Cut& cut, Shared& sh) {
+__device__ __forceinline__ void count_steps(const void* s, int64_t lo, int64_t hi, const Binning& bin, const Cut& cut, Shared& sh, float* top = nullptr) {
     const bool all = cut.s == kNone;
     clear_hist(sh);
     for (int j = threadIdx.x; j < kTopBins; j += kThreads) sh.place[j] = 0;
     __syncthreads();
+    float best = kNone;
     for_groups<BF16, 2>(s, lo, hi, threadIdx.x, kThreads, [&](const float (&v)[4], int i) {
+        if (top) best = max_of(best, max_of(max_of(v[0], v[1]), max_of(v[2], v[3])));
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float x = fminf(bin.at(v[j]), (float)(kBins - 1));
+            const float x = fmaxf(fminf(bin.at(v[j]), (float)(kBins - 1)), 0.0f);  // NaN goes to the last
             const int b = (int)x;
             if ((all | cut.keeps(v[j], i + j)) & (b < kBins - 1)) {
                 atomicAdd(&sh.count[b], 1u);
@@ -819,6 +861,7 @@ __device__ __forceinline__ void count_steps(const void* s, int64_t lo, int64_t h
             }
         }
     });
+    if (top) *top = best;
 }
 
 // The steps [first, last] that may hold the column in which the running weight reaches top_p of the whole, and the columns
@@ -850,15 +893,16 @@ __device__ __forceinline__ Window mass_window(const Binning& bin, double T, doub
 #pragma unroll
         for (int j = 0; j < per; ++j) {
             const float place = (float)sh.place[b0 + j] / (65536.0f * (float)max(count[j], 1u));
-            w[j] = (double)count[j] * weigh((float)((double)bin.top - wide * (b0 + j + (double)place)));
+            // an empty step above the best score may weigh too much for a number
+            w[j] = count[j] ? (double)count[j] * weigh((float)((double)bin.top - wide * (b0 + j + (double)place))) : 0.0;
         }
     } else {
         double x = weigh((float)((double)bin.top - wide * (b0 + 0.5)));
         const double ratio = exp2_step(wide, weigh);
 #pragma unroll
         for (int j = 0; j < per; ++j) {
-            w[j] = (double)count[j] * x;
-            square = fma(w[j], x, square);
+            w[j] = count[j] ? (double)count[j] * x : 0.0;
+            square = fma(w[j], count[j] ? x : 0.0, square);
             x *= ratio;
         }
     }
@@ -908,9 +952,11 @@ __device__ __forceinline__ void sum_window(const void* s, int64_t cols, const Se
         double w = 0.0;
         for_groups<BF16, 1>(s, g * segs.len, min(cols, (g + 1) * segs.len), lane, 64, [&](const float (&v)[4], int i) {
             bool in[4];
+            double weight[4];
+            weigh.scaled<4>(v, 0, weight);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                double x = weigh(v[j]);
+                double x = weight[j];
                 const float d = bin.at(v[j]);
                 const bool ok = ALL || cut.keeps(v[j], i + j);
                 z += ok ? x : 0.0;
@@ -1000,9 +1046,10 @@ __device__ __forceinline__ bool resolve_window(int n, double z, double better, c
     return true;
 }
 
-__device__ __forceinline__ double kept_weight(float v, int i, const Cut& cut, const Weigh& weigh, double min_p) {
-    const double w = weigh(v);
-    return (cut.keeps(v, i) & (w >= min_p)) ? w : 0.0;
+__device__ __forceinline__ void kept_weights(const float (&v)[4], int i, const Cut& cut, const Weigh& weigh, double min_p, double (&w)[4]) {
+    weigh.scaled<4>(v, 0, w);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = (cut.keeps(v[j], i + j) & (w[j] >= min_p)) ? w[j] : 0.0;
 }
 
 // weights of the kept columns of segments [g0, g1) -> sum(g, .)
@@ -1013,9 +1060,11 @@ __device__ __forceinline__ void sum_segments(const void* s, int64_t cols, const 
     for (int g = g0 + wave; g < g1; g += kWaves) {
         double w = 0.0;
         for_groups<BF16, 1>(s, g * segs.len, min(cols, (g + 1) * segs.len), lane, 64, [&](const float (&v)[4], int i) {
-            if (max_of(max_of(v[0], v[1]), max_of(v[2], v[3])) >= cut.s)
-                w += (kept_weight(v[0], i, cut, weigh, min_p) + kept_weight(v[1], i + 1, cut, weigh, min_p)) +
-                     (kept_weight(v[2], i + 2, cut, weigh, min_p) + kept_weight(v[3], i + 3, cut, weigh, min_p));
+            if (max_of(max_of(v[0], v[1]), max_of(v[2], v[3])) >= cut.s) {
+                double x[4];
+                kept_weights(v, i, cut, weigh, min_p, x);
+                w += (x[0] + x[1]) + (x[2] + x[3]);
+            }
         });
         w = wave_scan_f64(w);
         if (lane == 63) sum(g, w);
@@ -1072,8 +1121,9 @@ __device__ __forceinline__ void draw_columns(const SampleArgs& a, int64_t row, c
                 if (pick >= 0) break;
                 const int64_t i = i0 + t * kStep + lane * N;
                 double w[N], own = 0.0;
+                kept_weights(v[t], (int)i, cut, weigh, r.min_p, w);
 #pragma unroll
-                for (int k = 0; k < N; ++k) own += w[k] = kept_weight(v[t][k], (int)i + k, cut, weigh, r.min_p);
+                for (int k = 0; k < N; ++k) own += w[k];
                 double c = run + wave_scan_f64(own) - own;
                 // this lane's first column past the target, or without one its last of any weight
                 int at = -1, tail = -1;
@@ -1175,8 +1225,28 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int64_t row, con
             }
         }
     }
-    const Maxima m = scan_maxima<BF16>(s, 0, cols, 1);
-    const float top = best_of(m, sh), low = of_reverse_order(block_max_u64(reverse_order_of(m.low), sh));
+    // for top_p alone an eighth of the row is enough to lay out the steps, and the reading that counts them finds the best
+    // score; a best score above them (by more than a quarter of the range, or a T so low that there is no such room) costs
+    // a reading more
+    const bool sample = by_p && !by_k && cols >= 16 * kChunk;
+    Maxima m = scan_maxima<BF16>(s, 0, cols, sample ? 8 : 1);
+    float top = best_of(m, sh), low = of_reverse_order(block_max_u64(reverse_order_of(m.low), sh));
+    Binning bin{top, 0.0f};
+    bool counted = false;
+    if (sample && top > kNone && top < INFINITY) {
+        const Steps steps(top, low, r, cols);
+        if (steps.margin > 0.1 * steps.range) {
+            bin = steps.bins(top, steps.margin);
+            count_steps<BF16>(s, 0, cols, bin, Cut{kNone, -1}, sh, &m.best[0]);
+            top = unord_f32((uint32_t)block_max_u64(order_of(m.best[0]), sh));
+            counted = top <= bin.top;
+        }
+    }
+    if (sample && !counted) {
+        m = scan_maxima<BF16>(s, 0, cols, 1);
+        top = best_of(m, sh);
+        low = of_reverse_order(block_max_u64(reverse_order_of(m.low), sh));
+    }
     if (top == kNone) {
         all_draws(a, row, -1, 0.0f);
         return;
@@ -1189,7 +1259,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int64_t row, con
     Cut cut{kNone, -1};
     if (by_k) {
         // the step of the top_k-th column
-        const Binning bin = make_binning(top, fmax((double)top - (double)low, 0.0));
+        bin = make_binning(top, fmax((double)top - (double)low, 0.0));
         clear_hist(sh);
         for_groups<BF16, 2>(s, 0, cols, tid, kThreads, [&](const float (&v)[4], int) {
 #pragma unroll
@@ -1213,8 +1283,10 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int64_t row, con
     const auto to_seg = [&](int g, double w) { sh.seg[g + 1] = w; };
     bool summed = false;
     if (by_p) {
-        const Binning bin = mass_binning(top, low, r, cols);
-        count_steps<BF16>(s, 0, cols, bin, cut, sh);
+        if (!counted) {
+            bin = Steps(top, low, r, cols).bins(top, 0.0);
+            count_steps<BF16>(s, 0, cols, bin, cut, sh);
+        }
         __syncthreads();
         const Window win = mass_window(bin, r.T, r.top_p, weigh, sh);
         if (win.usable()) {
@@ -1289,6 +1361,10 @@ __device__ __forceinline__ void load_steps(const RowState* st, Shared& sh) {
     for (int j = threadIdx.x; j < kBins; j += kThreads) sh.count[j] = st->count[j];
     for (int j = threadIdx.x; j < kTopBins; j += kThreads) sh.place[j] = st->place[j];
 }
+__device__ __forceinline__ Binning row_steps(const RowState* st, const Row& r, int64_t cols) {
+    const float top = unord_f32(st->top);
+    return Steps(top, of_reverse_order(st->low), r, cols).bins(top, 0.0);
+}
 __device__ __forceinline__ bool finite(float top) { return top > kNone && top < INFINITY; }
 
 // Every part gives the score of its j-th best class; the ceil(top_k / j)-th best of those is one that top_k columns reach.
@@ -1361,7 +1437,7 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_find(SampleArgs a, S
         gather<BF16>(s, part.lo, part.hi, [&](float v) { return v >= bound; }, [&](uint64_t key) { push(sh.key, &sh.n, key); });
         append_list(p.keys + row * kList, &st->n, sh);
     } else if (r.top_p < 1.0 && finite(unord_f32(st->top))) {
-        count_steps<BF16>(s, part.lo, part.hi, mass_binning(unord_f32(st->top), of_reverse_order(st->low), r, a.cols), Cut{kNone, -1}, sh);
+        count_steps<BF16>(s, part.lo, part.hi, row_steps(st, r, a.cols), Cut{kNone, -1}, sh);
         __syncthreads();
         for (int j = threadIdx.x; j < kBins; j += kThreads)
             if (sh.count[j]) atomicAdd(&st->count[j], sh.count[j]);
@@ -1388,7 +1464,7 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_sum(SampleArgs a, Sp
         sum_segments<BF16>(s, a.cols, segs, part.g0, part.g1, Cut{kNone, -1}, weigh, r.min_p, [&](int g, double w) { seg[g + 1] = w; });
         return;
     }
-    const Binning bin = mass_binning(top, of_reverse_order(st->low), r, a.cols);
+    const Binning bin = row_steps(st, r, a.cols);
     load_steps(st, sh);
     if (threadIdx.x == 0) sh.n = 0;
     __syncthreads();
@@ -1439,7 +1515,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_split_draw(SampleArgs a, S
     const Weigh weigh(top, r.T, (int)a.cols);
     alone |= !finite(top);
     if (!alone && by_p) {
-        const Binning bin = mass_binning(top, of_reverse_order(st->low), r, a.cols);
+        const Binning bin = row_steps(st, r, a.cols);
         load_steps(st, sh);
         __syncthreads();
         const Window win = mass_window(bin, r.T, r.top_p, weigh, sh);

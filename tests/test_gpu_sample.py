@@ -88,6 +88,47 @@ def test_long_rows(rows, cols):
     check(S, u, top_p=0.7)
 
 
+def _odd_rows(cols, seed):
+    """Rows that a histogram laid over a part of a normal row's scores would not expect."""
+    g = torch.Generator().manual_seed(seed)
+    n = torch.randn(cols, generator=g)
+    rows = [torch.sort(n).values, torch.sort(n, descending=True).values, n.clone(), (n * 2).round(), torch.zeros(cols),
+            n.clone(), n.abs().pow(-1.5).clamp(max=1e6), n * 1e-3, n.clone(), n.clone(), n * 40, n.clone()]
+    rows[2][cols - 1] = 60.0                                   # one column holds nearly all the weight
+    rows[5][::2] = float("nan")
+    rows[5][1::4] = float("-inf")
+    rows[8][:] = float("-inf")
+    rows[8][cols - 3:] = torch.tensor([1.0, 3.0, 2.0])         # three columns, at the end
+    rows[9][:cols // 2] = torch.finfo(torch.float32).min       # masked by the lowest value
+    rows[11][cols // 3] = float("inf")
+    return torch.stack(rows)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("cols", [32768, 50000, 131071])
+def test_rows_of_unexpected_shapes(cols, dtype):
+    S = _odd_rows(cols, cols).to(dtype).to(DEV)
+    u = torch.rand(S.shape[0], 6, generator=torch.Generator().manual_seed(1)).to(DEV)
+    for kw in ({}, {"top_p": 0.9}, {"top_p": 0.9, "temperature": 0.05}, {"top_p": 0.99999}, {"top_p": 1e-6}, {"top_k": 50},
+               {"top_k": 1024, "top_p": 0.7}, {"top_k": 1500}, {"top_k": 6000, "top_p": 0.8, "min_p": 0.01},
+               {"top_p": 0.5, "min_p": 0.3}, {"top_p": 0.9, "temperature": 100.0}, {"top_k": cols - 1, "top_p": 0.95}):
+        check(S, u, **kw)
+
+
+def test_a_batch_that_fills_the_chip():
+    """768 rows and more take a workgroup each whatever their length."""
+    S = torch.randn(800, 40000, device=DEV, generator=torch.Generator(device=DEV).manual_seed(2))
+    S[:12] = _odd_rows(40000, 3).to(DEV)
+    u = torch.rand(800, 3, generator=torch.Generator().manual_seed(4)).to(DEV)
+    for kw in ({"top_p": 0.9}, {"top_k": 100}, {"min_p": 0.2}, {"top_k": 3000, "top_p": 0.9}):
+        idx, prob = lgx.sample_rows(S, u, **kw)
+        i2, p2 = check(S[:40], u[:40], **kw)  # the same rows in a batch that is split
+        assert torch.equal(idx[:40], i2) and torch.equal(prob[:40], p2)
+        check(S[780:], u[780:], **kw)
+        again = lgx.sample_rows(S, u, **kw)
+        assert torch.equal(again[0], idx) and torch.equal(again[1], prob)
+
+
 def test_many_draws_and_given_numbers_at_the_ends():
     S, _ = scores(3, 5000, 1)
     u = torch.rand(3, 777, generator=torch.Generator().manual_seed(2), dtype=torch.float64)
