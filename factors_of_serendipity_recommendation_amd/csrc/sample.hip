@@ -496,6 +496,16 @@ struct Binning {
     __device__ __forceinline__ float at(float s) const { return (top - s) * inv; }
     __device__ __forceinline__ int operator()(float s) const { return (int)fminf(at(s), (float)(kBins - 1)); }
 };
+// the largest score whose distance is at least x steps: at(s) < x iff s is above it (the distance falls with the score)
+__device__ __forceinline__ float score_at(const Binning& bin, float x) {
+    uint32_t lo = ord_f32(-INFINITY), hi = ord_f32(bin.top);  // at(lo) >= x; scores above top lie at less than any x > 0
+    if (!(bin.at(bin.top) < x)) return bin.top;
+    while (hi - lo > 1) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        if (bin.at(unord_f32(mid)) < x) hi = mid; else lo = mid;
+    }
+    return unord_f32(lo);
+}
 __device__ __forceinline__ Binning make_binning(float top, double range, int bins = kBins) {
     const double inv = (double)(bins - 1) / range;  // a range of 0: all the best score's equals in bin 0
     return Binning{top, (float)fmin(inv, 1e30)};
@@ -948,34 +958,35 @@ __device__ __forceinline__ void sum_window(const void* s, int64_t cols, const Se
                                            Sum sum, double& z, double& better) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     z = better = 0.0;
+    const float above = win.first > 0 ? score_at(bin, win.from) : INFINITY, least = score_at(bin, win.to);
+    const bool masks = min_p > 0.0;
     for (int g = g0 + wave; g < g1; g += kWaves) {
         double w = 0.0;
         for_groups<BF16, 1>(s, g * segs.len, min(cols, (g + 1) * segs.len), lane, 64, [&](const float (&v)[4], int i) {
-            bool in[4];
-            double weight[4];
-            weigh.scaled<4>(v, 0, weight);
+            double x[4];
+            weigh.scaled<4>(v, 0, x);
+            bool in = false;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                double x = weight[j];
-                const float d = bin.at(v[j]);
                 const bool ok = ALL || cut.keeps(v[j], i + j);
-                z += ok ? x : 0.0;
-                x = d < win.from ? x : 0.0;
-                if (min_p > 0.0) {
-                    better += x;
-                    w += x >= min_p ? x : 0.0;
-                } else {
-                    w += x;
+                if (ok) z += x[j];
+                if (v[j] > above) {
+                    if (masks) {
+                        better += x[j];
+                        if (x[j] >= min_p) w += x[j];
+                    } else {
+                        w += x[j];
+                    }
                 }
-                in[j] = !(d < win.from) & (d < win.to) & ok;
+                in |= (v[j] > least) & !(v[j] > above);
             }
-            if (in[0] | in[1] | in[2] | in[3]) {
+            if (in) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (in[j]) put(column_key(v[j], i + j));
+                    if ((v[j] > least) & !(v[j] > above) && (ALL || cut.keeps(v[j], i + j))) put(column_key(v[j], i + j));
             }
         });
-        if (!(min_p > 0.0)) better += w;
+        if (!masks) better += w;
         w = wave_scan_f64(w);
         if (lane == 63) sum(g, w);
     }
@@ -1053,15 +1064,20 @@ __device__ __forceinline__ void kept_weights(const float (&v)[4], int i, const C
 }
 
 // weights of the kept columns of segments [g0, g1) -> sum(g, .)
-template <bool BF16, typename Sum>
+template <bool BF16, bool ALL, typename Sum>
 __device__ __forceinline__ void sum_segments(const void* s, int64_t cols, const Segments& segs, int g0, int g1, const Cut& cut,
                                              const Weigh& weigh, double min_p, Sum sum) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const bool masks = min_p > 0.0;
     for (int g = g0 + wave; g < g1; g += kWaves) {
         double w = 0.0;
         for_groups<BF16, 1>(s, g * segs.len, min(cols, (g + 1) * segs.len), lane, 64, [&](const float (&v)[4], int i) {
-            if (max_of(max_of(v[0], v[1]), max_of(v[2], v[3])) >= cut.s) {
-                double x[4];
+            if (!ALL && !(max_of(max_of(v[0], v[1]), max_of(v[2], v[3])) >= cut.s)) return;
+            double x[4];
+            if (ALL && !masks) {
+                weigh.scaled<4>(v, 0, x);
+                w += (x[0] + x[1]) + (x[2] + x[3]);
+            } else {
                 kept_weights(v, i, cut, weigh, min_p, x);
                 w += (x[0] + x[1]) + (x[2] + x[3]);
             }
@@ -1310,7 +1326,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int64_t row, con
     }
     if (!summed) {
         __syncthreads();
-        sum_segments<BF16>(s, cols, segs, 0, segs.n, cut, weigh, r.min_p, to_seg);
+        sum_segments<BF16, !K && !P>(s, cols, segs, 0, segs.n, cut, weigh, r.min_p, to_seg);
     }
     draw_columns<BF16>(a, row, r, s, segs, cut, weigh, 0, 1, sh);
 }
@@ -1461,7 +1477,7 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_sum(SampleArgs a, Sp
     if (!finite(top)) return;
     const Weigh weigh(top, r.T, (int)a.cols);
     if (!(r.top_p < 1.0)) {
-        sum_segments<BF16>(s, a.cols, segs, part.g0, part.g1, Cut{kNone, -1}, weigh, r.min_p, [&](int g, double w) { seg[g + 1] = w; });
+        sum_segments<BF16, true>(s, a.cols, segs, part.g0, part.g1, Cut{kNone, -1}, weigh, r.min_p, [&](int g, double w) { seg[g + 1] = w; });
         return;
     }
     const Binning bin = row_steps(st, r, a.cols);
