@@ -275,10 +275,17 @@ __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
     return v;  // lane 63 holds it
 }
 
+struct alignas(16) Pair {
+    uint64_t w, key;
+};
 struct Shared {
     union {
         uint64_t wide[kBins / 2];
         uint32_t count[kBins];
+        struct {
+            Pair pair[kShort];
+            float prob[kShort];
+        };
     };
     uint64_t place[kTopBins];  // in 2^-16 of a step
     uint64_t key[kList];       // gathered columns
@@ -571,56 +578,55 @@ __device__ __forceinline__ void finish_short(const SampleArgs& a, int64_t row, c
     const int tid = threadIdx.x;
     const int n_wave = __builtin_amdgcn_readfirstlane(tid) < n ? n : 0;  // waves without a column skip the loops
     const uint64_t mine = tid < n ? sh.key[tid] : 0;
-    const uint64_t w = tid < n ? weigh.fixed_kept(key_score(mine)) : 0;
-    if (tid < n) sh.wide[tid] = w;
+    const double weight = weigh(key_score(mine));
+    const uint64_t w = tid < n ? max(weigh.fixed(key_score(mine)), (uint64_t)(weight > 0.0 ? 1 : 0)) : 0;
+    // (weight, key) pairs side by side: a step of the loops is one read
+    if (tid < n) sh.pair[tid] = Pair{w, mine};
     __syncthreads();
     int rank = 0;
     uint64_t better = 0;
-    if (r.top_p < 1.0) {
-#pragma unroll 4
-        for (int j = 0; j < n_wave; ++j) {
-            const uint64_t x = sh.wide[j];
-            const bool b = sh.key[j] > mine;
-            rank += b;
-            better += b ? x : 0;
-        }
-    } else {
 #pragma unroll 8
-        for (int j = 0; j < n_wave; ++j) rank += sh.key[j] > mine;
+    for (int j = 0; j < n_wave; ++j) {
+        const Pair p = sh.pair[j];
+        const bool b = p.key > mine;
+        rank += b;
+        better += b ? p.w : 0;
     }
     bool keep = tid < n && rank < r.top_k;
     if (r.top_p < 1.0) {
         const double target = r.top_p * (double)block_sum_u64(keep ? w : 0, sh);
         keep &= rank == 0 || (double)better < target;
     }
-    keep &= (w > 0) & (weigh(key_score(mine)) >= r.min_p);
+    keep &= (w > 0) & (weight >= r.min_p);
     __syncthreads();
-    if (tid < n) sh.wide[tid] = keep ? w : 0;
+    if (tid < n) sh.pair[tid].w = keep ? w : 0;
     __syncthreads();
     uint64_t upto = 0;
-#pragma unroll 4
+#pragma unroll 8
     for (int j = 0; j < n_wave; ++j) {
-        const uint64_t x = sh.wide[j];
-        upto += (uint32_t)sh.key[j] >= (uint32_t)mine ? x : 0;  // the low half falls with the column
+        const Pair p = sh.pair[j];
+        upto += (uint32_t)p.key >= (uint32_t)mine ? p.w : 0;  // the low half falls with the column
     }
     const uint64_t total = block_max_u64(keep ? upto : 0, sh);  // (the barriers also end the loop above)
-    const auto put = [&](int64_t j, uint64_t key) {
+    const float prob = (float)(ldexp(weight, weigh.unit) / (double)total);
+    const auto put = [&](int64_t j, uint64_t key, float p) {
         a.out_idx[row * a.n_draws + j] = key_index(key);
-        if (a.out_prob) a.out_prob[row * a.n_draws + j] = (float)(ldexp(weigh(key_score(key)), weigh.unit) / (double)total);
+        if (a.out_prob) a.out_prob[row * a.n_draws + j] = p;
     };
     // a draw is the column with upto - w <= target < upto; a number at the end of the range counts as the last column's
     if (a.n_draws <= n) {
-        for (int j = tid; j < (int)a.n_draws; j += kThreads) sh.wide[j] = min((uint64_t)(draw_number(a, row, j) * (double)total), total - 1);
+        for (int j = tid; j < (int)a.n_draws; j += kThreads) sh.pair[j].w = min((uint64_t)(draw_number(a, row, j) * (double)total), total - 1);
         __syncthreads();
         if (keep)
 #pragma unroll 4
             for (int j = 0; j < (int)a.n_draws; ++j) {
-                const uint64_t target = sh.wide[j];
-                if ((target < upto) & (target >= upto - w)) put(j, mine);
+                const uint64_t target = sh.pair[j].w;
+                if ((target < upto) & (target >= upto - w)) put(j, mine, prob);
             }
         return;
     }
-    if (tid < n) sh.wide[tid] = keep ? upto : 0;
+    if (tid < n) sh.pair[tid].w = keep ? upto : 0;
+    if (tid < n) sh.prob[tid] = prob;
     __syncthreads();
     for (int64_t j = tid; j < a.n_draws; j += kThreads) {
         const uint64_t target = min((uint64_t)(draw_number(a, row, j) * (double)total), total - 1);
@@ -628,12 +634,12 @@ __device__ __forceinline__ void finish_short(const SampleArgs& a, int64_t row, c
         int at = 0;
 #pragma unroll 4
         for (int c = 0; c < n; ++c) {
-            const uint64_t x = sh.wide[c];
+            const uint64_t x = sh.pair[c].w;
             const bool nearer = (x > target) & (x < least);
             least = nearer ? x : least;
             at = nearer ? c : at;
         }
-        put(j, sh.key[at]);
+        put(j, sh.pair[at].key, sh.prob[at]);
     }
 }
 
