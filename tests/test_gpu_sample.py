@@ -115,6 +115,19 @@ def test_rows_of_unexpected_shapes(cols, dtype):
         check(S, u, **kw)
 
 
+@pytest.mark.parametrize("cols", [4097, 70000])
+def test_unrestricted_rows_whose_parts_differ_by_all_of_the_range(cols):
+    """Parts of a row whose weights underflow against the row's best score, though not against their own."""
+    steps = torch.arange(cols).div(300, rounding_mode="floor").float()
+    rows = [steps * 40 - 5000, 5000 - steps * 40, -steps, torch.full((cols,), -745.2), torch.full((cols,), -743.0)]
+    rows[3][cols - 2] = 0.0     # what the other columns weigh rounds to 0 in f64
+    rows[4][cols // 2] = 0.0    # and here to a few of its smallest units
+    S = torch.stack(rows).to(DEV)
+    u = torch.tensor([0.0, 2.0 ** -24, 0.25, 0.5, 1 - 2.0 ** -24]).repeat(5, 1).to(DEV)
+    check(S, u)
+    check(S, u, temperature=20.0)
+
+
 def test_a_batch_that_fills_the_chip():
     """768 rows and more take a workgroup each whatever their length."""
     S = torch.randn(800, 40000, device=DEV, generator=torch.Generator(device=DEV).manual_seed(2))
