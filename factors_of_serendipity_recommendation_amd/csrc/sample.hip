@@ -232,7 +232,6 @@ struct Weigh {
 
 // ------------------------------------------------------------------------------------ wave and workgroup steps
 __device__ __forceinline__ double shfl_f64(double v, int src) { return __longlong_as_double((int64_t)shfl_u64(__double_as_longlong(v), src)); }
-__device__ __forceinline__ double shfl_xor_f64(double v, int m) { return __longlong_as_double((int64_t)shfl_xor_u64(__double_as_longlong(v), m)); }
 
 // v from the lane that a DPP row operation names, 0 where it names none
 template <int CTRL, int ROWS>
@@ -462,6 +461,7 @@ struct Row {
 __device__ __forceinline__ Row row_settings(const SampleArgs& a, int64_t row) {
     Row r;
     r.T = a.T_rows ? (double)a.T_rows[row] : a.T;
+    if (r.T > 0.0) r.T = fmax(r.T, 1e-300);  // below it 1 / T is none, and no two f32 scores lie so near anyway
     r.top_p = a.p_rows ? (double)a.p_rows[row] : a.top_p;
     const double m = a.m_rows ? (double)a.m_rows[row] : a.min_p;
     r.min_p = m > 0.0 ? fmin(m, 1.0) : 0.0;
@@ -831,7 +831,7 @@ __device__ __forceinline__ void push(Keys keys, Count n, uint64_t key) {
 template <bool BF16, typename Take, typename Put>
 __device__ __forceinline__ void gather(const void* s, int64_t lo, int64_t hi, Take take, Put put) {
     for_groups<BF16, 4>(s, lo, hi, threadIdx.x, kThreads, [&](const float (&v)[4], int i) {
-        if (take(v[0]) | take(v[1]) | take(v[2]) | take(v[3])) {
+        if ((int)take(v[0]) | (int)take(v[1]) | (int)take(v[2]) | (int)take(v[3])) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 if (take(v[j])) put(column_key(v[j], i + j));
@@ -1724,7 +1724,7 @@ int launch_sample(const SampleArgs& a, void* ws, int parts, hipStream_t stream) 
                       reinterpret_cast<double*>(w + l.sums), reinterpret_cast<float*>(w + l.seg_top), parts};
     const dim3 grid((unsigned)parts, (unsigned)a.rows);
     const dim3 draws((unsigned)std::min<int64_t>(ceil_div(a.n_draws, (int64_t)kWaves), parts), (unsigned)a.rows);
-    const bool find = a.k_rows || a.p_rows || a.top_k > 0 || a.top_p < 1.0;
+    const bool find = a.k_rows || a.p_rows || (a.top_k > 0 && a.top_k < a.cols) || a.top_p < 1.0;
     if (!find && !a.m_rows && !(a.min_p > 0.0)) {
         sample_own_sum<BF16><<<grid, kThreads, 0, stream>>>(a, p);
         LGX_LAUNCH_CHECK();

@@ -9,6 +9,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import math
+import operator
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -650,8 +651,10 @@ def _row_setting(name: str, v, rows: int, dev: torch.device, dtype: torch.dtype,
         if dtype == torch.int32 and v.dtype != torch.int32:
             if v.dtype.is_floating_point or v.dtype == torch.bool:
                 raise TypeError(f"sample_rows: {name} must hold integers, got {v.dtype}")
-            v = v.clamp(0, 2 ** 31 - 1)
+            v = v.to(torch.int64).clamp(0, 2 ** 31 - 1)
         return 0, v.to(dtype).contiguous()
+    if dtype == torch.int32:
+        v = operator.index(v)
     if not lo <= v <= hi:
         raise ValueError(f"sample_rows: {name} = {v} outside [{lo}, {hi}]")
     return v, None

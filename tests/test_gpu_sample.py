@@ -128,6 +128,34 @@ def test_unrestricted_rows_whose_parts_differ_by_all_of_the_range(cols):
     check(S, u, temperature=20.0)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,cols", [(6, 300), (6, 32768), (6, 70000), (800, 33000)])
+def test_long_runs_of_undefined_scores(rows, cols, dtype):
+    """Whole lanes, segments and parts of a row without a number; a few temperatures below what f32 holds."""
+    g = torch.Generator().manual_seed(cols)
+    S = torch.randn(6, cols, generator=g).to(dtype)
+    nan = float("nan")
+    S[0, :cols // 2] = nan
+    S[1, cols // 3:] = nan
+    S[2, torch.arange(cols) // 64 % 3 > 0] = nan
+    S[3] = nan
+    S[4], S[4, cols - 2] = nan, -7.0
+    S[5, 1:] = float("-inf")
+    S[5, 2:cols // 2] = nan
+    S = S.repeat(-(-rows // 6), 1)[:rows].to(DEV)
+    u = torch.rand(rows, 3, generator=g).to(DEV)
+    for kw in ({}, {"top_p": 0.9}, {"top_k": 5}, {"top_k": 1500}, {"min_p": 0.3}, {"top_k": 100, "top_p": 0.5},
+               {"temperature": 5e-324}, {"temperature": 1e-310, "top_p": 0.5}, {"temperature": 1e-45, "min_p": 0.1},
+               {"temperature": 5e-324, "top_k": 3}):
+        idx, prob = check(S[:12], u[:12], **kw) if rows > 12 else check(S, u, **kw)
+        if rows > 12:
+            all_idx, all_prob = lgx.sample_rows(S, u, **kw)
+            assert torch.equal(all_idx[:12], idx) and torch.equal(all_prob[:12], prob)
+            every = torch.arange(6, rows - rows % 6, 6)
+            assert (all_idx[3::6] == -1).all() and (all_idx[4::6] == cols - 2).all() and (all_idx[5::6] == 0).all()
+            assert torch.equal(all_prob[every + 3], torch.zeros_like(all_prob[every + 3]))
+
+
 def test_a_batch_that_fills_the_chip():
     """768 rows and more take a workgroup each whatever their length."""
     S = torch.randn(800, 40000, device=DEV, generator=torch.Generator(device=DEV).manual_seed(2))
@@ -212,6 +240,20 @@ def test_settings_per_row():
     n = torch.full((64,), float("nan"), device=DEV)  # no restriction
     c, d = lgx.sample_rows(S, u, top_p=n, min_p=n), lgx.sample_rows(S, u)
     assert torch.equal(c[0], d[0])
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64])
+def test_top_k_of_any_integer_type(dtype):
+    S, u = scores(8, 500, 3)
+    k = torch.tensor([0, 1, 2, 5, 17, 63, 100, 127], device=DEV)
+    for a, b in zip(lgx.sample_rows(S, u, top_k=k.to(dtype)), check(S, u, top_k=k)):
+        assert torch.equal(a, b)
+    S, u = scores(2, 40000, 4)
+    for a, b in zip(lgx.sample_rows(S, u, top_k=50000), check(S, u)):  # past the row's end: all of it
+        assert torch.equal(a, b)
+    for bad in (2.5, 2.0, "3", None):
+        with pytest.raises(TypeError):
+            lgx.sample_rows(S, u, top_k=bad)
 
 
 def test_strided_rows_and_empty_calls():
