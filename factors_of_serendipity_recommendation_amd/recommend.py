@@ -67,6 +67,23 @@ def topk_candidates(emb_user: torch.Tensor, emb_item: torch.Tensor, candidates: 
     return ragged_topk(scores, indptr, items, K)
 
 
+def _check_mask(mask: Tuple[torch.Tensor, torch.Tensor], n_users: int, n_items: int) -> None:
+    """Raises unless mask is a CSR of n_users lists of ids in [0, n_items): its entries become offsets."""
+    indptr, indices = mask
+    if indptr.dim() != 1 or indices.dim() != 1 or indptr.numel() != n_users + 1:
+        raise ValueError(f"mask indptr must have {n_users + 1} entries, got {tuple(indptr.shape)}")
+    if indptr.dtype != torch.int64 or indices.dtype != torch.int32:
+        raise TypeError(f"mask must be (int64 indptr, int32 indices), got ({indptr.dtype}, {indices.dtype})")
+    nnz = indices.numel()
+    bad = (indptr[0] != 0) | (indptr[-1] != nnz) | (indptr[1:] < indptr[:-1]).any()
+    out = ((indices < 0) | (indices >= n_items)).any()
+    bad, out = torch.stack((bad, out)).tolist()
+    if bad:
+        raise ValueError(f"mask indptr must rise from 0 to the {nnz} indices")
+    if out:
+        raise IndexError(f"masked item id out of range for {n_items} items")
+
+
 def sample_recommendations(emb_user: torch.Tensor, emb_item, users: torch.Tensor, u: torch.Tensor,
                            mask: Optional[Tuple[torch.Tensor, torch.Tensor]] = None, temperature=1.0, top_k=0,
                            top_p=1.0, min_p=0.0,
@@ -85,13 +102,16 @@ def sample_recommendations(emb_user: torch.Tensor, emb_item, users: torch.Tensor
     n_users, n_items = users.numel(), emb_item.shape[0]
     if users.dim() != 1 or u.shape[:1] != users.shape:
         raise ValueError(f"users {tuple(users.shape)} and u {tuple(u.shape)} must list the same users")
-    if mask is not None and mask[0].numel() != n_users + 1:
-        raise ValueError(f"mask indptr must have {n_users + 1} entries, got {mask[0].numel()}")
+    if mask is not None:
+        _check_mask(mask, n_users, n_items)
+    settings = {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p}
+    for n, v in settings.items():
+        if torch.is_tensor(v) and v.shape != users.shape:
+            raise ValueError(f"{n} must be a number or one per user ([{n_users}]), got {tuple(v.shape)}")
     if n_users and (int(users.min()) < 0 or int(users.max()) >= emb_user.shape[0]):
         raise IndexError(f"user id out of range for {emb_user.shape[0]} users")
     items = torch.empty(u.shape, dtype=torch.int32, device=u.device)
     prob = torch.empty(u.shape, dtype=torch.float32, device=u.device)
-    settings = {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p}
     step = ops.dense_chunk_users(n_items, chunk_bytes)
     for c0 in range(0, n_users, step):
         c1 = min(n_users, c0 + step)

@@ -151,6 +151,29 @@ def test_score_mx_gathers_rows_and_flags_bad_ones(kind):
     assert torch.equal(lgx.score_mx(q[3:9], items[100:200]), want[3:9, 100:200])
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16", "mx"])
+@pytest.mark.parametrize("B,d", [(20, 90), (32, 256), (50, 64), (40, 600), (100, 290)])
+def test_rows_outside_the_table_and_undefined_blocks_of_every_form(B, d, kind):
+    """Strided queries at odd addresses, repeated and outside rows, NaN blocks at both ends of a row: each reaches its own
+    scores only, and in every form of the product the rest equals the same rows scored one by one."""
+    base = table(64, d + 9, B, torch.bfloat16 if kind == "bf16" else torch.float32)
+    base[2, 3 + d - 1], base[5, 3] = float("inf"), float("nan")
+    x, y = base[:, 3:3 + d], table(777, d, d)
+    y[4, 0], y[700, d - 1] = float("nan"), float("-inf")
+    items = lgx.mx_quantize(y)
+    rows = torch.randint(0, 64, (B,), generator=torch.Generator().manual_seed(d)).to(DEV)
+    rows[1], rows[7], rows[B - 1], rows[B - 2], rows[3] = -1, 64, 2 ** 33, 5, 2
+    got = lgx.score_mx(lgx.mx_quantize(x) if kind == "mx" else x, items, user_rows=rows)
+    outside = (rows < 0) | (rows >= 64)
+    bad = (outside | (rows == 2) | (rows == 5))[:, None].expand(B, 777).clone()
+    bad[:, 4], bad[:, 700] = True, True
+    assert torch.equal(torch.isnan(got), bad)
+    for j in (0, 2, B // 2, B - 3):
+        if not bad[j, 0]:
+            one = lgx.score_mx(lgx.mx_quantize(x), items, user_rows=rows[j:j + 1])
+            assert torch.equal(torch.nan_to_num(got[j], 7.0), torch.nan_to_num(one[0], 7.0))
+
+
 def test_score_mx_keeps_a_nan_block_to_its_rows():
     x, y = table(4, 64, 1), table(200, 64, 2)
     x[1, 5], y[17, 60] = float("nan"), float("inf")

@@ -342,6 +342,13 @@ def test_sample_recommendations_masks_and_draws(packed):
         recommend.sample_recommendations(eu, items, users + 1, u)
     with pytest.raises(ValueError):
         recommend.sample_recommendations(eu, items, users, u[:4])
+    for T in (torch.ones(6, device=DEV), torch.ones(5, 1, device=DEV)):
+        with pytest.raises(ValueError):
+            recommend.sample_recommendations(eu, items, users, u, mask, temperature=T)
+    with pytest.raises(IndexError):
+        recommend.sample_recommendations(eu, items, users, u, (mask[0], mask[1] + 1))
+    none = recommend.sample_recommendations(eu, items, users[:0], u[:0], (mask[0][:1], mask[1][:0]), temperature=T[:0, 0])
+    assert none[0].shape == none[1].shape == (0, 40)
 
 
 def test_chain_captured_and_replayed():

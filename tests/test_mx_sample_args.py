@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import factors_of_serendipity_recommendation_amd as lgx
-from factors_of_serendipity_recommendation_amd import _lib
+from factors_of_serendipity_recommendation_amd import _lib, recommend
 
 P = ctypes.c_void_p(4096)  # an aligned address that a refused call never touches
 ODD = ctypes.c_void_p(4100)
@@ -101,3 +101,21 @@ def test_sample_entry_point_refuses_bad_arguments():
     assert call(cols=0) == 1 and call(cols=2 ** 31, ld=2 ** 31) == 1 and call(ld=99) == 1
     assert call(rows=2 ** 31) == 3
     assert call(S=None) == 1 and call(u=None) == 1 and call(idx=None) == 1
+
+
+def test_mask_of_sample_recommendations_is_checked():
+    ip, ix = torch.tensor([0, 2, 2, 3]), torch.tensor([0, 9, 4], dtype=torch.int32)
+    check = recommend._check_mask
+    check((ip, ix), 3, 10)
+    check((torch.zeros(1, dtype=torch.int64), ix[:0]), 0, 10)
+    check((torch.zeros(4, dtype=torch.int64), ix[:0]), 3, 0)
+    for bad in ((ip, ix, 2, 10), (ip[:-1], ix, 2, 10), (ip + 1, ix, 3, 10), (torch.tensor([0, 3, 2, 3]), ix, 3, 10),
+                (ip.view(2, 2), ix, 3, 10), (ip, ix.view(1, 3), 3, 10)):
+        with pytest.raises(ValueError):
+            check(bad[:2], *bad[2:])
+    for indices, n_items in ((ix, 9), (ix - 1, 10)):
+        with pytest.raises(IndexError):
+            check((ip, indices), 3, n_items)
+    for types in ((ip.int(), ix), (ip, ix.long()), (ip.float(), ix)):
+        with pytest.raises(TypeError):
+            check(types, 3, 10)
