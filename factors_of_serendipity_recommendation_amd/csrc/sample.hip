@@ -1424,16 +1424,22 @@ __global__ __launch_bounds__(kThreads, 6) void sample_rows_kernel(SampleArgs a) 
 // The same steps with a row cut into `parts` runs of segments, a workgroup each, and a launch per reading; what the
 // workgroups of a row tell each other goes through the workspace, in integers whose order does not matter or in slots
 // of their own.  A row that needs one of the rare ways is left to its first workgroup in the last launch.
+struct Counted {
+    uint32_t count[kBins];
+    uint64_t place[kTopBins];
+};
 struct RowState {          // all zero at the start
     uint64_t best;         // best column key (rows that draw the best column only)
     uint32_t top, low;     // order bits of the best score, reversed ones of the low score
     uint32_t bound;        // order bits of a score that top_k columns reach (top_k)
     uint32_t n;            // columns gathered
-    uint32_t count[kBins];
-    uint64_t place[kTopBins];
+    uint32_t part_top;     // order bits of the best score of the part of the row that was looked at first
+    Counted steps;
 };
 struct SplitArgs {
     RowState* state;
+    Counted* again;  // [rows], zero at the start: where the steps laid out from a part of the row missed its best score
+    bool sample;     // top_p's steps are laid out from an eighth of the row
     uint64_t* keys;  // [rows, kList]
     double* seg;     // [rows, kSegs + 1]
     double* sums;    // [rows, parts, 2]: z, better (top_p); order bits of the part's class bound (top_k); best column key
@@ -1457,15 +1463,40 @@ struct Part {
         hi = min(cols, g1 * segs.len);
     }
 };
-__device__ __forceinline__ void load_steps(const RowState* st, Shared& sh) {
-    for (int j = threadIdx.x; j < kBins; j += kThreads) sh.count[j] = st->count[j];
-    for (int j = threadIdx.x; j < kTopBins; j += kThreads) sh.place[j] = st->place[j];
+__device__ __forceinline__ void load_steps(const Counted& c, Shared& sh) {
+    for (int j = threadIdx.x; j < kBins; j += kThreads) sh.count[j] = c.count[j];
+    for (int j = threadIdx.x; j < kTopBins; j += kThreads) sh.place[j] = c.place[j];
 }
+__device__ __forceinline__ void add_steps(Counted& c, const Shared& sh) {
+    for (int j = threadIdx.x; j < kBins; j += kThreads)
+        if (sh.count[j]) atomicAdd(&c.count[j], sh.count[j]);
+    for (int j = threadIdx.x; j < kTopBins; j += kThreads)
+        if (sh.place[j]) atomicAdd((unsigned long long*)&c.place[j], (unsigned long long)sh.place[j]);
+}
+__device__ __forceinline__ bool finite(float top) { return top > kNone && top < INFINITY; }
+// the row's steps: the ones laid out from its best score, or with room above from a part of the row's; false without them
 __device__ __forceinline__ Binning row_steps(const RowState* st, const Row& r, int64_t cols) {
     const float top = unord_f32(st->top);
     return Steps(top, of_reverse_order(st->low), r, cols).bins(top, 0.0);
 }
-__device__ __forceinline__ bool finite(float top) { return top > kNone && top < INFINITY; }
+__device__ __forceinline__ bool part_steps(const RowState* st, const Row& r, int64_t cols, Binning& bin) {
+    const float top = unord_f32(st->part_top);
+    if (!finite(top)) return false;
+    const Steps steps(top, of_reverse_order(st->low), r, cols);
+    bin = steps.bins(top, steps.margin);
+    return steps.margin > 0.1 * steps.range;
+}
+// what the columns were counted by, and the counts
+__device__ __forceinline__ const Counted& counted_steps(const SplitArgs& p, int64_t row, const Row& r, int64_t cols, Binning& bin) {
+    const RowState* st = p.state + row;
+    if (p.sample) {
+        if (part_steps(st, r, cols, bin) && unord_f32(st->top) <= bin.top) return st->steps;
+        bin = row_steps(st, r, cols);
+        return p.again[row];
+    }
+    bin = row_steps(st, r, cols);
+    return st->steps;
+}
 
 // Without any restriction two launches do: the segments' own weights, and the draws
 template <bool BF16>
@@ -1527,7 +1558,8 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_top(SampleArgs a, Sp
     }
     const bool by_k = listed(a, r);
     if (by_k && r.top_k > kList / 2) return;
-    const Maxima m = scan_maxima<BF16>(s, part.lo, part.hi, by_k ? list_stride(part.lo, part.hi, r.top_k) : 1);
+    const bool sample = p.sample && r.top_p < 1.0;
+    const Maxima m = scan_maxima<BF16>(s, part.lo, part.hi, by_k ? list_stride(part.lo, part.hi, r.top_k) : sample ? 8 : 1);
     if (by_k) {
         const float bound = class_bound(m, part_rank(r.top_k, p.parts), sh);
         if (threadIdx.x == 0) reinterpret_cast<uint64_t*>(p.sums)[(row * p.parts + blockIdx.x) * 2] = order_of(bound);
@@ -1536,7 +1568,7 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_top(SampleArgs a, Sp
     const uint32_t top = (uint32_t)order_of(best_of(m, sh));
     const uint32_t low = (uint32_t)block_max_u64(reverse_order_of(m.low), sh);
     if (threadIdx.x == 0) {
-        atomicMax(&st->top, top);
+        atomicMax(sample ? &st->part_top : &st->top, top);
         atomicMax(&st->low, low);
     }
 }
@@ -1576,14 +1608,40 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_find(SampleArgs a, S
         __syncthreads();
         gather<BF16>(s, part.lo, part.hi, [&](float v) { return v >= bound; }, [&](uint64_t key) { push(sh.key, &sh.n, key); });
         append_list(p.keys + row * kList, &st->n, sh);
+    } else if (r.top_p < 1.0 && p.sample) {
+        Binning bin;
+        float top;
+        if (part_steps(st, r, a.cols, bin)) {
+            count_steps<BF16>(s, part.lo, part.hi, bin, Cut{kNone, -1}, sh, &top);
+            __syncthreads();
+            add_steps(st->steps, sh);
+        } else {
+            const Maxima m = scan_maxima<BF16>(s, part.lo, part.hi, 1);
+            top = max_of(max_of(m.best[0], m.best[1]), max_of(m.best[2], m.best[3]));
+        }
+        const uint32_t order = (uint32_t)block_max_u64(order_of(top), sh);
+        if (threadIdx.x == 0) atomicMax(&st->top, order);
     } else if (r.top_p < 1.0 && finite(unord_f32(st->top))) {
         count_steps<BF16>(s, part.lo, part.hi, row_steps(st, r, a.cols), Cut{kNone, -1}, sh);
         __syncthreads();
-        for (int j = threadIdx.x; j < kBins; j += kThreads)
-            if (sh.count[j]) atomicAdd(&st->count[j], sh.count[j]);
-        for (int j = threadIdx.x; j < kTopBins; j += kThreads)
-            if (sh.place[j]) atomicAdd((unsigned long long*)&st->place[j], (unsigned long long)sh.place[j]);
+        add_steps(st->steps, sh);
     }
+}
+
+// The rows whose best score lies above the steps that a part of them laid out (by more than a quarter of the range), or
+// whose T is so low that no room could be left
+template <bool BF16>
+__global__ __launch_bounds__(kThreads, 6) void sample_split_again(SampleArgs a, SplitArgs p) {
+    __shared__ Shared sh;
+    const int64_t row = blockIdx.y;
+    const Row r = row_settings(a, row);
+    const Part part(Segments(a.cols), a.cols, blockIdx.x, p.parts);
+    if (part.lo >= part.hi || best_only(r) || listed(a, r) || !(r.top_p < 1.0) || !finite(unord_f32(p.state[row].top))) return;
+    Binning bin;
+    if (&counted_steps(p, row, r, a.cols, bin) != p.again + row) return;
+    count_steps<BF16>(row_scores<BF16>(a, row), part.lo, part.hi, bin, Cut{kNone, -1}, sh);
+    __syncthreads();
+    add_steps(p.again[row], sh);
 }
 
 template <bool BF16>
@@ -1604,8 +1662,8 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_sum(SampleArgs a, Sp
         sum_segments<BF16, true>(s, a.cols, segs, part.g0, part.g1, Cut{kNone, -1}, weigh, r.min_p, [&](int g, double w) { seg[g + 1] = w; });
         return;
     }
-    const Binning bin = row_steps(st, r, a.cols);
-    load_steps(st, sh);
+    Binning bin;
+    load_steps(counted_steps(p, row, r, a.cols, bin), sh);
     if (threadIdx.x == 0) sh.n = 0;
     __syncthreads();
     const Window win = mass_window(bin, r.T, r.top_p, weigh, sh);
@@ -1655,8 +1713,8 @@ __global__ __launch_bounds__(kThreads, 4) void sample_split_draw(SampleArgs a, S
     const Weigh weigh(top, r.T, (int)a.cols);
     alone |= !finite(top);
     if (!alone && by_p) {
-        const Binning bin = row_steps(st, r, a.cols);
-        load_steps(st, sh);
+        Binning bin;
+        load_steps(counted_steps(p, row, r, a.cols, bin), sh);
         __syncthreads();
         const Window win = mass_window(bin, r.T, r.top_p, weigh, sh);
         alone = !win.usable();
@@ -1693,11 +1751,15 @@ int split_parts(int64_t rows, int64_t cols) {
     return (int)ceil_div((int64_t)segs.n, ceil_div((int64_t)segs.n, parts));  // none without a segment
 }
 
-// the workspace: states, keys, segment sums, sums
+// parts of a row that are long enough for an eighth of them to show what the row is like
+bool split_sample(int64_t cols, int parts) { return cols / parts >= 16 * kChunk; }
+
+// the workspace: states, second counts, keys, segment sums, sums
 struct SplitLayout {
-    size_t keys, seg, sums, seg_top, bytes;
-    SplitLayout(int64_t rows, int parts) {
-        keys = align_up((size_t)rows * sizeof(RowState));
+    size_t again, keys, seg, sums, seg_top, bytes;
+    SplitLayout(int64_t rows, int64_t cols, int parts) {
+        again = (size_t)rows * sizeof(RowState);
+        keys = align_up(again + (split_sample(cols, parts) ? (size_t)rows * sizeof(Counted) : 0));
         seg = keys + align_up((size_t)rows * kList * 8);
         sums = seg + align_up((size_t)rows * (kSegs + 1) * 8);
         seg_top = sums + align_up((size_t)rows * parts * 16);
@@ -1718,13 +1780,14 @@ int launch_sample(const SampleArgs& a, void* ws, int parts, hipStream_t stream) 
         LGX_LAUNCH_CHECK();
         return LGX_OK;
     }
-    const SplitLayout l(a.rows, parts);
+    const SplitLayout l(a.rows, a.cols, parts);
+    const bool by_p = a.p_rows || a.top_p < 1.0, sample = by_p && split_sample(a.cols, parts);
     char* w = static_cast<char*>(ws);
-    const SplitArgs p{reinterpret_cast<RowState*>(w), reinterpret_cast<uint64_t*>(w + l.keys), reinterpret_cast<double*>(w + l.seg),
+    const SplitArgs p{reinterpret_cast<RowState*>(w), reinterpret_cast<Counted*>(w + l.again), sample, reinterpret_cast<uint64_t*>(w + l.keys), reinterpret_cast<double*>(w + l.seg),
                       reinterpret_cast<double*>(w + l.sums), reinterpret_cast<float*>(w + l.seg_top), parts};
     const dim3 grid((unsigned)parts, (unsigned)a.rows);
     const dim3 draws((unsigned)std::min<int64_t>(ceil_div(a.n_draws, (int64_t)kWaves), parts), (unsigned)a.rows);
-    const bool find = a.k_rows || a.p_rows || (a.top_k > 0 && a.top_k < a.cols) || a.top_p < 1.0;
+    const bool find = by_p || a.k_rows || (a.top_k > 0 && a.top_k < a.cols);
     if (!find && !a.m_rows && !(a.min_p > 0.0)) {
         sample_own_sum<BF16><<<grid, kThreads, 0, stream>>>(a, p);
         LGX_LAUNCH_CHECK();
@@ -1732,13 +1795,17 @@ int launch_sample(const SampleArgs& a, void* ws, int parts, hipStream_t stream) 
         LGX_LAUNCH_CHECK();
         return LGX_OK;
     }
-    const int64_t words = a.rows * (int64_t)(sizeof(RowState) / 4);
+    const int64_t words = a.rows * (int64_t)((sizeof(RowState) + (sample ? sizeof(Counted) : 0)) / 4);
     sample_clear<<<(unsigned)std::min<int64_t>(1024, ceil_div(words, (int64_t)256)), 256, 0, stream>>>(reinterpret_cast<uint32_t*>(w), words);
     LGX_LAUNCH_CHECK();
     sample_split_top<BF16><<<grid, kThreads, 0, stream>>>(a, p);
     LGX_LAUNCH_CHECK();
     if (find) {
         sample_split_find<BF16><<<grid, kThreads, 0, stream>>>(a, p);
+        LGX_LAUNCH_CHECK();
+    }
+    if (sample) {
+        sample_split_again<BF16><<<grid, kThreads, 0, stream>>>(a, p);
         LGX_LAUNCH_CHECK();
     }
     sample_split_sum<BF16><<<grid, kThreads, 0, stream>>>(a, p);
@@ -1756,7 +1823,7 @@ using namespace lgx;
 extern "C" int lgx_sample_rows_workspace(int64_t rows, int64_t cols, int64_t n_draws, size_t* ws_bytes) {
     LGX_REQUIRE(ws_bytes && rows >= 0 && cols >= 1 && n_draws >= 0, LGX_ERR_INVALID_ARG,
                 "lgx_sample_rows_workspace: bad arguments");
-    *ws_bytes = SplitLayout(rows, split_parts(rows, cols)).bytes;
+    *ws_bytes = SplitLayout(rows, cols, split_parts(rows, cols)).bytes;
     return LGX_OK;
 }
 
@@ -1775,7 +1842,7 @@ extern "C" int lgx_sample_rows(const void* S, int dtype, int64_t rows, int64_t c
     LGX_REQUIRE(rows < (1LL << 31), LGX_ERR_UNSUPPORTED, "lgx_sample_rows: %lld rows is too many", (long long)rows);
     LGX_REQUIRE(S && u && out_idx, LGX_ERR_INVALID_ARG, "lgx_sample_rows: null pointer");
     const int parts = split_parts(rows, cols);
-    const size_t need = SplitLayout(rows, parts).bytes;
+    const size_t need = SplitLayout(rows, cols, parts).bytes;
     LGX_REQUIRE(need == 0 || (ws && ws_bytes >= need && reinterpret_cast<uintptr_t>(ws) % 16 == 0), LGX_ERR_WORKSPACE,
                 "lgx_sample_rows: workspace %zu < %zu", ws_bytes, need);
     const SampleArgs a{S, rows, cols, ld, u, u_dtype == LGX_DTYPE_F64, n_draws, temperature, top_p, min_p, top_k,

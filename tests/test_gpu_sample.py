@@ -115,6 +115,23 @@ def test_rows_of_unexpected_shapes(cols, dtype):
         check(S, u, **kw)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_of_unexpected_shapes_in_a_batch_of_long_rows(dtype):
+    """Parts of 35,000 columns, of which an eighth is looked at first."""
+    S = _odd_rows(140000, 5).to(dtype).to(DEV)
+    u = torch.rand(12, 4, generator=torch.Generator().manual_seed(1)).to(DEV)
+    many, u_many = S.repeat(59, 1), u.repeat(59, 1)
+    for kw in ({"top_p": 0.9}, {"top_p": 0.9, "temperature": 0.05}, {"top_p": 0.99999}, {"top_p": 1e-6, "min_p": 0.5},
+               {"top_p": 0.9, "temperature": 100.0}, {"top_p": 0.5, "top_k": 900}, {"top_p": 0.5, "top_k": 3000}):
+        want = check(S, u, **kw)
+        for g, w in zip(lgx.sample_rows(many, u_many, **kw), want):
+            assert torch.equal(g, w.repeat(59, 1)), kw
+    p = torch.tensor([0.3, 1.0, 0.8], device=DEV).repeat(236)  # 12 rows take 12 settings
+    want = check(S, u, top_p=p[:12])
+    for g, w in zip(lgx.sample_rows(many, u_many, top_p=p), want):
+        assert torch.equal(g, w.repeat(59, 1))
+
+
 @pytest.mark.parametrize("cols", [4097, 70000])
 def test_unrestricted_rows_whose_parts_differ_by_all_of_the_range(cols):
     """Parts of a row whose weights underflow against the row's best score, though not against their own."""
