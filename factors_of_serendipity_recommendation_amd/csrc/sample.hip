@@ -417,6 +417,12 @@ __device__ __forceinline__ void find_fine(double target, Shared& sh) {
     __syncthreads();
 }
 
+// what the wave's lanes wrote to LDS is there for its other lanes (its LDS instructions run in order)
+__device__ __forceinline__ void wave_lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // bitonic sort of sh.key[0, n), descending, n <= kList; keys past n become 0
 __device__ __forceinline__ void sort_keys(int n, Shared& sh) {
     int size = 64;
@@ -426,9 +432,13 @@ __device__ __forceinline__ void sort_keys(int n, Shared& sh) {
         if (j >= n) sh.key[j] = 0;
     for (int k = 2; k <= size; k <<= 1)
         for (int d = k >> 1; d > 0; d >>= 1) {
-            __syncthreads();
+            // up to a distance of 64 a wave works on 128 keys of its own
+            if (k == 2 || d >= 64)
+                __syncthreads();
+            else
+                wave_lds_order();
             for (int t = threadIdx.x; t < size / 2; t += kThreads) {
-                const int i = (t / d) * 2 * d + t % d;
+                const int i = 2 * t - (t & (d - 1));
                 const uint64_t x = sh.key[i], y = sh.key[i + d];
                 if ((x < y) == ((i & k) == 0)) {
                     sh.key[i] = y;
@@ -441,15 +451,20 @@ __device__ __forceinline__ void sort_keys(int n, Shared& sh) {
 
 // sh.w[0, n) -> its inclusive running sums, in order
 __device__ __forceinline__ void scan_list(int n, Shared& sh) {
-    constexpr int per = kList / 64;
+    constexpr int per = kList / kThreads;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lo = threadIdx.x * per;
+    double v[per], own = 0.0;
     __syncthreads();
-    if (threadIdx.x < 64) {
-        const int lane = threadIdx.x, lo = lane * per, hi = min(n, lo + per);
-        double own = 0.0;
-        for (int j = lo; j < hi; ++j) own += sh.w[j];
-        double run = wave_scan_f64(own) - own;
-        for (int j = lo; j < hi; ++j) sh.w[j] = run += sh.w[j];
-    }
+#pragma unroll
+    for (int j = 0; j < per; ++j) own += v[j] = lo + j < n ? sh.w[lo + j] : 0.0;
+    const double incl = wave_scan_f64(own);
+    if (lane == 63) sh.dpart[wave] = incl;
+    __syncthreads();
+    double run = incl - own;
+    for (int w = 0; w < wave; ++w) run += sh.dpart[w];
+#pragma unroll
+    for (int j = 0; j < per; ++j)
+        if (lo + j < n) sh.w[lo + j] = run += v[j];
     __syncthreads();
 }
 
@@ -1244,6 +1259,9 @@ __device__ __forceinline__ const void* row_scores(const SampleArgs& a, int64_t r
 }
 
 __device__ __forceinline__ bool listed(const SampleArgs& a, const Row& r) { return r.top_k > 0 && r.top_k < a.cols; }
+__device__ __forceinline__ bool unrestricted(const SampleArgs& a, const Row& r) {
+    return !listed(a, r) && !(r.top_p < 1.0) && !(r.min_p > 0.0);
+}
 
 __device__ __forceinline__ float best_of(const Maxima& m, Shared& sh) {
     return unord_f32((uint32_t)block_max_u64(order_of(max_of(max_of(m.best[0], m.best[1]), max_of(m.best[2], m.best[3]))), sh));
@@ -1312,16 +1330,15 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int64_t row, con
             const Maxima m = scan_maxima<BF16>(s, 0, cols, list_stride(0, cols, r.top_k));
             bound = class_bound(m, r.top_k, sh);
         }
-        if (cols <= kList || bound > kNone) {
-            __syncthreads();
-            if (tid == 0) sh.n = 0;
-            __syncthreads();
-            gather<BF16>(s, 0, cols, [&](float v) { return (v >= bound) & (v > kNone); }, to_list);
-            __syncthreads();
-            if (sh.n <= kList) {
-                draw_list<BF16>(a, row, r, s, (int)sh.n, sh);
-                return;
-            }
+        // without a bound there are few scores
+        __syncthreads();
+        if (tid == 0) sh.n = 0;
+        __syncthreads();
+        gather<BF16>(s, 0, cols, [&](float v) { return (v >= bound) & (v > kNone); }, to_list);
+        __syncthreads();
+        if (sh.n <= kList) {
+            draw_list<BF16>(a, row, r, s, (int)sh.n, sh);
+            return;
         }
     }
     // for top_p alone an eighth of the row is enough to lay out the steps, and the reading that counts them finds the best
@@ -1431,7 +1448,6 @@ struct Counted {
 struct RowState {          // all zero at the start
     uint64_t best;         // best column key (rows that draw the best column only)
     uint32_t top, low;     // order bits of the best score, reversed ones of the low score
-    uint32_t bound;        // order bits of a score that top_k columns reach (top_k)
     uint32_t n;            // columns gathered
     uint32_t part_top;     // order bits of the best score of the part of the row that was looked at first
     Counted steps;
@@ -1498,6 +1514,13 @@ __device__ __forceinline__ const Counted& counted_steps(const SplitArgs& p, int6
     return st->steps;
 }
 
+__device__ __forceinline__ void load_own(const SplitArgs& p, int64_t row, const Segments& segs, Shared& sh) {
+    for (int j = threadIdx.x; j < segs.n; j += kThreads) {
+        sh.seg[j + 1] = p.seg[row * (kSegs + 1) + j + 1];
+        sh.seg_top[j] = p.seg_top[row * kSegs + j];
+    }
+}
+
 // Without any restriction two launches do: the segments' own weights, and the draws
 template <bool BF16>
 __global__ __launch_bounds__(kThreads, 6) void sample_own_sum(SampleArgs a, SplitArgs p) {
@@ -1531,10 +1554,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_own_draw(SampleArgs a, Spl
         all_draws(a, row, best ? key_index(best) : -1, best ? 1.0f : 0.0f);
         return;
     }
-    for (int j = threadIdx.x; j < segs.n; j += kThreads) {
-        sh.seg[j + 1] = p.seg[row * (kSegs + 1) + j + 1];
-        sh.seg_top[j] = p.seg_top[row * kSegs + j];
-    }
+    load_own(p, row, segs, sh);
     draw_own<BF16>(a, row, r, row_scores<BF16>(a, row), segs, blockIdx.x, gridDim.x, sh);
 }
 
@@ -1557,7 +1577,7 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_top(SampleArgs a, Sp
         return;
     }
     const bool by_k = listed(a, r);
-    if (by_k && r.top_k > kList / 2) return;
+    if ((by_k && r.top_k > kList / 2) || unrestricted(a, r)) return;
     const bool sample = p.sample && r.top_p < 1.0;
     const Maxima m = scan_maxima<BF16>(s, part.lo, part.hi, by_k ? list_stride(part.lo, part.hi, r.top_k) : sample ? 8 : 1);
     if (by_k) {
@@ -1599,14 +1619,11 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_find(SampleArgs a, S
             sh.key[j] = reinterpret_cast<const uint64_t*>(p.sums)[(row * p.parts + j) * 2];
         sort_keys(p.parts, sh);
         const int64_t j = part_rank(r.top_k, p.parts);
-        const uint32_t order = (uint32_t)sh.key[(r.top_k + j - 1) / j - 1];
-        const float bound = unord_f32(order);
-        if (threadIdx.x == 0 && blockIdx.x == 0) st->bound = order;
-        if (!(bound > kNone)) return;
+        const float bound = unord_f32((uint32_t)sh.key[(r.top_k + j - 1) / j - 1]);  // without one there are few scores
         __syncthreads();
         if (threadIdx.x == 0) sh.n = 0;
         __syncthreads();
-        gather<BF16>(s, part.lo, part.hi, [&](float v) { return v >= bound; }, [&](uint64_t key) { push(sh.key, &sh.n, key); });
+        gather<BF16>(s, part.lo, part.hi, [&](float v) { return (v >= bound) & (v > kNone); }, [&](uint64_t key) { push(sh.key, &sh.n, key); });
         append_list(p.keys + row * kList, &st->n, sh);
     } else if (r.top_p < 1.0 && p.sample) {
         Binning bin;
@@ -1655,6 +1672,13 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_sum(SampleArgs a, Sp
     if (part.lo >= part.hi || best_only(r) || listed(a, r)) return;
     const void* s = row_scores<BF16>(a, row);
     double* seg = p.seg + row * (kSegs + 1);
+    if (unrestricted(a, r)) {
+        sum_own<BF16>(s, a.cols, segs, part.g0, part.g1, Weigh(0.0f, r.T, (int)a.cols), [&](int g, double w, float t) {
+            seg[g + 1] = w;
+            p.seg_top[row * kSegs + g] = t;
+        });
+        return;
+    }
     const float top = unord_f32(st->top);
     if (!finite(top)) return;
     const Weigh weigh(top, r.T, (int)a.cols);
@@ -1695,10 +1719,15 @@ __global__ __launch_bounds__(kThreads, 4) void sample_split_draw(SampleArgs a, S
         if (first) all_draws(a, row, st->best ? key_index(st->best) : -1, st->best ? 1.0f : 0.0f);
         return;
     }
+    if (unrestricted(a, r)) {
+        load_own(p, row, segs, sh);
+        draw_own<BF16>(a, row, r, s, segs, blockIdx.x, gridDim.x, sh);
+        return;
+    }
     const int n = (int)min(st->n, (uint32_t)kList + 1);
     bool alone = n > kList;
     const bool by_k = listed(a, r);
-    if (by_k && !alone && unord_f32(st->bound) > kNone) {  // 0, a NaN, where none was found
+    if (by_k && r.top_k <= kList / 2 && !alone) {
         if (!first) return;
         for (int j = tid; j < n; j += kThreads) sh.key[j] = p.keys[row * kList + j];
         __syncthreads();
@@ -1711,7 +1740,11 @@ __global__ __launch_bounds__(kThreads, 4) void sample_split_draw(SampleArgs a, S
     const bool by_p = r.top_p < 1.0;
     const float top = unord_f32(st->top);
     const Weigh weigh(top, r.T, (int)a.cols);
-    alone |= !finite(top);
+    if (!by_k && !finite(top)) {
+        if (!first) return;
+        if (top == INFINITY) draw_infinite<BF16>(a, row, r, s, sh); else all_draws(a, row, -1, 0.0f);
+        return;
+    }
     if (!alone && by_p) {
         Binning bin;
         load_steps(counted_steps(p, row, r, a.cols, bin), sh);
