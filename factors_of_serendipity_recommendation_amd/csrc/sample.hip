@@ -449,23 +449,28 @@ __device__ __forceinline__ void sort_keys(int n, Shared& sh) {
     __syncthreads();
 }
 
-// sh.w[0, n) -> its inclusive running sums, in order
-__device__ __forceinline__ void scan_list(int n, Shared& sh) {
-    constexpr int per = kList / kThreads;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lo = threadIdx.x * per;
-    double v[per], own = 0.0;
+// v[0, n), n <= PER * kThreads, in LDS -> its inclusive running sums, in order; the last place above 0 (0 without one)
+template <int PER>
+__device__ __forceinline__ int running_sums(double* v, int n, Shared& sh) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lo = threadIdx.x * PER;
+    double x[PER], own = 0.0;
+    uint32_t last = 0;
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < per; ++j) own += v[j] = lo + j < n ? sh.w[lo + j] : 0.0;
+    for (int j = 0; j < PER; ++j) {
+        x[j] = lo + j < n ? v[lo + j] : 0.0;
+        own += x[j];
+        if (x[j] > 0.0) last = lo + j;
+    }
     const double incl = wave_scan_f64(own);
     if (lane == 63) sh.dpart[wave] = incl;
     __syncthreads();
     double run = incl - own;
     for (int w = 0; w < wave; ++w) run += sh.dpart[w];
 #pragma unroll
-    for (int j = 0; j < per; ++j)
-        if (lo + j < n) sh.w[lo + j] = run += v[j];
-    __syncthreads();
+    for (int j = 0; j < PER; ++j)
+        if (lo + j < n) v[lo + j] = run += x[j];
+    return (int)block_max_u64(last, sh);
 }
 
 // ------------------------------------------------------------------------------------ one row
@@ -701,7 +706,7 @@ __device__ __forceinline__ void finish_list(const SampleArgs& a, int64_t row, co
     // min_p cuts a prefix of the ranking; top_p looks at all of top_k
     int keep = n;
     if (r.top_p < 1.0) {
-        scan_list(n, sh);
+        running_sums<kList / kThreads>(sh.w, n, sh);
         const double target = r.top_p * sh.w[n - 1];
         // column j stays iff the sum before it is below the target
         int lo = 1, hi = n;
@@ -727,10 +732,8 @@ __device__ __forceinline__ void finish_list(const SampleArgs& a, int64_t row, co
         const uint64_t key = sh.key[j];
         sh.w[j] = key ? weigh(unord_f32((uint32_t)key)) : 0.0;
     }
-    scan_list(keep, sh);
+    const int end = running_sums<kList / kThreads>(sh.w, keep, sh);  // the last column with any weight
     const double total = sh.w[keep - 1];
-    int end = keep - 1;  // the last column with any weight
-    while (end > 0 && !(sh.w[end] > sh.w[end - 1])) --end;
     for (int64_t j = threadIdx.x; j < a.n_draws; j += kThreads) {
         const double target = draw_number(a, row, j) * total;
         int lo = 0, hi = end;
@@ -1163,19 +1166,10 @@ __device__ __forceinline__ void draw_columns(const SampleArgs& a, int64_t row, c
                              const Weigh& weigh, int part, int parts, Shared& sh) {
     constexpr int N = Vec<BF16>::N, kStep = 64 * N;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    __syncthreads();
-    if (tid < 64) {
-        const int per = (segs.n + 63) / 64, lo = lane * per, hi = min(segs.n, lo + per);
-        double own = 0.0;
-        for (int j = lo; j < hi; ++j) own += sh.seg[j + 1];
-        double run = wave_scan_f64(own) - own;
-        for (int j = lo; j < hi; ++j) sh.seg[j + 1] = run += sh.seg[j + 1];
-        if (lane == 0) sh.seg[0] = 0.0;
-    }
+    const int last_seg = running_sums<kSegs / kThreads>(sh.seg + 1, segs.n, sh);  // the last segment with any weight
+    if (tid == 0) sh.seg[0] = 0.0;
     __syncthreads();
     const double total = sh.seg[segs.n];
-    int last_seg = segs.n - 1;  // the last segment with any weight
-    while (last_seg > 0 && !(sh.seg[last_seg + 1] > sh.seg[last_seg])) --last_seg;
     for (int64_t j = wave + (int64_t)part * kWaves; j < a.n_draws; j += (int64_t)parts * kWaves) {
         const double target = draw_number(a, row, j) * total;
         int lo = 0, hi = last_seg;  // the first segment whose end passes the target
