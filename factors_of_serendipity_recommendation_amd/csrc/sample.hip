@@ -30,6 +30,25 @@ constexpr int kAim = 384;  // columns a list is made of, where one chunk in seve
 constexpr int kShort = 256;  // columns that are compared with each other, a step per pair, instead of sorted
 constexpr int kSegs = 1024;  // column segments with sums of their own: a draw scans one of them
 
+// The columns' segments, at most kSegs: of up to eight steps of a wave each (so that their one reduction is shared), and as
+// many for every wave of the `parts` workgroups of a row
+struct Segments {
+    static constexpr int64_t kStep = 64 * 4, kMost = 8;
+    int64_t len;
+    int n, part;  // a workgroup's
+    explicit Segments(int64_t cols, int parts = 1) {
+        const int64_t waves = kWaves * parts, steps = (cols + kStep * waves - 1) / (kStep * waves);
+        int64_t each = (steps + kMost - 1) / kMost;
+        const int64_t more = (steps + kMost - 2) / (kMost - 1);  // a step shorter, if that leaves a wave fewer empty ones
+        if (more * ((steps + more - 1) / more) < each * ((steps + each - 1) / each)) each = more;
+        if (each > kSegs / waves) each = kSegs / waves;
+        len = (steps + each - 1) / each * kStep;
+        n = (int)((cols + len - 1) / len);
+        part = kWaves * (int)each;
+    }
+    int parts() const { return (n + part - 1) / part; }
+};
+
 struct SampleArgs {
     const void* S;
     int64_t rows, cols, ld;
@@ -42,6 +61,7 @@ struct SampleArgs {
     const int32_t* k_rows;
     int32_t* out_idx;
     float* out_prob;
+    Segments segs;  // of a row that one workgroup takes
 };
 
 // ------------------------------------------------------------------------------------ scores and weights
@@ -526,11 +546,14 @@ struct Binning {
 };
 // the largest score whose distance is at least x steps: at(s) < x iff s is above it (the distance falls with the score)
 __device__ __forceinline__ float score_at(const Binning& bin, float x) {
-    uint32_t lo = ord_f32(-INFINITY), hi = ord_f32(bin.top);  // at(lo) >= x; scores above top lie at less than any x > 0
     if (!(bin.at(bin.top) < x)) return bin.top;
+    // at(lo) >= x > at(hi); scores above top lie at less than any x > 0.  Every lane tries a place between them
+    uint32_t lo = ord_f32(-INFINITY), hi = __builtin_amdgcn_readfirstlane(ord_f32(bin.top));
     while (hi - lo > 1) {
-        const uint32_t mid = lo + (hi - lo) / 2;
-        if (bin.at(unord_f32(mid)) < x) hi = mid; else lo = mid;
+        const uint32_t step = (hi - lo + 64) / 65, mine = lo + step * ((threadIdx.x & 63) + 1);
+        const int n = __popcll(__ballot(mine < hi && !(bin.at(unord_f32(mine)) < x)));
+        hi = min(hi, lo + step * (n + 1));
+        lo += step * n;
     }
     return unord_f32(lo);
 }
@@ -772,18 +795,46 @@ __device__ __forceinline__ void draw_infinite(const SampleArgs& a, int64_t row, 
     }
 }
 
-// The columns' segments: `len` columns each, a multiple of a wave's step and at least four of those in a long row (so
-// that their one reduction is shared), and at most kSegs of them
-struct Segments {
-    int64_t len;
-    int n;
-    __host__ __device__ explicit Segments(int64_t cols) {
-        constexpr int64_t step = 64 * 4;
-        const int64_t least = (cols + kSegs * step - 1) / (kSegs * step);
-        len = (cols > 16 * step * kWaves && least < 4 ? 4 : least) * step;
-        n = (int)((cols + len - 1) / len);
+// f(four scores, column of the first) over the segments [g0, g1), done(segment) behind each.  A wave takes a run of them as
+// one stream: its addresses are a scalar and the lane's place, and the next step is on its way across their ends
+template <bool BF16, typename F, typename D>
+__device__ __forceinline__ void for_segments(const void* s, int64_t cols, const Segments& segs, int g0, int g1, F f, D done) {
+    constexpr int N = Vec<BF16>::N, kStep = Segments::kStep;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int each = (g1 - g0 + kWaves - 1) / kWaves, last = min(g1, g0 + (wave + 1) * each), per = (int)segs.len / kStep;
+    int g = g0 + wave * each, left = per;
+    if (g >= last) return;
+    const int64_t lo = g * segs.len, hi = min(cols, last * segs.len);
+    const int steps = (int)((hi - lo) / kStep);
+    const char* at = static_cast<const char*>(s) + lo * (BF16 ? 2 : 4);
+    Vec<BF16> v;
+    if (steps) {
+        v.load(at, lane * N);
+        v.arrive();
     }
-};
+#pragma unroll 1
+    for (int k = 0; k < steps; ++k) {
+        Vec<BF16> next;
+        at += kStep * (BF16 ? 2 : 4);
+        if (k + 1 < steps) next.load(at, lane * N);
+        float x[4];
+        v.values(x);
+        f(x, (int)lo + k * kStep + lane * N);
+        if (--left == 0) {
+            done(g++);
+            left = per;
+        }
+        v = next;
+    }
+    if (lo + (int64_t)steps * kStep < hi) {
+        const int64_t i = lo + (int64_t)steps * kStep + lane * N;
+        float x[4];
+        load_tail<BF16>(x, s, i, hi);
+        f(x, (int)min(i, hi));
+        left = 0;
+    }
+    if (left < per) done(g);
+}
 
 // what the first reading finds: the best scores of the thread's four classes of columns, and a low score that sets the
 // width of the steps (of a quarter of the columns, masks of the type's lowest value left out)
@@ -977,44 +1028,47 @@ __device__ __forceinline__ Window mass_window(const Binning& bin, double T, doub
 
 // One reading of the segments [g0, g1) with exact weights: z = all that the cut keeps, better = what lies before the
 // window, sum(g, .) = of that what min_p keeps.  The window's columns are put.  z and better of this lane.
+template <bool BF16, bool ALL, bool MASKS, typename Put, typename Sum>
+__device__ __forceinline__ void sum_window(const void* s, int64_t cols, const Segments& segs, int g0, int g1, float above, float least,
+                                           const Cut& cut, const Weigh& weigh, double min_p, Put put, Sum sum, double& z, double& better) {
+    const int lane = threadIdx.x & 63;
+    double w = 0.0;
+    z = better = 0.0;
+    for_segments<BF16>(s, cols, segs, g0, g1, [&](const float (&v)[4], int i) {
+        double x[4];
+        weigh.scaled<4>(v, 0, x);
+        uint64_t in[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const bool before = v[j] > above;
+            if (ALL || cut.keeps(v[j], i + j)) z += x[j];
+            if (before) {
+                if (MASKS) better += x[j];
+                if (!MASKS || x[j] >= min_p) w += x[j];
+            }
+            in[j] = __ballot(v[j] > least) & ~__ballot(before);
+        }
+        if (in[0] | in[1] | in[2] | in[3]) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if ((in[j] >> lane & 1) && (ALL || cut.keeps(v[j], i + j))) put(column_key(v[j], i + j));
+        }
+    }, [&](int g) {
+        if (!MASKS) better += w;
+        w = wave_scan_f64(w);
+        if (lane == 63) sum(g, w);
+        w = 0.0;
+    });
+}
 template <bool BF16, bool ALL, typename Put, typename Sum>
 __device__ __forceinline__ void sum_window(const void* s, int64_t cols, const Segments& segs, int g0, int g1, const Binning& bin,
                                            const Window& win, const Cut& cut, const Weigh& weigh, double min_p, Put put,
                                            Sum sum, double& z, double& better) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    z = better = 0.0;
     const float above = win.first > 0 ? score_at(bin, win.from) : INFINITY, least = score_at(bin, win.to);
-    const bool masks = min_p > 0.0;
-    for (int g = g0 + wave; g < g1; g += kWaves) {
-        double w = 0.0;
-        for_groups<BF16, 1>(s, g * segs.len, min(cols, (g + 1) * segs.len), lane, 64, [&](const float (&v)[4], int i) {
-            double x[4];
-            weigh.scaled<4>(v, 0, x);
-            bool in = false;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const bool ok = ALL || cut.keeps(v[j], i + j);
-                if (ok) z += x[j];
-                if (v[j] > above) {
-                    if (masks) {
-                        better += x[j];
-                        if (x[j] >= min_p) w += x[j];
-                    } else {
-                        w += x[j];
-                    }
-                }
-                in |= (v[j] > least) & !(v[j] > above);
-            }
-            if (in) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if ((v[j] > least) & !(v[j] > above) && (ALL || cut.keeps(v[j], i + j))) put(column_key(v[j], i + j));
-            }
-        });
-        if (!masks) better += w;
-        w = wave_scan_f64(w);
-        if (lane == 63) sum(g, w);
-    }
+    if (min_p > 0.0)
+        sum_window<BF16, ALL, true>(s, cols, segs, g0, g1, above, least, cut, weigh, min_p, put, sum, z, better);
+    else
+        sum_window<BF16, ALL, false>(s, cols, segs, g0, g1, above, least, cut, weigh, min_p, put, sum, z, better);
 }
 
 // The cut of top_p among the window's columns sh.key[0, n), and their kept weights added to the segments.  False if the
@@ -1092,24 +1146,21 @@ __device__ __forceinline__ void kept_weights(const float (&v)[4], int i, const C
 template <bool BF16, bool ALL, typename Sum>
 __device__ __forceinline__ void sum_segments(const void* s, int64_t cols, const Segments& segs, int g0, int g1, const Cut& cut,
                                              const Weigh& weigh, double min_p, Sum sum) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const bool masks = min_p > 0.0;
-    for (int g = g0 + wave; g < g1; g += kWaves) {
-        double w = 0.0;
-        for_groups<BF16, 1>(s, g * segs.len, min(cols, (g + 1) * segs.len), lane, 64, [&](const float (&v)[4], int i) {
-            if (!ALL && !(max_of(max_of(v[0], v[1]), max_of(v[2], v[3])) >= cut.s)) return;
-            double x[4];
-            if (ALL && !masks) {
-                weigh.scaled<4>(v, 0, x);
-                w += (x[0] + x[1]) + (x[2] + x[3]);
-            } else {
-                kept_weights(v, i, cut, weigh, min_p, x);
-                w += (x[0] + x[1]) + (x[2] + x[3]);
-            }
-        });
+    double w = 0.0;
+    for_segments<BF16>(s, cols, segs, g0, g1, [&](const float (&v)[4], int i) {
+        if (!ALL && !(max_of(max_of(v[0], v[1]), max_of(v[2], v[3])) >= cut.s)) return;
+        double x[4];
+        if (ALL && !masks)
+            weigh.scaled<4>(v, 0, x);
+        else
+            kept_weights(v, i, cut, weigh, min_p, x);
+        w += (x[0] + x[1]) + (x[2] + x[3]);
+    }, [&](int g) {
         w = wave_scan_f64(w);
-        if (lane == 63) sum(g, w);
-    }
+        if ((threadIdx.x & 63) == 63) sum(g, w);
+        w = 0.0;
+    });
 }
 
 // The same without any restriction, in one reading: a segment's weights against the segment's own best score,
@@ -1119,21 +1170,30 @@ __device__ __forceinline__ void sum_segments(const void* s, int64_t cols, const 
 template <bool BF16, typename Sum>
 __device__ __forceinline__ void sum_own(const void* s, int64_t cols, const Segments& segs, int g0, int g1, const Weigh& like, Sum sum) {
     constexpr int U = 4, N = Vec<BF16>::N;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     for (int g = g0 + wave; g < g1; g += kWaves) {
         const int64_t end = min(cols, (g + 1) * segs.len);
         double w = 0.0;
         float top = kNone;
         for (int64_t i0 = g * segs.len; i0 < end; i0 += U * 64 * N) {
             float v[U][4], best = kNone;
+            const bool whole = i0 + U * 64 * N <= end;
+            if (whole) {
+                Vec<BF16> x[U];
 #pragma unroll
-            for (int k = 0; k < U; ++k) {
-                const int64_t i = i0 + (k * 64 + lane) * N;
-                Vec<BF16> x;
-                x.none();
-                if (i + N <= end) x.load(s, i);
-                x.values(v[k]);
-                if (i < end && i + N > end) load_tail<BF16>(v[k], s, i, end);
+                for (int k = 0; k < U; ++k) x[k].load(s, i0 + (k * 64 + lane) * N);
+#pragma unroll
+                for (int k = 0; k < U; ++k) x[k].values(v[k]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < U; ++k) {
+                    const int64_t i = i0 + (k * 64 + lane) * N;
+                    Vec<BF16> x;
+                    x.none();
+                    if (i + N <= end) x.load(s, i);
+                    x.values(v[k]);
+                    if (i < end && i + N > end) load_tail<BF16>(v[k], s, i, end);
+                }
             }
 #pragma unroll
             for (int k = 0; k < U; ++k) best = max_of(best, max_of(max_of(v[k][0], v[k][1]), max_of(v[k][2], v[k][3])));
@@ -1148,11 +1208,18 @@ __device__ __forceinline__ void sum_own(const void* s, int64_t cols, const Segme
             }
             weigh.m = (double)top;
             if (top == INFINITY) continue;
-#pragma unroll
-            for (int k = 0; k < U; ++k) {
+            auto add = [&](const float (&s)[4]) {
                 double x[4];
-                weigh.scaled<4>(v[k], 0, x);
+                weigh.scaled<4>(s, 0, x);
                 w += (x[0] + x[1]) + (x[2] + x[3]);
+            };
+            if (whole) {
+#pragma unroll
+                for (int k = 0; k < U; ++k) add(v[k]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < U; ++k)
+                    if (i0 + k * 64 * N < end) add(v[k]);
             }
         }
         w = wave_scan_f64(w);
@@ -1308,12 +1375,11 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int64_t row, con
     }
     const bool by_k = K && listed(a, r), by_p = P && r.top_p < 1.0;
     if (!K && !P && !(r.min_p > 0.0)) {
-        const Segments own(cols);
-        sum_own<BF16>(s, cols, own, 0, own.n, Weigh(0.0f, r.T, cols), [&](int g, double w, float t) {
+        sum_own<BF16>(s, cols, a.segs, 0, a.segs.n, Weigh(0.0f, r.T, cols), [&](int g, double w, float t) {
             sh.seg[g + 1] = w;
             sh.seg_top[g] = t;
         });
-        draw_own<BF16>(a, row, r, s, own, 0, 1, sh);
+        draw_own<BF16>(a, row, r, s, a.segs, 0, 1, sh);
         return;
     }
     const auto to_list = [&](uint64_t key) { push(sh.key, &sh.n, key); };
@@ -1389,7 +1455,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int64_t row, con
             cut = descend<BF16, false>(s, cols, cut, (double)r.top_k, weigh, sh);
         }
     }
-    const Segments segs(cols);
+    const Segments& segs = a.segs;
     const auto to_seg = [&](int g, double w) { sh.seg[g + 1] = w; };
     bool summed = false;
     if (by_p) {
@@ -1454,7 +1520,8 @@ struct SplitArgs {
     double* seg;     // [rows, kSegs + 1]
     double* sums;    // [rows, parts, 2]: z, better (top_p); order bits of the part's class bound (top_k); best column key
     float* seg_top;  // [rows, kSegs]
-    int parts;
+    Segments segs;
+    int parts;       // of them, a workgroup each
 };
 
 __global__ __launch_bounds__(256) void sample_clear(uint32_t* p, int64_t n) {
@@ -1465,11 +1532,10 @@ __global__ __launch_bounds__(256) void sample_clear(uint32_t* p, int64_t n) {
 struct Part {
     int g0, g1;
     int64_t lo, hi;
-    __device__ __forceinline__ Part(const Segments& segs, int64_t cols, int part, int parts) {
-        const int per = (segs.n + parts - 1) / parts;
-        g0 = min(segs.n, part * per);
-        g1 = min(segs.n, g0 + per);
-        lo = min(cols, g0 * segs.len);
+    __device__ __forceinline__ Part(const Segments& segs, int64_t cols, int part) {
+        g0 = part * segs.part;
+        g1 = min(segs.n, g0 + segs.part);
+        lo = g0 * segs.len;
         hi = min(cols, g1 * segs.len);
     }
 };
@@ -1521,8 +1587,8 @@ __global__ __launch_bounds__(kThreads, 6) void sample_own_sum(SampleArgs a, Spli
     __shared__ Shared sh;
     const int64_t row = blockIdx.y;
     const Row r = row_settings(a, row);
-    const Segments segs(a.cols);
-    const Part part(segs, a.cols, blockIdx.x, p.parts);
+    const Segments& segs = p.segs;
+    const Part part(segs, a.cols, blockIdx.x);
     const void* s = row_scores<BF16>(a, row);
     if (best_only(r)) {
         const uint64_t best = block_max_u64(scan_best<BF16>(s, part.lo, part.hi, threadIdx.x, kThreads), sh);
@@ -1539,7 +1605,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_own_draw(SampleArgs a, Spl
     __shared__ Shared sh;
     const int64_t row = blockIdx.y;
     const Row r = row_settings(a, row);
-    const Segments segs(a.cols);
+    const Segments& segs = p.segs;
     if (best_only(r)) {
         if (blockIdx.x) return;
         uint64_t best = 0;
@@ -1561,8 +1627,7 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_top(SampleArgs a, Sp
     __shared__ Shared sh;
     const int64_t row = blockIdx.y;
     const Row r = row_settings(a, row);
-    const Part part(Segments(a.cols), a.cols, blockIdx.x, p.parts);
-    if (part.lo >= part.hi) return;
+    const Part part(p.segs, a.cols, blockIdx.x);
     RowState* st = p.state + row;
     const void* s = row_scores<BF16>(a, row);
     if (best_only(r)) {
@@ -1603,9 +1668,9 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_find(SampleArgs a, S
     __shared__ Shared sh;
     const int64_t row = blockIdx.y;
     const Row r = row_settings(a, row);
-    const Part part(Segments(a.cols), a.cols, blockIdx.x, p.parts);
+    const Part part(p.segs, a.cols, blockIdx.x);
     RowState* st = p.state + row;
-    if (part.lo >= part.hi || best_only(r)) return;
+    if (best_only(r)) return;
     const void* s = row_scores<BF16>(a, row);
     if (listed(a, r)) {
         if (r.top_k > kList / 2) return;
@@ -1646,8 +1711,8 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_again(SampleArgs a, 
     __shared__ Shared sh;
     const int64_t row = blockIdx.y;
     const Row r = row_settings(a, row);
-    const Part part(Segments(a.cols), a.cols, blockIdx.x, p.parts);
-    if (part.lo >= part.hi || best_only(r) || listed(a, r) || !(r.top_p < 1.0) || !finite(unord_f32(p.state[row].top))) return;
+    const Part part(p.segs, a.cols, blockIdx.x);
+    if (best_only(r) || listed(a, r) || !(r.top_p < 1.0) || !finite(unord_f32(p.state[row].top))) return;
     Binning bin;
     if (&counted_steps(p, row, r, a.cols, bin) != p.again + row) return;
     count_steps<BF16>(row_scores<BF16>(a, row), part.lo, part.hi, bin, Cut{kNone, -1}, sh);
@@ -1660,10 +1725,10 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_sum(SampleArgs a, Sp
     __shared__ Shared sh;
     const int64_t row = blockIdx.y;
     const Row r = row_settings(a, row);
-    const Segments segs(a.cols);
-    const Part part(segs, a.cols, blockIdx.x, p.parts);
+    const Segments& segs = p.segs;
+    const Part part(segs, a.cols, blockIdx.x);
     RowState* st = p.state + row;
-    if (part.lo >= part.hi || best_only(r) || listed(a, r)) return;
+    if (best_only(r) || listed(a, r)) return;
     const void* s = row_scores<BF16>(a, row);
     double* seg = p.seg + row * (kSegs + 1);
     if (unrestricted(a, r)) {
@@ -1706,7 +1771,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_split_draw(SampleArgs a, S
     const int tid = threadIdx.x;
     const bool first = blockIdx.x == 0;
     const Row r = row_settings(a, row);
-    const Segments segs(a.cols);
+    const Segments& segs = p.segs;
     const RowState* st = p.state + row;
     const void* s = row_scores<BF16>(a, row);
     if (best_only(r)) {
@@ -1769,24 +1834,25 @@ __global__ __launch_bounds__(kThreads, 4) void sample_split_draw(SampleArgs a, S
 }
 
 // How many workgroups share a row: none where a workgroup per row fills the chip (three fit a CU), else enough to fill it
-// four times over (rows with other settings cost other amounts), of at least four segments
+// four times over (rows with other settings cost other amounts), of at least two steps for every wave
 constexpr int64_t kFill = 768, kSplitGroups = 4 * kFill;
-int split_parts(int64_t rows, int64_t cols) {
-    if (rows <= 0 || rows >= kFill || cols <= 32768) return 1;
-    const Segments segs(cols);
-    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(kSplitGroups / rows, segs.n / 4));
-    return (int)ceil_div((int64_t)segs.n, ceil_div((int64_t)segs.n, parts));  // none without a segment
+Segments split_segments(int64_t rows, int64_t cols) {
+    int64_t parts = 1;
+    if (rows > 0 && rows < kFill && cols > 32768)
+        parts = std::min({kSplitGroups / rows, cols / (2 * kWaves * Segments::kStep), (int64_t)kSegs / kWaves});
+    return Segments(cols, (int)parts);
 }
 
 // parts of a row that are long enough for an eighth of them to show what the row is like
-bool split_sample(int64_t cols, int parts) { return cols / parts >= 16 * kChunk; }
+bool split_sample(const Segments& segs) { return segs.part * segs.len >= 16 * kChunk; }
 
 // the workspace: states, second counts, keys, segment sums, sums
 struct SplitLayout {
     size_t again, keys, seg, sums, seg_top, bytes;
-    SplitLayout(int64_t rows, int64_t cols, int parts) {
+    SplitLayout(int64_t rows, const Segments& segs) {
+        const int parts = segs.parts();
         again = (size_t)rows * sizeof(RowState);
-        keys = align_up(again + (split_sample(cols, parts) ? (size_t)rows * sizeof(Counted) : 0));
+        keys = align_up(again + (split_sample(segs) ? (size_t)rows * sizeof(Counted) : 0));
         seg = keys + align_up((size_t)rows * kList * 8);
         sums = seg + align_up((size_t)rows * (kSegs + 1) * 8);
         seg_top = sums + align_up((size_t)rows * parts * 16);
@@ -1795,7 +1861,8 @@ struct SplitLayout {
 };
 
 template <bool BF16>
-int launch_sample(const SampleArgs& a, void* ws, int parts, hipStream_t stream) {
+int launch_sample(const SampleArgs& a, void* ws, const Segments& segs, hipStream_t stream) {
+    const int parts = segs.parts();
     if (parts == 1) {
         const unsigned grid = (unsigned)a.rows;
         if (a.k_rows || (a.top_k > 0 && a.top_k < a.cols))
@@ -1807,11 +1874,11 @@ int launch_sample(const SampleArgs& a, void* ws, int parts, hipStream_t stream) 
         LGX_LAUNCH_CHECK();
         return LGX_OK;
     }
-    const SplitLayout l(a.rows, a.cols, parts);
-    const bool by_p = a.p_rows || a.top_p < 1.0, sample = by_p && split_sample(a.cols, parts);
+    const SplitLayout l(a.rows, segs);
+    const bool by_p = a.p_rows || a.top_p < 1.0, sample = by_p && split_sample(segs);
     char* w = static_cast<char*>(ws);
     const SplitArgs p{reinterpret_cast<RowState*>(w), reinterpret_cast<Counted*>(w + l.again), sample, reinterpret_cast<uint64_t*>(w + l.keys), reinterpret_cast<double*>(w + l.seg),
-                      reinterpret_cast<double*>(w + l.sums), reinterpret_cast<float*>(w + l.seg_top), parts};
+                      reinterpret_cast<double*>(w + l.sums), reinterpret_cast<float*>(w + l.seg_top), segs, parts};
     const dim3 grid((unsigned)parts, (unsigned)a.rows);
     const dim3 draws((unsigned)std::min<int64_t>(ceil_div(a.n_draws, (int64_t)kWaves), parts), (unsigned)a.rows);
     const bool find = by_p || a.k_rows || (a.top_k > 0 && a.top_k < a.cols);
@@ -1850,7 +1917,7 @@ using namespace lgx;
 extern "C" int lgx_sample_rows_workspace(int64_t rows, int64_t cols, int64_t n_draws, size_t* ws_bytes) {
     LGX_REQUIRE(ws_bytes && rows >= 0 && cols >= 1 && n_draws >= 0, LGX_ERR_INVALID_ARG,
                 "lgx_sample_rows_workspace: bad arguments");
-    *ws_bytes = SplitLayout(rows, cols, split_parts(rows, cols)).bytes;
+    *ws_bytes = SplitLayout(rows, split_segments(rows, cols)).bytes;
     return LGX_OK;
 }
 
@@ -1868,11 +1935,11 @@ extern "C" int lgx_sample_rows(const void* S, int dtype, int64_t rows, int64_t c
     if (rows == 0 || n_draws == 0) return LGX_OK;
     LGX_REQUIRE(rows < (1LL << 31), LGX_ERR_UNSUPPORTED, "lgx_sample_rows: %lld rows is too many", (long long)rows);
     LGX_REQUIRE(S && u && out_idx, LGX_ERR_INVALID_ARG, "lgx_sample_rows: null pointer");
-    const int parts = split_parts(rows, cols);
-    const size_t need = SplitLayout(rows, cols, parts).bytes;
+    const Segments segs = split_segments(rows, cols);
+    const size_t need = SplitLayout(rows, segs).bytes;
     LGX_REQUIRE(need == 0 || (ws && ws_bytes >= need && reinterpret_cast<uintptr_t>(ws) % 16 == 0), LGX_ERR_WORKSPACE,
                 "lgx_sample_rows: workspace %zu < %zu", ws_bytes, need);
     const SampleArgs a{S, rows, cols, ld, u, u_dtype == LGX_DTYPE_F64, n_draws, temperature, top_p, min_p, top_k,
-                       temperature_rows, top_p_rows, min_p_rows, top_k_rows, out_idx, out_prob};
-    return dtype == LGX_DTYPE_BF16 ? launch_sample<true>(a, ws, parts, stream) : launch_sample<false>(a, ws, parts, stream);
+                       temperature_rows, top_p_rows, min_p_rows, top_k_rows, out_idx, out_prob, Segments(cols)};
+    return dtype == LGX_DTYPE_BF16 ? launch_sample<true>(a, ws, segs, stream) : launch_sample<false>(a, ws, segs, stream);
 }
