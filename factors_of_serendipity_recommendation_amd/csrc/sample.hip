@@ -26,6 +26,7 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kBins = 4096;  // of 32 bits, or half as many of 64
 constexpr int kTopBins = 512;  // the first of them, whose columns' places within the step are summed too
 constexpr int kList = 2048;  // columns that are gathered in LDS
+constexpr int kFar = 8192;   // and in the workspace, of a row that several workgroups share
 constexpr int kAim = 384;  // columns a list is made of, where one chunk in several is looked at first
 constexpr int kShort = 256;  // columns that are compared with each other, a step per pair, instead of sorted
 constexpr int kSegs = 1024;  // column segments with sums of their own: a draw scans one of them
@@ -951,10 +952,12 @@ __device__ __forceinline__ void count_steps(const void* s, int64_t lo, int64_t h
 }
 
 // The steps [first, last] that may hold the column in which the running weight reaches top_p of the whole, and the columns
-// in them; the likeliest step alone where those are too many.  The weight w at the mean place of a step's columns stands
-// for each of them.  Past the first steps, where single columns weigh little, the middle is their place: they lie anywhere
-// in the step's width of d, an error of w d / (T sqrt 12) each.  Four times its root of squares, and 5e-6 of the whole
-// (the slope of their number within a step), are allowed for.
+// in them.  The weight w at the mean place of a step's columns stands for each of them.  Past the first steps, where single
+// columns weigh little, the middle is their place: they lie anywhere in the step's width of d, an error of w d / (T sqrt 12)
+// each, or of that for all of a step's columns together where they share a score, as bf16 ones do.  Four times its root of
+// squares, and 5e-6 of the whole (the slope of their number within a step), are allowed for.  Where that is more than `limit`
+// columns, f32 ones fill their step evenly enough for a part of it to do: at most a step to both sides of where the target lies
+// in it (0.35 of the limit; they lie 0.01 of a step off).
 __device__ __forceinline__ double exp2_step(double distance, const Weigh& weigh) {
     Weigh one = weigh;
     one.m = 0.0;
@@ -964,9 +967,10 @@ struct Window {
     int first, last;
     uint64_t columns;
     float from, to;
-    __device__ __forceinline__ bool usable() const { return last < kBins - 1 && columns > 0 && columns <= kList; }
+    __device__ __forceinline__ bool usable(int limit) const { return last < kBins - 1 && columns > 0 && columns <= limit; }
 };
-__device__ __forceinline__ Window mass_window(const Binning& bin, double T, double top_p, const Weigh& weigh, Shared& sh) {
+template <bool BF16>
+__device__ __forceinline__ Window mass_window(const Binning& bin, double T, double top_p, const Weigh& weigh, int limit, Shared& sh) {
     constexpr int per = kBins / kThreads;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const double wide = 1.0 / (double)bin.inv;
@@ -988,7 +992,7 @@ __device__ __forceinline__ Window mass_window(const Binning& bin, double T, doub
 #pragma unroll
         for (int j = 0; j < per; ++j) {
             w[j] = count[j] ? (double)count[j] * x : 0.0;
-            square = fma(w[j], count[j] ? x : 0.0, square);
+            square = fma(w[j], BF16 ? w[j] : count[j] ? x : 0.0, square);
             x *= ratio;
         }
     }
@@ -1013,7 +1017,10 @@ __device__ __forceinline__ Window mass_window(const Binning& bin, double T, doub
         const double next = run + w[j];
         if (next >= t1 && run < t1) sh.bin = b0 + j;
         if (next >= t2 && run < t2) sh.bin2 = b0 + j;
-        if (next >= t3 && run < t3) sh.bin3 = b0 + j;
+        if (next >= t3 && run < t3) {
+            sh.bin3 = b0 + j;
+            sh.below = (uint64_t)__double_as_longlong(b0 + j + (t3 - run) / w[j]);
+        }
         run = next;
     }
     __syncthreads();
@@ -1022,7 +1029,16 @@ __device__ __forceinline__ Window mass_window(const Binning& bin, double T, doub
 #pragma unroll
     for (int j = 0; j < per; ++j) inside += b0 + j >= win.first && b0 + j <= win.last ? count[j] : 0;
     win.columns = block_sum_u64(inside, sh);
-    if (win.columns > kList) win = Window{(int)sh.bin3, (int)sh.bin3, sh.count[sh.bin3], (float)sh.bin3, (float)(sh.bin3 + 1)};
+    if (win.columns > (uint64_t)limit) {
+        const int b = (int)sh.bin3;
+        win = Window{b, b, sh.count[b], (float)b, (float)(b + 1)};
+        if (!BF16 && b > 0 && b < kBins - 2) {
+            const float at = (float)__longlong_as_double((int64_t)sh.below);
+            const uint32_t most = max(max(sh.count[b - 1], sh.count[b + 1]), sh.count[b]);
+            const float half = fminf(1.0f, 0.35f * (float)limit / (float)most);
+            win = Window{(int)(at - half), (int)(at + half), min((uint64_t)limit, (uint64_t)most), at - half, at + half};
+        }
+    }
     return win;
 }
 
@@ -1064,58 +1080,88 @@ template <bool BF16, bool ALL, typename Put, typename Sum>
 __device__ __forceinline__ void sum_window(const void* s, int64_t cols, const Segments& segs, int g0, int g1, const Binning& bin,
                                            const Window& win, const Cut& cut, const Weigh& weigh, double min_p, Put put,
                                            Sum sum, double& z, double& better) {
-    const float above = win.first > 0 ? score_at(bin, win.from) : INFINITY, least = score_at(bin, win.to);
+    const float above = win.from > 0.0f ? score_at(bin, win.from) : INFINITY, least = score_at(bin, win.to);
     if (min_p > 0.0)
         sum_window<BF16, ALL, true>(s, cols, segs, g0, g1, above, least, cut, weigh, min_p, put, sum, z, better);
     else
         sum_window<BF16, ALL, false>(s, cols, segs, g0, g1, above, least, cut, weigh, min_p, put, sum, z, better);
 }
 
-// The cut of top_p among the window's columns sh.key[0, n), and their kept weights added to the segments.  False if the
-// exact sums show that the cut lies elsewhere.
-__device__ __forceinline__ bool resolve_window(int n, double z, double better, const Binning& bin, const Window& win, const Row& r, const Segments& segs, const Weigh& weigh, Cut& cut, Shared& sh) {
+// The cut of top_p among the window's columns, and their kept weights added to the segments.  each(f): f(key) for this
+// thread's of them.  False if the exact sums show that the cut lies elsewhere.
+template <typename Each>
+__device__ __forceinline__ bool resolve_window(Each each, int64_t cols, double z, double better, const Binning& bin, const Window& win,
+                                               const Row& r, const Segments& segs, const Weigh& weigh, Cut& cut, Shared& sh) {
     const int tid = threadIdx.x;
     const double target = r.top_p * z, scale = ldexp(1.0, -weigh.unit);
     // kThreads smaller steps within the window, of weights, and the columns of the one that reaches the target
-    constexpr int per = kList / kThreads;
     const float fine = (float)kThreads / (win.to - win.from);
-    uint64_t mine[per], whole = 0, w[per];
-    int at[per];
+    const auto step = [&](float v) { return min(kThreads - 1, max(0, (int)((bin.at(v) - win.from) * fine))); };
+    uint64_t whole = 0;
     clear_fine(sh);
-#pragma unroll
-    for (int j = 0; j < per; ++j) {
-        mine[j] = tid + j * kThreads < n ? sh.key[tid + j * kThreads] : 0;
-        at[j] = -1;
-        w[j] = 0;
-        if (mine[j]) {
-            const float v = key_score(mine[j]);
-            w[j] = weigh.fixed(v);
-            whole += w[j];
-            at[j] = min(kThreads - 1, (int)((bin.at(v) - win.from) * fine));
-            atomicAdd((unsigned long long*)&sh.wide[at[j]], (unsigned long long)w[j]);
-        }
-    }
+    each([&](uint64_t key) {
+        const float v = key_score(key);
+        const uint64_t w = weigh.fixed(v);
+        whole += w;
+        atomicAdd((unsigned long long*)&sh.wide[step(v)], (unsigned long long)w);
+    });
     whole = block_sum_u64(whole, sh);
     if (!whole || !(better < target && better + (double)whole * scale >= target)) return false;
     find_fine((target - better) / scale, sh);
     const int b = (int)sh.bin;
     const double before = better + (double)sh.below * scale;
+    uint32_t most = 0, least = 0;  // order bits, reversed ones
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < per; ++j)
-        if (at[j] == b) {
-            const uint32_t k = atomicAdd(&sh.n, 1u);
-            sh.key[k] = mine[j];
-            sh.wide[k] = w[j];
-        }
-    __syncthreads();
-    // each thread adds up what ranks before its columns: the last one below the target is the cut
-    const int m = (int)sh.n;
+    each([&](uint64_t key) {
+        if (step(key_score(key)) != b) return;
+        const uint32_t order = (uint32_t)order_of(key_score(key));
+        most = max(most, order);
+        least = max(least, ~order);
+        const uint32_t k = atomicAdd(&sh.n, 1u);
+        if (k < kList) sh.key[k] = key;
+    });
+    block_max2(most, least, sh);
+    int m = (int)sh.n;
     uint64_t last = 0;  // of the keys below the target the smallest, complemented
-    for (int c = tid; c < m; c += kThreads) {
-        uint64_t sum = 0;
-        for (int j = 0; j < m; ++j) sum += sh.key[j] > sh.key[c] ? sh.wide[j] : 0;
-        if (before + (double)sum * scale < target) last = max(last, ~sh.key[c]);
+    if (m > 64 && most == ~least) {
+        // equal scores: the first `want` of them in column order, found in kThreads runs of columns
+        const double each_w = (double)weigh.fixed(unord_f32(most)) * scale;
+        double want = floor((target - before) / each_w);
+        if (!(before + want * each_w < target)) want -= 1.0;
+        if (before + (want + 1.0) * each_w < target) want += 1.0;
+        const uint32_t run = (uint32_t)((cols + kThreads - 1) / kThreads);
+        const int equals = m;
+        clear_fine(sh);
+        each([&](uint64_t key) {
+            if (step(key_score(key)) == b) atomicAdd((unsigned long long*)&sh.wide[(uint32_t)key_index(key) / run], 1ull);
+        });
+        find_fine(fmin(want + 1.0, (double)equals), sh);
+        const uint32_t piece = sh.bin;
+        const int64_t rank = (int64_t)fmin(want, (double)(equals - 1)) - (int64_t)sh.below;
+        __syncthreads();
+        each([&](uint64_t key) {
+            if (step(key_score(key)) != b || (uint32_t)key_index(key) / run != piece) return;
+            const uint32_t k = atomicAdd(&sh.n, 1u);
+            if (k < kList) sh.key[k] = key;
+        });
+        __syncthreads();
+        m = (int)sh.n;
+        if (m > kList) return false;
+        for (int c = tid; c < m; c += kThreads) {
+            int64_t n = 0;
+            for (int j = 0; j < m; ++j) n += sh.key[j] > sh.key[c];
+            if (n == rank) last = ~sh.key[c];
+        }
+    } else {
+        if (m > kList) return false;
+        for (int c = tid; c < m; c += kThreads) sh.wide[c] = weigh.fixed(key_score(sh.key[c]));
+        __syncthreads();
+        // each thread adds up what ranks before its columns: the last one below the target is the cut
+        for (int c = tid; c < m; c += kThreads) {
+            uint64_t sum = 0;
+            for (int j = 0; j < m; ++j) sum += sh.key[j] > sh.key[c] ? sh.wide[j] : 0;
+            if (before + (double)sum * scale < target) last = max(last, ~sh.key[c]);
+        }
     }
     last = block_max_u64(last, sh);
     if (!last) return false;
@@ -1124,13 +1170,11 @@ __device__ __forceinline__ bool resolve_window(int n, double z, double better, c
     __syncthreads();
     for (int j = tid; j < segs.n; j += kThreads) sh.wide[j] = 0;
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < per; ++j) {
-        const uint64_t k = mine[j];
+    each([&](uint64_t k) {
         const float v = key_score(k);
-        if (k && k >= key && weigh(v) >= r.min_p)
+        if (k >= key && weigh(v) >= r.min_p)
             atomicAdd((unsigned long long*)&sh.wide[(uint32_t)key_index(k) / (uint32_t)segs.len], (unsigned long long)weigh.fixed_kept(v));
-    }
+    });
     __syncthreads();
     for (int j = tid; j < segs.n; j += kThreads) sh.seg[j + 1] += (double)sh.wide[j] * scale;
     return true;
@@ -1464,8 +1508,8 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int64_t row, con
             count_steps<BF16>(s, 0, cols, bin, cut, sh);
         }
         __syncthreads();
-        const Window win = mass_window(bin, r.T, r.top_p, weigh, sh);
-        if (win.usable()) {
+        const Window win = mass_window<BF16>(bin, r.T, r.top_p, weigh, kList, sh);
+        if (win.usable(kList)) {
             double z, better;
             if (K && by_k)
                 sum_window<BF16, false>(s, cols, segs, 0, segs.n, bin, win, cut, weigh, r.min_p, to_list, to_seg, z, better);
@@ -1473,7 +1517,15 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int64_t row, con
                 sum_window<BF16, true>(s, cols, segs, 0, segs.n, bin, win, cut, weigh, r.min_p, to_list, to_seg, z, better);
             z = block_sum_f64(z, sh);
             better = block_sum_f64(better, sh);
-            summed = resolve_window((int)min(sh.n, (uint32_t)kList), z, better, bin, win, r, segs, weigh, cut, sh);
+            const uint32_t n = sh.n;
+            uint64_t mine[kList / kThreads];
+#pragma unroll
+            for (int j = 0; j < kList / kThreads; ++j) mine[j] = tid + j * kThreads < n ? sh.key[tid + j * kThreads] : 0;
+            summed = n <= kList && resolve_window([&](auto f) {
+#pragma unroll
+                for (int j = 0; j < kList / kThreads; ++j)
+                    if (mine[j]) f(mine[j]);
+            }, cols, z, better, bin, win, r, segs, weigh, cut, sh);
         }
         if (!summed) {
             uint64_t sum = 0;
@@ -1516,7 +1568,8 @@ struct SplitArgs {
     RowState* state;
     Counted* again;  // [rows], zero at the start: where the steps laid out from a part of the row missed its best score
     bool sample;     // top_p's steps are laid out from an eighth of the row
-    uint64_t* keys;  // [rows, kList]
+    uint64_t* keys;  // [rows, list]
+    int list;
     double* seg;     // [rows, kSegs + 1]
     double* sums;    // [rows, parts, 2]: z, better (top_p); order bits of the part's class bound (top_k); best column key
     float* seg_top;  // [rows, kSegs]
@@ -1652,15 +1705,25 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_top(SampleArgs a, Sp
     }
 }
 
+// a column to the workgroup's list in LDS, to the row's `list` ones in the workspace once that is full
+__device__ __forceinline__ void push_far(uint64_t* keys, uint32_t* count, uint32_t list, Shared& sh, uint64_t key) {
+    const uint32_t at = atomicAdd(&sh.n, 1u);
+    if (at < kList) {
+        sh.key[at] = key;
+    } else {
+        const uint32_t far = atomicAdd(count, 1u);
+        if (far < list) keys[far] = key;
+    }
+}
 // the workgroup's list behind the row's
-__device__ __forceinline__ void append_list(uint64_t* keys, uint32_t* count, Shared& sh) {
+__device__ __forceinline__ void append_list(uint64_t* keys, uint32_t* count, uint32_t list, Shared& sh) {
     __syncthreads();
-    const uint32_t n = sh.n;
+    const uint32_t n = min(sh.n, (uint32_t)kList);
     if (threadIdx.x == 0) sh.bin = atomicAdd(count, n);
     __syncthreads();
     const uint32_t at = sh.bin;
-    for (uint32_t j = threadIdx.x; j < min(n, (uint32_t)kList); j += kThreads)
-        if (at + j < kList) keys[at + j] = sh.key[j];
+    for (uint32_t j = threadIdx.x; j < n; j += kThreads)
+        if (at + j < list) keys[at + j] = sh.key[j];
 }
 
 template <bool BF16>
@@ -1682,8 +1745,8 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_find(SampleArgs a, S
         __syncthreads();
         if (threadIdx.x == 0) sh.n = 0;
         __syncthreads();
-        gather<BF16>(s, part.lo, part.hi, [&](float v) { return (v >= bound) & (v > kNone); }, [&](uint64_t key) { push(sh.key, &sh.n, key); });
-        append_list(p.keys + row * kList, &st->n, sh);
+        gather<BF16>(s, part.lo, part.hi, [&](float v) { return (v >= bound) & (v > kNone); }, [&](uint64_t key) { push_far(p.keys + row * p.list, &st->n, kList, sh, key); });
+        append_list(p.keys + row * p.list, &st->n, kList, sh);
     } else if (r.top_p < 1.0 && p.sample) {
         Binning bin;
         float top;
@@ -1749,12 +1812,13 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_sum(SampleArgs a, Sp
     load_steps(counted_steps(p, row, r, a.cols, bin), sh);
     if (threadIdx.x == 0) sh.n = 0;
     __syncthreads();
-    const Window win = mass_window(bin, r.T, r.top_p, weigh, sh);
-    if (!win.usable()) return;
+    const Window win = mass_window<BF16>(bin, r.T, r.top_p, weigh, p.list, sh);
+    if (!win.usable(p.list)) return;
     double z, better;
     sum_window<BF16, true>(s, a.cols, segs, part.g0, part.g1, bin, win, Cut{kNone, -1}, weigh, r.min_p,
-                           [&](uint64_t key) { push(sh.key, &sh.n, key); }, [&](int g, double w) { seg[g + 1] = w; }, z, better);
-    append_list(p.keys + row * kList, &st->n, sh);
+                           [&](uint64_t key) { push_far(p.keys + row * p.list, &st->n, p.list, sh, key); },
+                           [&](int g, double w) { seg[g + 1] = w; }, z, better);
+    append_list(p.keys + row * p.list, &st->n, p.list, sh);
     z = block_sum_f64(z, sh);
     better = block_sum_f64(better, sh);
     if (threadIdx.x == 0) {
@@ -1783,12 +1847,13 @@ __global__ __launch_bounds__(kThreads, 4) void sample_split_draw(SampleArgs a, S
         draw_own<BF16>(a, row, r, s, segs, blockIdx.x, gridDim.x, sh);
         return;
     }
-    const int n = (int)min(st->n, (uint32_t)kList + 1);
-    bool alone = n > kList;
     const bool by_k = listed(a, r);
+    const int list = by_k ? kList : p.list, n = (int)min(st->n, (uint32_t)list + 1);
+    bool alone = n > list;
+    const uint64_t* keys = p.keys + row * p.list;
     if (by_k && r.top_k <= kList / 2 && !alone) {
         if (!first) return;
-        for (int j = tid; j < n; j += kThreads) sh.key[j] = p.keys[row * kList + j];
+        for (int j = tid; j < n; j += kThreads) sh.key[j] = keys[j];
         __syncthreads();
         draw_list<BF16>(a, row, r, s, n, sh);
         return;
@@ -1808,19 +1873,20 @@ __global__ __launch_bounds__(kThreads, 4) void sample_split_draw(SampleArgs a, S
         Binning bin;
         load_steps(counted_steps(p, row, r, a.cols, bin), sh);
         __syncthreads();
-        const Window win = mass_window(bin, r.T, r.top_p, weigh, sh);
-        alone = !win.usable();
+        const Window win = mass_window<BF16>(bin, r.T, r.top_p, weigh, p.list, sh);
+        alone = !win.usable(p.list);
         if (!alone) {
             __syncthreads();
             for (int j = tid; j < segs.n; j += kThreads) sh.seg[j + 1] = seg[j + 1];
-            for (int j = tid; j < n; j += kThreads) sh.key[j] = p.keys[row * kList + j];
             double z = 0.0, better = 0.0;
             for (int j = 0; j < p.parts; ++j) {
                 z += p.sums[(row * p.parts + j) * 2];
                 better += p.sums[(row * p.parts + j) * 2 + 1];
             }
             __syncthreads();
-            alone = !resolve_window(n, z, better, bin, win, r, segs, weigh, cut, sh);
+            alone = !resolve_window([&](auto f) {
+                for (int j = tid; j < n; j += kThreads) f(keys[j]);
+            }, a.cols, z, better, bin, win, r, segs, weigh, cut, sh);
         }
     } else if (!alone) {
         for (int j = tid; j < segs.n; j += kThreads) sh.seg[j + 1] = seg[j + 1];
@@ -1845,15 +1911,16 @@ Segments split_segments(int64_t rows, int64_t cols) {
 
 // parts of a row that are long enough for an eighth of them to show what the row is like
 bool split_sample(const Segments& segs) { return segs.part * segs.len >= 16 * kChunk; }
+int split_list(int64_t cols) { return cols > 131072 ? kFar : kList; }
 
 // the workspace: states, second counts, keys, segment sums, sums
 struct SplitLayout {
     size_t again, keys, seg, sums, seg_top, bytes;
-    SplitLayout(int64_t rows, const Segments& segs) {
+    SplitLayout(int64_t rows, int64_t cols, const Segments& segs) {
         const int parts = segs.parts();
         again = (size_t)rows * sizeof(RowState);
         keys = align_up(again + (split_sample(segs) ? (size_t)rows * sizeof(Counted) : 0));
-        seg = keys + align_up((size_t)rows * kList * 8);
+        seg = keys + align_up((size_t)rows * split_list(cols) * 8);
         sums = seg + align_up((size_t)rows * (kSegs + 1) * 8);
         seg_top = sums + align_up((size_t)rows * parts * 16);
         bytes = parts > 1 ? seg_top + align_up((size_t)rows * kSegs * 4) : 0;
@@ -1874,10 +1941,10 @@ int launch_sample(const SampleArgs& a, void* ws, const Segments& segs, hipStream
         LGX_LAUNCH_CHECK();
         return LGX_OK;
     }
-    const SplitLayout l(a.rows, segs);
+    const SplitLayout l(a.rows, a.cols, segs);
     const bool by_p = a.p_rows || a.top_p < 1.0, sample = by_p && split_sample(segs);
     char* w = static_cast<char*>(ws);
-    const SplitArgs p{reinterpret_cast<RowState*>(w), reinterpret_cast<Counted*>(w + l.again), sample, reinterpret_cast<uint64_t*>(w + l.keys), reinterpret_cast<double*>(w + l.seg),
+    const SplitArgs p{reinterpret_cast<RowState*>(w), reinterpret_cast<Counted*>(w + l.again), sample, reinterpret_cast<uint64_t*>(w + l.keys), split_list(a.cols), reinterpret_cast<double*>(w + l.seg),
                       reinterpret_cast<double*>(w + l.sums), reinterpret_cast<float*>(w + l.seg_top), segs, parts};
     const dim3 grid((unsigned)parts, (unsigned)a.rows);
     const dim3 draws((unsigned)std::min<int64_t>(ceil_div(a.n_draws, (int64_t)kWaves), parts), (unsigned)a.rows);
@@ -1917,7 +1984,7 @@ using namespace lgx;
 extern "C" int lgx_sample_rows_workspace(int64_t rows, int64_t cols, int64_t n_draws, size_t* ws_bytes) {
     LGX_REQUIRE(ws_bytes && rows >= 0 && cols >= 1 && n_draws >= 0, LGX_ERR_INVALID_ARG,
                 "lgx_sample_rows_workspace: bad arguments");
-    *ws_bytes = SplitLayout(rows, split_segments(rows, cols)).bytes;
+    *ws_bytes = SplitLayout(rows, cols, split_segments(rows, cols)).bytes;
     return LGX_OK;
 }
 
@@ -1936,7 +2003,7 @@ extern "C" int lgx_sample_rows(const void* S, int dtype, int64_t rows, int64_t c
     LGX_REQUIRE(rows < (1LL << 31), LGX_ERR_UNSUPPORTED, "lgx_sample_rows: %lld rows is too many", (long long)rows);
     LGX_REQUIRE(S && u && out_idx, LGX_ERR_INVALID_ARG, "lgx_sample_rows: null pointer");
     const Segments segs = split_segments(rows, cols);
-    const size_t need = SplitLayout(rows, segs).bytes;
+    const size_t need = SplitLayout(rows, cols, segs).bytes;
     LGX_REQUIRE(need == 0 || (ws && ws_bytes >= need && reinterpret_cast<uintptr_t>(ws) % 16 == 0), LGX_ERR_WORKSPACE,
                 "lgx_sample_rows: workspace %zu < %zu", ws_bytes, need);
     const SampleArgs a{S, rows, cols, ld, u, u_dtype == LGX_DTYPE_F64, n_draws, temperature, top_p, min_p, top_k,

@@ -88,6 +88,17 @@ def test_long_rows(rows, cols):
     check(S, u, top_p=0.7)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_top_p_where_many_columns_lie_near_the_cut(dtype):
+    """Thousands of columns in the step that holds the cut, of one score among bf16 ones."""
+    S, u = scores(3, 1000000, 11, dtype, sigma=1.65)
+    S[2] = torch.sort(S[2]).values
+    for p, T in ((0.5, 2.0), (0.9, 1.0), (0.95, 0.7), (0.99, 1.0), (0.99, 0.5)):
+        check(S, u, top_p=p, temperature=T, min_p=1e-4 if p == 0.9 else 0.0)
+    S, u = scores(1, 12000000, 12, dtype)
+    check(S, u, top_p=0.9)
+
+
 def _odd_rows(cols, seed):
     """Rows that a histogram laid over a part of a normal row's scores would not expect."""
     g = torch.Generator().manual_seed(seed)
