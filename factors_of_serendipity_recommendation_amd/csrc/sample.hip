@@ -1899,13 +1899,16 @@ __global__ __launch_bounds__(kThreads, 4) void sample_split_draw(SampleArgs a, S
     draw_columns<BF16>(a, row, r, s, segs, cut, weigh, blockIdx.x, gridDim.x, sh);
 }
 
-// How many workgroups share a row: none where a workgroup per row fills the chip (three fit a CU), else enough to fill it
-// four times over (rows with other settings cost other amounts), of at least two steps for every wave
+// How many workgroups share a row: none where a workgroup per row fills the chip (three fit a CU; 1024 x 300,000 f32, top_p: 523
+// us, by two of them 633), except that of rows past 2^19 columns more bf16 ones share a score than a workgroup can list
+// (1024 x 1M bf16, top_p: 3.5 ms, by three of them 1.8; f32 2.0 and 2.1).  Else enough to fill it four times over (rows with
+// other settings cost other amounts), of at least two steps for every wave
+// (more than 16 kFill rows again none: their lists would take gigabytes)
 constexpr int64_t kFill = 768, kSplitGroups = 4 * kFill;
 Segments split_segments(int64_t rows, int64_t cols) {
     int64_t parts = 1;
-    if (rows > 0 && rows < kFill && cols > 32768)
-        parts = std::min({kSplitGroups / rows, cols / (2 * kWaves * Segments::kStep), (int64_t)kSegs / kWaves});
+    if (rows > 0 && rows < (cols > 1 << 19 ? 16 * kFill : kFill) && cols > 32768)
+        parts = std::min({std::max<int64_t>(2, kSplitGroups / rows), cols / (2 * kWaves * Segments::kStep), (int64_t)kSegs / kWaves});
     return Segments(cols, (int)parts);
 }
 

@@ -97,6 +97,12 @@ def test_top_p_where_many_columns_lie_near_the_cut(dtype):
         check(S, u, top_p=p, temperature=T, min_p=1e-4 if p == 0.9 else 0.0)
     S, u = scores(1, 12000000, 12, dtype)
     check(S, u, top_p=0.9)
+    S, u = scores(4, 600000, 13, dtype, sigma=1.65)
+    many, u_many = S.repeat(200, 1), u.repeat(200, 1)
+    for kw in ({"top_p": 0.9}, {"top_k": 40}, {"temperature": 0.8}):
+        want = check(S, u, **kw)
+        for g, w in zip(lgx.sample_rows(many, u_many, **kw), want):
+            assert torch.equal(g, w.repeat(200, 1)), kw
 
 
 def _odd_rows(cols, seed):
