@@ -113,8 +113,9 @@ __device__ __forceinline__ void load_tail(float (&v)[4], const void* s, int64_t 
 }
 
 // f(four scores, column of the first) over columns [lo, hi) by `width` lanes, this one being `me`; a lane takes
-// its columns in ascending order.  U = 1, 2: so many groups at a time with the next ones on their way (f takes long); U = 4:
-// four groups on their way at once.  What is past the end comes as -inf
+// its columns in ascending order.  U = 1, 2: so many groups at a time with the next ones on their way (f takes long); U = 4, 8:
+// so many on their way at once (8 bytes each of bf16 rows: 1024 x 91,599, top_k 100, 78 us with eight, 83 with four).  What is
+// past the end comes as -inf
 template <bool BF16, int U, typename F>
 __device__ __forceinline__ void for_groups(const void* s, int64_t lo, int64_t hi, int me, int width, F f) {
     constexpr int N = Vec<BF16>::N;
@@ -527,7 +528,7 @@ template <bool BF16>
 __device__ __forceinline__ uint64_t scan_best(const void* s, int64_t lo, int64_t hi, int me, int width) {
     float best = kNone;
     int at = -1;
-    for_groups<BF16, 4>(s, lo, hi, me, width, [&](const float (&v)[4], int i) {
+    for_groups<BF16, BF16 ? 8 : 4>(s, lo, hi, me, width, [&](const float (&v)[4], int i) {
         if (max_of(max_of(v[0], v[1]), max_of(v[2], v[3])) > best) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -851,7 +852,7 @@ constexpr int64_t kChunk = kThreads * 4;  // columns of one step of the workgrou
 template <bool BF16>
 __device__ __forceinline__ Maxima scan_maxima(const void* s, int64_t lo, int64_t hi, int64_t stride) {
     Maxima m{{kNone, kNone, kNone, kNone}, INFINITY};
-    for_groups<BF16, 4>(s, lo, hi, threadIdx.x, kThreads * stride, [&](const float (&v)[4], int) {
+    for_groups<BF16, BF16 ? 8 : 4>(s, lo, hi, threadIdx.x, kThreads * stride, [&](const float (&v)[4], int) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) m.best[j] = max_of(m.best[j], v[j]);
         m.low = v[0] > -1e30f ? fminf(m.low, v[0]) : m.low;
@@ -904,7 +905,7 @@ __device__ __forceinline__ void push(Keys keys, Count n, uint64_t key) {
 // put(key) for the columns of [lo, hi) that `take` names
 template <bool BF16, typename Take, typename Put>
 __device__ __forceinline__ void gather(const void* s, int64_t lo, int64_t hi, Take take, Put put) {
-    for_groups<BF16, 4>(s, lo, hi, threadIdx.x, kThreads, [&](const float (&v)[4], int i) {
+    for_groups<BF16, BF16 ? 8 : 4>(s, lo, hi, threadIdx.x, kThreads, [&](const float (&v)[4], int i) {
         if ((int)take(v[0]) | (int)take(v[1]) | (int)take(v[2]) | (int)take(v[3])) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -1547,8 +1548,8 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int64_t row, con
     draw_columns<BF16>(a, row, r, s, segs, cut, weigh, 0, 1, sh);
 }
 
-// 2048 x 40,981 f32, top_p: 175 us (2 1/8 readings, of which the memory's share is 126); 1024 x 91,599 bf16, top_k 100: 83 us (one
-// reading and a quarter, 42).  Held to 80 registers (three workgroups a CU) with 8 to 10 spilled
+// 2048 x 40,981 f32, top_p: 175 us (2 1/8 readings, of which the memory's share is 126); 1024 x 91,599 bf16, top_k 100: 78 us (one
+// reading and a third, 44).  Held to 80 registers (three workgroups a CU) with 8 to 10 spilled
 template <bool BF16, bool K, bool P>
 __global__ __launch_bounds__(kThreads, 6) void sample_rows_kernel(SampleArgs a) {
     __shared__ Shared sh;
