@@ -38,14 +38,19 @@ constexpr int kSegs = 1024;  // column segments with sums of their own: a draw s
 // The columns' segments, at most kSegs: of up to eight steps of a wave each (so that their one reduction is shared), and as
 // many for every wave of the `parts` workgroups of a row
 struct Segments {
-    static constexpr int64_t kStep = 64 * 4, kMost = 8;
+    static constexpr int64_t kStep = 64 * 4;
     int64_t len;
     int n, part;  // a workgroup's
-    explicit Segments(int64_t cols, int parts = 1) {
+    Segments(int64_t cols, int64_t n_draws, int parts = 1) {
         const int64_t waves = kWaves * parts, steps = (cols + kStep * waves - 1) / (kStep * waves);
-        int64_t each = (steps + kMost - 1) / kMost;
-        const int64_t more = (steps + kMost - 2) / (kMost - 1);  // a step shorter, if that leaves a wave fewer empty ones
-        if (more * ((steps + more - 1) / more) < each * ((steps + each - 1) / each)) each = more;
+        // a segment's reduction costs about a third of a step of its sum, and a draw scans one segment
+        int64_t most = 8;
+        while (most > 1 && 3 * most * most * n_draws > steps * waves) --most;
+        int64_t each = (steps + most - 1) / most;
+        if (most > 1) {
+            const int64_t more = (steps + most - 2) / (most - 1);  // a step shorter, if that leaves a wave fewer empty ones
+            if (more * ((steps + more - 1) / more) < each * ((steps + each - 1) / each)) each = more;
+        }
         if (each > kSegs / waves) each = kSegs / waves;
         len = (steps + each - 1) / each * kStep;
         n = (int)((cols + len - 1) / len);
@@ -53,6 +58,12 @@ struct Segments {
     }
     int parts() const { return (n + part - 1) / part; }
 };
+
+// whether a row that one workgroup takes is drawn from by running weights of groups of columns instead of segments
+constexpr int kGroup = 16;
+__host__ __device__ __forceinline__ bool grouped(int64_t cols, int64_t n_draws) {
+    return cols <= kList || (cols <= kGroup * kList && n_draws > kWaves);
+}
 
 struct SampleArgs {
     const void* S;
@@ -1276,6 +1287,67 @@ __device__ __forceinline__ void sum_own(const void* s, int64_t cols, const Segme
     }
 }
 
+// A row of at most kGroup x kList columns by one workgroup: the running weights of groups of columns in LDS, which every thread
+// searches for a draw of its own: 256 x 14,687 f32 with min_p, 100 draws 12 us (a wave a draw, on segments, 35), 20 draws 13 (16);
+// one draw of 1000 columns 7.3 (7.0), of 14,687 a wave's still: the groups take another reading
+template <bool BF16>
+__device__ __forceinline__ bool draw_groups(const SampleArgs& a, int64_t row, const Row& r, const void* s, const Cut& cut,
+                                            const Weigh& weigh, Shared& sh) {
+    constexpr int N = Vec<BF16>::N;
+    if (!grouped(a.cols, a.n_draws)) return false;
+    const int cols = (int)a.cols, size = (cols + N * kList - 1) / (N * kList) * N, n = (cols + size - 1) / size;
+    const auto weights = [&](int i, double (&w)[N]) {
+        float v[N];
+        if (i + N <= cols) {
+            Vec<BF16> x;
+            x.load(s, i);
+            x.values(v);
+        } else {
+            load_tail<BF16>(v, s, i, cols);
+        }
+        kept_weights(v, i, cut, weigh, r.min_p, w);
+    };
+    __syncthreads();
+    for (int g = threadIdx.x; g < n; g += kThreads) {
+        double sum = 0.0;
+        for (int i = g * size; i < min(cols, (g + 1) * size); i += N) {
+            double w[N];
+            weights(i, w);
+            sum += (w[0] + w[1]) + (w[2] + w[3]);
+        }
+        sh.w[g] = sum;
+    }
+    const int end = running_sums<kList / kThreads>(sh.w, n, sh);
+    const double total = sh.w[n - 1];
+    for (int64_t j = threadIdx.x; j < a.n_draws; j += kThreads) {
+        const double target = draw_number(a, row, j) * total;
+        int lo = 0, hi = end;  // the first group whose end passes the target
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (sh.w[mid] > target) hi = mid; else lo = mid + 1;
+        }
+        double run = lo ? sh.w[lo - 1] : 0.0, weight = 0.0;
+        int pick = -1;  // its first column past the target, or without one its last of any weight
+        bool past = false;
+        for (int i = lo * size; i < min(cols, (lo + 1) * size) && !past; i += N) {
+            double w[N];
+            weights(i, w);
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                run += w[k];
+                if (w[k] > 0.0 && !past) {
+                    pick = i + k;
+                    weight = w[k];
+                    past = run > target;
+                }
+            }
+        }
+        a.out_idx[row * a.n_draws + j] = pick;
+        if (a.out_prob) a.out_prob[row * a.n_draws + j] = (float)(weight / total);
+    }
+    return true;
+}
+
 // the draws part, part + parts, ... (in groups of kWaves) from the segment sums sh.seg[1, n]
 template <bool BF16>
 __device__ __forceinline__ void draw_columns(const SampleArgs& a, int64_t row, const Row& r, const void* s, const Segments& segs, const Cut& cut,
@@ -1423,7 +1495,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int64_t row, con
         return;
     }
     const bool by_k = K && listed(a, r), by_p = P && r.top_p < 1.0;
-    if (!K && !P && !(r.min_p > 0.0)) {
+    if (!K && !P && !(r.min_p > 0.0) && !grouped(cols, a.n_draws)) {
         sum_own<BF16>(s, cols, a.segs, 0, a.segs.n, Weigh(0.0f, r.T, cols), [&](int g, double w, float t) {
             sh.seg[g + 1] = w;
             sh.seg_top[g] = t;
@@ -1432,8 +1504,10 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int64_t row, con
         return;
     }
     const auto to_list = [&](uint64_t key) { push(sh.key, &sh.n, key); };
-    // the list of the columns that reach the bound of the first ones
-    if (by_k && r.top_k <= kList / 2) {
+    // the list of the columns that reach the bound of the first ones, or of all of a short row
+    if (K && (by_k ? r.top_k <= kList / 2 : by_p && cols <= kShort)) {
+        Row first = r;
+        if (!by_k) first.top_k = cols;
         float bound = kNone;
         if (cols > kList) {
             const Maxima m = scan_maxima<BF16>(s, 0, cols, list_stride(0, cols, r.top_k));
@@ -1446,7 +1520,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int64_t row, con
         gather<BF16>(s, 0, cols, [&](float v) { return (v >= bound) & (v > kNone); }, to_list);
         __syncthreads();
         if (sh.n <= kList) {
-            draw_list<BF16>(a, row, r, s, (int)sh.n, sh);
+            draw_list<BF16>(a, row, first, s, (int)sh.n, sh);
             return;
         }
     }
@@ -1541,6 +1615,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int64_t row, con
             cut = descend<BF16, true>(s, cols, cut, r.top_p * (double)block_sum_u64(sum, sh), weigh, sh);
         }
     }
+    if (draw_groups<BF16>(a, row, r, s, cut, weigh, sh)) return;
     if (!summed) {
         __syncthreads();
         sum_segments<BF16, !K && !P>(s, cols, segs, 0, segs.n, cut, weigh, r.min_p, to_seg);
@@ -1914,11 +1989,11 @@ __global__ __launch_bounds__(kThreads, 4) void sample_split_draw(SampleArgs a, S
 // other settings cost other amounts), of at least two steps for every wave
 // (more than 16 kFill rows again none: their lists would take gigabytes)
 constexpr int64_t kFill = 768, kSplitGroups = 4 * kFill;
-Segments split_segments(int64_t rows, int64_t cols) {
+Segments split_segments(int64_t rows, int64_t cols, int64_t n_draws) {
     int64_t parts = 1;
     if (rows > 0 && rows < (cols > 1 << 19 ? 16 * kFill : kFill) && cols > 32768)
         parts = std::min({std::max<int64_t>(2, kSplitGroups / rows), cols / (2 * kWaves * Segments::kStep), (int64_t)kSegs / kWaves});
-    return Segments(cols, (int)parts);
+    return Segments(cols, n_draws, (int)parts);
 }
 
 // parts of a row that are long enough for an eighth of them to show what the row is like
@@ -1944,9 +2019,10 @@ int launch_sample(const SampleArgs& a, void* ws, const Segments& segs, hipStream
     const int parts = segs.parts();
     if (parts == 1) {
         const unsigned grid = (unsigned)a.rows;
-        if (a.k_rows || (a.top_k > 0 && a.top_k < a.cols))
+        const bool by_p = a.p_rows || a.top_p < 1.0;
+        if (a.k_rows || (a.top_k > 0 && a.top_k < a.cols) || (by_p && a.cols <= kShort))
             sample_rows_kernel<BF16, true, true><<<grid, kThreads, 0, stream>>>(a);
-        else if (a.p_rows || a.top_p < 1.0)
+        else if (by_p)
             sample_rows_kernel<BF16, false, true><<<grid, kThreads, 0, stream>>>(a);
         else
             sample_rows_kernel<BF16, false, false><<<grid, kThreads, 0, stream>>>(a);
@@ -1996,7 +2072,7 @@ using namespace lgx;
 extern "C" int lgx_sample_rows_workspace(int64_t rows, int64_t cols, int64_t n_draws, size_t* ws_bytes) {
     LGX_REQUIRE(ws_bytes && rows >= 0 && cols >= 1 && n_draws >= 0, LGX_ERR_INVALID_ARG,
                 "lgx_sample_rows_workspace: bad arguments");
-    *ws_bytes = SplitLayout(rows, cols, split_segments(rows, cols)).bytes;
+    *ws_bytes = SplitLayout(rows, cols, split_segments(rows, cols, n_draws)).bytes;
     return LGX_OK;
 }
 
@@ -2014,11 +2090,12 @@ extern "C" int lgx_sample_rows(const void* S, int dtype, int64_t rows, int64_t c
     if (rows == 0 || n_draws == 0) return LGX_OK;
     LGX_REQUIRE(rows < (1LL << 31), LGX_ERR_UNSUPPORTED, "lgx_sample_rows: %lld rows is too many", (long long)rows);
     LGX_REQUIRE(S && u && out_idx, LGX_ERR_INVALID_ARG, "lgx_sample_rows: null pointer");
-    const Segments segs = split_segments(rows, cols);
+    const Segments segs = split_segments(rows, cols, n_draws);
     const size_t need = SplitLayout(rows, cols, segs).bytes;
     LGX_REQUIRE(need == 0 || (ws && ws_bytes >= need && reinterpret_cast<uintptr_t>(ws) % 16 == 0), LGX_ERR_WORKSPACE,
                 "lgx_sample_rows: workspace %zu < %zu", ws_bytes, need);
     const SampleArgs a{S, rows, cols, ld, u, u_dtype == LGX_DTYPE_F64, n_draws, temperature, top_p, min_p, top_k,
-                       temperature_rows, top_p_rows, min_p_rows, top_k_rows, out_idx, out_prob, Segments(cols)};
+                       temperature_rows, top_p_rows, min_p_rows, top_k_rows, out_idx, out_prob,
+                       Segments(cols, grouped(cols, n_draws) ? 1 : n_draws)};
     return dtype == LGX_DTYPE_BF16 ? launch_sample<true>(a, ws, segs, stream) : launch_sample<false>(a, ws, segs, stream);
 }
