@@ -732,48 +732,126 @@ __device__ __forceinline__ int shrink_list(int n, int64_t top_k, Shared& sh) {
     return (int)sh.n;
 }
 
-// the same for longer lists: sorted by rank, cut, and sorted by column
+// Of the keys `mine` (each thread's, 0 for none) the last in rank before which less than `target` lies: columns, or MASS: fixed
+// weights.  kThreads steps of the score name the step that holds it, whose keys are compared with each other
+template <bool MASS>
+__device__ __forceinline__ uint64_t list_cut(const uint64_t (&mine)[kList / kThreads], double target, const Weigh& weigh, Shared& sh) {
+    constexpr int per = kList / kThreads;
+    uint64_t* members = reinterpret_cast<uint64_t*>(sh.w);
+    const auto measure = [&](uint64_t key) { return MASS ? weigh.fixed(key_score(key)) : 1ull; };
+    uint32_t most = 0, least = 0;  // order bits, reversed ones
+#pragma unroll
+    for (int j = 0; j < per; ++j)
+        if (mine[j]) {
+            most = max(most, (uint32_t)(mine[j] >> 32));
+            least = max(least, ~(uint32_t)(mine[j] >> 32));
+        }
+    block_max2(most, least, sh);
+    const float top = unord_f32(most);
+    const Binning bin = make_binning(top, (double)top - (double)unord_f32(~least), kThreads);
+    clear_fine(sh);
+#pragma unroll
+    for (int j = 0; j < per; ++j)
+        if (mine[j]) atomicAdd((unsigned long long*)&sh.wide[bin.fine(key_score(mine[j]))], (unsigned long long)measure(mine[j]));
+    find_fine(target, sh);
+    const int b = (int)sh.bin;
+    const double before = (double)sh.below;
+#pragma unroll
+    for (int j = 0; j < per; ++j)
+        if (mine[j] && bin.fine(key_score(mine[j])) == b) members[atomicAdd(&sh.n, 1u)] = mine[j];
+    __syncthreads();
+    const int m = (int)sh.n;
+    uint64_t last = 0;  // of the keys below the target the smallest, complemented
+    for (int c = threadIdx.x; c < m; c += kThreads) {
+        uint64_t sum = 0;
+        for (int j = 0; j < m; ++j) sum += members[j] > members[c] ? measure(members[j]) : 0;
+        if (before + (double)sum < target) last = max(last, ~members[c]);
+    }
+    return ~block_max_u64(last, sh);
+}
+
+// the same for longer lists: cut by rank, and placed in column order by kThreads runs of columns
 __device__ __forceinline__ void finish_list(const SampleArgs& a, int64_t row, const Row& r, int n, const Weigh& weigh, Shared& sh) {
     if (n > kShort && r.top_k < n) n = shrink_list(n, r.top_k, sh);
     if (n <= kShort) {
         finish_short(a, row, r, n, weigh, sh);
         return;
     }
-    sort_keys(n, sh);
-    n = (int)min((int64_t)n, r.top_k);
-    for (int j = threadIdx.x; j < n; j += kThreads) sh.w[j] = weigh(key_score(sh.key[j]));
+    constexpr int per = kList / kThreads;
+    uint64_t mine[per], cut = 1;
     __syncthreads();
+#pragma unroll
+    for (int j = 0; j < per; ++j) mine[j] = threadIdx.x + j * kThreads < n ? sh.key[threadIdx.x + j * kThreads] : 0;
+    const auto keep = [&](auto f) {
+#pragma unroll
+        for (int j = 0; j < per; ++j)
+            if (!f(mine[j])) mine[j] = 0;
+    };
+    if (r.top_k < n) {
+        cut = list_cut<false>(mine, (double)r.top_k, weigh, sh);
+        keep([&](uint64_t key) { return key >= cut; });
+    }
     // min_p cuts a prefix of the ranking; top_p looks at all of top_k
-    int keep = n;
     if (r.top_p < 1.0) {
-        running_sums<kList / kThreads>(sh.w, n, sh);
-        const double target = r.top_p * sh.w[n - 1];
-        // column j stays iff the sum before it is below the target
-        int lo = 1, hi = n;
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (sh.w[mid - 1] < target) lo = mid + 1; else hi = mid;
-        }
-        keep = lo;
-        // (lo is the first count whose sum reaches the target)
-        __syncthreads();
+        uint64_t whole = 0;
+#pragma unroll
+        for (int j = 0; j < per; ++j) whole += mine[j] ? weigh.fixed(key_score(mine[j])) : 0;
+        whole = block_sum_u64(whole, sh);
+        cut = list_cut<true>(mine, r.top_p * (double)whole, weigh, sh);
+        keep([&](uint64_t key) { return key >= cut; });
     }
-    // the kept ones in column order
-    for (int j = threadIdx.x; j < keep; j += kThreads) {
-        const uint64_t key = sh.key[j];
-        const double w = weigh(key_score(key));
-        // ~column descending = column ascending; the score rides along in the low half
-        sh.wide[j] = w >= r.min_p ? (uint64_t)(uint32_t)key << 32 | (uint32_t)(key >> 32) : 0ull;
+    if (r.min_p > 0.0) keep([&](uint64_t key) { return key && weigh(key_score(key)) >= r.min_p; });
+    uint32_t last = 0, first = 0;  // columns, the first complemented
+#pragma unroll
+    for (int j = 0; j < per; ++j)
+        if (mine[j]) {
+            last = max(last, (uint32_t)key_index(mine[j]));
+            first = max(first, ~(uint32_t)key_index(mine[j]));
+        }
+    block_max2(last, first, sh);
+    first = ~first;
+    const uint32_t run = (last - first) / kThreads + 1;
+    const auto place = [&](uint64_t key) { return ((uint32_t)key_index(key) - first) / run; };
+    clear_fine(sh);
+#pragma unroll
+    for (int j = 0; j < per; ++j)
+        if (mine[j]) atomicAdd((unsigned long long*)&sh.wide[place(mine[j])], 1ull);
+    __syncthreads();
+    const uint64_t own = sh.wide[threadIdx.x], incl = wave_scan_u64(own);
+    if ((threadIdx.x & 63) == 63) sh.part[threadIdx.x >> 6] = incl;
+    __syncthreads();
+    uint64_t begin = incl - own;
+    n = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        if (w < (int)(threadIdx.x >> 6)) begin += sh.part[w];
+        n += (int)sh.part[w];
+    }
+    sh.wide[threadIdx.x] = begin;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < per; ++j)
+        if (mine[j]) sh.key[atomicAdd((unsigned long long*)&sh.wide[place(mine[j])], 1ull)] = mine[j];
+    __syncthreads();
+    int at[per];
+#pragma unroll
+    for (int j = 0; j < per; ++j) {
+        if (!mine[j]) continue;
+        const uint32_t p = place(mine[j]);
+        const int end = (int)sh.wide[p];
+        at[j] = p ? (int)sh.wide[p - 1] : 0;
+        const int begins = at[j];
+        for (int c = begins; c < end; ++c) at[j] += key_index(sh.key[c]) < key_index(mine[j]);
     }
     __syncthreads();
-    for (int j = threadIdx.x; j < keep; j += kThreads) sh.key[j] = sh.wide[j];
-    sort_keys(keep, sh);
-    for (int j = threadIdx.x; j < keep; j += kThreads) {
-        const uint64_t key = sh.key[j];
-        sh.w[j] = key ? weigh(unord_f32((uint32_t)key)) : 0.0;
-    }
-    const int end = running_sums<kList / kThreads>(sh.w, keep, sh);  // the last column with any weight
-    const double total = sh.w[keep - 1];
+#pragma unroll
+    for (int j = 0; j < per; ++j)
+        if (mine[j]) {
+            sh.key[at[j]] = mine[j];
+            sh.w[at[j]] = weigh(key_score(mine[j]));
+        }
+    const int end = running_sums<kList / kThreads>(sh.w, n, sh);  // the last column with any weight
+    const double total = sh.w[n - 1];
     for (int64_t j = threadIdx.x; j < a.n_draws; j += kThreads) {
         const double target = draw_number(a, row, j) * total;
         int lo = 0, hi = end;
@@ -782,8 +860,8 @@ __device__ __forceinline__ void finish_list(const SampleArgs& a, int64_t row, co
             if (sh.w[mid] > target) hi = mid; else lo = mid + 1;
         }
         const uint64_t key = sh.key[lo];
-        a.out_idx[row * a.n_draws + j] = (int32_t)(0xffffffffu - (uint32_t)(key >> 32));
-        if (a.out_prob) a.out_prob[row * a.n_draws + j] = (float)(weigh(unord_f32((uint32_t)key)) / total);
+        a.out_idx[row * a.n_draws + j] = key_index(key);
+        if (a.out_prob) a.out_prob[row * a.n_draws + j] = (float)(weigh(key_score(key)) / total);
     }
 }
 
