@@ -32,7 +32,7 @@ constexpr int kTopBins = 512;  // the first of them, whose columns' places withi
 constexpr int kList = 2048;  // columns that are gathered in LDS
 constexpr int kFar = 8192;   // and in the workspace, of a row that several workgroups share
 constexpr int kAim = 384;  // columns a list is made of, where one chunk in several is looked at first
-constexpr int kShort = 256;  // columns that are compared with each other, a step per pair, instead of sorted
+constexpr int kShort = 160;  // columns that are compared with each other, a step per pair, instead of placed
 constexpr int kSegs = 1024;  // column segments with sums of their own: a draw scans one of them
 
 // The columns' segments, at most kSegs: of up to eight steps of a wave each (so that their one reduction is shared), and as
@@ -772,8 +772,10 @@ __device__ __forceinline__ uint64_t list_cut(const uint64_t (&mine)[kList / kThr
 
 // the same for longer lists: cut by rank, and placed in column order by kThreads runs of columns
 __device__ __forceinline__ void finish_list(const SampleArgs& a, int64_t row, const Row& r, int n, const Weigh& weigh, Shared& sh) {
-    if (n > kShort && r.top_k < n) n = shrink_list(n, r.top_k, sh);
-    if (n <= kShort) {
+    // comparing takes two steps a column, and four times that a draw: 256 x 100 f32, one draw: 10 us, 100 draws: 17; placing 12
+    const auto few = [&](int n) { return n + 2 * min((int64_t)n, a.n_draws) <= kShort; };
+    if (!few(n) && r.top_k < n) n = shrink_list(n, r.top_k, sh);
+    if (few(n)) {
         finish_short(a, row, r, n, weigh, sh);
         return;
     }
@@ -1583,7 +1585,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int64_t row, con
     }
     const auto to_list = [&](uint64_t key) { push(sh.key, &sh.n, key); };
     // the list of the columns that reach the bound of the first ones, or of all of a short row
-    if (K && (by_k ? r.top_k <= kList / 2 : by_p && cols <= kShort)) {
+    if (K && (by_k ? r.top_k <= kList / 2 : by_p && cols <= kList)) {
         Row first = r;
         if (!by_k) first.top_k = cols;
         float bound = kNone;
@@ -2098,7 +2100,7 @@ int launch_sample(const SampleArgs& a, void* ws, const Segments& segs, hipStream
     if (parts == 1) {
         const unsigned grid = (unsigned)a.rows;
         const bool by_p = a.p_rows || a.top_p < 1.0;
-        if (a.k_rows || (a.top_k > 0 && a.top_k < a.cols) || (by_p && a.cols <= kShort))
+        if (a.k_rows || (a.top_k > 0 && a.top_k < a.cols) || (by_p && a.cols <= kList))
             sample_rows_kernel<BF16, true, true><<<grid, kThreads, 0, stream>>>(a);
         else if (by_p)
             sample_rows_kernel<BF16, false, true><<<grid, kThreads, 0, stream>>>(a);
