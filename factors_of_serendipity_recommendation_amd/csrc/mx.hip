@@ -20,6 +20,10 @@ using f32x4 = float __attribute__((ext_vector_type(4)));
 using f32x2 = float __attribute__((ext_vector_type(2)));
 using f32x16 = float __attribute__((ext_vector_type(16)));
 using i32x8 = int __attribute__((ext_vector_type(8)));
+// at any multiple of an element
+using f32x4u = float __attribute__((ext_vector_type(4), aligned(4)));
+using u32x2u = uint32_t __attribute__((ext_vector_type(2), aligned(2)));
+using u32x4u = uint32_t __attribute__((ext_vector_type(4), aligned(2)));
 
 // the codes of 8 scaled elements, element 0 in the low nibble of byte 0 (v_cvt_scalef32_pk_fp4_f32 rounds
 // to nearest even and saturates at 6; the scale is applied by the caller, so its own is 1)
@@ -32,13 +36,18 @@ __device__ __forceinline__ uint32_t pack8(const float (&y)[8]) {
     return r;
 }
 
+// 8 elements from 16-byte boundaries (VEC) or anywhere
+template <bool VEC>
 __device__ __forceinline__ void load8_f32(const float* p, float (&x)[8]) {
-    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+    using V = std::conditional_t<VEC, f32x4, f32x4u>;
+    const f32x4 a = *reinterpret_cast<const V*>(p), b = *reinterpret_cast<const V*>(p + 4);
 #pragma unroll
     for (int j = 0; j < 4; ++j) x[j] = a[j], x[4 + j] = b[j];
 }
+template <bool VEC>
 __device__ __forceinline__ void load8_bf16(const uint16_t* p, float (&x)[8]) {
-    const u32x4 a = *reinterpret_cast<const u32x4*>(p);
+    using V = std::conditional_t<VEC, u32x4, u32x4u>;
+    const u32x4 a = *reinterpret_cast<const V*>(p);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         x[2 * j] = __uint_as_float(a[j] << 16);
@@ -60,7 +69,8 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t a) {
 
 // 4 lanes per block, 8 elements a lane.  VEC: rows are 16-byte aligned and d % 8 == 0.  rows_of (optional):
 // the source row of every output row, a row outside [0, n_src) gives NaN blocks.  Bound by memory: 1M x 256 f32, 1.16 GB, in
-// 237 us (4.9 TB/s, a copy's rate); 70,839 x 64 in 4.6 us.
+// 237 us (4.9 TB/s, a copy's rate); 70,839 x 64 in 4.6 us.  Rows at odd addresses are loaded as wide, at any multiple of an
+// element (100,000 x 601 f32 43 us, element by element 101).
 template <bool BF16, bool VEC>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const void* __restrict__ X, const int64_t* __restrict__ rows_of,
                                                           int64_t n_src, int64_t units, int64_t nb, int64_t d, int64_t ld,
@@ -78,14 +88,12 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const void* __restrict
     }
     float x[8] = {};
     if (!bad) {
-        if (VEC) {
-            if (c0 < d) {
-                if (BF16)
-                    load8_bf16(static_cast<const uint16_t*>(X) + src * ld + c0, x);
-                else
-                    load8_f32(static_cast<const float*>(X) + src * ld + c0, x);
-            }
-        } else {
+        if (c0 + 8 <= d) {
+            if (BF16)
+                load8_bf16<VEC>(static_cast<const uint16_t*>(X) + src * ld + c0, x);
+            else
+                load8_f32<VEC>(static_cast<const float*>(X) + src * ld + c0, x);
+        } else if (!VEC) {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 if (c0 + j < d)
@@ -112,7 +120,8 @@ __device__ __forceinline__ float scale_value(uint32_t b) {  // 2^(b - 127); b = 
     return b == 255u ? __builtin_nanf("") : __uint_as_float(b ? b << 23 : 0x00400000u);
 }
 
-// 4 lanes per block, 8 elements a lane (the layout of the quantiser).  1M x 256 to f32: 237 us
+// 4 lanes per block, 8 elements a lane (the layout of the quantiser).  1M x 256 to f32: 237 us; 100,000 x 601 55 us
+// (element by element 146)
 template <bool BF16, bool VEC>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint8_t* __restrict__ codes,
                                                             const uint8_t* __restrict__ scales, int64_t units, int64_t nb,
@@ -135,11 +144,11 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint8_t* __res
     for (int j = 0; j < 8; ++j) v[j] = p[j / 2][j % 2] * s;
     if (BF16) {
         uint16_t* o = static_cast<uint16_t*>(out) + row * d + c0;
-        if (VEC) {
+        if (VEC || c0 + 8 <= d) {
             u32x4 w;
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
-            *reinterpret_cast<u32x4*>(o) = w;
+            *reinterpret_cast<std::conditional_t<VEC, u32x4, u32x4u>*>(o) = w;
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -147,9 +156,10 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint8_t* __res
         }
     } else {
         float* o = static_cast<float*>(out) + row * d + c0;
-        if (VEC) {
-            *reinterpret_cast<f32x4*>(o) = f32x4{v[0], v[1], v[2], v[3]};
-            *reinterpret_cast<f32x4*>(o + 4) = f32x4{v[4], v[5], v[6], v[7]};
+        if (VEC || c0 + 8 <= d) {
+            using V = std::conditional_t<VEC, f32x4, f32x4u>;
+            *reinterpret_cast<V*>(o) = f32x4{v[0], v[1], v[2], v[3]};
+            *reinterpret_cast<V*>(o + 4) = f32x4{v[4], v[5], v[6], v[7]};
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -265,9 +275,9 @@ __device__ __forceinline__ void load_query(Frag<HB>& f, const MxArgs& a, int64_t
                 if (a.q_vec) {
                     if (c0 + 8 * i < a.d) {
                         if (QD == LGX_DTYPE_BF16)
-                            load8_bf16(reinterpret_cast<const uint16_t*>(a.q) + at, x[i]);
+                            load8_bf16<true>(reinterpret_cast<const uint16_t*>(a.q) + at, x[i]);
                         else
-                            load8_f32(reinterpret_cast<const float*>(a.q) + at, x[i]);
+                            load8_f32<true>(reinterpret_cast<const float*>(a.q) + at, x[i]);
                     }
                 } else {
 #pragma unroll
@@ -315,10 +325,6 @@ __device__ __forceinline__ void mma_steps(f32x16 (&acc)[4], const Frag<HB>& q, c
 #pragma unroll
         for (int t = 0; t < 4; ++t) acc[t] = mma<3>(q.c[HB > 3 ? 3 : 0], it[t].c[HB > 3 ? 3 : 0], acc[t], q.s, it[t].s);
 }
-
-// rows of the score matrix start at any multiple of an element
-using f32x4u = float __attribute__((ext_vector_type(4), aligned(4)));
-using u32x2u = uint32_t __attribute__((ext_vector_type(2), aligned(2)));
 
 // 32 users x 128 items of results.  The items' tile t of lane l is item base + 4 (l % 32) + t, so that a lane's
 // four results of one user are neighbours in the output row: one 16-byte store (512 bytes of a row per
