@@ -196,8 +196,20 @@ __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c, uint32_t sa, u
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(frag(a), frag(b), c, 4, 4, KK, (int)sa, KK, (int)sb);
 }
 
-// within 2^-22 relative (the reciprocal instruction is 1 ulp off; an IEEE division made the stores wait)
-__device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + expf(-x)); }
+// e^-x by one instruction, |x| 2^-24 off for the rounding of x log2(e): below 2^-17 where the result is not 0, enough for
+// bf16 results.  f32 ones take the product's rest in: within 2^-22 with the reciprocal's 1 ulp.  2048 x 40,981 with expf: bf16
+// 59 us (34), f32 79 (76); an IEEE division made the stores wait
+template <bool BF16>
+__device__ __forceinline__ float sigmoid(float x) {
+    constexpr float c = -1.44269502f, c_rest = (float)(-1.4426950408889634074 - (double)c);  // -log2(e)
+    const float t = x * c;
+    float e = __builtin_amdgcn_exp2f(t);
+    if (!BF16) {
+        const float rest = __builtin_amdgcn_fmed3f(fmaf(x, c_rest, fmaf(x, c, -t)), -0.01f, 0.01f);  // (no number for infinite x)
+        e *= fmaf(rest, 0.69314718f, 1.0f);
+    }
+    return __builtin_amdgcn_rcpf(1.0f + e);
+}
 
 using u32u = uint32_t __attribute__((aligned(1)));
 using u16u = uint16_t __attribute__((aligned(1)));
@@ -351,7 +363,7 @@ __device__ __forceinline__ void store_tile(const MxArgs& a, const f32x16 (&acc)[
         if (u_lane + r >= a.B) continue;
         float v[4];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) v[t] = SIG ? sigmoid(acc[t][i]) : acc[t][i];
+        for (int t = 0; t < 4; ++t) v[t] = SIG ? sigmoid<BF16>(acc[t][i]) : acc[t][i];
         if (BF16) {
             uint16_t* o = static_cast<uint16_t*>(a.out) + (u0 + r) * a.n_items + base + off;
             if (left >= 4) {
@@ -379,7 +391,7 @@ constexpr int kUserTiles = 8;  // tiles of 32 users a workgroup of score_mx_shor
 // Rows of at most 8 blocks (d <= 256), HB = ceil(nb / 2): a wave keeps 128 items in registers and walks the
 // users' tiles; the next tile's rows are loaded before this one's scores are stored, so that no load waits
 // behind a store.  Bound by the writes of the score matrix: 1024 x 1M x 256 f32, 4.1 GB, in 0.76 ms (the same stores
-// without loads and products 0.755); 2048 x 40,981 x 64 with the sigmoid 69 us.
+// without loads and products 0.755); 2048 x 40,981 x 64 with the sigmoid 66 us.
 template <int HB, bool BF16, bool SIG, bool NT>
 __global__ __launch_bounds__(256, 2) void score_mx_short(MxArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);

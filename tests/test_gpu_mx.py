@@ -136,6 +136,17 @@ def test_score_mx_matches_64_bits(B, I, d, kind):
     assert ((got - torch.sigmoid(want)).abs() <= bound / 4 + 2.0 ** -20).all()
 
 
+@pytest.mark.parametrize("B,I,d,scale", [(5, 700, 64, 0.5), (70, 641, 100, 1.0), (40, 300, 600, 0.5), (300, 1000, 64, 8.0)])
+def test_sigmoid_in_bf16(B, I, d, scale):
+    """One rounding to bf16 beside the score's own error (a slope of at most 1/4) and the f32 arithmetic's; scores of hundreds
+    end at 0 and 1."""
+    t, items = lgx.mx_quantize(table(B, d, B) * scale), lgx.mx_quantize(table(I, d, I) * scale)
+    q, it = values64(t), values64(items)
+    want, bound = torch.sigmoid(q @ it.T), score_bound(q, it)
+    got = lgx.score_mx(t, items, apply_sigmoid=True, dtype=torch.bfloat16).double().cpu()
+    assert ((got - want).abs() <= bound / 4 + 2.0 ** -17 * want + 2.0 ** -9 * (want + bound) * 2 + 1e-38).all()
+
+
 @pytest.mark.parametrize("kind", ["f32", "mx"])
 def test_score_mx_gathers_rows_and_flags_bad_ones(kind):
     x, items = table(40, 96, 1), lgx.mx_quantize(table(333, 96, 2))
