@@ -686,16 +686,21 @@ def sample_rows(S: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
         raise ValueError(f"sample_rows: u must be [{rows}] or [{rows}, n], got {tuple(u.shape)}")
     n = u.shape[1] if u.dim() == 2 else 1
     with _on(dev):
-        t, t_rows = _row_setting("temperature", temperature, rows, dev, torch.float32, 0.0, float("inf"))
-        k, k_rows = _row_setting("top_k", top_k, rows, dev, torch.int32, 0, 2 ** 63 - 1)
-        p, p_rows = _row_setting("top_p", top_p, rows, dev, torch.float32, 0.0, 1.0)
-        m, m_rows = _row_setting("min_p", min_p, rows, dev, torch.float32, 0.0, 1.0)
-        idx = u.new_empty(u.shape, dtype=torch.int32)
-        prob = u.new_empty(u.shape, dtype=torch.float32)
+        if (type(temperature) is float and type(top_k) is int and type(top_p) is float and type(min_p) is float
+                and temperature >= 0.0 and 0 <= top_k < 2 ** 63 and 0.0 <= top_p <= 1.0 and 0.0 <= min_p <= 1.0):
+            t, k, p, m = temperature, top_k, top_p, min_p  # what most calls give, without four calls' time
+            t_rows = k_rows = p_rows = m_rows = None
+        else:
+            t, t_rows = _row_setting("temperature", temperature, rows, dev, torch.float32, 0.0, float("inf"))
+            k, k_rows = _row_setting("top_k", top_k, rows, dev, torch.int32, 0, 2 ** 63 - 1)
+            p, p_rows = _row_setting("top_p", top_p, rows, dev, torch.float32, 0.0, 1.0)
+            m, m_rows = _row_setting("min_p", min_p, rows, dev, torch.float32, 0.0, 1.0)
+        u = u.contiguous()
+        idx = torch.empty_like(u, dtype=torch.int32)
+        prob = torch.empty_like(u, dtype=torch.float32)
         if cols == 0:
             return idx.fill_(-1), prob.zero_()
         S, ld = _row_stride(S)
-        u = u.contiguous()
         L = _lib.lib()
         ws = ctypes.c_size_t(0)
         _lib.check(L.lgx_sample_rows_workspace(rows, cols, n, ctypes.byref(ws)), "lgx_sample_rows_workspace")
