@@ -689,14 +689,14 @@ extern "C" int lgx_score_mx(const void* Q, const uint8_t* q_scales, int q_dtype,
     LGX_REQUIRE(n_items < (1LL << 27), LGX_ERR_UNSUPPORTED, "lgx_score_mx: %lld items is too many (< 2^27)",
                 (long long)n_items);
     if (B == 0 || n_items == 0) return LGX_OK;
-    LGX_REQUIRE(Q && item_codes && item_scales && scores, LGX_ERR_INVALID_ARG, "lgx_score_mx: null pointer");
+    LGX_REQUIRE((Q || n_q == 0) && item_codes && item_scales && scores, LGX_ERR_INVALID_ARG, "lgx_score_mx: null pointer");
     LGX_REQUIRE(user_rows || B <= n_q, LGX_ERR_INVALID_ARG, "lgx_score_mx: %lld queries of %lld rows", (long long)B,
                 (long long)n_q);
     LGX_REQUIRE(aligned(item_codes, 16), LGX_ERR_INVALID_ARG, "lgx_score_mx: codes must be 16-byte aligned");
     const int64_t nb = ceil_div(d, (int64_t)kBlock);
     MxArgs a{static_cast<const uint8_t*>(Q), q_scales, user_rows, n_q, item_codes, item_scales, B, n_items, nb, scores, d, q_ld, false};
     if (q_dtype == LGX_DTYPE_MXFP4) {
-        LGX_REQUIRE(q_scales && aligned(Q, 16), LGX_ERR_INVALID_ARG, "lgx_score_mx: query codes must be 16-byte aligned, with scales");
+        LGX_REQUIRE((q_scales || n_q == 0) && aligned(Q, 16), LGX_ERR_INVALID_ARG, "lgx_score_mx: query codes must be 16-byte aligned, with scales");
     } else {
         LGX_REQUIRE(q_ld >= d, LGX_ERR_INVALID_ARG, "lgx_score_mx: q_ld=%lld < d", (long long)q_ld);
         size_t need = 0;

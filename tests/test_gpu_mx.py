@@ -185,6 +185,16 @@ def test_rows_outside_the_table_and_undefined_blocks_of_every_form(B, d, kind):
             assert torch.equal(torch.nan_to_num(got[j], 7.0), torch.nan_to_num(one[0], 7.0))
 
 
+def test_rows_of_an_empty_table():
+    """Every row lies outside it."""
+    for B, d in ((3, 64), (50, 64), (3, 320), (50, 320)):
+        x, it = torch.empty(0, d, device=DEV), lgx.mx_quantize(table(100, d, 1))
+        rows = torch.arange(B, device=DEV)
+        for q in (x, x.bfloat16(), lgx.mx_quantize(x)):
+            assert torch.isnan(lgx.score_mx(q, it, user_rows=rows)).all()
+            assert lgx.score_mx(q, it).shape == (0, 100)
+
+
 def test_score_mx_keeps_a_nan_block_to_its_rows():
     x, y = table(4, 64, 1), table(200, 64, 2)
     x[1, 5], y[17, 60] = float("nan"), float("inf")
