@@ -1715,27 +1715,34 @@ __global__ __launch_bounds__(kThreads, 6) void sample_rows_kernel(SampleArgs a) 
 // The same steps with a row cut into `parts` runs of segments, a workgroup each, and a launch per reading; what the
 // workgroups of a row tell each other goes through the workspace, in integers whose order does not matter or in slots
 // of their own.  A row that needs one of the rare ways is left to its first workgroup in the last launch.
-// 512 x 1M f32 with settings per row: top 192 us (a third of the rows is read whole: 0.7 GB), find 264 (62 %), again 10, sum 267
-// (a quarter with top_p, a twelfth without restrictions), draw 49 (the lists' sorts), clear 7.
+// 512 x 1M f32 with settings per row: top 192 us (a third of the rows is read whole: 0.7 GB), find 261 (62 %), again 10, sum 270
+// (a quarter with top_p, a twelfth without restrictions), draw 35, clear 7.
 struct Counted {
     uint32_t count[kBins];
     uint64_t place[kTopBins];
 };
-struct RowState {          // all zero at the start
-    uint64_t best;         // best column key (rows that draw the best column only)
-    uint32_t top, low;     // order bits of the best score, reversed ones of the low score
-    uint32_t n;            // columns gathered
-    uint32_t part_top;     // order bits of the best score of the part of the row that was looked at first
+// the best and a low score of what the first reading looked at
+struct Extent {
+    float top, low;
+};
+struct RowState {   // cleared at the start
+    uint32_t n;     // columns gathered
+    uint32_t top;   // order bits of the best score, of rows of which an eighth was looked at first
+    Extent extent;  // where there is a second launch
     Counted steps;
 };
 struct SplitArgs {
     RowState* state;
-    Counted* again;  // [rows], zero at the start: where the steps laid out from a part of the row missed its best score
+    Counted* again;  // [rows], cleared too: where the steps laid out from an eighth of the row missed its best score
     bool sample;     // top_p's steps are laid out from an eighth of the row
+    bool clear;      // by the first reading
+    bool find;       // there is a second launch
     uint64_t* keys;  // [rows, list]
     int list;
     double* seg;     // [rows, kSegs + 1]
-    double* sums;    // [rows, parts, 2]: z, better (top_p); order bits of the part's class bound (top_k); best column key
+    uint64_t* first;  // [rows, parts], what the part's first reading found: the class bound's order bits (top_k), the best column
+                      // key (rows that draw it only), or the best score's order bits above the low score's reversed ones
+    double* sums;     // [rows, parts, 2]: z, better (top_p)
     float* seg_top;  // [rows, kSegs]
     Segments segs;
     int parts;       // of them, a workgroup each
@@ -1767,28 +1774,37 @@ __device__ __forceinline__ void add_steps(Counted& c, const Shared& sh) {
         if (sh.place[j]) atomicAdd((unsigned long long*)&c.place[j], (unsigned long long)sh.place[j]);
 }
 __device__ __forceinline__ bool finite(float top) { return top > kNone && top < INFINITY; }
-// the row's steps: the ones laid out from its best score, or with room above from a part of the row's; false without them
-__device__ __forceinline__ Binning row_steps(const RowState* st, const Row& r, int64_t cols) {
-    const float top = unord_f32(st->top);
-    return Steps(top, of_reverse_order(st->low), r, cols).bins(top, 0.0);
+__device__ __forceinline__ Extent first_extent(const SplitArgs& p, int64_t row, Shared& sh) {
+    uint32_t top = 0, low = 0;
+    for (int j = threadIdx.x; j < p.parts; j += kThreads) {
+        const uint64_t x = p.first[row * p.parts + j];
+        top = max(top, (uint32_t)(x >> 32));
+        low = max(low, (uint32_t)x);
+    }
+    block_max2(top, low, sh);
+    return Extent{unord_f32(top), of_reverse_order(low)};
 }
-__device__ __forceinline__ bool part_steps(const RowState* st, const Row& r, int64_t cols, Binning& bin) {
-    const float top = unord_f32(st->part_top);
-    if (!finite(top)) return false;
-    const Steps steps(top, of_reverse_order(st->low), r, cols);
-    bin = steps.bins(top, steps.margin);
+__device__ __forceinline__ Extent known_extent(const SplitArgs& p, int64_t row, Shared& sh) {
+    return p.find ? p.state[row].extent : first_extent(p, row, sh);
+}
+__device__ __forceinline__ bool eighth(const SplitArgs& p, const Row& r) { return p.sample && r.top_p < 1.0; }
+__device__ __forceinline__ float best_score(const SplitArgs& p, int64_t row, const Row& r, const Extent& e) {
+    return eighth(p, r) ? unord_f32(p.state[row].top) : e.top;
+}
+// steps with room above what an eighth of the row showed; false without them
+__device__ __forceinline__ bool eighth_steps(const Extent& e, const Row& r, int64_t cols, Binning& bin) {
+    if (!finite(e.top)) return false;
+    const Steps steps(e.top, e.low, r, cols);
+    bin = steps.bins(e.top, steps.margin);
     return steps.margin > 0.1 * steps.range;
 }
 // what the columns were counted by, and the counts
-__device__ __forceinline__ const Counted& counted_steps(const SplitArgs& p, int64_t row, const Row& r, int64_t cols, Binning& bin) {
-    const RowState* st = p.state + row;
-    if (p.sample) {
-        if (part_steps(st, r, cols, bin) && unord_f32(st->top) <= bin.top) return st->steps;
-        bin = row_steps(st, r, cols);
-        return p.again[row];
-    }
-    bin = row_steps(st, r, cols);
-    return st->steps;
+__device__ __forceinline__ const Counted& counted_steps(const SplitArgs& p, int64_t row, const Row& r, int64_t cols, const Extent& e,
+                                                        Binning& bin) {
+    const float top = best_score(p, row, r, e);
+    if (p.sample && eighth_steps(e, r, cols, bin) && top <= bin.top) return p.state[row].steps;
+    bin = Steps(top, e.low, r, cols).bins(top, 0.0);
+    return p.sample ? p.again[row] : p.state[row].steps;
 }
 
 __device__ __forceinline__ void load_own(const SplitArgs& p, int64_t row, const Segments& segs, Shared& sh) {
@@ -1796,6 +1812,13 @@ __device__ __forceinline__ void load_own(const SplitArgs& p, int64_t row, const 
         sh.seg[j + 1] = p.seg[row * (kSegs + 1) + j + 1];
         sh.seg_top[j] = p.seg_top[row * kSegs + j];
     }
+}
+
+__device__ __forceinline__ void draw_best(const SampleArgs& a, const SplitArgs& p, int64_t row, Shared& sh) {
+    uint64_t best = 0;
+    for (int j = threadIdx.x; j < p.parts; j += kThreads) best = max(best, p.first[row * p.parts + j]);
+    best = block_max_u64(best, sh);
+    all_draws(a, row, best ? key_index(best) : -1, best ? 1.0f : 0.0f);
 }
 
 // Without any restriction two launches do: the segments' own weights, and the draws
@@ -1809,7 +1832,7 @@ __global__ __launch_bounds__(kThreads, 6) void sample_own_sum(SampleArgs a, Spli
     const void* s = row_scores<BF16>(a, row);
     if (best_only(r)) {
         const uint64_t best = block_max_u64(scan_best<BF16>(s, part.lo, part.hi, threadIdx.x, kThreads), sh);
-        if (threadIdx.x == 0) reinterpret_cast<uint64_t*>(p.sums)[(row * p.parts + blockIdx.x) * 2] = best;
+        if (threadIdx.x == 0) p.first[row * p.parts + blockIdx.x] = best;
         return;
     }
     sum_own<BF16>(s, a.cols, segs, part.g0, part.g1, Weigh(0.0f, r.T, (int)a.cols), [&](int g, double w, float t) {
@@ -1825,10 +1848,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_own_draw(SampleArgs a, Spl
     const Segments& segs = p.segs;
     if (best_only(r)) {
         if (blockIdx.x) return;
-        uint64_t best = 0;
-        for (int j = threadIdx.x; j < p.parts; j += kThreads) best = max(best, reinterpret_cast<const uint64_t*>(p.sums)[(row * p.parts + j) * 2]);
-        best = block_max_u64(best, sh);
-        all_draws(a, row, best ? key_index(best) : -1, best ? 1.0f : 0.0f);
+        draw_best(a, p, row, sh);
         return;
     }
     load_own(p, row, segs, sh);
@@ -1845,28 +1865,28 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_top(SampleArgs a, Sp
     const int64_t row = blockIdx.y;
     const Row r = row_settings(a, row);
     const Part part(p.segs, a.cols, blockIdx.x);
-    RowState* st = p.state + row;
     const void* s = row_scores<BF16>(a, row);
-    if (best_only(r)) {
-        const uint64_t best = block_max_u64(scan_best<BF16>(s, part.lo, part.hi, threadIdx.x, kThreads), sh);
-        if (threadIdx.x == 0) atomicMax((unsigned long long*)&st->best, (unsigned long long)best);
-        return;
-    }
     const bool by_k = listed(a, r);
-    if ((by_k && r.top_k > kList / 2) || unrestricted(a, r)) return;
-    const bool sample = p.sample && r.top_p < 1.0;
-    const Maxima m = scan_maxima<BF16>(s, part.lo, part.hi, by_k ? list_stride(part.lo, part.hi, r.top_k) : sample ? 8 : 1);
-    if (by_k) {
-        const float bound = class_bound(m, part_rank(r.top_k, p.parts), sh);
-        if (threadIdx.x == 0) reinterpret_cast<uint64_t*>(p.sums)[(row * p.parts + blockIdx.x) * 2] = order_of(bound);
-        return;
+    uint64_t found = 0;
+    if (best_only(r)) {
+        found = block_max_u64(scan_best<BF16>(s, part.lo, part.hi, threadIdx.x, kThreads), sh);
+    } else if (by_k ? r.top_k <= kList / 2 : !unrestricted(a, r)) {
+        const int64_t stride = by_k ? list_stride(part.lo, part.hi, r.top_k) : eighth(p, r) ? 8 : 1;
+        const Maxima m = scan_maxima<BF16>(s, part.lo, part.hi, stride);
+        if (by_k) {
+            found = order_of(class_bound(m, part_rank(r.top_k, p.parts), sh));
+        } else {
+            const uint64_t top = order_of(best_of(m, sh));
+            found = top << 32 | block_max_u64(reverse_order_of(m.low), sh);
+        }
     }
-    const uint32_t top = (uint32_t)order_of(best_of(m, sh));
-    const uint32_t low = (uint32_t)block_max_u64(reverse_order_of(m.low), sh);
-    if (threadIdx.x == 0) {
-        atomicMax(sample ? &st->part_top : &st->top, top);
-        atomicMax(&st->low, low);
-    }
+    if (threadIdx.x == 0) p.first[row * p.parts + blockIdx.x] = found;
+    if (!p.clear) return;
+    const auto clear = [&](void* at, int words) {
+        for (int j = blockIdx.x * kThreads + threadIdx.x; j < words; j += p.parts * kThreads) static_cast<uint32_t*>(at)[j] = 0;
+    };
+    clear(p.state + row, sizeof(RowState) / 4);
+    if (p.sample) clear(p.again + row, sizeof(Counted) / 4);
 }
 
 // a column to the workgroup's list in LDS, to the row's `list` ones in the workspace once that is full
@@ -1902,7 +1922,7 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_find(SampleArgs a, S
     if (listed(a, r)) {
         if (r.top_k > kList / 2) return;
         for (int j = threadIdx.x; j < p.parts; j += kThreads)
-            sh.key[j] = reinterpret_cast<const uint64_t*>(p.sums)[(row * p.parts + j) * 2];
+            sh.key[j] = p.first[row * p.parts + j];
         sort_keys(p.parts, sh);
         const int64_t j = part_rank(r.top_k, p.parts);
         const float bound = unord_f32((uint32_t)sh.key[(r.top_k + j - 1) / j - 1]);  // without one there are few scores
@@ -1911,10 +1931,15 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_find(SampleArgs a, S
         __syncthreads();
         gather<BF16>(s, part.lo, part.hi, [&](float v) { return (v >= bound) & (v > kNone); }, [&](uint64_t key) { push_far(p.keys + row * p.list, &st->n, kList, sh, key); });
         append_list(p.keys + row * p.list, &st->n, kList, sh);
-    } else if (r.top_p < 1.0 && p.sample) {
+        return;
+    }
+    if (unrestricted(a, r) || (blockIdx.x && !(r.top_p < 1.0))) return;
+    const Extent e = first_extent(p, row, sh);
+    if (blockIdx.x == 0 && threadIdx.x == 0) st->extent = e;
+    if (eighth(p, r)) {
         Binning bin;
         float top;
-        if (part_steps(st, r, a.cols, bin)) {
+        if (eighth_steps(e, r, a.cols, bin)) {
             count_steps<BF16>(s, part.lo, part.hi, bin, Cut{kNone, -1}, sh, &top);
             __syncthreads();
             add_steps(st->steps, sh);
@@ -1924,8 +1949,8 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_find(SampleArgs a, S
         }
         const uint32_t order = (uint32_t)block_max_u64(order_of(top), sh);
         if (threadIdx.x == 0) atomicMax(&st->top, order);
-    } else if (r.top_p < 1.0 && finite(unord_f32(st->top))) {
-        count_steps<BF16>(s, part.lo, part.hi, row_steps(st, r, a.cols), Cut{kNone, -1}, sh);
+    } else if (r.top_p < 1.0 && finite(e.top)) {
+        count_steps<BF16>(s, part.lo, part.hi, Steps(e.top, e.low, r, a.cols).bins(e.top, 0.0), Cut{kNone, -1}, sh);
         __syncthreads();
         add_steps(st->steps, sh);
     }
@@ -1941,7 +1966,7 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_again(SampleArgs a, 
     const Part part(p.segs, a.cols, blockIdx.x);
     if (best_only(r) || listed(a, r) || !(r.top_p < 1.0) || !finite(unord_f32(p.state[row].top))) return;
     Binning bin;
-    if (&counted_steps(p, row, r, a.cols, bin) != p.again + row) return;
+    if (&counted_steps(p, row, r, a.cols, p.state[row].extent, bin) != p.again + row) return;
     count_steps<BF16>(row_scores<BF16>(a, row), part.lo, part.hi, bin, Cut{kNone, -1}, sh);
     __syncthreads();
     add_steps(p.again[row], sh);
@@ -1965,7 +1990,8 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_sum(SampleArgs a, Sp
         });
         return;
     }
-    const float top = unord_f32(st->top);
+    const Extent extent = known_extent(p, row, sh);
+    const float top = best_score(p, row, r, extent);
     if (!finite(top)) return;
     const Weigh weigh(top, r.T, (int)a.cols);
     if (!(r.top_p < 1.0)) {
@@ -1973,7 +1999,7 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_sum(SampleArgs a, Sp
         return;
     }
     Binning bin;
-    load_steps(counted_steps(p, row, r, a.cols, bin), sh);
+    load_steps(counted_steps(p, row, r, a.cols, extent, bin), sh);
     if (threadIdx.x == 0) sh.n = 0;
     __syncthreads();
     const Window win = mass_window<BF16>(bin, r.T, r.top_p, weigh, p.list, sh);
@@ -2003,7 +2029,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_split_draw(SampleArgs a, S
     const RowState* st = p.state + row;
     const void* s = row_scores<BF16>(a, row);
     if (best_only(r)) {
-        if (first) all_draws(a, row, st->best ? key_index(st->best) : -1, st->best ? 1.0f : 0.0f);
+        if (first) draw_best(a, p, row, sh);
         return;
     }
     if (unrestricted(a, r)) {
@@ -2026,7 +2052,8 @@ __global__ __launch_bounds__(kThreads, 4) void sample_split_draw(SampleArgs a, S
     Cut cut{kNone, -1};
     const double* seg = p.seg + row * (kSegs + 1);
     const bool by_p = r.top_p < 1.0;
-    const float top = unord_f32(st->top);
+    const Extent extent = by_k ? Extent{0.0f, 0.0f} : known_extent(p, row, sh);  // (a top_k row comes here with no list)
+    const float top = best_score(p, row, r, extent);
     const Weigh weigh(top, r.T, (int)a.cols);
     if (!by_k && !finite(top)) {
         if (!first) return;
@@ -2035,7 +2062,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_split_draw(SampleArgs a, S
     }
     if (!alone && by_p) {
         Binning bin;
-        load_steps(counted_steps(p, row, r, a.cols, bin), sh);
+        load_steps(counted_steps(p, row, r, a.cols, extent, bin), sh);
         __syncthreads();
         const Window win = mass_window<BF16>(bin, r.T, r.top_p, weigh, p.list, sh);
         alone = !win.usable(p.list);
@@ -2080,15 +2107,16 @@ Segments split_segments(int64_t rows, int64_t cols, int64_t n_draws) {
 bool split_sample(const Segments& segs) { return segs.part * segs.len >= 16 * kChunk; }
 int split_list(int64_t cols) { return cols > 131072 ? kFar : kList; }
 
-// the workspace: states, second counts, keys, segment sums, sums
+// the workspace: states, second counts, keys, segment sums, first findings, sums, segments' best scores
 struct SplitLayout {
-    size_t again, keys, seg, sums, seg_top, bytes;
+    size_t again, keys, seg, first, sums, seg_top, bytes;
     SplitLayout(int64_t rows, int64_t cols, const Segments& segs) {
         const int parts = segs.parts();
         again = (size_t)rows * sizeof(RowState);
         keys = align_up(again + (split_sample(segs) ? (size_t)rows * sizeof(Counted) : 0));
         seg = keys + align_up((size_t)rows * split_list(cols) * 8);
-        sums = seg + align_up((size_t)rows * (kSegs + 1) * 8);
+        first = seg + align_up((size_t)rows * (kSegs + 1) * 8);
+        sums = first + align_up((size_t)rows * parts * 8);
         seg_top = sums + align_up((size_t)rows * parts * 16);
         bytes = parts > 1 ? seg_top + align_up((size_t)rows * kSegs * 4) : 0;
     }
@@ -2111,12 +2139,16 @@ int launch_sample(const SampleArgs& a, void* ws, const Segments& segs, hipStream
     }
     const SplitLayout l(a.rows, a.cols, segs);
     const bool by_p = a.p_rows || a.top_p < 1.0, sample = by_p && split_sample(segs);
+    const bool find = by_p || a.k_rows || (a.top_k > 0 && a.top_k < a.cols);
+    // a launch more costs a small batch 2 us (64 x 131,072, top_k 50: 57, 55 without), the clearing inside a reading of many rows 10
+    // (512 x 1M with settings per row: 738 us, 727 with the launch)
+    const int64_t words = a.rows * (int64_t)((sizeof(RowState) + (sample ? sizeof(Counted) : 0)) / 4);
+    const bool clear = words <= 1 << 21;
     char* w = static_cast<char*>(ws);
-    const SplitArgs p{reinterpret_cast<RowState*>(w), reinterpret_cast<Counted*>(w + l.again), sample, reinterpret_cast<uint64_t*>(w + l.keys), split_list(a.cols), reinterpret_cast<double*>(w + l.seg),
-                      reinterpret_cast<double*>(w + l.sums), reinterpret_cast<float*>(w + l.seg_top), segs, parts};
+    const SplitArgs p{reinterpret_cast<RowState*>(w), reinterpret_cast<Counted*>(w + l.again), sample, clear, find, reinterpret_cast<uint64_t*>(w + l.keys), split_list(a.cols), reinterpret_cast<double*>(w + l.seg),
+                      reinterpret_cast<uint64_t*>(w + l.first), reinterpret_cast<double*>(w + l.sums), reinterpret_cast<float*>(w + l.seg_top), segs, parts};
     const dim3 grid((unsigned)parts, (unsigned)a.rows);
     const dim3 draws((unsigned)std::min<int64_t>(ceil_div(a.n_draws, (int64_t)kWaves), parts), (unsigned)a.rows);
-    const bool find = by_p || a.k_rows || (a.top_k > 0 && a.top_k < a.cols);
     if (!find && !a.m_rows && !(a.min_p > 0.0)) {
         sample_own_sum<BF16><<<grid, kThreads, 0, stream>>>(a, p);
         LGX_LAUNCH_CHECK();
@@ -2124,9 +2156,10 @@ int launch_sample(const SampleArgs& a, void* ws, const Segments& segs, hipStream
         LGX_LAUNCH_CHECK();
         return LGX_OK;
     }
-    const int64_t words = a.rows * (int64_t)((sizeof(RowState) + (sample ? sizeof(Counted) : 0)) / 4);
-    sample_clear<<<(unsigned)std::min<int64_t>(1024, ceil_div(words, (int64_t)256)), 256, 0, stream>>>(reinterpret_cast<uint32_t*>(w), words);
-    LGX_LAUNCH_CHECK();
+    if (!clear) {
+        sample_clear<<<1024, 256, 0, stream>>>(reinterpret_cast<uint32_t*>(w), words);
+        LGX_LAUNCH_CHECK();
+    }
     sample_split_top<BF16><<<grid, kThreads, 0, stream>>>(a, p);
     LGX_LAUNCH_CHECK();
     if (find) {
