@@ -520,6 +520,9 @@ __device__ __forceinline__ Row row_settings(const SampleArgs& a, int64_t row) {
     r.T = a.T_rows ? (double)a.T_rows[row] : a.T;
     if (r.T > 0.0) r.T = fmax(r.T, 1e-300);  // below it 1 / T is none, and no two f32 scores lie so near anyway
     r.top_p = a.p_rows ? (double)a.p_rows[row] : a.top_p;
+    // within 1e-15 of top_p is reached: of equal weights that lie on it to the last bit (0.9 of ten), a sum's order and what weighs
+    // next to nothing would decide
+    if (r.top_p < 1.0) r.top_p *= 1.0 - 1e-15;
     const double m = a.m_rows ? (double)a.m_rows[row] : a.min_p;
     r.min_p = m > 0.0 ? fmin(m, 1.0) : 0.0;
     r.top_k = a.k_rows ? (int64_t)a.k_rows[row] : a.top_k;
@@ -640,9 +643,10 @@ __device__ __forceinline__ void finish_short(const SampleArgs& a, int64_t row, c
     const int n_wave = __builtin_amdgcn_readfirstlane(tid) < n ? n : 0;  // waves without a column skip the loops
     const uint64_t mine = tid < n ? sh.key[tid] : 0;
     const double weight = weigh(key_score(mine));
-    const uint64_t w = tid < n ? max(weigh.fixed(key_score(mine)), (uint64_t)(weight > 0.0 ? 1 : 0)) : 0;
+    const uint64_t plain = tid < n ? weigh.fixed(key_score(mine)) : 0;
+    const uint64_t w = max(plain, (uint64_t)(tid < n && weight > 0.0 ? 1 : 0));  // to be drawn
     // (weight, key) pairs side by side: a step of the loops is one read
-    if (tid < n) sh.pair[tid] = Pair{w, mine};
+    if (tid < n) sh.pair[tid] = Pair{plain, mine};
     __syncthreads();
     int rank = 0;
     uint64_t better = 0;
@@ -655,7 +659,7 @@ __device__ __forceinline__ void finish_short(const SampleArgs& a, int64_t row, c
     }
     bool keep = tid < n && rank < r.top_k;
     if (r.top_p < 1.0) {
-        const double target = r.top_p * (double)block_sum_u64(keep ? w : 0, sh);
+        const double target = r.top_p * (double)block_sum_u64(keep ? plain : 0, sh);
         keep &= rank == 0 || (double)better < target;
     }
     keep &= (w > 0) & (weight >= r.min_p);
@@ -1187,7 +1191,9 @@ __device__ __forceinline__ void sum_window(const void* s, int64_t cols, const Se
 // thread's of them.  False if the exact sums show that the cut lies elsewhere.
 template <typename Each>
 __device__ __forceinline__ bool resolve_window(Each each, int64_t cols, double z, double better, const Binning& bin, const Window& win,
-                                               const Row& r, const Segments& segs, const Weigh& weigh, Cut& cut, Shared& sh) {
+                                               const Row& r, const Segments& segs, Weigh weigh, Cut& cut, Shared& sh) {
+    static_assert(kFar <= 1 << 13, "units of 2^-49");
+    weigh.unit = 49;  // these columns' weights add up to at most kFar
     const int tid = threadIdx.x;
     const double target = r.top_p * z, scale = ldexp(1.0, -weigh.unit);
     // kThreads smaller steps within the window, of weights, and the columns of the one that reaches the target
@@ -1540,7 +1546,7 @@ __device__ __forceinline__ void draw_list(const SampleArgs& a, int64_t row, cons
     else if (key_score(best) == INFINITY)
         draw_infinite<BF16>(a, row, r, s, sh);
     else
-        finish_list(a, row, r, n, Weigh(key_score(best), r.T, (int)a.cols), sh);
+        finish_list(a, row, r, n, Weigh(key_score(best), r.T, n), sh);
 }
 
 // the draws of a row without restrictions, from its segments' weights against their own best scores (sh.seg, sh.seg_top)

@@ -472,7 +472,8 @@ int lgx_score_mx(const void* Q, const uint8_t* q_scales, int q_dtype, int64_t n_
  *   weight w_i = exp((s_i - m) / T); scores of -inf and NaN are excluded; +inf shares the row equally.
  *   ranking: higher score first, ties -> lower column.  Kept are, in this order:
  *   top_k  the first top_k columns (top_k <= 0: all);
- *   top_p  of these the shortest prefix whose weight reaches top_p of theirs, one at least (top_p >= 1: all);
+ *   top_p  of these the shortest prefix whose weight reaches top_p of theirs to 1e-15, one at least (top_p >= 1:
+ *          all);
  *   min_p  of these the ones with w_i >= min_p.
  *   A draw with the given number u is the first kept column i, in column order, with
  *   sum_{j <= i, kept} w_j > u * sum_{kept} w_j.  T not above 0 (or NaN): the best column.  A

@@ -234,6 +234,23 @@ def test_equal_scores_are_cut_and_drawn_in_column_order():
     check(S, u[:1], top_k=900)
 
 
+@pytest.mark.parametrize("cols", [12, 300, 3000, 70000])
+def test_top_p_on_the_border_of_equal_scores(cols):
+    """Ten equal columns hold all that f64 can see of the row: top_p of them is 0.9 or 0.5 to the last bit, whatever the others weigh."""
+    S = torch.full((3, cols), -200.0)
+    S[0, cols // 2 - 5:cols // 2 + 5] = 0.0
+    S[1, torch.randperm(cols, generator=torch.Generator().manual_seed(cols))[:10]] = 0.0
+    S[2, :9], S[2, cols - 1] = 0.0, 0.0
+    u = torch.tensor([0.0, 0.3, 0.6, 0.999]).repeat(3, 1).to(DEV)
+    for dtype in (torch.float32, torch.bfloat16):
+        for kw in ({"top_p": 0.9}, {"top_p": 0.5}, {"top_p": 0.9, "top_k": 11}, {"top_p": 0.5, "top_k": 200},
+                   {"top_p": 0.9, "top_k": 1500}):
+            if kw.get("top_k", 0) <= cols:
+                prob = check(S.to(dtype).to(DEV), u, **kw)[1]
+                kept = 9 if kw["top_p"] == 0.9 else 5
+                assert ((prob.double() * kept - 1).abs() <= 2.0 ** -24 + 1e-12).all()
+
+
 def test_masked_infinite_and_undefined_scores():
     inf, nan, low = float("inf"), float("nan"), torch.finfo(torch.float32).min
     S = torch.full((10, 300), -inf, device=DEV)
