@@ -210,14 +210,12 @@ __device__ __forceinline__ double fma_const(double a, double b, double c) {
 struct Weigh {
     double m, c;   // c = log2(e) / T
     double floor;  // the distance whose weight underflows
-    int unit;      // log2 of the fixed-point unit
-    __device__ __forceinline__ Weigh(float top, double T, int cols) {
+    int unit;      // log2 of the fixed-point unit of a list's weights, of which 64 bits hold 2^12
+    __device__ __forceinline__ Weigh(float top, double T) {
         m = (double)top;
         c = 1.4426950408889634074 / fmin(T, 1e300);
         floor = -1100.0 / c;
-        unit = 62;  // the sum of all weights is at most cols
-        while (unit > 0 && (1ll << (62 - unit)) < (int64_t)cols) --unit;
-        unit = min(unit, 51);
+        unit = 51;
     }
     template <int N>
     __device__ __forceinline__ void scaled(const float (&s)[N], int e, double (&w)[N]) const {
@@ -332,7 +330,7 @@ struct Shared {
     };
     uint64_t part[kWaves];
     double dpart[kWaves];
-    uint64_t below;
+    uint64_t below, below2;
     uint32_t bin, bin2, bin3, n;
 };
 
@@ -582,36 +580,104 @@ __device__ __forceinline__ Binning make_binning(float top, double range, int bin
     return Binning{top, (float)fmin(inv, 1e30)};
 }
 
-// The cut of top_k (MASS false: `target` columns) or top_p (`target` of the fixed weights), among the columns of
-// key >= cut, by descent over the score bits; ties are counted off in column order
+// Sums of weights by atomics, for rows of any length: integers, whose order does not matter, of 128 bits in units of 2^-84.  2^31
+// weights fit, and what all of them lose to the unit is 2^-53 of the best one (in 64 bits a unit would have to grow with the row:
+// of 12M columns that share a score the cut lay 33 off, of 100M 22,743).  A bin's low word is in sh.wide, its high one in sh.key
+using u128 = unsigned __int128;
+constexpr int kMassUnit = 84;
+__device__ __forceinline__ double mass_value(u128 x) {  // in units; never falls as x grows (the high word is below 2^53)
+    return fma((double)(uint64_t)(x >> 64), 0x1p64, (double)(uint64_t)x);
+}
+__device__ __forceinline__ void add_mass(int bin, double w, Shared& sh) {  // w in units
+    const uint32_t hi = (uint32_t)(w * 0x1p-64);
+    const uint64_t lo = (uint64_t)fma(-(double)hi, 0x1p64, w);
+    const uint64_t sum = atomicAdd((unsigned long long*)&sh.wide[bin], (unsigned long long)lo) + lo;
+    const uint32_t up = hi + (sum < lo ? 1 : 0);
+    if (up) atomicAdd((unsigned long long*)&sh.key[bin], (unsigned long long)up);
+}
+__device__ __forceinline__ void clear_mass(Shared& sh) {
+    static_assert(kList == kBins / 2, "a high word a bin");
+    __syncthreads();
+    for (int j = threadIdx.x; j < kList; j += kThreads) sh.wide[j] = sh.key[j] = 0;
+    __syncthreads();
+}
+__device__ __forceinline__ u128 bin_mass(int bin, const Shared& sh) { return (u128)sh.key[bin] << 64 | sh.wide[bin]; }
+// find_bin over these sums with `base` before them.  The first time the target is that part of the whole
+// -> sh.bin, sh.below2 and sh.below = the sum before it, base included
+__device__ __forceinline__ void find_mass(double& target, u128 base, bool first, Shared& sh) {
+    constexpr int per = kBins / 2 / kThreads;
+    const int tid = threadIdx.x, wave = tid >> 6;
+    __syncthreads();
+    u128 own = 0;
+    for (int j = 0; j < per; ++j) own += bin_mass(tid * per + j, sh);
+    const u128 incl = ((u128)wave_scan_u64((uint64_t)(own >> 64)) << 64) + ((u128)wave_scan_u64((uint64_t)own >> 32) << 32) +
+                      wave_scan_u64((uint32_t)own);
+    if ((tid & 63) == 63) {
+        sh.part[wave] = (uint64_t)incl;
+        sh.dpart[wave] = __longlong_as_double((int64_t)(incl >> 64));
+    }
+    __syncthreads();
+    u128 run = base + incl - own, all = base;
+    for (int w = 0; w < kWaves; ++w) {
+        const u128 x = (u128)(uint64_t)__double_as_longlong(sh.dpart[w]) << 64 | sh.part[w];
+        if (w < wave) run += x;
+        all += x;
+    }
+    const double whole = mass_value(all);
+    target = fmin(first ? target * whole : target, whole);
+    if (own && mass_value(run + own) >= target && (run == base || mass_value(run) < target))
+        for (int j = 0; j < per; ++j) {
+            const u128 h = bin_mass(tid * per + j, sh), next = run + h;
+            if (h && mass_value(next) >= target) {
+                sh.bin = (uint32_t)(tid * per + j);
+                sh.below = (uint64_t)run;
+                sh.below2 = (uint64_t)(run >> 64);
+                break;
+            }
+            run = next;
+        }
+    __syncthreads();
+}
+
+// The cut of top_k (MASS false: `target` columns) or top_p (that part of the weights), among the columns that `cut`
+// keeps, by descent over the score bits; ties are counted off in column order
 template <bool BF16, bool MASS>
 __device__ __forceinline__ Cut descend(const void* s, int cols, const Cut& cut, double target, const Weigh& weigh, Shared& sh) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    uint64_t above = 0;   // counted in better bins than this digit's
+    u128 above = 0;       // counted in better bins than this digit's
     uint32_t prefix = 0;  // the score bits found so far
 #pragma unroll 1
     for (int digit = 0; digit < 3; ++digit) {
         const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0;
         const int open = digit == 0 ? 32 : digit == 1 ? 21 : 10;  // bits not yet found
         const uint32_t mask = (1u << (open - shift)) - 1u;
-        clear_hist(sh);
+        if (MASS) clear_mass(sh); else clear_hist(sh);
         for_groups<BF16, 1>(s, 0, cols, tid, kThreads, [&](const float (&v)[4], int i) {
-#pragma unroll
+#pragma unroll 1  // (four copies of it cost the callers registers)
             for (int j = 0; j < 4; ++j) {
                 const uint32_t k = score_key(v[j]);
-                if (cut.keeps(v[j], i + j) && (open == 32 || (k >> open) == (prefix >> open)))
-                    atomicAdd((unsigned long long*)&sh.wide[mask - ((k >> shift) & mask)],
-                              (unsigned long long)(MASS ? weigh.fixed(v[j]) : 1ull));
+                if (!cut.keeps(v[j], i + j) || (open < 32 && (k >> open) != (prefix >> open))) continue;
+                const int bin = (int)(mask - ((k >> shift) & mask));
+                if (MASS)
+                    add_mass(bin, weigh.scaled(v[j], kMassUnit), sh);
+                else
+                    atomicAdd((unsigned long long*)&sh.wide[bin], 1ull);
             }
         });
-        find_bin(sh.wide, target - (double)above, sh);
+        if (MASS)
+            find_mass(target, above, digit == 0, sh);
+        else
+            find_bin(sh.wide, target - (double)(uint64_t)above, sh);
         prefix |= (mask - sh.bin) << shift;
-        above += sh.below;
+        if (MASS)
+            above = (u128)sh.below2 << 64 | sh.below;
+        else
+            above += sh.below;
     }
     __syncthreads();
     const float value = unord_f32(prefix);
-    const uint64_t each = MASS ? max(weigh.fixed(value), (uint64_t)1) : 1ull;
-    const double want_f = ceil((target - (double)above) / (double)each);
+    const double each = MASS ? weigh.scaled(value, kMassUnit) : 1.0;
+    const double want_f = ceil((target - mass_value(above)) / each);
     int64_t want = want_f < 1.0 ? 1 : (int64_t)fmin(want_f, (double)cols);
     int found = -1;  // the column of the last one taken
     for (int64_t i0 = 0; i0 < cols; i0 += kThreads) {
@@ -1546,7 +1612,7 @@ __device__ __forceinline__ void draw_list(const SampleArgs& a, int64_t row, cons
     else if (key_score(best) == INFINITY)
         draw_infinite<BF16>(a, row, r, s, sh);
     else
-        finish_list(a, row, r, n, Weigh(key_score(best), r.T, n), sh);
+        finish_list(a, row, r, n, Weigh(key_score(best), r.T), sh);
 }
 
 // the draws of a row without restrictions, from its segments' weights against their own best scores (sh.seg, sh.seg_top)
@@ -1562,7 +1628,7 @@ __device__ __forceinline__ void draw_own(const SampleArgs& a, int64_t row, const
     } else if (top == INFINITY) {
         if (part == 0) draw_infinite<BF16>(a, row, r, s, sh);
     } else {
-        const Weigh weigh(top, r.T, (int)a.cols);
+        const Weigh weigh(top, r.T);
         for (int j = threadIdx.x; j < segs.n; j += kThreads) sh.seg[j + 1] *= weigh(sh.seg_top[j]);
         draw_columns<BF16>(a, row, r, s, segs, Cut{kNone, -1}, weigh, part, parts, sh);
     }
@@ -1582,7 +1648,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int64_t row, con
     }
     const bool by_k = K && listed(a, r), by_p = P && r.top_p < 1.0;
     if (!K && !P && !(r.min_p > 0.0) && !grouped(cols, a.n_draws)) {
-        sum_own<BF16>(s, cols, a.segs, 0, a.segs.n, Weigh(0.0f, r.T, cols), [&](int g, double w, float t) {
+        sum_own<BF16>(s, cols, a.segs, 0, a.segs.n, Weigh(0.0f, r.T), [&](int g, double w, float t) {
             sh.seg[g + 1] = w;
             sh.seg_top[g] = t;
         });
@@ -1640,7 +1706,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int64_t row, con
         draw_infinite<BF16>(a, row, r, s, sh);
         return;
     }
-    const Weigh weigh(top, r.T, cols);
+    const Weigh weigh(top, r.T);
     Cut cut{kNone, -1};
     if (by_k) {
         // the step of the top_k-th column
@@ -1692,14 +1758,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int64_t row, con
                     if (mine[j]) f(mine[j]);
             }, cols, z, better, bin, win, r, segs, weigh, cut, sh);
         }
-        if (!summed) {
-            uint64_t sum = 0;
-            for_groups<BF16, 1>(s, 0, cols, tid, kThreads, [&](const float (&v)[4], int i) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) sum += cut.keeps(v[j], i + j) ? weigh.fixed(v[j]) : 0;
-            });
-            cut = descend<BF16, true>(s, cols, cut, r.top_p * (double)block_sum_u64(sum, sh), weigh, sh);
-        }
+        if (!summed) cut = descend<BF16, true>(s, cols, cut, r.top_p, weigh, sh);
     }
     if (draw_groups<BF16>(a, row, r, s, cut, weigh, sh)) return;
     if (!summed) {
@@ -1710,7 +1769,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int64_t row, con
 }
 
 // 2048 x 40,981 f32, top_p: 175 us (2 1/8 readings, of which the memory's share is 126); 1024 x 91,599 bf16, top_k 100: 78 us (one
-// reading and a third, 44).  Held to 80 registers (three workgroups a CU) with 8 to 10 spilled
+// reading and a third, 44).  Held to 80 registers (three workgroups a CU) with 8 to 13 spilled
 template <bool BF16, bool K, bool P>
 __global__ __launch_bounds__(kThreads, 6) void sample_rows_kernel(SampleArgs a) {
     __shared__ Shared sh;
@@ -1841,7 +1900,7 @@ __global__ __launch_bounds__(kThreads, 6) void sample_own_sum(SampleArgs a, Spli
         if (threadIdx.x == 0) p.first[row * p.parts + blockIdx.x] = best;
         return;
     }
-    sum_own<BF16>(s, a.cols, segs, part.g0, part.g1, Weigh(0.0f, r.T, (int)a.cols), [&](int g, double w, float t) {
+    sum_own<BF16>(s, a.cols, segs, part.g0, part.g1, Weigh(0.0f, r.T), [&](int g, double w, float t) {
         p.seg[row * (kSegs + 1) + g + 1] = w;
         p.seg_top[row * kSegs + g] = t;
     });
@@ -1990,7 +2049,7 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_sum(SampleArgs a, Sp
     const void* s = row_scores<BF16>(a, row);
     double* seg = p.seg + row * (kSegs + 1);
     if (unrestricted(a, r)) {
-        sum_own<BF16>(s, a.cols, segs, part.g0, part.g1, Weigh(0.0f, r.T, (int)a.cols), [&](int g, double w, float t) {
+        sum_own<BF16>(s, a.cols, segs, part.g0, part.g1, Weigh(0.0f, r.T), [&](int g, double w, float t) {
             seg[g + 1] = w;
             p.seg_top[row * kSegs + g] = t;
         });
@@ -1999,7 +2058,7 @@ __global__ __launch_bounds__(kThreads, 6) void sample_split_sum(SampleArgs a, Sp
     const Extent extent = known_extent(p, row, sh);
     const float top = best_score(p, row, r, extent);
     if (!finite(top)) return;
-    const Weigh weigh(top, r.T, (int)a.cols);
+    const Weigh weigh(top, r.T);
     if (!(r.top_p < 1.0)) {
         sum_segments<BF16, true>(s, a.cols, segs, part.g0, part.g1, Cut{kNone, -1}, weigh, r.min_p, [&](int g, double w) { seg[g + 1] = w; });
         return;
@@ -2060,7 +2119,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_split_draw(SampleArgs a, S
     const bool by_p = r.top_p < 1.0;
     const Extent extent = by_k ? Extent{0.0f, 0.0f} : known_extent(p, row, sh);  // (a top_k row comes here with no list)
     const float top = best_score(p, row, r, extent);
-    const Weigh weigh(top, r.T, (int)a.cols);
+    const Weigh weigh(top, r.T);
     if (!by_k && !finite(top)) {
         if (!first) return;
         if (top == INFINITY) draw_infinite<BF16>(a, row, r, s, sh); else all_draws(a, row, -1, 0.0f);

@@ -3,6 +3,8 @@
 The drawn columns must be equal: the kernel's weights and sums carry 64 bits, as the reference's do, so
 they differ only where a random number lies within ~1e-14 of a border.  Probabilities are one rounding to
 f32 off: 2^-24 relative, plus 1e-12 for the weights."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -103,6 +105,39 @@ def test_top_p_where_many_columns_lie_near_the_cut(dtype):
         want = check(S, u, **kw)
         for g, w in zip(lgx.sample_rows(many, u_many, **kw), want):
             assert torch.equal(g, w.repeat(200, 1)), kw
+
+
+def _head_and_tail(tail, n, p):
+    """A column at 0 and n at `tail`, T = 1, top_p = p: (kept columns of the tail, weight of one, kept weight).  p (1 + n w) lies
+    at least a hundredth of a column from the border of two columns, and 64 bits lose a thousandth of one at most (2e-15 of the whole)."""
+    w = math.exp(tail)
+    x = (p * (1 + n * w) - 1) / w
+    assert 0.01 < x - math.floor(x) < 0.99 and 2e-15 * (1 + n * w) < 1.1e-3 * w
+    return math.ceil(x), w, 1 + math.ceil(x) * w
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,tail,p", [(4000000, -15.25, 0.75), (12000000, -16.375, 0.75), (12000000, -16.375, 0.6),
+                                      (100000000, -18.375, 0.75), (1000000, -27.0, 1 - 1e-6), (33000, -21.0, 1 - 1e-5)])
+def test_top_p_among_millions_of_equal_scores_behind_a_heavy_one(n, tail, p, dtype):
+    """The cut lies deep in one score's columns, each of which weighs next to nothing against the first."""
+    if dtype == torch.float32 and n > 50000000:
+        n, tail = n // 4, tail + math.log(4.0)  # (a score with as much weight in all)
+        tail = float(torch.tensor(tail))
+    kept, w, total = _head_and_tail(tail, n, p)
+    S = torch.full((1, n + 1), tail, dtype=dtype, device=DEV)
+    S[0, 0] = 0.0
+    assert S[0, 1].item() == tail
+    # the first column, some of the tail by the middles of theirs, and the end of the range: the last one kept
+    cols = sorted({1, 2, kept // 3, kept // 2, kept - 1, kept})
+    u = torch.tensor([[0.0] + [(1 + (c - 0.5) * w) / total for c in cols] + [1 - 2.0 ** -53]], dtype=torch.float64, device=DEV)
+    idx, prob = lgx.sample_rows(S, u, top_p=p)
+    assert idx[0].tolist() == [0] + cols + [kept]
+    want = torch.tensor([1.0] + [w] * (len(cols) + 1), dtype=torch.float64) / total
+    assert ((prob[0].double().cpu() - want).abs() <= (2.0 ** -24 + 1e-12) * want).all()
+    if n <= 100000:  # a batch that takes a workgroup a row
+        many = lgx.sample_rows(S.repeat(800, 1), u.repeat(800, 1), top_p=p)
+        assert torch.equal(many[0], idx.repeat(800, 1)) and torch.equal(many[1], prob.repeat(800, 1))
 
 
 def _odd_rows(cols, seed):
