@@ -2187,19 +2187,38 @@ struct SplitLayout {
     }
 };
 
+// the rows from `first` on
+SampleArgs rows_from(SampleArgs a, bool bf16, int64_t first) {
+    const auto from = [&](auto& p, int64_t each) { if (p) p += first * each; };
+    a.S = static_cast<const char*>(a.S) + first * a.ld * (bf16 ? 2 : 4);
+    a.u = static_cast<const char*>(a.u) + first * a.n_draws * (a.u_f64 ? 8 : 4);
+    from(a.T_rows, 1);
+    from(a.p_rows, 1);
+    from(a.m_rows, 1);
+    from(a.k_rows, 1);
+    from(a.out_idx, a.n_draws);
+    from(a.out_prob, a.n_draws);
+    a.rows -= first;
+    return a;
+}
+
 template <bool BF16>
 int launch_sample(const SampleArgs& a, void* ws, const Segments& segs, hipStream_t stream) {
     const int parts = segs.parts();
     if (parts == 1) {
-        const unsigned grid = (unsigned)a.rows;
         const bool by_p = a.p_rows || a.top_p < 1.0;
-        if (a.k_rows || (a.top_k > 0 && a.top_k < a.cols) || (by_p && a.cols <= kList))
-            sample_rows_kernel<BF16, true, true><<<grid, kThreads, 0, stream>>>(a);
-        else if (by_p)
-            sample_rows_kernel<BF16, false, true><<<grid, kThreads, 0, stream>>>(a);
-        else
-            sample_rows_kernel<BF16, false, false><<<grid, kThreads, 0, stream>>>(a);
-        LGX_LAUNCH_CHECK();
+        constexpr int64_t kMost = 1 << 22;  // rows of a launch: a grid has less than 2^32 threads
+        for (int64_t first = 0; first < a.rows; first += kMost) {
+            const SampleArgs b = rows_from(a, BF16, first);
+            const unsigned grid = (unsigned)std::min(kMost, b.rows);
+            if (a.k_rows || (a.top_k > 0 && a.top_k < a.cols) || (by_p && a.cols <= kList))
+                sample_rows_kernel<BF16, true, true><<<grid, kThreads, 0, stream>>>(b);
+            else if (by_p)
+                sample_rows_kernel<BF16, false, true><<<grid, kThreads, 0, stream>>>(b);
+            else
+                sample_rows_kernel<BF16, false, false><<<grid, kThreads, 0, stream>>>(b);
+            LGX_LAUNCH_CHECK();
+        }
         return LGX_OK;
     }
     const SplitLayout l(a.rows, a.cols, segs);

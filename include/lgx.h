@@ -483,7 +483,7 @@ int lgx_score_mx(const void* Q, const uint8_t* q_scales, int q_dtype, int64_t n_
  *   u [rows, n_draws] f32 or f64 (u_dtype) in [0, 1); values outside are taken as the nearest end.
  *   Each setting is one value for all rows or, where the *_rows pointer is given, one per row.
  * Weights and their sums are held in 64 bits, so that the column does not depend on how the sums
- * are split; results are the same for every call.  1 <= cols < 2^31.
+ * are split; results are the same for every call.  1 <= cols < 2^31 - 1, rows < 2^31.
  */
 int lgx_sample_rows_workspace(int64_t rows, int64_t cols, int64_t n_draws, size_t* ws_bytes);
 int lgx_sample_rows(const void* S, int dtype, int64_t rows, int64_t cols, int64_t ld, const void* u, int u_dtype,

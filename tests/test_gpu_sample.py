@@ -367,6 +367,26 @@ def test_offsets_past_32_bits():
     check(S[2198:].clone(), u[2198:], top_p=0.5)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_more_rows_than_a_launch_takes(dtype):
+    """8.4 million rows: more threads than a grid holds.  They draw what they draw in batches of a million."""
+    rows, g = 2 ** 23 + 5, torch.Generator(device=DEV).manual_seed(1)
+    S = torch.randn(rows, 3, device=DEV, generator=g).to(dtype)
+    u = torch.rand(rows, 2, device=DEV, generator=g)
+    T = torch.rand(rows, device=DEV, generator=g) + 0.1
+    k = torch.randint(0, 4, (rows,), device=DEV, generator=g)
+    p, m = torch.rand(rows, device=DEV, generator=g), torch.rand(rows, device=DEV, generator=g) * 0.1
+    for kw in ({}, {"top_k": 2}, {"temperature": T, "top_k": k, "top_p": p, "min_p": m}):
+        def at(lo, hi):
+            return {n: v[lo:hi] if torch.is_tensor(v) else v for n, v in kw.items()}
+
+        idx, prob = lgx.sample_rows(S, u, **kw)
+        for lo in range(0, rows, 2 ** 20):
+            want = lgx.sample_rows(S[lo:lo + 2 ** 20], u[lo:lo + 2 ** 20], **at(lo, lo + 2 ** 20))
+            assert torch.equal(idx[lo:lo + 2 ** 20], want[0]) and torch.equal(prob[lo:lo + 2 ** 20], want[1])
+        check(S[-9:], u[-9:], **at(rows - 9, rows))
+
+
 def test_frequencies_follow_the_probabilities():
     S, _ = scores(1, 40, 8)
     n = 200000
