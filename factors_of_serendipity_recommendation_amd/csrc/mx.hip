@@ -583,7 +583,6 @@ int launch_score(const MxArgs& a, int q_dtype, hipStream_t stream) {
         else { LGX_MX_STEPS(LGX_MX_FEW, LGX_DTYPE_MXFP4) }
     } else if (a.nb <= 8) {
         const int64_t gy = ceil_div(a.B, (int64_t)(kUserTiles * 32));
-        LGX_REQUIRE(gy < 65536, LGX_ERR_UNSUPPORTED, "lgx_score_mx: %lld queries is too many", (long long)a.B);
         const int64_t gx = ceil_div(a.n_items, (int64_t)512);
         const dim3 grid((unsigned)(NT ? gx : 8 * ceil_div(gx, (int64_t)8)), (unsigned)gy);
         LGX_MX_STEPS(LGX_MX_SHORT, 0)
@@ -594,7 +593,9 @@ int launch_score(const MxArgs& a, int q_dtype, hipStream_t stream) {
         const int uw = a.B > 32 ? 2 : 1, nu = a.B > 64 ? 2 : 1;
         const int64_t user_tiles = ceil_div(a.B, (int64_t)(uw * nu * 32));
         const int64_t grid = 8 * ceil_div(ceil_div(a.n_items, (int64_t)(512 / uw)), (int64_t)8) * user_tiles;
-        LGX_REQUIRE(grid < (1LL << 31), LGX_ERR_UNSUPPORTED, "lgx_score_mx: %lld queries is too many", (long long)a.B);
+        // (scores of so many tiles would not fit the memory)
+        LGX_REQUIRE(grid < (1LL << 24), LGX_ERR_UNSUPPORTED, "lgx_score_mx: %lld queries of %lld items is too many", (long long)a.B,
+                    (long long)a.n_items);
         if (nu == 2) score_mx_long<2, 2, BF16, SIG, NT><<<(unsigned)grid, 256, 0, stream>>>(a, (int)user_tiles);
         else if (uw == 2) score_mx_long<2, 1, BF16, SIG, NT><<<(unsigned)grid, 256, 0, stream>>>(a, (int)user_tiles);
         else score_mx_long<1, 1, BF16, SIG, NT><<<(unsigned)grid, 256, 0, stream>>>(a, (int)user_tiles);
@@ -609,22 +610,29 @@ bool quantised_inside(int64_t B, int64_t d) { return B <= 32 && d <= 8 * kBlock;
 
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
+// Rows (queries) of a launch: a grid holds less than 2^32 threads, and 64 blocks take 256
+constexpr int64_t kMostBlocks = 1 << 28, kMostQueries = 1 << 22;
+
 int launch_quantize(const void* X, const int64_t* rows_of, int64_t n_src, int64_t rows, int64_t d, int64_t ld, int dtype,
                     uint8_t* codes, uint8_t* scales, hipStream_t stream) {
-    const int64_t nb = ceil_div(d, (int64_t)kBlock), units = rows * nb;
-    const int64_t grid = ceil_div(units, (int64_t)64);
-    LGX_REQUIRE(grid < (1LL << 31), LGX_ERR_UNSUPPORTED, "lgx_mx_quantize: %lld rows is too many", (long long)rows);
+    const int64_t nb = ceil_div(d, (int64_t)kBlock), most = kMostBlocks / nb;
     const int size = dtype == LGX_DTYPE_BF16 ? 2 : 4;
     const bool vec = d % 8 == 0 && (ld * size) % 16 == 0 && aligned(X, 16);
-#define LGX_MXQ(BF, V)                                                                                          \
-    mx_quantize_kernel<BF, V><<<(unsigned)grid, 256, 0, stream>>>(X, rows_of, n_src, units, nb, d, ld, codes, scales)
-    if (dtype == LGX_DTYPE_BF16) {
-        if (vec) LGX_MXQ(true, true); else LGX_MXQ(true, false);
-    } else {
-        if (vec) LGX_MXQ(false, true); else LGX_MXQ(false, false);
+#define LGX_MXQ(BF, V)                                                                                                  \
+    mx_quantize_kernel<BF, V><<<grid, 256, 0, stream>>>(static_cast<const char*>(X) + (rows_of ? 0 : first * ld * size),  \
+                                                        rows_of ? rows_of + first : nullptr, n_src, units, nb, d, ld,     \
+                                                        codes + first * nb * 16, scales + first * nb)
+    for (int64_t first = 0; first < rows; first += most) {
+        const int64_t units = std::min(most, rows - first) * nb;
+        const unsigned grid = (unsigned)ceil_div(units, (int64_t)64);
+        if (dtype == LGX_DTYPE_BF16) {
+            if (vec) LGX_MXQ(true, true); else LGX_MXQ(true, false);
+        } else {
+            if (vec) LGX_MXQ(false, true); else LGX_MXQ(false, false);
+        }
+        LGX_LAUNCH_CHECK();
     }
 #undef LGX_MXQ
-    LGX_LAUNCH_CHECK();
     return LGX_OK;
 }
 
@@ -640,7 +648,7 @@ extern "C" int lgx_mx_quantize(const void* X, int64_t rows, int64_t d, int64_t l
     LGX_REQUIRE(d >= 1 && d <= kMaxD && ld >= d, LGX_ERR_UNSUPPORTED, "lgx_mx_quantize: d=%lld outside [1, %lld] or ld=%lld < d",
                 (long long)d, (long long)kMaxD, (long long)ld);
     LGX_REQUIRE(aligned(codes, 16), LGX_ERR_INVALID_ARG, "lgx_mx_quantize: codes must be 16-byte aligned");
-    if (rows == 0) return LGX_OK;
+    LGX_REQUIRE(rows < (1LL << 36), LGX_ERR_UNSUPPORTED, "lgx_mx_quantize: %lld rows is too many", (long long)rows);
     return launch_quantize(X, nullptr, rows, rows, d, ld, dtype, codes, scales, as_hip(stream));
 }
 
@@ -654,17 +662,24 @@ extern "C" int lgx_mx_dequantize(const uint8_t* codes, const uint8_t* scales, in
                 (long long)kMaxD);
     LGX_REQUIRE(aligned(codes, 16), LGX_ERR_INVALID_ARG, "lgx_mx_dequantize: codes must be 16-byte aligned");
     if (rows == 0) return LGX_OK;
-    const int64_t nb = ceil_div(d, (int64_t)kBlock), units = rows * nb, grid = ceil_div(units, (int64_t)64);
-    LGX_REQUIRE(grid < (1LL << 31), LGX_ERR_UNSUPPORTED, "lgx_mx_dequantize: %lld rows is too many", (long long)rows);
+    LGX_REQUIRE(rows < (1LL << 36), LGX_ERR_UNSUPPORTED, "lgx_mx_dequantize: %lld rows is too many", (long long)rows);
+    const int64_t nb = ceil_div(d, (int64_t)kBlock), most = kMostBlocks / nb;
+    const int size = dtype == LGX_DTYPE_BF16 ? 2 : 4;
     const bool vec = d % 8 == 0 && aligned(out, 16);
-#define LGX_MXD(BF, V) mx_dequantize_kernel<BF, V><<<(unsigned)grid, 256, 0, stream>>>(codes, scales, units, nb, d, out)
-    if (dtype == LGX_DTYPE_BF16) {
-        if (vec) LGX_MXD(true, true); else LGX_MXD(true, false);
-    } else {
-        if (vec) LGX_MXD(false, true); else LGX_MXD(false, false);
+#define LGX_MXD(BF, V)                                                                                              \
+    mx_dequantize_kernel<BF, V><<<grid, 256, 0, stream>>>(codes + first * nb * 16, scales + first * nb, units, nb, d, \
+                                                          static_cast<char*>(out) + first * d * size)
+    for (int64_t first = 0; first < rows; first += most) {
+        const int64_t units = std::min(most, rows - first) * nb;
+        const unsigned grid = (unsigned)ceil_div(units, (int64_t)64);
+        if (dtype == LGX_DTYPE_BF16) {
+            if (vec) LGX_MXD(true, true); else LGX_MXD(true, false);
+        } else {
+            if (vec) LGX_MXD(false, true); else LGX_MXD(false, false);
+        }
+        LGX_LAUNCH_CHECK();
     }
 #undef LGX_MXD
-    LGX_LAUNCH_CHECK();
     return LGX_OK;
 }
 
@@ -718,8 +733,21 @@ extern "C" int lgx_score_mx(const void* Q, const uint8_t* q_scales, int q_dtype,
     // Rows that start on a 128-byte line write whole lines, which go past the L2 (1024 x 1 M f32: 0.79 against
     // 0.94 ms); the ends of other rows' stores share lines, which the L2 merges (2048 x 40,981: 119 us past it).
     const bool nt = aligned(scores, 128) && n_items * (out_dtype == LGX_DTYPE_BF16 ? 2 : 4) % 128 == 0;
-#define LGX_SMX(BF, SG) (nt ? launch_score<BF, SG, true>(a, q_dtype, stream) : launch_score<BF, SG, false>(a, q_dtype, stream))
-    if (out_dtype == LGX_DTYPE_BF16) return apply_sigmoid ? LGX_SMX(true, true) : LGX_SMX(true, false);
-    return apply_sigmoid ? LGX_SMX(false, true) : LGX_SMX(false, false);
+#define LGX_SMX(BF, SG) (nt ? launch_score<BF, SG, true>(b, q_dtype, stream) : launch_score<BF, SG, false>(b, q_dtype, stream))
+    for (int64_t first = 0; first < B; first += kMostQueries) {
+        MxArgs b = a;
+        b.B = std::min(kMostQueries, B - first);
+        b.out = static_cast<char*>(scores) + first * n_items * (out_dtype == LGX_DTYPE_BF16 ? 2 : 4);
+        if (b.user_rows) {
+            b.user_rows += first;
+        } else if (first) {  // packed rows: more of them than a wave quantises by itself
+            b.q += first * nb * 16;
+            b.qs += first * nb;
+        }
+        const int rc = out_dtype == LGX_DTYPE_BF16 ? (apply_sigmoid ? LGX_SMX(true, true) : LGX_SMX(true, false))
+                                                   : (apply_sigmoid ? LGX_SMX(false, true) : LGX_SMX(false, false));
+        if (rc) return rc;
+    }
 #undef LGX_SMX
+    return LGX_OK;
 }

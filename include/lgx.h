@@ -443,7 +443,7 @@ int lgx_list_dot_reduce(const void* table, int64_t d, int dtype, int64_t n_users
  * lgx_mx_quantize: X [rows, d] f32 or bf16, row stride ld >= d elements.  b = max(E - 2, 0) with E the
  * exponent field of the block's largest magnitude, so that magnitude lands in [4, 8); elements round to
  * the nearest magnitude, ties to the even code, and saturate at 6.  A block holding an infinity or a NaN
- * gets b = 255.  1 <= d <= 65536.
+ * gets b = 255.  1 <= d <= 65536, rows < 2^36.
  * lgx_mx_dequantize: -> out [rows, d] f32 or bf16 contiguous; every value is exact in both types.
  */
 int lgx_mx_quantize(const void* X, int64_t rows, int64_t d, int64_t ld, int dtype, uint8_t* codes, uint8_t* scales,
@@ -456,8 +456,8 @@ int lgx_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows,
  *   Q [n_q, d]: q_dtype MXFP4 (Q = codes, q_scales = scales, q_ld ignored), or f32 / bf16 with row stride
  *   q_ld (q_scales NULL), which the call first quantises as lgx_mx_quantize does.
  *   user_rows [B] int64 (NULL: row b, B <= n_q): the rows of Q; a row outside [0, n_q) is never read and
- *   scores NaN.  n_items < 2^27 (32-bit lane offsets), 1 <= d <= 65536.  Workspace: lgx_score_mx_workspace (0 where none is
- *   needed).
+ *   scores NaN.  n_items < 2^27 (32-bit lane offsets), 1 <= d <= 65536; any B (millions of queries go in several
+ *   launches).  Workspace: lgx_score_mx_workspace (0 where none is needed).
  */
 int lgx_score_mx_workspace(int64_t B, int64_t d, int q_dtype, size_t* ws_bytes);
 int lgx_score_mx(const void* Q, const uint8_t* q_scales, int q_dtype, int64_t n_q, int64_t q_ld,

@@ -232,6 +232,43 @@ def test_tables_pass_2_31_bytes_of_scores():
     assert torch.equal(S[2190:, 999000:], want)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_more_rows_than_a_launch_takes(dtype):
+    """2^30 rows of one element: four launches' blocks, of more threads than one grid holds.  A row of one element x is
+    +-4 scales, where x lies below 5 of them, or 6."""
+    rows, part = 2 ** 30 + 3, 2 ** 27
+    x = torch.empty(rows, 1, dtype=dtype, device=DEV)
+    for r in x.split(part):
+        r.normal_()
+    t = lgx.mx_quantize(x)
+    back = lgx.mx_dequantize(t, torch.bfloat16)
+    for a in range(0, rows, part):
+        v = x[a:a + part].float()
+        unit = torch.exp2(torch.floor(torch.log2(v.abs().double()).clamp(min=-140)) - 2).float()
+        unit = torch.where(v.abs() >= 8 * unit, unit * 2, torch.where(v.abs() < 4 * unit, unit / 2, unit))  # log2 rounds
+        want = torch.where(v.abs() <= 5 * unit, 4 * unit, 6 * unit) * torch.sign(v)
+        assert torch.equal(back[a:a + part].float(), want)
+        del v, unit, want
+
+
+@pytest.mark.parametrize("B,d,kind", [(2 ** 24 + 300, 40, "f32"), (2 ** 24 + 300, 40, "mx"), (2 ** 22 + 1, 64, "f32"),
+                                      (2 ** 22 + 1, 64, "mx"), (2 ** 22 + 1, 290, "f32"), (2 ** 28 + 129, 290, "mx")])
+def test_more_queries_than_a_launch_takes(B, d, kind):
+    """Millions of queries of a few rows: each scores what the row scores in a small batch."""
+    x, items = table(7, d, d), lgx.mx_quantize(table(1 if B > 2 ** 27 else 3, d, 2))
+    q = lgx.mx_quantize(x) if kind == "mx" else x
+    few = torch.arange(50, device=DEV) % 7
+    want = lgx.score_mx(q, items, user_rows=few)[:7]
+    rows = torch.randint(0, 7, (B,), device=DEV, generator=torch.Generator(device=DEV).manual_seed(d))
+    rows[-1], rows[-2] = 7, 3  # outside: NaN
+    got = lgx.score_mx(q, items, user_rows=rows)
+    assert torch.isnan(got[-1]).all()
+    assert torch.equal(got[:-1], want[rows[:-1]])
+    if kind == "mx" and B < 2 ** 23:  # and rows without a list
+        many = lgx.MXTable(q.codes[rows % 7], q.scales[rows % 7], d)
+        assert torch.equal(lgx.score_mx(many, items), want[rows % 7])
+
+
 def test_mx_refusals():
     x = table(4, 64, 1)
     t = lgx.mx_quantize(x)
