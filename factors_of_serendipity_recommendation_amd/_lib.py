@@ -121,6 +121,8 @@ SIGNATURES = {
     "lgx_sample_rows_workspace": (_c_int, [_c_i64, _c_i64, _c_i64, _sz_p]),
     "lgx_sample_rows": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _vp, _c_int, _c_i64, ctypes.c_double, _vp, _c_i64,
                                  _vp, ctypes.c_double, _vp, ctypes.c_double, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "lgx_sample_rows_f64": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _vp, _c_int, _c_i64, ctypes.c_double, _vp, _c_i64,
+                                     _vp, ctypes.c_double, _vp, ctypes.c_double, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
     "lgx_synth_edges": (_c_int, [ctypes.c_uint64, _vp, _c_i64, _vp, _vp, _c_i64, _c_i64, _vp, _vp, _vp]),
     "lgx_fill_normal": (_c_int, [_vp, _c_i64, ctypes.c_float, ctypes.c_uint64, _c_int, _vp]),
     "lgx_fill_normal_at": (_c_int, [_vp, _c_i64, _c_i64, ctypes.c_float, ctypes.c_uint64, _c_int, _vp]),

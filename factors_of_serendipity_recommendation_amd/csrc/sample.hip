@@ -69,11 +69,11 @@ struct SampleArgs {
     const void* S;
     int64_t rows, cols, ld;
     const void* u;
-    int u_f64;
+    int u_f64, rows_f64;
     int64_t n_draws;
     double T, top_p, min_p;
     int64_t top_k;
-    const float *T_rows, *p_rows, *m_rows;
+    const void *T_rows, *p_rows, *m_rows;  // f32, or f64 (rows_f64)
     const int32_t* k_rows;
     int32_t* out_idx;
     float* out_prob;
@@ -515,13 +515,16 @@ struct Row {
 };
 __device__ __forceinline__ Row row_settings(const SampleArgs& a, int64_t row) {
     Row r;
-    r.T = a.T_rows ? (double)a.T_rows[row] : a.T;
+    const auto setting = [&](const void* of_rows, double all) {
+        return !of_rows ? all : a.rows_f64 ? static_cast<const double*>(of_rows)[row] : (double)static_cast<const float*>(of_rows)[row];
+    };
+    r.T = setting(a.T_rows, a.T);
     if (r.T > 0.0) r.T = fmax(r.T, 1e-300);  // below it 1 / T is none, and no two f32 scores lie so near anyway
-    r.top_p = a.p_rows ? (double)a.p_rows[row] : a.top_p;
+    r.top_p = setting(a.p_rows, a.top_p);
     // within 1e-15 of top_p is reached: of equal weights that lie on it to the last bit (0.9 of ten), a sum's order and what weighs
     // next to nothing would decide
     if (r.top_p < 1.0) r.top_p *= 1.0 - 1e-15;
-    const double m = a.m_rows ? (double)a.m_rows[row] : a.min_p;
+    const double m = setting(a.m_rows, a.min_p);
     r.min_p = m > 0.0 ? fmin(m, 1.0) : 0.0;
     r.top_k = a.k_rows ? (int64_t)a.k_rows[row] : a.top_k;
     return r;
@@ -2189,15 +2192,13 @@ struct SplitLayout {
 
 // the rows from `first` on
 SampleArgs rows_from(SampleArgs a, bool bf16, int64_t first) {
-    const auto from = [&](auto& p, int64_t each) { if (p) p += first * each; };
     a.S = static_cast<const char*>(a.S) + first * a.ld * (bf16 ? 2 : 4);
     a.u = static_cast<const char*>(a.u) + first * a.n_draws * (a.u_f64 ? 8 : 4);
-    from(a.T_rows, 1);
-    from(a.p_rows, 1);
-    from(a.m_rows, 1);
-    from(a.k_rows, 1);
-    from(a.out_idx, a.n_draws);
-    from(a.out_prob, a.n_draws);
+    for (const void** p : {&a.T_rows, &a.p_rows, &a.m_rows})
+        if (*p) *p = static_cast<const char*>(*p) + first * (a.rows_f64 ? 8 : 4);
+    if (a.k_rows) a.k_rows += first;
+    a.out_idx += first * a.n_draws;
+    if (a.out_prob) a.out_prob += first * a.n_draws;
     a.rows -= first;
     return a;
 }
@@ -2273,11 +2274,13 @@ extern "C" int lgx_sample_rows_workspace(int64_t rows, int64_t cols, int64_t n_d
     return LGX_OK;
 }
 
-extern "C" int lgx_sample_rows(const void* S, int dtype, int64_t rows, int64_t cols, int64_t ld, const void* u, int u_dtype,
-                               int64_t n_draws, double temperature, const float* temperature_rows, int64_t top_k,
-                               const int32_t* top_k_rows, double top_p, const float* top_p_rows, double min_p,
-                               const float* min_p_rows, int32_t* out_idx, float* out_prob, void* ws, size_t ws_bytes,
-                               lgx_stream_t stream_) {
+namespace lgx {
+namespace {
+
+int sample_entry(const void* S, int dtype, int64_t rows, int64_t cols, int64_t ld, const void* u, int u_dtype, int64_t n_draws,
+                 double temperature, const void* temperature_rows, int64_t top_k, const int32_t* top_k_rows, double top_p,
+                 const void* top_p_rows, double min_p, const void* min_p_rows, bool rows_f64, int32_t* out_idx, float* out_prob,
+                 void* ws, size_t ws_bytes, lgx_stream_t stream_) {
     hipStream_t stream = as_hip(stream_);
     LGX_REQUIRE(dtype == LGX_DTYPE_F32 || dtype == LGX_DTYPE_BF16, LGX_ERR_INVALID_ARG, "lgx_sample_rows: dtype");
     LGX_REQUIRE(u_dtype == LGX_DTYPE_F32 || u_dtype == LGX_DTYPE_F64, LGX_ERR_INVALID_ARG, "lgx_sample_rows: dtype of u");
@@ -2291,8 +2294,29 @@ extern "C" int lgx_sample_rows(const void* S, int dtype, int64_t rows, int64_t c
     const size_t need = SplitLayout(rows, cols, segs).bytes;
     LGX_REQUIRE(need == 0 || (ws && ws_bytes >= need && reinterpret_cast<uintptr_t>(ws) % 16 == 0), LGX_ERR_WORKSPACE,
                 "lgx_sample_rows: workspace %zu < %zu", ws_bytes, need);
-    const SampleArgs a{S, rows, cols, ld, u, u_dtype == LGX_DTYPE_F64, n_draws, temperature, top_p, min_p, top_k,
+    const SampleArgs a{S, rows, cols, ld, u, u_dtype == LGX_DTYPE_F64, rows_f64, n_draws, temperature, top_p, min_p, top_k,
                        temperature_rows, top_p_rows, min_p_rows, top_k_rows, out_idx, out_prob,
                        Segments(cols, grouped(cols, n_draws) ? 1 : n_draws)};
     return dtype == LGX_DTYPE_BF16 ? launch_sample<true>(a, ws, segs, stream) : launch_sample<false>(a, ws, segs, stream);
+}
+
+}  // namespace
+}  // namespace lgx
+
+extern "C" int lgx_sample_rows(const void* S, int dtype, int64_t rows, int64_t cols, int64_t ld, const void* u, int u_dtype,
+                               int64_t n_draws, double temperature, const float* temperature_rows, int64_t top_k,
+                               const int32_t* top_k_rows, double top_p, const float* top_p_rows, double min_p,
+                               const float* min_p_rows, int32_t* out_idx, float* out_prob, void* ws, size_t ws_bytes,
+                               lgx_stream_t stream) {
+    return sample_entry(S, dtype, rows, cols, ld, u, u_dtype, n_draws, temperature, temperature_rows, top_k, top_k_rows, top_p,
+                        top_p_rows, min_p, min_p_rows, false, out_idx, out_prob, ws, ws_bytes, stream);
+}
+
+extern "C" int lgx_sample_rows_f64(const void* S, int dtype, int64_t rows, int64_t cols, int64_t ld, const void* u, int u_dtype,
+                                   int64_t n_draws, double temperature, const double* temperature_rows, int64_t top_k,
+                                   const int32_t* top_k_rows, double top_p, const double* top_p_rows, double min_p,
+                                   const double* min_p_rows, int32_t* out_idx, float* out_prob, void* ws, size_t ws_bytes,
+                                   lgx_stream_t stream) {
+    return sample_entry(S, dtype, rows, cols, ld, u, u_dtype, n_draws, temperature, temperature_rows, top_k, top_k_rows, top_p,
+                        top_p_rows, min_p, min_p_rows, true, out_idx, out_prob, ws, ws_bytes, stream);
 }

@@ -642,6 +642,9 @@ def score_mx(Q, items: MXTable, user_rows: Optional[torch.Tensor] = None, apply_
 
 
 # ------------------------------------------------------------------------------------ draws
+_HELD_IN_F32 = (torch.float32, torch.bfloat16, torch.float16, torch.bool, torch.uint8, torch.int8, torch.int16)
+
+
 def _row_setting(name: str, v, rows: int, dev: torch.device, dtype: torch.dtype, lo: float, hi: float):
     """(value for all rows, per-row tensor or None) of one sample_rows setting."""
     if torch.is_tensor(v):
@@ -670,7 +673,8 @@ def sample_rows(S: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     lower column; 0 = all), of these the shortest prefix with top_p of their weight, of these the ones
     with weight >= min_p.  A draw is the first kept column, in column order, whose cumulative weight
     exceeds u times the whole.  temperature 0 is the best column.  Each setting is a number or a tensor
-    [rows] (then T <= 0 and NaN mean the best column, top_k <= 0 all).
+    [rows] of any real type, top_k's of an integer one (then T <= 0 and NaN mean the best column, top_k <= 0
+    all).  A tensor's values count as they are: a float32 top_p of 0.6 is 0.60000002, a float64 one what the number is.
 
     Returns (columns int32, their probabilities f32), both shaped as u; -1 and 0 for a row with nothing to
     draw from.  Not differentiable."""
@@ -690,11 +694,15 @@ def sample_rows(S: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
                 and temperature >= 0.0 and 0 <= top_k < 2 ** 63 and 0.0 <= top_p <= 1.0 and 0.0 <= min_p <= 1.0):
             t, k, p, m = temperature, top_k, top_p, min_p  # what most calls give, without four calls' time
             t_rows = k_rows = p_rows = m_rows = None
+            wide = False
         else:
-            t, t_rows = _row_setting("temperature", temperature, rows, dev, torch.float32, 0.0, float("inf"))
+            # in 64 bits where one of them is of a type that 32 do not hold
+            wide = any(torch.is_tensor(v) and v.dtype not in _HELD_IN_F32 for v in (temperature, top_p, min_p))
+            real = torch.float64 if wide else torch.float32
+            t, t_rows = _row_setting("temperature", temperature, rows, dev, real, 0.0, float("inf"))
             k, k_rows = _row_setting("top_k", top_k, rows, dev, torch.int32, 0, 2 ** 63 - 1)
-            p, p_rows = _row_setting("top_p", top_p, rows, dev, torch.float32, 0.0, 1.0)
-            m, m_rows = _row_setting("min_p", min_p, rows, dev, torch.float32, 0.0, 1.0)
+            p, p_rows = _row_setting("top_p", top_p, rows, dev, real, 0.0, 1.0)
+            m, m_rows = _row_setting("min_p", min_p, rows, dev, real, 0.0, 1.0)
         u = u.contiguous()
         idx = torch.empty_like(u, dtype=torch.int32)
         prob = torch.empty_like(u, dtype=torch.float32)
@@ -705,10 +713,11 @@ def sample_rows(S: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
         ws = ctypes.c_size_t(0)
         _lib.check(L.lgx_sample_rows_workspace(rows, cols, n, ctypes.byref(ws)), "lgx_sample_rows_workspace")
         work = u.new_empty(ws.value, dtype=torch.uint8) if ws.value else None
-        _lib.check(L.lgx_sample_rows(S.data_ptr(), dt, rows, cols, ld, u.data_ptr(),
-                                     _lib.LGX_DTYPE_F64 if u.dtype == torch.float64 else _lib.LGX_DTYPE_F32, n, float(t),
-                                     _ptr(t_rows), int(k), _ptr(k_rows), float(p), _ptr(p_rows), float(m), _ptr(m_rows),
-                                     idx.data_ptr(), prob.data_ptr(), _ptr(work), ws.value, _stream_ptr(dev)),
+        sample = L.lgx_sample_rows_f64 if wide else L.lgx_sample_rows
+        _lib.check(sample(S.data_ptr(), dt, rows, cols, ld, u.data_ptr(),
+                          _lib.LGX_DTYPE_F64 if u.dtype == torch.float64 else _lib.LGX_DTYPE_F32, n, float(t),
+                          _ptr(t_rows), int(k), _ptr(k_rows), float(p), _ptr(p_rows), float(m), _ptr(m_rows),
+                          idx.data_ptr(), prob.data_ptr(), _ptr(work), ws.value, _stream_ptr(dev)),
                    "lgx_sample_rows")
     return idx, prob
 

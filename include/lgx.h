@@ -481,7 +481,8 @@ int lgx_score_mx(const void* Q, const uint8_t* q_scales, int q_dtype, int64_t n_
  * out_idx [rows, n_draws] int32, out_prob [rows, n_draws] f32 = w_i / sum_{kept} w_j (NULL: not wanted).  A
  * row with nothing to draw from gives -1 and 0.
  *   u [rows, n_draws] f32 or f64 (u_dtype) in [0, 1); values outside are taken as the nearest end.
- *   Each setting is one value for all rows or, where the *_rows pointer is given, one per row.
+ *   Each setting is one value for all rows or, where the *_rows pointer is given, one per row: in 32 bits, or for
+ *   lgx_sample_rows_f64 in 64 bits.
  * Weights and their sums are held in 64 bits, so that the column does not depend on how the sums
  * are split; results are the same for every call.  1 <= cols < 2^31 - 1, rows < 2^31.
  */
@@ -491,6 +492,11 @@ int lgx_sample_rows(const void* S, int dtype, int64_t rows, int64_t cols, int64_
                     const int32_t* top_k_rows, double top_p, const float* top_p_rows, double min_p,
                     const float* min_p_rows, int32_t* out_idx, float* out_prob, void* ws, size_t ws_bytes,
                     lgx_stream_t stream);
+int lgx_sample_rows_f64(const void* S, int dtype, int64_t rows, int64_t cols, int64_t ld, const void* u, int u_dtype,
+                        int64_t n_draws, double temperature, const double* temperature_rows, int64_t top_k,
+                        const int32_t* top_k_rows, double top_p, const double* top_p_rows, double min_p,
+                        const double* min_p_rows, int32_t* out_idx, float* out_prob, void* ws, size_t ws_bytes,
+                        lgx_stream_t stream);
 
 /* ---------------------------------------------------------------- synthetic graphs (bench) */
 /*

@@ -328,6 +328,39 @@ def test_settings_per_row():
     assert torch.equal(c[0], d[0])
 
 
+@pytest.mark.parametrize("cols", [300, 3000, 70000])
+def test_settings_per_row_keep_64_bits(cols):
+    """A float64 tensor of settings is what the same numbers are, row by row; so are mixed types."""
+    g = torch.Generator().manual_seed(cols)
+    S = torch.full((6, cols), -200.0)
+    S[:, torch.randperm(cols, generator=g)[:10]] = 0.0          # ten equal columns hold all of the weight
+    u = torch.tensor([[0.0, 0.15, 0.35, 0.55, 0.75, 0.999]] * 6, dtype=torch.float64)
+    S, u = S.to(DEV), u.to(DEV)
+    p = [0.6, 0.3, 0.8, 0.9, 0.1, 1.0]
+    _, prob = check(S, u, top_p=torch.tensor(p, dtype=torch.float64, device=DEV))  # u = 0 with top_p 1: a column of e^-200
+    assert torch.equal((1 / prob[:, 1]).round().int().cpu(), torch.tensor([6, 3, 8, 9, 1, 10], dtype=torch.int32))
+    _, prob = check(S, u, top_p=torch.tensor(p, device=DEV))     # f32 values are their own: 0.6 is 0.60000002, 0.3 0.30000001
+    assert torch.equal((1 / prob[:, 1]).round().int().cpu(), torch.tensor([7, 4, 9, 9, 2, 10], dtype=torch.int32))
+    T = torch.tensor([1e-50, 1e-300, 5e-324, 0.0, -1e-50, 1e60], dtype=torch.float64, device=DEV)
+    idx, _ = check(S, u, temperature=T)
+    assert [len(set(r)) for r in idx.tolist()] == [6, 6, 6, 1, 1, 6]  # below what f32 holds is not the best column alone
+    w = math.exp(-0.5)
+    S[:, S[0].argmax()] = 0.5                                     # the others weigh w
+    m = torch.tensor([w * (1 - 1e-10), w * (1 + 1e-10), 0.0, 1.0, w * (1 - 1e-9), w * (1 + 1e-9)], dtype=torch.float64, device=DEV)
+    _, prob = check(S, u, min_p=m)
+    assert (prob[[1, 3, 5]] == 1.0).all() and (prob[[0, 4], 1] < 1.0).all()
+    S, u = scores(6, cols, 7)
+    kw = {"temperature": torch.rand(6, generator=g, dtype=torch.float64).to(DEV) + 0.3,
+          "top_p": torch.rand(6, generator=g).to(DEV) * 0.5 + 0.5, "min_p": torch.tensor([0, 0, 1, 0, 0, 1], device=DEV)}
+    for more in ({}, {"top_k": torch.tensor([0, 5, 50, 0, 200, 1000], device=DEV)}):
+        idx, prob = check(S, u, **kw, **more)
+        for r in range(6):
+            one = lgx.sample_rows(S[r:r + 1], u[r:r + 1], **{n: v[r].item() for n, v in {**kw, **more}.items()})
+            assert torch.equal(one[0], idx[r:r + 1]) and torch.equal(one[1], prob[r:r + 1])
+    assert torch.equal(lgx.sample_rows(S, u, temperature=torch.full((6,), 0.5, dtype=torch.float16, device=DEV))[0],
+                       lgx.sample_rows(S, u, temperature=0.5)[0])
+
+
 @pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64])
 def test_top_k_of_any_integer_type(dtype):
     S, u = scores(8, 500, 3)

@@ -103,6 +103,19 @@ def test_sample_entry_point_refuses_bad_arguments():
     assert call(S=None) == 1 and call(u=None) == 1 and call(idx=None) == 1
 
 
+def test_sample_entry_point_of_64_bit_settings_refuses_the_same():
+    L = _lib.lib()
+
+    def call(S=P, rows=4, cols=100, ld=100, u=P, ud=0, idx=P):
+        return L.lgx_sample_rows_f64(S, 0, rows, cols, ld, u, ud, 1, 1.0, P, 0, None, 1.0, P, 0.0, P, idx, None, None, 0, None)
+
+    assert call(rows=0) == 0
+    assert call(rows=-1) == 1 and call(ud=1) == 1 and call(cols=0) == 1 and call(ld=99) == 1
+    assert call(rows=2 ** 31) == 3
+    assert call(S=None) == 1 and call(u=None) == 1 and call(idx=None) == 1
+    assert call(rows=1, cols=100000, ld=100000) == 4 and b"workspace" in _err()
+
+
 def test_mask_of_sample_recommendations_is_checked():
     ip, ix = torch.tensor([0, 2, 2, 3]), torch.tensor([0, 9, 4], dtype=torch.int32)
     check = recommend._check_mask
