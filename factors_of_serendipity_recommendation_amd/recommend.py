@@ -75,8 +75,10 @@ def _check_mask(mask: Tuple[torch.Tensor, torch.Tensor], n_users: int, n_items: 
     if indptr.dtype != torch.int64 or indices.dtype != torch.int32:
         raise TypeError(f"mask must be (int64 indptr, int32 indices), got ({indptr.dtype}, {indices.dtype})")
     nnz = indices.numel()
-    bad = (indptr[0] != 0) | (indptr[-1] != nnz) | (indptr[1:] < indptr[:-1]).any()
-    out = ((indices < 0) | (indices >= n_items)).any()
+    # lists that are all empty come with an index that none of them holds (ops.lists_to_device_csr)
+    ends = (indptr[-1] == nnz) | ((indptr[-1] == 0) & (nnz == 1))
+    bad = (indptr[0] != 0) | ~ends | (indptr[1:] < indptr[:-1]).any()
+    out = ((indices < 0) | (indices >= n_items)).any() & (indptr[-1] > 0)
     bad, out = torch.stack((bad, out)).tolist()
     if bad:
         raise ValueError(f"mask indptr must rise from 0 to the {nnz} indices")

@@ -490,6 +490,21 @@ def test_sample_recommendations_masks_and_draws(packed):
     assert none[0].shape == none[1].shape == (0, 40)
 
 
+@pytest.mark.parametrize("packed", [False, True])
+def test_sample_recommendations_with_a_mask_of_empty_lists(packed):
+    """Users without train positives draw what they draw without a mask; so do chunks in which every list is empty."""
+    eu, ei = _tables(9, 300, 32, 2)
+    items, users = lgx.mx_quantize(ei) if packed else ei, torch.arange(9, device=DEV)
+    u = torch.rand(9, 4, generator=torch.Generator().manual_seed(3)).to(DEV)
+    want = recommend.sample_recommendations(eu, items, users, u, top_p=0.9)
+    got = recommend.sample_recommendations(eu, items, users, u, ops.lists_to_device_csr([[]] * 9, DEV), top_p=0.9)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    mask = ops.lists_to_device_csr([[], [], [], list(range(300)), [], [], [], [], []], DEV)
+    got = recommend.sample_recommendations(eu, items, users, u, mask, top_p=0.9, chunk_bytes=2 * 300 * 4)
+    other = torch.arange(9) != 3
+    assert (got[0][3] == -1).all() and torch.equal(got[0][other], want[0][other])
+
+
 def test_chain_captured_and_replayed():
     """quantise -> score -> draw captured once and replayed over changed inputs, with eager work between the
     replays; a second graph of other sizes lives beside it."""

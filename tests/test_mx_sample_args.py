@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import factors_of_serendipity_recommendation_amd as lgx
-from factors_of_serendipity_recommendation_amd import _lib, recommend
+from factors_of_serendipity_recommendation_amd import _lib, ops, recommend
 
 P = ctypes.c_void_p(4096)  # an aligned address that a refused call never touches
 ODD = ctypes.c_void_p(4100)
@@ -132,3 +132,19 @@ def test_mask_of_sample_recommendations_is_checked():
     for types in ((ip.int(), ix), (ip, ix.long()), (ip.float(), ix)):
         with pytest.raises(TypeError):
             check(types, 3, 10)
+
+
+def test_mask_of_empty_lists():
+    """What the framework itself makes of lists without an item: an indptr of zeros and a single index."""
+    for users in (0, 1, 3):
+        mask = ops.lists_to_device_csr([[] for _ in range(users)], "cpu")
+        for n_items in (0, 1, 10):
+            recommend._check_mask(mask, users, n_items)
+        assert not ops.dense_mask_offsets(mask, 10, 0, users).numel()
+    zeros = torch.zeros(3, dtype=torch.int64)
+    with pytest.raises(ValueError):
+        recommend._check_mask((zeros, torch.zeros(2, dtype=torch.int32)), 2, 10)
+    with pytest.raises(ValueError):
+        recommend._check_mask((torch.tensor([0, 1, 0]), torch.zeros(1, dtype=torch.int32)), 2, 10)
+    with pytest.raises(ValueError):
+        recommend._check_mask((zeros + 1, torch.zeros(1, dtype=torch.int32)), 2, 10)
