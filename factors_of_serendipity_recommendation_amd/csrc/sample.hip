@@ -535,8 +535,8 @@ __device__ __forceinline__ double draw_number(const SampleArgs& a, int64_t row, 
     return fmin(fmax(u, 0.0), 1.0);
 }
 
-// v_med3 ignores NaN (so does the maximum, but the compiler first makes signalling NaN quiet: two instructions)
-__device__ __forceinline__ float max_of(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
+// The larger of two scores, the number of a number and a NaN; NaN of two NaN, which the next maximum with a number drops
+__device__ __forceinline__ float max_of(float a, float b) { return fmaxf(a, b); }
 
 // the best of the columns [lo, hi) as a key, 0 without one
 template <bool BF16>
