@@ -205,7 +205,7 @@ __device__ __forceinline__ float sigmoid(float x) {
     const float t = x * c;
     float e = __builtin_amdgcn_exp2f(t);
     if (!BF16) {
-        const float rest = __builtin_amdgcn_fmed3f(fmaf(x, c_rest, fmaf(x, c, -t)), -0.01f, 0.01f);  // (no number for infinite x)
+        const float rest = __builtin_amdgcn_fmed3f(fmaf(x, c_rest, fmaf(x, c, -t)), -0.01f, 0.01f);  // infinite x: of a NaN the lower bound, which leaves 0 and infinity as they are
         e *= fmaf(rest, 0.69314718f, 1.0f);
     }
     return __builtin_amdgcn_rcpf(1.0f + e);

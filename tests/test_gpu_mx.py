@@ -147,6 +147,21 @@ def test_sigmoid_in_bf16(B, I, d, scale):
     assert ((got - want).abs() <= bound / 4 + 2.0 ** -17 * want + 2.0 ** -9 * (want + bound) * 2 + 1e-38).all()
 
 
+@pytest.mark.parametrize("B,d", [(3, 64), (50, 100), (50, 300)])
+def test_sigmoid_of_infinite_and_undefined_scores(B, d):
+    """Scores past f32's range are 0 and 1, undefined ones stay so."""
+    x, y = torch.full((B, d), 1e30, device=DEV), torch.full((7, d), 1e30, device=DEV)
+    y[1], y[2], y[3, 0], y[4] = -1e30, 0.0, float("nan"), 1e-30
+    q, it = lgx.mx_quantize(x), lgx.mx_quantize(y)
+    raw = lgx.score_mx(q, it)
+    assert (raw[:, 0] == float("inf")).all() and (raw[:, 1] == float("-inf")).all()
+    want = torch.tensor([1.0, 0.0, 0.5, float("nan"), 1.0, 1.0, 1.0], device=DEV).expand(B, 7)
+    for dtype in (torch.float32, torch.bfloat16):
+        got = lgx.score_mx(q, it, apply_sigmoid=True, dtype=dtype).float()
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        assert torch.equal(torch.nan_to_num(got, 7.0), torch.nan_to_num(want, 7.0))
+
+
 @pytest.mark.parametrize("kind", ["f32", "mx"])
 def test_score_mx_gathers_rows_and_flags_bad_ones(kind):
     x, items = table(40, 96, 1), lgx.mx_quantize(table(333, 96, 2))
