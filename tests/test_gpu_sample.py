@@ -556,3 +556,29 @@ def test_two_streams_at_once():
                 got.append(work())
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+
+
+def test_two_streams_with_inputs_of_their_own():
+    """Rows shared by workgroups, and queries quantised by the call: what a call keeps in its workspace between its launches
+    is its own, while another stream's calls on other numbers and settings of the same sizes are under way."""
+    def work(seed, kw):
+        eu, ei = _tables(40, 90000, 64, seed)
+        t = lgx.mx_quantize(ei)
+        u = torch.rand(40, 4, generator=torch.Generator().manual_seed(seed)).to(DEV)
+        return lambda: (S := lgx.score_mx(eu, t), *lgx.sample_rows(S, u, **kw))
+
+    for settings in (({"top_p": 0.9}, {"top_p": 0.5, "temperature": 0.3}), ({"top_p": 0.8}, {"top_k": 300}), ({"top_k": 50}, {}),
+                     ({"min_p": 0.01}, {"top_k": 900, "top_p": 0.7})):
+        works = [work(seed, kw) for seed, kw in enumerate(settings, 5)]
+        want = [w() for w in works]
+        assert not torch.equal(want[0][1], want[1][1])
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in works]
+        got = []
+        for _ in range(6):
+            for j, (s, w) in enumerate(zip(streams, works)):
+                with torch.cuda.stream(s):
+                    got.append((j, w()))
+        torch.cuda.synchronize()
+        for j, g in got:
+            assert all(torch.equal(a, b) for a, b in zip(g, want[j])), settings
