@@ -69,7 +69,7 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t a) {
 
 // 4 lanes per block, 8 elements a lane.  VEC: rows are 16-byte aligned and d % 8 == 0.  rows_of (optional):
 // the source row of every output row, a row outside [0, n_src) gives NaN blocks.  Bound by memory: 1M x 256 f32, 1.16 GB, in
-// 237 us (4.9 TB/s, a copy's rate); 70,839 x 64 in 4.6 us.  Rows at odd addresses are loaded as wide, at any multiple of an
+// 234 us (5.0 TB/s, a copy's rate); 70,839 x 64 in 4.5 us.  Rows at odd addresses are loaded as wide, at any multiple of an
 // element (100,000 x 601 f32 43 us, element by element 101).
 template <bool BF16, bool VEC>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const void* __restrict__ X, const int64_t* __restrict__ rows_of,
@@ -120,7 +120,7 @@ __device__ __forceinline__ float scale_value(uint32_t b) {  // 2^(b - 127); b = 
     return b == 255u ? __builtin_nanf("") : __uint_as_float(b ? b << 23 : 0x00400000u);
 }
 
-// 4 lanes per block, 8 elements a lane (the layout of the quantiser).  1M x 256 to f32: 237 us; 100,000 x 601 55 us
+// 4 lanes per block, 8 elements a lane (the layout of the quantiser).  1M x 256 to f32: 237 us (in a loop of calls 214, the quantiser 201); 100,000 x 601 50 us
 // (element by element 146)
 template <bool BF16, bool VEC>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint8_t* __restrict__ codes,
@@ -197,8 +197,8 @@ __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c, uint32_t sa, u
 }
 
 // e^-x by one instruction, |x| 2^-24 off for the rounding of x log2(e): below 2^-17 where the result is not 0, enough for
-// bf16 results.  f32 ones take the product's rest in: within 2^-22 with the reciprocal's 1 ulp.  2048 x 40,981 with expf: bf16
-// 59 us (34), f32 79 (76); an IEEE division made the stores wait
+// bf16 results.  f32 ones take the product's rest in: within 2^-22 with the reciprocal's 1 ulp.  A call of 2048 x 40,981 with expf: bf16
+// 59 us (34), f32 79 (74); an IEEE division made the stores wait
 template <bool BF16>
 __device__ __forceinline__ float sigmoid(float x) {
     constexpr float c = -1.44269502f, c_rest = (float)(-1.4426950408889634074 - (double)c);  // -log2(e)
@@ -391,7 +391,7 @@ constexpr int kUserTiles = 8;  // tiles of 32 users a workgroup of score_mx_shor
 // Rows of at most 8 blocks (d <= 256), HB = ceil(nb / 2): a wave keeps 128 items in registers and walks the
 // users' tiles; the next tile's rows are loaded before this one's scores are stored, so that no load waits
 // behind a store.  Bound by the writes of the score matrix: 1024 x 1M x 256 f32, 4.1 GB, in 0.76 ms (the same stores
-// without loads and products 0.755); 2048 x 40,981 x 64 with the sigmoid 66 us.
+// without loads and products 0.755); 2048 x 40,981 x 64 with the sigmoid 70 us (62 at best; a call 74 to 78).
 template <int HB, bool BF16, bool SIG, bool NT>
 __global__ __launch_bounds__(256, 2) void score_mx_short(MxArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -421,7 +421,9 @@ __global__ __launch_bounds__(256, 2) void score_mx_short(MxArgs a) {
 }
 
 // The same for one tile of users: a wave keeps that, quantised by itself, and walks the items, the next 128 on their way.
-// Bound by the reading of the table: 1 x 1M x 256, 136 MB, in 29 us.
+// Bound by the reading of the table: 1 x 1M x 256, 136 MB, in 29 us.  Four steps (d of 193 to 256) take all 256 registers and
+// spill 12 to 28 of them, 64 where it packs the queries and writes bf16 scores without the sigmoid: a call of 1 x 1M x 256 takes 36 us
+// there, 31 with the sigmoid, 30 with f32 scores.
 template <int QD, int HB, bool BF16, bool SIG, bool NT>
 __global__ __launch_bounds__(256, 2) void score_mx_few(MxArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -457,8 +459,10 @@ __global__ __launch_bounds__(256, 2) void score_mx_few(MxArgs a) {
 // blocks 8 at a time through LDS: read from there a row's 16 bytes a lane cost a line each (333 x 91,599 x 1000: 93 us, its
 // address unit busy throughout), while 8 lanes fetch the 128 bytes of a row together.  The next 8 blocks are on their way
 // in registers during the products.  Block b of a row lies at slot b ^ (r % 8) of the row's 128 bytes, of an item's at b ^ (r / 4 %
-// 8), so that 8 lanes that read one block of 8 rows (items: every fourth) touch all banks.  333 x 91,599 x 1000 bf16: 45 us, for 49 MB of
-// codes (23 us of memory time with the 61 MB of scores).
+// 8), so that 8 lanes that read one block of 8 rows (items: every fourth) touch all banks.  333 x 91,599 x 1000 bf16: 43 to 45 us, for 49 MB of
+// codes (23 us of memory time with the 61 MB of scores): 1080 workgroups of two a CU are 2.1 fillings of the chip, of 384 users.  Few
+// users leave CUs idle (184 workgroups): 1 x 91,599 x 1000 12 us with packed queries, 15 with f32 ones, which a launch of its own packs;
+// 8 x 200,000 x 768 16 and 19 (17 us of memory time).
 template <int UW, int NU, bool BF16, bool SIG, bool NT>
 __global__ __launch_bounds__(256, 2) void score_mx_long(MxArgs a, int user_tiles) {
     constexpr int kUsers = UW * NU * 32, kItems = 4 / UW * 128, kRows = kUsers + kItems;

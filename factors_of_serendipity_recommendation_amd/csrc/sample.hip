@@ -8,12 +8,15 @@
 // top_p: a histogram of the distances to the best score, in 4096 equal steps, counts columns; a count times the weight
 // at the columns' mean place in the step is close enough to name the step or two in which the running weight reaches its target.
 // The next reading sums the exact weights of everything better, and gathers those steps' columns, among which the cut is
-// found.  What does not fit (a top_k of thousands, sums that show the cut elsewhere) takes a descent over the 32 score bits.
+// found.  What does not fit (a top_k of thousands, sums that show the cut elsewhere) takes a descent over the 32 score bits, by
+// one workgroup also where several share a row: 1 x 1M f32 with top_k 1024 37 us, 1025 333, 5000 415; 64 x 1M 117, 470, 512; 2048 x
+// 40,981 with top_k 1000 132, 5000 210.
 // Without restrictions one reading does, each segment of the row weighed against its own best score.
 //
 // Which column a given number draws depends on every weight before it, and with a million columns the borders
 // between columns lie 1e-6 of the total apart, so 24 bits are not enough: weights are computed in f64 and
-// summed in f64 in a fixed order, and what atomics add are integers (so that their order does not matter).
+// summed in f64 in a fixed order, and what atomics add are integers (so that their order does not matter): the columns of a list
+// or of top_p's window in units of 2^-51 and 2^-49 of the best weight, which 64 bits hold thousands of, rows of any length in 2^-84.
 //
 // Bounds: a reading runs at up to 5.6 TB/s; the exact sums take 29 vector instructions a step of 64 columns, 16 of them the
 // weight (2 of the difference, 4 of the exponent's split, a polynomial of degree 9, the scaling), 4 cycles each at the 2.0 GHz that
@@ -125,7 +128,7 @@ __device__ __forceinline__ void load_tail(float (&v)[4], const void* s, int64_t 
 
 // f(four scores, column of the first) over columns [lo, hi) by `width` lanes, this one being `me`; a lane takes
 // its columns in ascending order.  U = 1, 2: so many groups at a time with the next ones on their way (f takes long); U = 4, 8:
-// so many on their way at once (8 bytes each of bf16 rows: 1024 x 91,599, top_k 100, 78 us with eight, 83 with four).  What is
+// so many on their way at once (8 bytes each of bf16 rows: 1024 x 91,599, top_k 100, 73.5 us with eight, 78.6 with four).  What is
 // past the end comes as -inf
 template <bool BF16, int U, typename F>
 __device__ __forceinline__ void for_groups(const void* s, int64_t lo, int64_t hi, int me, int width, F f) {
@@ -1380,8 +1383,8 @@ __device__ __forceinline__ void sum_segments(const void* s, int64_t cols, const 
 
 // The same without any restriction, in one reading: a segment's weights against the segment's own best score,
 // sum(g, weights, best score).  A wave keeps 1024 columns in registers between finding their best and weighing them.
-// Against a reading for the best score and one for the sums: 2048 x 91,599 f32 214 us (295), 64 x 1M 65 us (104), 64 x 40,981
-// bf16 14 us (21).  A segment's sum is above 0 iff its best column's weight is, so no draw meets a segment without columns
+// Against a reading for the best score and one for the sums: 2048 x 91,599 f32 190 us (295), 64 x 1M 65 us (104), 64 x 40,981
+// bf16 15 us (21).  A segment's sum is above 0 iff its best column's weight is, so no draw meets a segment without columns
 template <bool BF16, typename Sum>
 __device__ __forceinline__ void sum_own(const void* s, int64_t cols, const Segments& segs, int g0, int g1, const Weigh& like, Sum sum) {
     constexpr int U = 4, N = Vec<BF16>::N;
@@ -1443,7 +1446,7 @@ __device__ __forceinline__ void sum_own(const void* s, int64_t cols, const Segme
 }
 
 // A row of at most kGroup x kList columns by one workgroup: the running weights of groups of columns in LDS, which every thread
-// searches for a draw of its own: 256 x 14,687 f32 with min_p, 100 draws 12 us (a wave a draw, on segments, 35), 20 draws 13 (16);
+// searches for a draw of its own: 256 x 14,687 f32 with min_p, 100 draws 12.8 us (a wave a draw, on segments, 35), 20 draws 12.6 (16);
 // one draw of 1000 columns 7.3 (7.0), of 14,687 a wave's still: the groups take another reading
 template <bool BF16>
 __device__ __forceinline__ bool draw_groups(const SampleArgs& a, int64_t row, const Row& r, const void* s, const Cut& cut,
@@ -1771,7 +1774,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int64_t row, con
     draw_columns<BF16>(a, row, r, s, segs, cut, weigh, 0, 1, sh);
 }
 
-// 2048 x 40,981 f32, top_p: 175 us (2 1/8 readings, of which the memory's share is 126); 1024 x 91,599 bf16, top_k 100: 78 us (one
+// 2048 x 40,981 f32, top_p: 166 to 173 us (2 1/8 readings, of which the memory's share is 126), min_p 117; 1024 x 91,599 bf16, top_k 100: 74 us (one
 // reading and a third, 44).  Held to 80 registers (three workgroups a CU) with 8 to 13 spilled
 template <bool BF16, bool K, bool P>
 __global__ __launch_bounds__(kThreads, 6) void sample_rows_kernel(SampleArgs a) {
@@ -1783,7 +1786,7 @@ __global__ __launch_bounds__(kThreads, 6) void sample_rows_kernel(SampleArgs a) 
 // The same steps with a row cut into `parts` runs of segments, a workgroup each, and a launch per reading; what the
 // workgroups of a row tell each other goes through the workspace, in integers whose order does not matter or in slots
 // of their own.  A row that needs one of the rare ways is left to its first workgroup in the last launch.
-// 512 x 1M f32 with settings per row: top 192 us (a third of the rows is read whole: 0.7 GB), find 261 (62 %), again 10, sum 270
+// 512 x 1M f32 with settings per row: top 194 us (a third of the rows is read whole: 0.7 GB), find 267 (62 %), again 11, sum 281
 // (a quarter with top_p, a twelfth without restrictions), draw 35, clear 7.
 struct Counted {
     uint32_t count[kBins];

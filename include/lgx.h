@@ -472,8 +472,8 @@ int lgx_score_mx(const void* Q, const uint8_t* q_scales, int q_dtype, int64_t n_
  *   weight w_i = exp((s_i - m) / T); scores of -inf and NaN are excluded; +inf shares the row equally.
  *   ranking: higher score first, ties -> lower column.  Kept are, in this order:
  *   top_k  the first top_k columns (top_k <= 0: all);
- *   top_p  of these the shortest prefix whose weight reaches top_p of theirs to 1e-15, one at least (top_p >= 1:
- *          all);
+ *   top_p  of these the shortest prefix whose weight reaches top_p (1 - 1e-15) of theirs, one at least (top_p >= 1:
+ *          all): equal weights whose sum is top_p of the whole end there, however it is rounded;
  *   min_p  of these the ones with w_i >= min_p.
  *   A draw with the given number u is the first kept column i, in column order, with
  *   sum_{j <= i, kept} w_j > u * sum_{kept} w_j.  T not above 0 (or NaN): the best column.  A
@@ -483,8 +483,11 @@ int lgx_score_mx(const void* Q, const uint8_t* q_scales, int q_dtype, int64_t n_
  *   u [rows, n_draws] f32 or f64 (u_dtype) in [0, 1); values outside are taken as the nearest end.
  *   Each setting is one value for all rows or, where the *_rows pointer is given, one per row: in 32 bits, or for
  *   lgx_sample_rows_f64 in 64 bits.
- * Weights and their sums are held in 64 bits, so that the column does not depend on how the sums
- * are split; results are the same for every call.  1 <= cols < 2^31 - 1, rows < 2^31.
+ * Weights are f64 within 1e-13 of their value, and what the kept ones add up to is summed in f64 in an order that is fixed
+ * for a shape and its settings: a draw is the definition's unless u lies within 1e-11 of a border (1e-13 without top_p).  The
+ * weights that top_p is compared with add up in integers, each within 2^-50 of the best weight (2^-84 where the cut is found by its
+ * score's bits): where the prefix ends within 1e-11 of the best weight of a border, a neighbouring column can end it.  Results are
+ * the same for every call.  1 <= cols < 2^31 - 1, rows < 2^31.
  */
 int lgx_sample_rows_workspace(int64_t rows, int64_t cols, int64_t n_draws, size_t* ws_bytes);
 int lgx_sample_rows(const void* S, int dtype, int64_t rows, int64_t cols, int64_t ld, const void* u, int u_dtype,
